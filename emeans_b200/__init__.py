@@ -13,6 +13,10 @@ It mirrors the reference's interfaces for this path:
   (crates/emeans-cluster/src/backend.rs:126-133).
 - :func:`knn_self` / :func:`knn` follow crates/emeans-cluster/src/knn.rs:17-64.
 
+Beyond the reference, the engine takes one gradient step of a head over the
+rows (``Engine.layer_norm``, ``Engine.linear_cross_entropy``, :class:`AdamW`;
+``emeans_b200.head`` puts them together).
+
 There is no CPU fallback: without the built library or a B200 the calls
 raise.
 """
@@ -28,16 +32,21 @@ from typing import Optional, Sequence
 import numpy as np
 
 __all__ = ["Engine", "Buffer", "B200Assigner", "EngineError", "Config", "Trained",
-           "DedupConfig", "DedupResult", "dedup", "dedup_with_neighbors",
+           "DedupConfig", "DedupResult", "dedup", "dedup_with_neighbors", "AdamW", "AdamWTensor",
            "knn", "knn_self", "L2", "IP", "lib_path", "load"]
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 _LIB_NAME = "libemeans_b200.so"
 
 L2, IP = 0, 1
-F32, U32 = 0, 1
+F32, U32, BF16, F16, F8 = 0, 1, 2, 3, 4
+# Host element types of the buffer types: numpy has no bf16 or 8-bit float, so
+# those travel as their bits.
+_HOST = {F32: np.float32, U32: np.uint32, BF16: np.uint16, F16: np.float16, F8: np.uint8}
 OK, INVALID_ARGUMENT, ERROR, INTERNAL = 0, 1, 2, 3
 NONE_ID = 0xFFFFFFFF
+IGNORE = 0xFFFFFFFF      # target of a row without a label
+ADAMW_BLOCK = 256        # elements that share a scale of the 8-bit states
 GPU_KMAX = 16
 
 _lib = None
@@ -62,6 +71,13 @@ class _DedupOut(C.Structure):
                 ("anchors", C.c_void_p), ("sizes", C.c_void_p), ("nn_sim", C.c_void_p),
                 ("n_groups", C.c_uint64), ("linked_pairs", C.c_uint64),
                 ("split_components", C.c_uint64)]
+
+
+class _AdamWTensor(C.Structure):
+    """eb_adamw_tensor (include/emeans_b200.h)."""
+    _fields_ = [("p", C.c_void_p), ("g", C.c_void_p), ("m", C.c_void_p), ("v", C.c_void_p),
+                ("m_scale", C.c_void_p), ("v_scale", C.c_void_p), ("copy", C.c_void_p),
+                ("weight_decay", C.c_double)]
 
 
 class EngineError(RuntimeError):
@@ -118,6 +134,7 @@ def load():
         "eb_last_error": (C.c_char_p, []),
         "eb_version": (C.c_char_p, []),
         "eb_engine_create": (I, [I, C.POINTER(P)]),
+        "eb_engine_create_on": (I, [I, P, C.POINTER(P)]),
         "eb_engine_destroy": (I, [P]),
         "eb_engine_name": (I, [P, C.c_char_p, S]),
         "eb_flush": (I, [P]),
@@ -162,6 +179,14 @@ def load():
         "eb_dedup_with_neighbors": (I, [P, S, S, P, P, S, P, P, P, C.POINTER(_DedupConfig),
                                         C.POINTER(_DedupOut)]),
         "eb_dedup": (I, [P, P, S, S, P, P, P, C.POINTER(_DedupConfig), C.POINTER(_DedupOut)]),
+        "eb_layer_norm": (I, [P, P, S, S, S, P, P, C.c_float, P, S, P, P]),
+        "eb_layer_norm_backward": (I, [P, P, S, P, S, S, S, P, P, P, P, S, P, P]),
+        "eb_linear_ce": (I, [P, P, S, S, S, P, S, S, P, C.c_float, P, P]),
+        "eb_linear_ce_backward": (I, [P, P, S, S, S, P, S, S, P, C.c_float, P, P, P, S, P, S]),
+        "eb_adamw_create": (I, [P, P, S, C.POINTER(P)]),
+        "eb_adamw_destroy": (I, [P, P]),
+        "eb_adamw_step": (I, [P, P, C.c_double, C.c_uint64, C.c_double, C.c_double, C.c_double,
+                              C.c_float]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
@@ -205,15 +230,16 @@ class Buffer:
         return load().eb_buf_ptr(self.h) or 0
 
     def read(self, lo: int = 0, hi: Optional[int] = None) -> np.ndarray:
-        """``Device::read_f32/u32``: waits for queued work."""
+        """``Device::read_f32/u32``: waits for queued work. bf16 and 8-bit
+        elements come back as their bits (uint16, uint8)."""
         hi = len(self) if hi is None else hi
-        out = np.empty(max(hi - lo, 0), np.float32 if self.dtype == F32 else np.uint32)
+        out = np.empty(max(hi - lo, 0), _HOST[self.dtype])
         _check(load().eb_buf_read(self.engine.h, self.h, lo, hi, _ptr(out)))
         return out
 
     def write(self, offset: int, values) -> None:
         """``Device::write_f32/u32``."""
-        v = _f32(values) if self.dtype == F32 else _u32(values)
+        v = np.ascontiguousarray(values, dtype=_HOST[self.dtype])
         _check(load().eb_buf_write(self.engine.h, self.h, offset, _ptr(v), v.size))
 
     def free(self) -> None:
@@ -266,12 +292,18 @@ _LAWS = {"auto": 0, "throughput": 1, "quality": 2}
 
 
 class Engine:
-    """One engine (stream, scratch, bound data) on one CUDA device."""
+    """One engine (stream, scratch, bound data) on one CUDA device. With
+    ``stream`` (a cudaStream_t, such as ``torch.cuda.current_stream().cuda_stream``)
+    its work is queued there instead of on a stream of its own, in order with
+    the caller's; the stream must outlive the engine."""
 
-    def __init__(self, device: int = 0):
+    def __init__(self, device: int = 0, stream: Optional[int] = None):
         lib = load()
         h = C.c_void_p()
-        _check(lib.eb_engine_create(device, C.byref(h)))
+        if stream is None:
+            _check(lib.eb_engine_create(device, C.byref(h)))
+        else:
+            _check(lib.eb_engine_create_on(device, stream, C.byref(h)))
         self.h = h.value
         self.device = device
 
@@ -350,13 +382,19 @@ class Engine:
         x = _f32(x).ravel()
         return self._new(load().eb_bind, _ptr(x), x.size // d, d, dtype=F32)
 
+    def zeros(self, dtype: int, n: int) -> Buffer:
+        """A zeroed buffer of n elements of any buffer type."""
+        return self._new(load().eb_buf_alloc, dtype, n, dtype=dtype)
+
     def wrap(self, tensor) -> Buffer:
-        """A non-owning view of a torch CUDA tensor (float32 or int32/uint32)."""
+        """A non-owning view of a torch CUDA tensor (float32, int32/uint32,
+        bfloat16, float16 or float8_e4m3fn)."""
         import torch
 
         assert tensor.is_cuda and tensor.is_contiguous()
-        dtype = F32 if tensor.dtype == torch.float32 else U32
-        assert tensor.dtype in (torch.float32, torch.int32, torch.uint32)
+        dtype = {torch.float32: F32, torch.int32: U32, torch.uint32: U32, torch.bfloat16: BF16,
+                 torch.float16: F16, torch.float8_e4m3fn: F8}.get(tensor.dtype)
+        assert dtype is not None, tensor.dtype
         return self._new(load().eb_buf_wrap, dtype, tensor.data_ptr(), tensor.numel(), dtype=dtype,
                          owner=tensor)
 
@@ -440,6 +478,49 @@ class Engine:
         decay = np.float32(1.0 - alpha)
         _check(load().eb_ema_update(self.h, positions.h, usage.h, sums.h, counts.h, k, d,
                                     float(a32), float(decay), int(alpha == 1.0)))
+
+    # ---- training operators
+    def layer_norm(self, x: Buffer, rows: int, d: int, weight: Optional[Buffer],
+                   bias: Optional[Buffer], y: Buffer, eps: float = 1e-5,
+                   mean: Optional[Buffer] = None, rstd: Optional[Buffer] = None, ldx: int = 0,
+                   ldy: int = 0):
+        """y = (x - mean) rstd weight + bias of each row (eb_layer_norm): f32,
+        bf16 or f16 rows, ``ldx`` / ``ldy`` elements apart (0: d). mean and
+        rstd keep the statistics for the backward pass."""
+        _check(load().eb_layer_norm(self.h, x.h, rows, d, ldx, weight.h if weight else None,
+                                    bias.h if bias else None, eps, y.h, ldy,
+                                    mean.h if mean else None, rstd.h if rstd else None))
+
+    def layer_norm_backward(self, dy: Buffer, x: Buffer, rows: int, d: int,
+                            weight: Optional[Buffer], mean: Buffer, rstd: Buffer,
+                            dx: Optional[Buffer], dweight: Optional[Buffer] = None,
+                            dbias: Optional[Buffer] = None, lddy: int = 0, ldx: int = 0,
+                            lddx: int = 0):
+        """The gradients of ``layer_norm`` (eb_layer_norm_backward)."""
+        _check(load().eb_layer_norm_backward(
+            self.h, dy.h, lddy, x.h, ldx, rows, d, weight.h if weight else None, mean.h, rstd.h,
+            dx.h if dx else None, lddx, dweight.h if dweight else None,
+            dbias.h if dbias else None))
+
+    def linear_cross_entropy(self, x: Buffer, n: int, d: int, w: Buffer, k: int, targets: Buffer,
+                             loss: Buffer, lse: Buffer, scale: float = 1.0, ldx: int = 0,
+                             ldw: int = 0):
+        """loss[i] = log sum_j exp(z_ij) - z[i, targets[i]] with the scores z =
+        scale x . w of n rows against k prototypes, which are never stored
+        (eb_linear_ce); rows with target ``IGNORE`` have loss 0."""
+        _check(load().eb_linear_ce(self.h, x.h, n, d, ldx, w.h, k, ldw, targets.h, scale, loss.h,
+                                   lse.h))
+
+    def linear_cross_entropy_backward(self, x: Buffer, n: int, d: int, w: Buffer, k: int,
+                                      targets: Buffer, lse: Buffer, dloss: Buffer,
+                                      dx: Optional[Buffer], dw: Optional[Buffer],
+                                      scale: float = 1.0, ldx: int = 0, ldw: int = 0,
+                                      lddx: int = 0, lddw: int = 0):
+        """The gradients of ``linear_cross_entropy`` from its lse and the rows'
+        loss gradients ``dloss`` (n, or one for all) (eb_linear_ce_backward)."""
+        _check(load().eb_linear_ce_backward(self.h, x.h, n, d, ldx, w.h, k, ldw, targets.h, scale,
+                                            lse.h, dloss.h, dx.h if dx else None, lddx,
+                                            dw.h if dw else None, lddw))
 
     # ---- Assigner::assign and the device loop
     def assign(self, rows, d: int, centroids, metric: int, ids=None):
@@ -526,7 +607,8 @@ class Engine:
 
     def view(self, buf: "Buffer", offset: int, length: int, dtype: int) -> "Buffer":
         """A non-owning view of buf's elements offset .. offset + length
-        (4-byte elements; the view's start must be 16-byte aligned). A range
+        (``dtype`` of the same size as buf's; the view's start must be 16-byte
+        aligned). A range
         past buf's end is refused (INVALID_ARGUMENT), as the C calls refuse
         one."""
         offset, length = int(offset), int(length)
@@ -534,7 +616,10 @@ class Engine:
             raise EngineError(INVALID_ARGUMENT,
                               f"view {offset} .. {offset + length} is outside the buffer's "
                               f"{len(buf)} elements")
-        return self._new(load().eb_buf_wrap, dtype, buf.ptr + 4 * offset, length,
+        size = np.dtype(_HOST[dtype]).itemsize
+        if size != np.dtype(_HOST[buf.dtype]).itemsize:
+            raise EngineError(INVALID_ARGUMENT, "a view's elements must be as large as its buffer's")
+        return self._new(load().eb_buf_wrap, dtype, buf.ptr + size * offset, length,
                          dtype=dtype, owner=buf)
 
     def group(self):
@@ -622,6 +707,65 @@ class Engine:
             obj, tr, lab, sco = best
             out.append((k, self.internal_scores(x, d, lab, k), tr, lab, sco, obj))
         return out
+
+
+@dataclass
+class AdamWTensor:
+    """One tensor of an AdamW step (eb_adamw_tensor): parameters and gradients
+    in f32 or bf16, moments in f32, or in 8 bits with their scales."""
+    p: Buffer
+    g: Buffer
+    m: Buffer
+    v: Buffer
+    m_scale: Optional[Buffer] = None
+    v_scale: Optional[Buffer] = None
+    copy: Optional[Buffer] = None
+    weight_decay: float = 0.0
+
+
+class AdamW:
+    """AdamW over many tensors, one kernel a step (eb_adamw_create,
+    eb_adamw_step). The buffers are the caller's; the plan keeps them alive."""
+
+    def __init__(self, engine: Engine, tensors: Sequence[AdamWTensor]):
+        self.engine = engine
+        self.tensors = list(tensors)
+        arr = (_AdamWTensor * max(len(self.tensors), 1))()
+        for a, t in zip(arr, self.tensors):
+            for f in ("p", "g", "m", "v", "m_scale", "v_scale", "copy"):
+                b = getattr(t, f)
+                setattr(a, f, b.h if b is not None else None)
+            a.weight_decay = t.weight_decay
+        h = C.c_void_p()
+        self.h = None
+        _check(load().eb_adamw_create(engine.h, arr, len(self.tensors), C.byref(h)))
+        self.h = h.value
+
+    @staticmethod
+    def states(engine: Engine, n: int, eight_bit: bool = False) -> dict:
+        """Zeroed moments for n parameters, as AdamWTensor's keywords."""
+        if not eight_bit:
+            return {"m": engine.zeros_f32(n), "v": engine.zeros_f32(n)}
+        blocks = -(-n // ADAMW_BLOCK)
+        return {"m": engine.zeros(F8, n), "v": engine.zeros(F8, n),
+                "m_scale": engine.zeros_f32(blocks), "v_scale": engine.zeros_f32(blocks)}
+
+    def step(self, lr: float, step: int, beta1: float = 0.9, beta2: float = 0.999,
+             eps: float = 1e-8, grad_scale: float = 1.0):
+        """Step number ``step`` (from 1) over every tensor."""
+        _check(load().eb_adamw_step(self.engine.h, self.h, lr, step, beta1, beta2, eps,
+                                    grad_scale))
+
+    def free(self) -> None:
+        if self.h and self.engine.h:
+            load().eb_adamw_destroy(self.engine.h, self.h)
+        self.h = None
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
 
 
 def mean_objective(scores, spherical: bool) -> float:

@@ -69,6 +69,31 @@ void touched(eb_engine* e, eb_buf* b) {
   }
 }
 
+bool is_float(int dtype) { return dtype == EB_F32 || dtype == EB_BF16 || dtype == EB_F16; }
+
+void need_float(const eb_buf* b, const char* what) {
+  need(b, what);
+  eb::ensure(is_float(b->dtype), std::string(what) + " must be an f32, bf16 or f16 buffer");
+}
+
+// The row stride of a matrix argument: `ld`, or the row's length for 0; the
+// buffer must hold rows x d at that stride.
+size_t need_rows(const eb_buf* b, size_t rows, size_t d, size_t ld, const char* what) {
+  if (ld == 0) ld = d;
+  eb::ensure(ld >= d, std::string(what) + ": the row stride is shorter than a row");
+  if (rows > 0)
+    eb::ensure(b->len >= d && (rows - 1) <= (b->len - d) / ld,
+               std::string(what) + " is too short for its rows");
+  return ld;
+}
+
+// Buffers over the same memory, in part or whole.
+bool overlap(const eb_buf* a, const eb_buf* b) {
+  if (!a || !b || a->len == 0 || b->len == 0) return false;
+  const char *pa = static_cast<const char*>(a->ptr), *pb = static_cast<const char*>(b->ptr);
+  return pa < pb + b->len * eb::dtype_bytes(b->dtype) && pb < pa + a->len * eb::dtype_bytes(a->dtype);
+}
+
 // check_select (core/mod.rs:432-439).
 void check_select(size_t r0, size_t r1, const eb_buf* ids, size_t n) {
   eb::ensure(r0 <= r1, "bad row range");
@@ -87,7 +112,7 @@ eb_buf* new_buf(eb_engine* e, int dtype, size_t len) {
   b->dtype = dtype;
   b->len = len;
   b->owned = true;
-  size_t bytes = std::max<size_t>(len * 4, 16);
+  size_t bytes = std::max<size_t>(len * dtype_bytes(dtype), 16);
   cudaError_t st = cudaMallocAsync(&b->ptr, bytes, e->stream);
   e->device_allocs++;
   if (st != cudaSuccess) {
@@ -135,7 +160,12 @@ const char* eb_last_error(void) { return g_last_error.c_str(); }
 
 const char* eb_version(void) { return "emeans_b200 0.1 (sm_100a)"; }
 
-int eb_engine_create(int device, eb_engine** out) {
+}  // extern "C"
+
+namespace {
+
+// An engine on a stream of its own, or on the caller's.
+int create_engine(int device, bool own_stream, cudaStream_t stream, eb_engine** out) {
   return guard([&] {
     need(out, "out");
     *out = nullptr;
@@ -157,7 +187,9 @@ int eb_engine_create(int device, eb_engine** out) {
     cudaGetDevice(&prev);
     try {
       EB_CUDA(cudaSetDevice(device));
-      EB_CUDA(cudaStreamCreateWithFlags(&e->stream, cudaStreamNonBlocking));
+      e->owns_stream = own_stream;
+      e->stream = stream;
+      if (own_stream) EB_CUDA(cudaStreamCreateWithFlags(&e->stream, cudaStreamNonBlocking));
       EB_CUDA(cudaMalloc(&e->d_status, 16));
       EB_CUDA(cudaMemset(e->d_status, 0, 16));
       EB_CUDA(cudaMallocHost(&e->h_status, 16));
@@ -175,6 +207,18 @@ int eb_engine_create(int device, eb_engine** out) {
     if (prev >= 0) cudaSetDevice(prev);
     *out = e;
   });
+}
+
+}  // namespace
+
+extern "C" {
+
+int eb_engine_create(int device, eb_engine** out) {
+  return create_engine(device, true, nullptr, out);
+}
+
+int eb_engine_create_on(int device, void* stream, eb_engine** out) {
+  return create_engine(device, false, static_cast<cudaStream_t>(stream), out);
 }
 
 int eb_engine_destroy(eb_engine* e) {
@@ -202,7 +246,7 @@ int eb_engine_destroy(eb_engine* e) {
     cudaFreeHost(e->h_status);
     if (e->copy_stream) cudaStreamDestroy(e->copy_stream);
     if (e->down_stream) cudaStreamDestroy(e->down_stream);
-    cudaStreamDestroy(e->stream);
+    if (e->owns_stream) cudaStreamDestroy(e->stream);
     delete e;
   });
 }
@@ -308,7 +352,7 @@ int eb_buf_alloc(eb_engine* e, int dtype, size_t len, eb_buf** out) {
   return guard([&] {
     need(e, "engine");
     need(out, "out");
-    ensure(dtype == EB_F32 || dtype == EB_U32, "unknown dtype");
+    ensure(eb::dtype_bytes(dtype) != 0, "unknown dtype");
     DeviceGuard g(e);
     *out = eb::new_buf(e, dtype, len);
   });
@@ -318,7 +362,7 @@ int eb_buf_wrap(eb_engine* e, int dtype, void* dev_ptr, size_t len, eb_buf** out
   return guard([&] {
     need(e, "engine");
     need(out, "out");
-    ensure(dtype == EB_F32 || dtype == EB_U32, "unknown dtype");
+    ensure(eb::dtype_bytes(dtype) != 0, "unknown dtype");
     ensure(dev_ptr != nullptr || len == 0, "null device pointer");
     ensure(((uintptr_t)dev_ptr & 15) == 0, "device pointer must be 16-byte aligned");
     cudaPointerAttributes attr{};
@@ -359,7 +403,8 @@ int eb_buf_write(eb_engine* e, eb_buf* b, size_t offset, const void* host, size_
     if (len == 0) return;
     need(host, "host");
     DeviceGuard g(e);
-    eb::h2d(e, static_cast<char*>(b->ptr) + offset * 4, host, len * 4, e->stream);
+    const size_t es = eb::dtype_bytes(b->dtype);
+    eb::h2d(e, static_cast<char*>(b->ptr) + offset * es, host, len * es, e->stream);
     b->version++;
     eb::drop_f16(b);
     if (b->xnorm) {
@@ -377,7 +422,8 @@ int eb_buf_read(eb_engine* e, const eb_buf* b, size_t lo, size_t hi, void* host)
     DeviceGuard g(e);
     if (hi > lo) {
       need(host, "host");
-      eb::d2h(e, host, static_cast<const char*>(b->ptr) + lo * 4, (hi - lo) * 4, e->stream);
+      const size_t es = eb::dtype_bytes(b->dtype);
+      eb::d2h(e, host, static_cast<const char*>(b->ptr) + lo * es, (hi - lo) * es, e->stream);
     }
     eb::sync(e);
   });
@@ -387,11 +433,11 @@ int eb_buf_upload(eb_engine* e, int dtype, const void* host, size_t len, eb_buf*
   return guard([&] {
     need(e, "engine");
     need(out, "out");
-    ensure(dtype == EB_F32 || dtype == EB_U32, "unknown dtype");
+    ensure(eb::dtype_bytes(dtype) != 0, "unknown dtype");
     ensure(host != nullptr || len == 0, "host is null");
     DeviceGuard g(e);
     eb_buf* b = eb::new_buf(e, dtype, len);
-    if (len) eb::h2d(e, b->ptr, host, len * 4, e->stream);
+    if (len) eb::h2d(e, b->ptr, host, len * eb::dtype_bytes(dtype), e->stream);
     *out = b;
   });
 }
@@ -782,6 +828,287 @@ int eb_assign(eb_engine* e, const float* rows, size_t n, size_t d, const uint32_
     eb::d2h(e, labels, lab, m * 4, e->stream);
     eb::d2h(e, scores, sco, m * 4, e->stream);
     eb::sync(e);
+  });
+}
+
+int eb_layer_norm(eb_engine* e, const eb_buf* x, size_t rows, size_t d, size_t ldx,
+                  const eb_buf* weight, const eb_buf* bias, float eps, eb_buf* y, size_t ldy,
+                  eb_buf* mean, eb_buf* rstd) {
+  return guard([&] {
+    need(e, "engine");
+    need_float(x, "x");
+    need_float(y, "y");
+    ensure(y->dtype == x->dtype, "x and y must have one type");
+    ensure(d > 0, "d must be positive");
+    ensure(eps >= 0.0f, "eps must not be negative");
+    eb::LayerNormArgs a;
+    a.ldx = need_rows(x, rows, d, ldx, "x");
+    a.ldy = need_rows(y, rows, d, ldy, "y");
+    ensure(x->ptr != y->ptr || a.ldx == a.ldy, "y over x needs x's row stride");
+    ensure(x->ptr == y->ptr || !overlap(x, y), "y overlaps x");
+    a.wtype = EB_F32;
+    for (const eb_buf* b : {weight, bias}) {
+      if (!b) continue;
+      need_float(b, "weight and bias");
+      ensure(b->dtype == EB_F32 || b->dtype == x->dtype, "weight and bias must be f32 or of x's type");
+      ensure(b->len >= d, "weight and bias must hold d elements");
+      a.wtype = b->dtype;
+    }
+    ensure(!weight || !bias || weight->dtype == bias->dtype, "weight and bias must have one type");
+    for (const eb_buf* b : {mean, rstd}) {
+      if (!b) continue;
+      need_type(b, EB_F32, "mean and rstd");
+      ensure(b->len >= rows, "mean and rstd must hold one element a row");
+    }
+    DeviceGuard g(e);
+    touched(e, y);
+    touched(e, mean);
+    touched(e, rstd);
+    a.x = x->ptr;
+    a.rows = rows;
+    a.d = d;
+    a.weight = weight ? weight->ptr : nullptr;
+    a.bias = bias ? bias->ptr : nullptr;
+    a.eps = eps;
+    a.y = y->ptr;
+    a.mean = mean ? static_cast<float*>(mean->ptr) : nullptr;
+    a.rstd = rstd ? static_cast<float*>(rstd->ptr) : nullptr;
+    a.dtype = x->dtype;
+    eb::layer_norm(e, a);
+  });
+}
+
+int eb_layer_norm_backward(eb_engine* e, const eb_buf* dy, size_t lddy, const eb_buf* x,
+                           size_t ldx, size_t rows, size_t d, const eb_buf* weight,
+                           const eb_buf* mean, const eb_buf* rstd, eb_buf* dx, size_t lddx,
+                           eb_buf* dweight, eb_buf* dbias) {
+  return guard([&] {
+    need(e, "engine");
+    need_float(dy, "dy");
+    need_float(x, "x");
+    ensure(dy->dtype == x->dtype, "dy and x must have one type");
+    ensure(d > 0, "d must be positive");
+    eb::LayerNormBackwardArgs a;
+    a.lddy = need_rows(dy, rows, d, lddy, "dy");
+    a.ldx = need_rows(x, rows, d, ldx, "x");
+    a.lddx = d;
+    if (dx) {
+      need_float(dx, "dx");
+      ensure(dx->dtype == x->dtype, "dx and x must have one type");
+      a.lddx = need_rows(dx, rows, d, lddx, "dx");
+      ensure(dx->ptr != dy->ptr || a.lddx == a.lddy, "dx over dy needs dy's row stride");
+      ensure(dx->ptr == dy->ptr || !overlap(dx, dy), "dx overlaps dy");
+      ensure(!overlap(dx, x), "dx overlaps x");
+    }
+    a.wtype = EB_F32;
+    if (weight) {
+      need_float(weight, "weight");
+      ensure(weight->dtype == EB_F32 || weight->dtype == x->dtype,
+             "weight must be f32 or of x's type");
+      ensure(weight->len >= d, "weight must hold d elements");
+      a.wtype = weight->dtype;
+    }
+    need_type(mean, EB_F32, "mean");
+    need_type(rstd, EB_F32, "rstd");
+    ensure(mean->len >= rows && rstd->len >= rows, "mean and rstd must hold one element a row");
+    for (const eb_buf* b : {dweight, dbias}) {
+      if (!b) continue;
+      need_float(b, "dweight and dbias");
+      ensure(b->dtype == EB_F32 || b->dtype == x->dtype,
+             "dweight and dbias must be f32 or of x's type");
+      ensure(b->len >= d, "dweight and dbias must hold d elements");
+    }
+    DeviceGuard g(e);
+    touched(e, dx);
+    touched(e, dweight);
+    touched(e, dbias);
+    a.dy = dy->ptr;
+    a.x = x->ptr;
+    a.rows = rows;
+    a.d = d;
+    a.weight = weight ? weight->ptr : nullptr;
+    a.mean = static_cast<const float*>(mean->ptr);
+    a.rstd = static_cast<const float*>(rstd->ptr);
+    a.dx = dx ? dx->ptr : nullptr;
+    a.dweight = dweight ? dweight->ptr : nullptr;
+    a.dbias = dbias ? dbias->ptr : nullptr;
+    a.dtype = x->dtype;
+    a.dwtype = dweight ? dweight->dtype : EB_F32;
+    a.dbtype = dbias ? dbias->dtype : EB_F32;
+    eb::layer_norm_backward(e, a);
+  });
+}
+
+}  // extern "C"
+
+namespace {
+
+// The arguments both passes of the linear cross entropy share.
+eb::LinearCeArgs check_linear_ce(eb_engine* e, const eb_buf* x, size_t n, size_t d, size_t ldx,
+                                 const eb_buf* w, size_t k, size_t ldw, const eb_buf* targets,
+                                 float scale) {
+  need(e, "engine");
+  need_float(x, "x");
+  need_float(w, "w");
+  ensure(x->dtype == w->dtype, "x and w must have one type");
+  ensure(d > 0 && d <= 0x7FFFFF00ull, "d must be positive and fit 31 bits");
+  ensure(k > 0 && k <= 0x7FFFFF00ull, "k must be positive and fit 31 bits");
+  ensure(n <= 0x7FFFFF00ull, "n must fit 31 bits");
+  ensure(std::isfinite(scale) && scale > 0.0f, "scale must be positive and finite");
+  need_type(targets, EB_U32, "targets");
+  ensure(targets->len >= n, "targets must hold one element a row");
+  eb::LinearCeArgs a;
+  a.ldx = need_rows(x, n, d, ldx, "x");
+  a.ldw = need_rows(w, k, d, ldw, "w");
+  a.x = x->ptr;
+  a.n = n;
+  a.d = d;
+  a.w = w->ptr;
+  a.k = k;
+  a.targets = static_cast<const uint32_t*>(targets->ptr);
+  a.scale = scale;
+  a.dtype = x->dtype;
+  return a;
+}
+
+}  // namespace
+
+extern "C" {
+
+int eb_linear_ce(eb_engine* e, const eb_buf* x, size_t n, size_t d, size_t ldx, const eb_buf* w,
+                 size_t k, size_t ldw, const eb_buf* targets, float scale, eb_buf* loss,
+                 eb_buf* lse) {
+  return guard([&] {
+    const eb::LinearCeArgs a = check_linear_ce(e, x, n, d, ldx, w, k, ldw, targets, scale);
+    need_type(loss, EB_F32, "loss");
+    need_type(lse, EB_F32, "lse");
+    ensure(loss->len >= n && lse->len >= n, "loss and lse must hold one element a row");
+    ensure(!overlap(loss, lse), "loss overlaps lse");
+    for (const eb_buf* in : {x, w, targets})
+      ensure(!overlap(loss, in) && !overlap(lse, in), "an output overlaps an input");
+    DeviceGuard g(e);
+    touched(e, loss);
+    touched(e, lse);
+    eb::linear_ce(e, a, static_cast<float*>(loss->ptr), static_cast<float*>(lse->ptr));
+  });
+}
+
+int eb_linear_ce_backward(eb_engine* e, const eb_buf* x, size_t n, size_t d, size_t ldx,
+                          const eb_buf* w, size_t k, size_t ldw, const eb_buf* targets,
+                          float scale, const eb_buf* lse, const eb_buf* dloss, eb_buf* dx,
+                          size_t lddx, eb_buf* dw, size_t lddw) {
+  return guard([&] {
+    const eb::LinearCeArgs a = check_linear_ce(e, x, n, d, ldx, w, k, ldw, targets, scale);
+    need_type(lse, EB_F32, "lse");
+    ensure(lse->len >= n, "lse must hold one element a row");
+    need_type(dloss, EB_F32, "dloss");
+    ensure(dloss->len == 1 || dloss->len >= n, "dloss must hold one element, or one a row");
+    eb::LinearCeGrads q{};
+    for (const eb_buf* b : {dx, dw}) {
+      if (!b) continue;
+      need_float(b, "dx and dw");
+      ensure(b->dtype == EB_F32 || b->dtype == x->dtype, "dx and dw must be f32 or of x's type");
+      for (const eb_buf* in : {x, w, targets, lse, dloss})
+        ensure(!overlap(b, in), "an output overlaps an input");
+    }
+    ensure(!overlap(dx, dw), "dx overlaps dw");
+    if (dx) {
+      q.lddx = need_rows(dx, n, d, lddx, "dx");
+      q.dx = dx->ptr;
+      q.dxtype = dx->dtype;
+    }
+    if (dw) {
+      q.lddw = need_rows(dw, k, d, lddw, "dw");
+      q.dw = dw->ptr;
+      q.dwtype = dw->dtype;
+    }
+    q.lse = static_cast<const float*>(lse->ptr);
+    q.dloss = static_cast<const float*>(dloss->ptr);
+    q.one_dloss = dloss->len == 1;
+    DeviceGuard g(e);
+    touched(e, dx);
+    touched(e, dw);
+    eb::linear_ce_backward(e, a, q);
+  });
+}
+
+int eb_adamw_create(eb_engine* e, const eb_adamw_tensor* t, size_t count, eb_adamw** out) {
+  return guard([&] {
+    need(e, "engine");
+    need(out, "out");
+    *out = nullptr;
+    if (count) need(t, "tensors");
+    ensure(count <= 0x7FFFFFFFull, "too many tensors");
+    std::unordered_set<const void*> seen;
+    auto plan = std::make_unique<eb_adamw>();
+    for (size_t i = 0; i < count; i++) {
+      need(t[i].p, "p");
+      need(t[i].g, "g");
+      need(t[i].m, "m");
+      need(t[i].v, "v");
+      const size_t len = t[i].p->len;
+      for (const eb_buf* b : {(const eb_buf*)t[i].p, t[i].g})
+        ensure(b->dtype == EB_F32 || b->dtype == EB_BF16, "p and g must be f32 or bf16 buffers");
+      ensure((t[i].m_scale == nullptr) == (t[i].v_scale == nullptr),
+             "m_scale and v_scale must be given together");
+      const bool eight = t[i].m_scale != nullptr;
+      for (const eb_buf* b : {t[i].m, t[i].v})
+        ensure(b->dtype == (eight ? EB_F8 : EB_F32),
+               eight ? "8-bit m and v must be f8 buffers" : "m and v must be f32 buffers");
+      ensure(t[i].g->len == len && t[i].m->len == len && t[i].v->len == len,
+             "p, g, m and v must have one length");
+      if (eight) {
+        const size_t blocks = (len + EB_ADAMW_BLOCK - 1) / EB_ADAMW_BLOCK;
+        need_type(t[i].m_scale, EB_F32, "m_scale");
+        need_type(t[i].v_scale, EB_F32, "v_scale");
+        ensure(t[i].m_scale->len >= blocks && t[i].v_scale->len >= blocks,
+               "m_scale and v_scale must hold one element for each 256 of p");
+      }
+      if (t[i].copy) {
+        ensure(t[i].copy->dtype == EB_BF16, "copy must be a bf16 buffer");
+        ensure(t[i].copy->len >= len, "copy must be as long as p");
+      }
+      ensure(std::isfinite(t[i].weight_decay), "weight_decay must be finite");
+      if (len == 0) continue;
+      for (eb_buf* b : {t[i].p, t[i].m, t[i].v, t[i].m_scale, t[i].v_scale, t[i].copy}) {
+        if (!b) continue;
+        ensure(seen.insert(b->ptr).second, "a buffer is written twice");
+        plan->written.push_back(b);
+      }
+    }
+    DeviceGuard g(e);
+    try {
+      eb::adamw_create(e, t, count, plan.get());
+    } catch (...) {
+      if (plan->table) cudaFreeAsync(plan->table, e->stream);
+      throw;
+    }
+    *out = plan.release();
+  });
+}
+
+int eb_adamw_destroy(eb_engine* e, eb_adamw* plan) {
+  if (!plan) return EB_OK;
+  return guard([&] {
+    need(e, "engine");
+    DeviceGuard g(e);
+    if (plan->table) cudaFreeAsync(plan->table, e->stream);
+    delete plan;
+  });
+}
+
+int eb_adamw_step(eb_engine* e, eb_adamw* plan, double lr, uint64_t step, double beta1,
+                  double beta2, double eps, float grad_scale) {
+  return guard([&] {
+    need(e, "engine");
+    need(plan, "plan");
+    ensure(step >= 1, "step counts from 1");
+    ensure(std::isfinite(lr), "lr must be finite");
+    ensure(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0, "betas must be in [0, 1)");
+    ensure(std::isfinite(eps) && eps >= 0.0, "eps must be finite and not negative");
+    DeviceGuard g(e);
+    for (eb_buf* b : plan->written) touched(e, b);
+    eb::adamw_step(e, plan, lr, step, beta1, beta2, eps, grad_scale);
   });
 }
 

@@ -31,6 +31,21 @@ inline void ensure(bool ok, const char* msg) {
   if (!ok) throw Error(EB_INVALID_ARGUMENT, msg);
 }
 
+// Bytes of one element of a buffer of `dtype`; 0 for no such type.
+inline size_t dtype_bytes(int dtype) {
+  switch (dtype) {
+    case EB_F32:
+    case EB_U32:
+      return 4;
+    case EB_BF16:
+    case EB_F16:
+      return 2;
+    case EB_F8:
+      return 1;
+  }
+  return 0;
+}
+
 inline void cuda_check(cudaError_t st, const char* what) {
   if (st != cudaSuccess)
     throw Error(EB_ERROR, std::string(what) + ": " + cudaGetErrorString(st));
@@ -82,9 +97,17 @@ struct eb_buf {
   eb::Q8Copy* q8 = nullptr;
 };
 
+// A plan of an AdamW step: the tensors' table and their pieces' on the device.
+struct eb_adamw {
+  void* table = nullptr;
+  size_t pieces_at = 0, pieces = 0;
+  std::vector<eb_buf*> written;  // parameters, states, scales and copies
+};
+
 struct eb_engine {
   int device = 0;
   cudaStream_t stream = nullptr;
+  bool owns_stream = true;  // false: the caller's stream (eb_engine_create_on)
   uint32_t* d_status = nullptr;  // device error flags
   uint32_t* h_status = nullptr;  // pinned mirror
   std::unordered_map<std::string, eb::Scratch> scratch;
@@ -344,6 +367,65 @@ void drop_f16(eb_buf* b);  // drops both screen copies
 // The bound set's split copy (made on first use; null if xbuf is not a bound
 // set of that shape or there is no room).
 Fp16Copy* bound_copy(eb_engine* e, eb_buf* xbuf, const float* x, size_t n, size_t d);
+
+// ---- norm.cu: layer norm over rows of a float type (EB_F32, EB_BF16, EB_F16)
+struct LayerNormArgs {
+  const void* x;
+  size_t rows, d, ldx;
+  const void* weight;  // d of wtype, or null
+  const void* bias;
+  float eps;
+  void* y;
+  size_t ldy;
+  float* mean;  // rows, or null
+  float* rstd;
+  int dtype, wtype;
+};
+void layer_norm(eb_engine* e, const LayerNormArgs& a);
+struct LayerNormBackwardArgs {
+  const void* dy;
+  size_t lddy;
+  const void* x;
+  size_t ldx, rows, d;
+  const void* weight;
+  const float* mean;
+  const float* rstd;
+  void* dx;  // or null
+  size_t lddx;
+  void* dweight;  // or null
+  void* dbias;    // or null
+  int dtype, wtype, dwtype, dbtype;
+};
+void layer_norm_backward(eb_engine* e, const LayerNormBackwardArgs& a);
+
+// ---- linear_ce.cu: softmax cross entropy of x (n x d) against w (k x d)
+struct LinearCeArgs {
+  const void* x;
+  size_t n, d, ldx;
+  const void* w;
+  size_t k, ldw;
+  const uint32_t* targets;
+  float scale;
+  int dtype;
+};
+void linear_ce(eb_engine* e, const LinearCeArgs& a, float* loss, float* lse);
+struct LinearCeGrads {
+  const float* lse;
+  const float* dloss;  // n, or one for all rows
+  bool one_dloss;
+  void* dx;  // or null
+  size_t lddx;
+  int dxtype;
+  void* dw;  // or null
+  size_t lddw;
+  int dwtype;
+};
+void linear_ce_backward(eb_engine* e, const LinearCeArgs& a, const LinearCeGrads& g);
+
+// ---- adamw.cu: a plan's device tables, and one step over them
+void adamw_create(eb_engine* e, const eb_adamw_tensor* t, size_t count, eb_adamw* plan);
+void adamw_step(eb_engine* e, const eb_adamw* plan, double lr, uint64_t step, double b1, double b2,
+                double eps, float gscale);
 
 // ---- topk.cu
 void topk(eb_engine* e, const float* q, size_t m, const float* data, size_t n, size_t d,

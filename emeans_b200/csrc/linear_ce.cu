@@ -1,0 +1,849 @@
+// Softmax cross entropy of rows x (n x d) against prototypes w (k x d), and
+// its gradients, without keeping the n x k scores.
+//
+//   z_ij = scale x_i . w_j,  lse_i = log sum_j exp z_ij,  loss_i = lse_i - z_i,t(i)
+//   P_ij = g_i scale (exp(z_ij - lse_i) - [j = t(i)]),  dx = P w,  dw = P^T x
+//
+// All products run in one persistent tcgen05 kernel (k_gemm) with three
+// epilogues. Forward: the tile of scores stays in TMEM; its epilogue reduces
+// each row's 128 columns to (max, sum of exp) and k_ce_join adds those up.
+// Backward, a piece of the prototypes at a time: the scores again, turned
+// into P (16 bits, engine scratch), then dx += P w and dw = P^T x read that
+// piece. Operands are K-major or MN-major as they lie in memory (w is the
+// K-major operand of the scores and the MN-major one of dx), so nothing is
+// transposed.
+//
+// P is kept as (g_i / max|g|) (p - [j = t]), whose largest entries are
+// rounded with the least error (with one g for all rows they are near -1),
+// and max|g| scale multiplies the products in FP32. bf16 keeps P as bf16; f16
+// keeps it times 2^14 (probabilities down to 2^-28 stay normal); f32 keeps
+// two FP16 terms of P times 2^14.
+//
+// f32 operands: scaled by a power of two so that the largest is below 2^15
+// and split into two FP16 terms (22 bits, absolute floor 2^-39 of the
+// largest); three products hi.hi + hi.lo + lo.hi add into one FP32
+// accumulator. The dropped lo.lo term is 2^-22 of the product.
+//
+// Bound by the tensor cores, 2 n k d operations forward and 6 n k d backward
+// (three times that for f32); for few rows by reading w once.
+#include <cuda_runtime.h>
+#include <cudaTypedefs.h>
+
+#include <cmath>
+
+#include "elem.h"
+#include "engine.h"
+#include "tc.h"
+
+namespace eb {
+
+namespace {
+
+constexpr int BM = 128;   // rows of a tile a CTA holds (TMEM lanes)
+constexpr int BN = 256;   // columns of a tile (TMEM columns of one accumulator)
+constexpr int BK = 64;    // k-elements a stage: one 128-byte swizzle row
+constexpr int NTHREADS = 384;  // warp 0 loads, warp 1 issues products, warps 4-11 epilogue
+constexpr int HALF = BN / 2;   // columns an epilogue warp takes
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr float PSCALE = 16384.0f;  // f16 and f32: P is kept times 2^14
+
+enum Epi { LSE, PROB, OUT };
+
+// Scalars shared by a call's kernels (device scratch): bits of max|x|,
+// max|w| over the finite elements (f32 operands) and of max|dloss|.
+enum { S_X, S_W, S_G, S_WORDS };
+
+// The power of two that brings a largest magnitude (its bits) below 2^15.
+__device__ __forceinline__ float split_scale(uint32_t bits) {
+  if (bits == 0) return 1.0f;
+  const int e = max((int)(bits >> 23), 1) - 127;  // 2^e <= max < 2^(e+1)
+  const int s = min(max(14 - e, -126), 126);
+  return __uint_as_float((uint32_t)(s + 127) << 23);
+}
+
+struct GemmParams {
+  long M, N, K;
+  int mtiles, ntiles, splits, kb_split, kblocks, group;
+  uint32_t fmt;     // operand format of the instruction (0 f16, 1 bf16)
+  uint32_t* status;
+  const uint32_t* scal;
+  float scale;      // of the scores
+  int sx, sw;       // scal slots of the operands' split scales, or -1
+  // LSE
+  float2* part;     // [2 ntiles][M]: (max, sum) of a half tile's columns
+  float* zt;        // M: target scores, base 2
+  const uint32_t* targets;
+  // PROB
+  long col0;        // first column of the piece
+  const float* lse;
+  const float* dloss;
+  int one_dloss;
+  long k;           // columns in all
+  void* p_hi;
+  void* p_lo;
+  long ldp;
+  float pscale;     // what P is kept times: 1 (bf16) or PSCALE
+  // OUT: v = acc scale max|dloss| / pscale, to `out`, or through FP32 sums
+  void* out;
+  int otype;
+  long ldo;
+  float* accum;     // M x N, row stride N (+ split * M * N)
+  int read_acc, write_acc;
+};
+
+template <int CG, int PARTS>
+struct Shape {
+  static constexpr int A_ROWS = BM;
+  static constexpr int B_ROWS = BN / CG;
+  static constexpr int A_BYTES = A_ROWS * BK * 2;
+  static constexpr int B_BYTES = B_ROWS * BK * 2;
+  static constexpr int STAGE = PARTS * (A_BYTES + B_BYTES);
+  static constexpr int STAGES = 196608 / STAGE;
+  // Operand ring, barriers, and each epilogue warp's 32 x 32 block.
+  static constexpr size_t SMEM = 1024 + (size_t)STAGES * STAGE + 256 + 8 * 4096;
+  // k-blocks summed in one TMEM accumulator. The tensor cores' FP32 sums are
+  // cut, not rounded, at every step of 16 (about 2^-26 of the sum a product,
+  // always towards zero): 5.6e-6 of dx at k = 5,003 in one chain of three
+  // products a step. Two-term operands, which aim at FP32's own error, end a
+  // chain after CHAIN blocks and add it to the epilogue's registers, rounded.
+  static constexpr int CHAIN = PARTS == 2 ? 2 : 1 << 28;
+};
+
+// exp2 of a log2-domain difference (relative error 2^-22; inputs <= 0 but for
+// rounding).
+__device__ __forceinline__ float ex2(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+// Larger of two, NaN if either is (fmaxf would drop it).
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// Folds (m', s') into a running (max, sum of 2^(z - max)); (-inf, 0) is empty.
+__device__ __forceinline__ void fold(float& m, float& s, float2 v) {
+  const float top = max_nan(m, v.x);
+  if (top != -INFINITY) s = s * ex2(m - top) + v.y * ex2(v.x - top);
+  m = top;
+}
+
+// A warp's 32 x 32 block in shared memory: row r's four-column group g is
+// kept at group g ^ (r & 7), so that rows are written by their own threads
+// and read across lanes without bank conflicts.
+__device__ __forceinline__ float4* block4(float* blk, int r, int g) {
+  return reinterpret_cast<float4*>(blk) + r * 8 + (g ^ (r & 7));
+}
+__device__ __forceinline__ float block1(const float* blk, int r, int c) {
+  return blk[r * 32 + (((c >> 2) ^ (r & 7)) << 2) + (c & 3)];
+}
+
+// The tile and k-range of unit u: within a split, groups of `group` row tiles
+// pass over all column tiles, row tile fastest, so that the tiles in flight
+// share operands in L2.
+struct Unit {
+  int mt, nt, split, kb0, kb1;
+};
+__device__ __forceinline__ Unit unit_at(const GemmParams& P, int u) {
+  Unit r;
+  const int tiles = P.mtiles * P.ntiles;
+  r.split = u / tiles;
+  const int t = u % tiles, gn = P.group * P.ntiles;
+  const int g = t / gn, w = t % gn;
+  const int gm = min(P.group, P.mtiles - g * P.group);
+  r.mt = g * P.group + w % gm;
+  r.nt = w / gm;
+  r.kb0 = r.split * P.kb_split;
+  r.kb1 = min(r.kb0 + P.kb_split, P.kblocks);
+  return r;
+}
+
+// D = A B^T over tiles of CG * 128 rows by 256 columns. A is M x K (K-major)
+// or K x M (A_MN), B likewise N x K or K x N. With PARTS = 2 each operand is
+// two FP16 terms.
+template <int EPI, int CG, int PARTS, bool A_MN, bool B_MN>
+__global__ void __launch_bounds__(NTHREADS, 1)
+    k_gemm(const __grid_constant__ CUtensorMap a0, const __grid_constant__ CUtensorMap a1,
+           const __grid_constant__ CUtensorMap b0, const __grid_constant__ CUtensorMap b1,
+           const GemmParams P) {
+  using S = Shape<CG, PARTS>;
+  using namespace tc;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint64_t* full = (uint64_t*)(smem + S::STAGES * S::STAGE);
+  uint64_t* empty = full + S::STAGES;
+  uint64_t* tfull = empty + S::STAGES;
+  uint64_t* tempty = tfull + 2;
+  uint64_t* done = tempty + 2;
+  uint32_t* tmem_slot = (uint32_t*)(done + 1);
+  volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = CG == 2 ? cta_rank() : 0;
+  const int units = P.mtiles * P.ntiles * P.splits;
+  const int first = blockIdx.x / CG, step = gridDim.x / CG;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S::STAGES; s++) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; b++) {
+      mbar_init(&tfull[b], 1);
+      mbar_init(&tempty[b], 8 * CG);
+    }
+    mbar_init(done, 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) tmem_alloc<CG>(tmem_slot, 512);
+  __syncthreads();
+  if constexpr (CG == 2) cluster_sync();
+  fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait();
+
+  // With the sums in registers, the first warpgroup gives some of its own to
+  // the epilogue (128 x 72 + 256 x 216 = 384 x 168).
+  if (warp < 4) {
+    if constexpr (PARTS == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if (warp == 0 && lane == 0) {
+      int it = 0;
+      bool stop = false;
+      for (int u = first; u < units && !stop; u += step) {
+        const Unit q = unit_at(P, u);
+        const int am = (q.mt * CG + (int)rank) * BM, bn = q.nt * BN + (int)rank * S::B_ROWS;
+        for (int kb = q.kb0; kb < q.kb1; kb++, it++) {
+          const int s = it % S::STAGES;
+          if (!mbar_wait(&empty[s], ((it / S::STAGES) & 1) ^ 1, abort_flag)) {
+            stop = true;
+            break;
+          }
+          if (rank == 0) mbar_expect_tx(&full[s], CG * S::STAGE);
+          const uint32_t bar = CG == 2 ? map_rank(smem_u32(&full[s]), 0) : smem_u32(&full[s]);
+          uint8_t* st = smem + s * S::STAGE;
+#pragma unroll
+          for (int p = 0; p < PARTS; p++) {
+            const CUtensorMap* am_ = p ? &a1 : &a0;
+            const CUtensorMap* bm_ = p ? &b1 : &b0;
+            if constexpr (A_MN) {
+#pragma unroll
+              for (int c = 0; c < S::A_ROWS / 64; c++)
+                tma_load<CG>(st + c * 8192, am_, bar, am + c * 64, kb * BK);
+            } else {
+              tma_load<CG>(st, am_, bar, kb * BK, am);
+            }
+            st += S::A_BYTES;
+            if constexpr (B_MN) {
+#pragma unroll
+              for (int c = 0; c < S::B_ROWS / 64; c++)
+                tma_load<CG>(st + c * 8192, bm_, bar, bn + c * 64, kb * BK);
+            } else {
+              tma_load<CG>(st, bm_, bar, kb * BK, bn);
+            }
+            st += S::B_BYTES;
+          }
+        }
+      }
+      // No copy may still be landing when the CTA exits: the first CTA's full
+      // barriers count both CTAs' bytes (on the normal path these waits
+      // return at once).
+      if (rank == 0) {
+        for (int j = it > S::STAGES ? it - S::STAGES : 0; j < it; j++) {
+          const uint64_t t0 = now_ns();
+          while (!mbar_try(&full[j % S::STAGES], (j / S::STAGES) & 1) && now_ns() - t0 < WAIT_NS) {
+          }
+        }
+      }
+    }
+    if (warp == 1 && lane == 0 && rank == 0) {
+      const uint32_t idesc = (1u << 4) | (P.fmt << 7) | (P.fmt << 10) | ((A_MN ? 1u : 0u) << 15) |
+                             ((B_MN ? 1u : 0u) << 16) | ((uint32_t)(BN >> 3) << 17) |
+                             ((uint32_t)(CG * BM >> 4) << 24);
+      int it = 0, tc = 0;  // tc counts chains
+      bool stop = false;
+      for (int u = first; u < units && !stop; u += step) {
+        const Unit q = unit_at(P, u);
+        for (int k0 = q.kb0; k0 < q.kb1 && !stop; k0 += S::CHAIN, tc++) {
+          const int k1 = min(k0 + S::CHAIN, q.kb1);
+          const uint32_t d = tmem + (tc & 1) * BN;
+          if (!mbar_wait(&tempty[tc & 1], ((tc >> 1) & 1) ^ 1, abort_flag)) {
+            stop = true;
+            break;
+          }
+          fence_after();
+          for (int kb = k0; kb < k1; kb++, it++) {
+            const int s = it % S::STAGES;
+            if (!mbar_wait(&full[s], (it / S::STAGES) & 1, abort_flag)) {
+              stop = true;
+              break;
+            }
+            fence_after();
+            const uint32_t st = smem_u32(smem + s * S::STAGE);
+#pragma unroll
+            for (int kk = 0; kk < BK / 16; kk++) {
+              uint64_t da[PARTS], db[PARTS];
+#pragma unroll
+              for (int p = 0; p < PARTS; p++) {
+                const uint32_t a = st + p * (S::A_BYTES + S::B_BYTES), b = a + S::A_BYTES;
+                da[p] = A_MN ? desc_mn(a + kk * 2048, 8192) : desc_k(a + kk * 32);
+                db[p] = B_MN ? desc_mn(b + kk * 2048, 8192) : desc_k(b + kk * 32);
+              }
+              mma_f16<CG>(d, da[0], db[0], idesc, (kb > k0 || kk > 0) ? 1u : 0u);
+              if constexpr (PARTS == 2) {
+                mma_f16<CG>(d, da[0], db[1], idesc, 1u);
+                mma_f16<CG>(d, da[1], db[0], idesc, 1u);
+              }
+            }
+            mma_commit<CG>(&empty[s]);
+          }
+          if (!stop) mma_commit<CG>(&tfull[tc & 1]);
+        }
+      }
+      // Every product this thread issued is complete once `done` flips.
+      mma_commit<CG>(done);
+      const uint64_t t0 = now_ns();
+      while (!mbar_try(done, 0) && now_ns() - t0 < WAIT_NS) {
+      }
+    }
+  } else {
+    if constexpr (PARTS == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    // Epilogue: warp w reads TMEM lanes 32 (w % 4) .. + 31, one row a thread,
+    // and half (w - 4) / 4 of the tile's columns.
+    const int hf = (warp - 4) >> 2;
+    const int r = (warp & 3) * 32 + lane;
+    float* blk = (float*)(smem + S::STAGES * S::STAGE + 256) + (warp - 4) * 1024;
+    const uint32_t base = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(hf * HALF);
+    const float sc2 = [&] {
+      float v = P.scale * LOG2E;
+      if (P.sx >= 0) v /= split_scale(P.scal[P.sx]);
+      if (P.sw >= 0) v /= split_scale(P.scal[P.sw]);
+      return v;
+    }();
+    float factor = 1.0f, gmax = 0.0f;
+    if constexpr (EPI != LSE) {
+      gmax = P.one_dloss ? fabsf(P.dloss[0]) : __uint_as_float(P.scal[S_G]);
+      if constexpr (EPI == OUT) {
+        factor = P.scale / P.pscale * gmax;
+        if (P.sx >= 0) factor /= split_scale(P.scal[P.sx]);
+        if (P.sw >= 0) factor /= split_scale(P.scal[P.sw]);
+      }
+    }
+    const uint32_t release = CG == 2 ? map_rank(smem_u32(tempty), 0) : smem_u32(tempty);
+    int tc = 0;
+    bool stop = false;
+    for (int u = first; u < units && !stop; u += step) {
+      const Unit q = unit_at(P, u);
+      const long i = (long)(q.mt * CG + (int)rank) * BM + r;
+      const bool live = i < P.M;
+      const long c0 = (long)q.nt * BN + hf * HALF;
+      const int cols = (int)min((long)HALF, max(P.N - c0, 0l));
+      float m2 = -INFINITY, sum = 0.0f, lse2 = 0.0f, gr = 0.0f;
+      int tcol = -1;
+      if constexpr (EPI != OUT) {
+        const uint32_t t = live ? P.targets[i] : EB_IGNORE;
+        if (t != EB_IGNORE) {
+          const long rel = (long)t - (EPI == PROB ? P.col0 : 0l) - c0;
+          if (rel >= 0 && rel < cols) tcol = (int)rel;
+        }
+        if constexpr (EPI == PROB) {
+          if (live && (long)t < P.k && t != EB_IGNORE) {
+            lse2 = P.lse[i] * LOG2E;
+            const float g = P.dloss[P.one_dloss ? 0 : i];
+            gr = gmax > 0.0f ? g / gmax : g;  // g: 0, or NaN
+          }
+        }
+      }
+      // Waits for the next chain; then its TMEM columns are this warp's.
+      auto wait_chain = [&] {
+        stop = !mbar_wait(&tfull[tc & 1], (tc >> 1) & 1, abort_flag);
+        fence_after();
+        return !stop;
+      };
+      auto release_chain = [&] {
+        fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_at(release + (tc & 1) * 8);
+        tc++;
+      };
+      float acc[PARTS == 2 ? HALF : 1];
+      if constexpr (PARTS == 2) {
+#pragma unroll
+        for (int j = 0; j < HALF; j++) acc[j] = 0.0f;
+        for (int k0 = q.kb0; k0 < q.kb1; k0 += S::CHAIN) {
+          if (!wait_chain()) break;
+#pragma unroll
+          for (int h = 0; h < HALF / 16; h++) {
+            uint32_t raw[16];
+            tmem_ld16(base + (tc & 1) * BN + h * 16, raw);
+            ld_wait(raw);
+#pragma unroll
+            for (int j = 0; j < 16; j++) acc[h * 16 + j] += __uint_as_float(raw[j]);
+          }
+          release_chain();
+        }
+      } else {
+        wait_chain();
+      }
+      if (stop) break;
+#pragma unroll
+      for (int h = 0; h < HALF / 32; h++) {
+        if (EPI != LSE && h * 32 >= cols) break;
+        float v[32];
+        if constexpr (PARTS == 2) {
+#pragma unroll
+          for (int j = 0; j < 32; j++) v[j] = acc[h * 32 + j];
+        } else {
+          uint32_t raw[32];
+          tmem_ld32(base + (tc & 1) * BN + h * 32, raw);
+          ld_wait(raw);
+#pragma unroll
+          for (int j = 0; j < 32; j++) v[j] = __uint_as_float(raw[j]);
+        }
+        const int left = cols - h * 32;
+        if constexpr (EPI == LSE) {
+          float top = -INFINITY;
+#pragma unroll
+          for (int j = 0; j < 32; j++) {
+            v[j] = j < left ? v[j] * sc2 : -INFINITY;
+            top = max_nan(top, v[j]);
+            if (j + h * 32 == tcol) P.zt[i] = v[j];
+          }
+          const float m = max_nan(m2, top);
+          if (m != -INFINITY) {  // columns of -inf alone add nothing
+            sum *= ex2(m2 - m);
+#pragma unroll
+            for (int j = 0; j < 32; j++) sum += ex2(v[j] - m);
+            m2 = m;
+          }
+        } else {
+          if constexpr (EPI == PROB) {
+#pragma unroll
+            for (int j = 0; j < 32; j++) {
+              float p = ex2(fmaf(v[j], sc2, -lse2));
+              if (j + h * 32 == tcol) p -= 1.0f;
+              v[j] = j < left && gr != 0.0f ? p * gr : 0.0f;
+            }
+          }
+          __syncwarp();
+#pragma unroll
+          for (int g = 0; g < 8; g++)
+            *block4(blk, lane, g) = make_float4(v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]);
+          __syncwarp();
+          const long row0 = i - lane, col = c0 + h * 32;
+          const int rows = (int)min(32l, P.M - row0);
+          if constexpr (EPI == PROB) {
+            // Four lanes a row, eight columns each.
+            const int g = (lane & 3) * 2;
+            for (int rr = lane >> 2; rr < rows; rr += 8) {
+              if (col + g * 4 >= P.ldp) break;
+              const float4 a = *block4(blk, rr, g), b = *block4(blk, rr, g + 1);
+              const float f[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+              Pack<uint16_t, 8> hi, lo;
+#pragma unroll
+              for (int w = 0; w < 8; w++) {
+                if (PARTS == 1 && P.fmt) {
+                  hi.v[w] = __bfloat16_as_ushort(__float2bfloat16_rn(f[w]));
+                } else {
+                  const float t = f[w] * PSCALE;
+                  const __half q = __float2half_rn(t);
+                  hi.v[w] = __half_as_ushort(q);
+                  if (PARTS == 2) lo.v[w] = __half_as_ushort(__float2half_rn(t - __half2float(q)));
+                }
+              }
+              const long at = (row0 + rr) * P.ldp + col + g * 4;
+              *reinterpret_cast<Pack<uint16_t, 8>*>((uint16_t*)P.p_hi + at) = hi;
+              if (PARTS == 2) *reinterpret_cast<Pack<uint16_t, 8>*>((uint16_t*)P.p_lo + at) = lo;
+            }
+          } else if (lane < left) {
+            // One row at a time, one column a lane.
+            float* sum_at = P.accum + ((long)q.split * P.M + row0) * P.N + col + lane;
+            const size_t out_at = (size_t)(row0 * P.ldo + col + lane);
+#pragma unroll 4
+            for (int rr = 0; rr < rows; rr++) {
+              float o = block1(blk, rr, lane) * factor;
+              if (P.read_acc) o += sum_at[rr * P.N];
+              if (P.write_acc)
+                sum_at[rr * P.N] = o;
+              else
+                store_any(P.out, P.otype, out_at + rr * P.ldo, o);
+            }
+          }
+        }
+      }
+      if constexpr (PARTS == 1) release_chain();
+      if constexpr (EPI == LSE) {
+        if (live) P.part[(long)(q.nt * 2 + hf) * P.M + i] = make_float2(m2, sum);
+      }
+    }
+  }
+
+  __syncthreads();
+  if constexpr (CG == 2) cluster_sync();
+  if (warp == 1) {
+    fence_after();
+    tmem_free<CG>(tmem, 512);
+  }
+  if (threadIdx.x == 0 && *abort_flag) atomicOr(P.status, ST_WAIT_TIMEOUT);
+}
+
+// lse and loss of 32 rows from their half tiles' (max, sum): 32 threads a row
+// take every 32nd half tile, then the row's thread adds the 32 in order.
+__global__ void __launch_bounds__(1024)
+    k_ce_join(const float2* __restrict__ part, int parts, long n, long k,
+              const float* __restrict__ zt, const uint32_t* __restrict__ targets, float* loss,
+              float* lse, uint32_t* status) {
+  pdl_wait();
+  __shared__ float2 acc[32][33];
+  const int rx = threadIdx.x & 31, py = threadIdx.x >> 5;
+  const long i = (long)blockIdx.x * 32 + rx;
+  float m = -INFINITY, s = 0.0f;
+  if (i < n) {
+    for (int p = py; p < parts; p += 32) fold(m, s, part[(long)p * n + i]);
+  }
+  acc[py][rx] = make_float2(m, s);
+  __syncthreads();
+  if (py || i >= n) return;
+  for (int p = 1; p < 32; p++) fold(m, s, acc[p][rx]);
+  const float l2 = m + log2f(s);
+  lse[i] = l2 * LN2;
+  const uint32_t t = targets[i];
+  if (t == EB_IGNORE || (long)t >= k) {
+    loss[i] = 0.0f;
+    if (t != EB_IGNORE) atomicOr(status, ST_BAD_LABEL);
+  } else {
+    loss[i] = (l2 - zt[i]) * LN2;
+  }
+}
+
+// Largest magnitude over the finite elements of rows x d f32 values.
+__global__ void __launch_bounds__(256) k_ce_max(const float* __restrict__ x, long rows, long d,
+                                                long ld, uint32_t* out) {
+  pdl_wait();
+  uint32_t m = 0;
+  const long total = rows * d;
+  for (long q = (long)blockIdx.x * 256 + threadIdx.x; q < total; q += (long)gridDim.x * 256) {
+    const uint32_t b = __float_as_uint(x[ld == d ? q : q / d * ld + q % d]) & 0x7FFFFFFFu;
+    if (b < 0x7F800000u) m = max(m, b);
+  }
+  m = __reduce_max_sync(0xffffffffu, m);
+  if ((threadIdx.x & 31) == 0 && m) atomicMax(out, m);
+}
+
+// Rows of x as rows of dp 16-bit elements, zeros past d: f32 as two FP16
+// terms, 16-bit types as they are.
+template <bool SPLIT>
+__global__ void __launch_bounds__(256) k_ce_rows(const void* __restrict__ x, long rows, long d,
+                                                 long ld, long dp, const uint32_t* max_bits,
+                                                 uint16_t* hi, uint16_t* lo) {
+  pdl_wait();
+  const float s = SPLIT ? split_scale(*max_bits) : 1.0f;
+  const long total = rows * dp;
+  for (long q = (long)blockIdx.x * 256 + threadIdx.x; q < total; q += (long)gridDim.x * 256) {
+    const long i = q / dp, c = q % dp;
+    if constexpr (SPLIT) {
+      float v = c < d ? static_cast<const float*>(x)[i * ld + c] * s : 0.0f;
+      if (!isfinite(v)) v = NAN;
+      const __half h = __float2half_rn(v);
+      hi[q] = __half_as_ushort(h);
+      lo[q] = __half_as_ushort(__float2half_rn(v - __half2float(h)));
+    } else {
+      hi[q] = c < d ? static_cast<const uint16_t*>(x)[i * ld + c] : (uint16_t)0;
+    }
+  }
+}
+
+// out = the sum over splits, in order, of the partial products (M x N each),
+// plus the FP32 sums so far.
+__global__ void __launch_bounds__(256)
+    k_ce_reduce(const float* __restrict__ part, int splits, long M, long N, float* accum,
+                int read_acc, int write_acc, void* out, int otype, long ldo) {
+  pdl_wait();
+  const long total = M * N;
+  for (long q = (long)blockIdx.x * 256 + threadIdx.x; q < total; q += (long)gridDim.x * 256) {
+    float s = 0.0f;
+    for (int p = 0; p < splits; p++) s += part[(long)p * total + q];
+    if (read_acc) s += accum[q];
+    if (write_acc)
+      accum[q] = s;
+    else
+      store_any(out, otype, (size_t)(q / N * ldo + q % N), s);
+  }
+}
+
+// ---------------------------------------------------------------- host side
+
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+  static const PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+    cudaDriverEntryPointQueryResult q;
+    void* p = nullptr;
+    EB_CUDA(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q));
+    if (q != cudaDriverEntryPointSuccess || !p)
+      throw Error(EB_ERROR, "cuTensorMapEncodeTiled is not available from the driver");
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+  }();
+  return fn;
+}
+
+// A 16-bit operand: rows x cols, row stride ld (a multiple of 8), one or two
+// terms.
+struct Operand {
+  const uint16_t* hi;
+  const uint16_t* lo;  // null: one term
+  long rows, cols, ld;
+};
+
+// Boxes of 64 columns (128 bytes) by box_rows rows, 128-byte swizzle. Every
+// load's first column is a multiple of 64.
+CUtensorMap make_map(const uint16_t* base, const Operand& o, uint32_t box_rows) {
+  CUtensorMap m;
+  cuuint64_t dims[2] = {(cuuint64_t)o.cols, (cuuint64_t)o.rows};
+  cuuint64_t strides[1] = {(cuuint64_t)o.ld * 2};
+  cuuint32_t box[2] = {64, box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = encode_fn()(&m, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2,
+                           const_cast<uint16_t*>(base), dims, strides, box, estr,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) throw Error(EB_ERROR, "cuTensorMapEncodeTiled failed: " + std::to_string(r));
+  return m;
+}
+
+template <int EPI, int CG, int PARTS, bool A_MN, bool B_MN>
+void launch_gemm(eb_engine* e, const Operand& A, const Operand& B, const GemmParams& P) {
+  using S = Shape<CG, PARTS>;
+  const auto kern = k_gemm<EPI, CG, PARTS, A_MN, B_MN>;
+  EB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::SMEM));
+  const uint32_t ar = A_MN ? 64 : S::A_ROWS, br = B_MN ? 64 : S::B_ROWS;
+  const CUtensorMap a0 = make_map(A.hi, A, ar), a1 = PARTS == 2 ? make_map(A.lo, A, ar) : a0;
+  const CUtensorMap b0 = make_map(B.hi, B, br), b1 = PARTS == 2 ? make_map(B.lo, B, br) : b0;
+  const int units = P.mtiles * P.ntiles * P.splits;
+  const int clusters = std::min(units, e->num_sms / CG);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(clusters * CG));
+  cfg.blockDim = dim3(NTHREADS);
+  cfg.dynamicSmemBytes = S::SMEM;
+  cfg.stream = e->stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = EB_PDL;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = CG;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = CG == 2 ? 2 : 1;
+  cuda_check(cudaLaunchKernelEx(&cfg, kern, a0, a1, b0, b1, P), "linear cross entropy");
+  e->stats.kernel_launches++;
+}
+
+constexpr int CGS = 2;
+
+template <int EPI, bool A_MN, bool B_MN>
+void gemm(eb_engine* e, const Operand& A, const Operand& B, GemmParams P) {
+  const int tm = CGS * BM;
+  P.mtiles = (int)((P.M + tm - 1) / tm);
+  P.ntiles = (int)((P.N + BN - 1) / BN);
+  P.kblocks = (int)((P.K + BK - 1) / BK);
+  if (P.kb_split == 0) P.kb_split = P.kblocks;
+  P.splits = (P.kblocks + P.kb_split - 1) / P.kb_split;
+  P.group = std::min(P.mtiles, 16);
+  P.status = e->d_status;
+  if (A.lo)
+    launch_gemm<EPI, CGS, 2, A_MN, B_MN>(e, A, B, P);
+  else
+    launch_gemm<EPI, CGS, 1, A_MN, B_MN>(e, A, B, P);
+}
+
+// The 16-bit operand of a matrix: itself where TMA can read it (row stride a
+// multiple of 16 bytes), else a copy in scratch; f32 split into two terms.
+Operand operand(eb_engine* e, const void* x, size_t rows, size_t d, size_t ld, int dtype,
+                uint32_t* max_bits, const char* name) {
+  Operand o{};
+  o.rows = (long)rows;
+  o.cols = (long)d;
+  if (dtype != EB_F32 && ld % 8 == 0) {
+    o.hi = static_cast<const uint16_t*>(x);
+    o.ld = (long)ld;
+    return o;
+  }
+  const long dp = ((long)d + 7) / 8 * 8;
+  const bool split = dtype == EB_F32;
+  uint16_t* c = e->scratch_get<uint16_t>(name, rows * (size_t)dp * (split ? 2 : 1));
+  o.hi = c;
+  o.lo = split ? c + rows * (size_t)dp : nullptr;
+  o.ld = dp;
+  const unsigned grid =
+      (unsigned)std::min<size_t>((rows * (size_t)dp + 255) / 256, (size_t)e->num_sms * 16);
+  if (split) {
+    launch_pdl(e, k_ce_max, dim3(grid), dim3(256), 0, static_cast<const float*>(x), (long)rows,
+               (long)d, (long)ld, max_bits);
+    launch_pdl(e, k_ce_rows<true>, dim3(grid), dim3(256), 0, x, (long)rows, (long)d, (long)ld, dp,
+               (const uint32_t*)max_bits, c, c + rows * (size_t)dp);
+    e->stats.kernel_launches += 2;
+  } else {
+    launch_pdl(e, k_ce_rows<false>, dim3(grid), dim3(256), 0, x, (long)rows, (long)d, (long)ld, dp,
+               (const uint32_t*)nullptr, c, (uint16_t*)nullptr);
+    e->stats.kernel_launches++;
+  }
+  return o;
+}
+
+Operand rows_of(const Operand& o, long r0, long r1) {
+  Operand p = o;
+  p.hi += r0 * o.ld;
+  if (p.lo) p.lo += r0 * o.ld;
+  p.rows = r1 - r0;
+  return p;
+}
+
+GemmParams base_params(const LinearCeArgs& a, const uint32_t* scal) {
+  GemmParams P{};
+  P.scal = scal;
+  P.scale = a.scale;
+  P.fmt = a.dtype == EB_BF16 ? 1u : 0u;
+  P.sx = a.dtype == EB_F32 ? S_X : -1;
+  P.sw = a.dtype == EB_F32 ? S_W : -1;
+  P.targets = a.targets;
+  P.k = (long)a.k;
+  P.pscale = a.dtype == EB_BF16 ? 1.0f : PSCALE;
+  return P;
+}
+
+// A product into an output: over splits of k when the tiles alone would leave
+// most of the GPU idle.
+template <bool A_MN>
+void product(eb_engine* e, const Operand& A, const Operand& B, GemmParams P, float* accum,
+             bool read_acc, bool write_acc, void* out, int otype, long ldo) {
+  const long tiles = ((P.M + CGS * BM - 1) / (CGS * BM)) * ((P.N + BN - 1) / BN);
+  const long kblocks = (P.K + BK - 1) / BK, clusters = e->num_sms / CGS;
+  long splits = std::min(clusters / std::max(tiles, 1l), kblocks / 4);
+  if (splits > 1) {
+    P.kb_split = (int)((kblocks + splits - 1) / splits);
+    splits = (kblocks + P.kb_split - 1) / P.kb_split;
+  }
+  if (splits > 1) {
+    P.accum = e->scratch_get<float>("ce_splits", (size_t)(splits * P.M * P.N));
+    P.write_acc = 1;
+    gemm<OUT, A_MN, true>(e, A, B, P);
+    const unsigned grid =
+        (unsigned)std::min<long>((P.M * P.N + 255) / 256, (long)e->num_sms * 16);
+    launch_pdl(e, k_ce_reduce, dim3(grid), dim3(256), 0, (const float*)P.accum, (int)splits, P.M,
+               P.N, accum, (int)read_acc, (int)write_acc, out, otype, ldo);
+    e->stats.kernel_launches++;
+  } else {
+    P.kb_split = 0;
+    P.accum = accum;
+    P.read_acc = read_acc;
+    P.write_acc = write_acc;
+    P.out = out;
+    P.otype = otype;
+    P.ldo = ldo;
+    gemm<OUT, A_MN, true>(e, A, B, P);
+  }
+}
+
+}  // namespace
+
+void linear_ce(eb_engine* e, const LinearCeArgs& a, float* loss, float* lse) {
+  if (a.n == 0) return;
+  uint32_t* scal = e->scratch_get<uint32_t>("ce_scalars", S_WORDS);
+  if (a.dtype == EB_F32) EB_CUDA(cudaMemsetAsync(scal, 0, S_WORDS * 4, e->stream));
+  const Operand X = operand(e, a.x, a.n, a.d, a.ldx, a.dtype, scal + S_X, "ce_x");
+  const Operand W = operand(e, a.w, a.k, a.d, a.ldw, a.dtype, scal + S_W, "ce_w");
+  const int parts = 2 * (int)((a.k + BN - 1) / BN);
+  float2* part = e->scratch_get<float2>("ce_part", (size_t)parts * a.n);
+  float* zt = e->scratch_get<float>("ce_zt", a.n);
+  GemmParams P = base_params(a, scal);
+  P.M = (long)a.n;
+  P.N = (long)a.k;
+  P.K = (long)a.d;
+  P.part = part;
+  P.zt = zt;
+  gemm<LSE, false, false>(e, X, W, P);
+  launch_pdl(e, k_ce_join, dim3((unsigned)((a.n + 31) / 32)), dim3(1024), 0, (const float2*)part,
+             parts, (long)a.n, (long)a.k, (const float*)zt, a.targets, loss, lse, e->d_status);
+  e->stats.kernel_launches++;
+}
+
+void linear_ce_backward(eb_engine* e, const LinearCeArgs& a, const LinearCeGrads& g) {
+  if (!g.dx && !g.dw) return;
+  if (a.n == 0) {
+    if (g.dw)
+      EB_CUDA(cudaMemset2DAsync(g.dw, g.lddw * dtype_bytes(g.dwtype), 0,
+                                a.d * dtype_bytes(g.dwtype), a.k, e->stream));
+    return;
+  }
+  uint32_t* scal = e->scratch_get<uint32_t>("ce_scalars", S_WORDS);
+  if (a.dtype == EB_F32 || !g.one_dloss)
+    EB_CUDA(cudaMemsetAsync(scal, 0, S_WORDS * 4, e->stream));
+  const Operand X = operand(e, a.x, a.n, a.d, a.ldx, a.dtype, scal + S_X, "ce_x");
+  const Operand W = operand(e, a.w, a.k, a.d, a.ldw, a.dtype, scal + S_W, "ce_w");
+  if (!g.one_dloss) {
+    const unsigned grid = (unsigned)std::min<size_t>((a.n + 255) / 256, (size_t)e->num_sms);
+    launch_pdl(e, k_ce_max, dim3(grid), dim3(256), 0, g.dloss, (long)a.n, 1l, 1l, scal + S_G);
+    e->stats.kernel_launches++;
+  }
+  // Pieces: all rows by as many prototypes as the scratch holds (multiples
+  // of a tile); with so many rows that fewer than 2,048 prototypes would
+  // fit, the rows are cut too.
+  const int parts = a.dtype == EB_F32 ? 2 : 1;
+  const size_t room = ((size_t)256 << 20) / 2 / parts;  // elements of P
+  const size_t kpad = (a.k + BN - 1) / BN * BN;
+  size_t rows = a.n;
+  if (room / rows < std::min<size_t>(2048, kpad))
+    rows = std::max<size_t>(room / std::min<size_t>(2048, kpad) / 256 * 256, 256);
+  const size_t cols = std::min(kpad, std::max<size_t>(room / rows / BN * BN, BN));
+  uint16_t* p = e->scratch_get<uint16_t>("ce_p", rows * cols * parts);
+  const bool many_cols = cols < a.k, many_rows = rows < a.n;
+  float* dxacc = g.dx && many_cols ? e->scratch_get<float>("ce_dx", rows * a.d) : nullptr;
+  float* dwacc = g.dw && many_rows ? e->scratch_get<float>("ce_dw", a.k * a.d) : nullptr;
+  for (size_t r0 = 0; r0 < a.n; r0 += rows) {
+    const size_t r1 = std::min(a.n, r0 + rows);
+    const Operand Xr = rows_of(X, (long)r0, (long)r1);
+    for (size_t v0 = 0; v0 < a.k; v0 += cols) {
+      const size_t v1 = std::min(a.k, v0 + cols);
+      const Operand Wv = rows_of(W, (long)v0, (long)v1);
+      GemmParams P = base_params(a, scal);
+      P.M = (long)(r1 - r0);
+      P.N = (long)(v1 - v0);
+      P.K = (long)a.d;
+      P.targets = a.targets + r0;
+      P.lse = g.lse + r0;
+      P.dloss = g.one_dloss ? g.dloss : g.dloss + r0;
+      P.one_dloss = g.one_dloss;
+      P.col0 = (long)v0;
+      P.ldp = ((long)(v1 - v0) + 7) / 8 * 8;
+      P.p_hi = p;
+      P.p_lo = parts == 2 ? p + rows * cols : nullptr;
+      gemm<PROB, false, false>(e, Xr, Wv, P);
+      const Operand Pm{p, parts == 2 ? p + rows * cols : nullptr, P.M, P.N, P.ldp};
+      GemmParams Q = base_params(a, scal);
+      Q.dloss = P.dloss;
+      Q.one_dloss = P.one_dloss;
+      if (g.dx) {
+        Q.M = P.M;
+        Q.N = (long)a.d;
+        Q.K = P.N;
+        Q.sx = -1;
+        Q.sw = base_params(a, scal).sw;
+        product<false>(e, Pm, Wv, Q, dxacc, v0 > 0, v1 < a.k,
+                       static_cast<char*>(g.dx) + r0 * g.lddx * dtype_bytes(g.dxtype), g.dxtype,
+                       (long)g.lddx);
+      }
+      if (g.dw) {
+        Q.M = P.N;
+        Q.N = (long)a.d;
+        Q.K = P.M;
+        Q.sx = base_params(a, scal).sx;
+        Q.sw = -1;
+        product<true>(e, Pm, Xr, Q, dwacc ? dwacc + v0 * a.d : nullptr, r0 > 0, r1 < a.n,
+                      static_cast<char*>(g.dw) + v0 * g.lddw * dtype_bytes(g.dwtype), g.dwtype,
+                      (long)g.lddw);
+      }
+    }
+  }
+}
+
+}  // namespace eb

@@ -292,6 +292,7 @@ extern "C" int eb_set_group_shard(eb_engine* e, int mode) {
 extern "C" int eb_group_allgather(eb_engine* e, eb_buf* b, size_t words_per_rank) {
   try {
     eb::ensure(e != nullptr && b != nullptr, "engine and buffer are required");
+    eb::ensure(eb::dtype_bytes(b->dtype) == 4, "the buffer must hold 32-bit elements");
     eb::ensure(b->len / (size_t)e->world >= words_per_rank,
                "the buffer holds fewer than world x words_per_rank elements");
     if (e->world > 1 && words_per_rank > 0) {

@@ -50,9 +50,13 @@ extern "C" {
 #define EB_ERROR 2 /* CUDA/NCCL failure, out of memory, device-wait timeout */
 #define EB_INTERNAL 3
 
-/* Element types of engine buffers. */
+/* Element types of engine buffers. The last three are the training operators'
+ * (bfloat16, IEEE half, and the 8-bit float e4m3 of optimizer states). */
 #define EB_F32 0
 #define EB_U32 1
+#define EB_BF16 2
+#define EB_F16 3
+#define EB_F8 4
 
 /* Metric: crates/emeans-core/src/assign.rs:14-21. */
 #define EB_L2 0
@@ -72,6 +76,11 @@ const char* eb_version(void);
  * device that is not sm_100, fails with EB_ERROR
  * (crates/emeans-cuda/src/lib.rs:303-309: a missing driver is an error). */
 int eb_engine_create(int device, eb_engine** out);
+/* No counterpart in the reference. An engine whose work is queued on the
+ * caller's stream (a cudaStream_t; null is the legacy default stream) instead
+ * of one of its own, so that it is ordered with the caller's other work there
+ * without events. The stream must outlive the engine. */
+int eb_engine_create_on(int device, void* stream, eb_engine** out);
 int eb_engine_destroy(eb_engine* e);
 /* Device::name (core/mod.rs:77). Writes a NUL-terminated name. */
 int eb_engine_name(eb_engine* e, char* buf, size_t cap);
@@ -409,6 +418,100 @@ typedef struct {
  * place. sizes: k counts out, or NULL. */
 int eb_internal_scores(eb_engine* e, const float* x, size_t n, size_t d, const uint32_t* labels,
                        size_t k, eb_internal* out, uint64_t* sizes);
+
+/* ---------------------------------------------------------------- training operators
+ *
+ * No counterpart in the reference, which learns centroids by averaging alone.
+ * One gradient step of a head over the rows, trained against cluster labels:
+ * rows normalised, scored against one prototype per cluster under a softmax
+ * cross entropy, prototypes and norm weights stepped by AdamW. "Float" types
+ * are EB_F32, EB_BF16 and EB_F16; sums, statistics and products are held in
+ * 32 bits whatever the type, and outputs are rounded once (to nearest).
+ * Matrices are row-major with a row stride of ld elements (>= the row's
+ * length; 0: equal to it); elements between rows are neither read nor
+ * written. Shapes of zero rows are valid and launch nothing but the zeroing
+ * of the sums they leave. Outputs must not overlap inputs unless noted. */
+
+/* Layer norm of each of `rows` rows of d elements: y = (x - mean) rstd w + b,
+ * rstd = 1 / sqrt(var + eps) with var the mean squared deviation. x and y
+ * have one float type; weight and bias (d each; either may be null: ones,
+ * zeros) are f32 or of x's type, both alike. mean and rstd (f32, rows; may be
+ * null) keep the statistics for the backward pass. y may be x. */
+int eb_layer_norm(eb_engine* e, const eb_buf* x, size_t rows, size_t d, size_t ldx,
+                  const eb_buf* weight, const eb_buf* bias, float eps, eb_buf* y, size_t ldy,
+                  eb_buf* mean, eb_buf* rstd);
+
+/* Its backward pass from the statistics kept: with u = (x - mean) rstd and
+ * h = dy w, dx = rstd (h - avg(h) - u avg(h u)), dweight = sum over the rows
+ * of dy u, dbias = sum of dy. dy, x and dx have one float type; dweight and
+ * dbias are f32 or of x's type; any of dx, dweight, dbias may be null. dx may
+ * be dy. The sums are added in a fixed order (the same bits on every call
+ * with the same shapes). */
+int eb_layer_norm_backward(eb_engine* e, const eb_buf* dy, size_t lddy, const eb_buf* x,
+                           size_t ldx, size_t rows, size_t d, const eb_buf* weight,
+                           const eb_buf* mean, const eb_buf* rstd, eb_buf* dx, size_t lddx,
+                           eb_buf* dweight, eb_buf* dbias);
+
+/* The target of a row that carries no label: its loss and gradients are 0. */
+#define EB_IGNORE 0xFFFFFFFFu
+
+/* Softmax cross entropy of n rows x (n x d) against k prototypes w (k x d),
+ * the scores z = scale x . w never stored: lse[i] = log sum_j exp z_ij,
+ * loss[i] = lse[i] - z[i, targets[i]], or 0 where targets[i] is EB_IGNORE. A
+ * target >= k is reported by the next call that waits (EB_INVALID_ARGUMENT)
+ * and treated as EB_IGNORE. x and w have one float type; targets u32;
+ * loss and lse f32, n each. Products: 16-bit types on the tensor cores as
+ * they are; f32 as two scaled FP16 terms each (22 bits), three products. */
+int eb_linear_ce(eb_engine* e, const eb_buf* x, size_t n, size_t d, size_t ldx, const eb_buf* w,
+                 size_t k, size_t ldw, const eb_buf* targets, float scale, eb_buf* loss,
+                 eb_buf* lse);
+
+/* Its gradients from the lse kept by the forward call on the same inputs:
+ * with P_ij = dloss_i scale (exp(z_ij - lse_i) - [j == targets_i]),
+ * dx = P w (n x d) and dw = P^T x (k x d). dloss is f32: n elements, or one
+ * for all rows. P is formed a piece of the prototypes (and of the rows, when
+ * there are very many) at a time in the engine's scratch (up to 256 MB),
+ * rounded to x's type (f32: two FP16 terms). dx and dw: x's type or f32;
+ * either may be null. Sums are added in a fixed order. */
+int eb_linear_ce_backward(eb_engine* e, const eb_buf* x, size_t n, size_t d, size_t ldx,
+                          const eb_buf* w, size_t k, size_t ldw, const eb_buf* targets,
+                          float scale, const eb_buf* lse, const eb_buf* dloss, eb_buf* dx,
+                          size_t lddx, eb_buf* dw, size_t lddw);
+
+/* One tensor of an AdamW step. p: parameters (f32 or bf16); g: gradients (f32
+ * or bf16, as long as p); m, v: the moments, f32 and as long as p, or both in
+ * 8 bits: EB_F8 codes as long as p with m_scale / v_scale f32, one per 256
+ * elements (the last block may be shorter). 8-bit m is code x scale; 8-bit v
+ * holds the root, v = (code x scale)^2. copy (or null): bf16, receives the
+ * new parameters rounded. All-zero states are the right start in either form. */
+#define EB_ADAMW_BLOCK 256
+typedef struct {
+  eb_buf* p;
+  const eb_buf* g;
+  eb_buf* m;
+  eb_buf* v;
+  eb_buf* m_scale; /* null: m, v are f32 */
+  eb_buf* v_scale;
+  eb_buf* copy;
+  double weight_decay;
+} eb_adamw_tensor;
+typedef struct eb_adamw eb_adamw;
+
+/* A plan over `count` tensors: their addresses laid out on the device once.
+ * The buffers must outlive it. No buffer may be written by two tensors. */
+int eb_adamw_create(eb_engine* e, const eb_adamw_tensor* tensors, size_t count, eb_adamw** out);
+int eb_adamw_destroy(eb_engine* e, eb_adamw* plan);
+
+/* One step over every tensor in one kernel. In f32, each operation rounded
+ * by itself: g' = grad_scale g; m = beta1 m + (1 - beta1) g';
+ * v = beta2 v + (1 - beta2) (g' g');
+ * p = (1 - lr weight_decay) p - lr / (1 - beta1^step) (m / (sqrt(v) c + eps)),
+ * c = 1 / sqrt(1 - beta2^step). 8-bit states are then rounded to the nearest
+ * code under the block's largest value / 448; a root above zero never rounds
+ * to zero. A block that holds a non-finite moment gets a NaN scale. step
+ * counts from 1. */
+int eb_adamw_step(eb_engine* e, eb_adamw* plan, double lr, uint64_t step, double beta1,
+                  double beta2, double eps, float grad_scale);
 
 #ifdef __cplusplus
 }
