@@ -6,9 +6,9 @@
 // (no FMA contraction, IEEE divide and square root): the step's results do
 // not depend on how the compiler fuses it.
 //
-// 8-bit states: 256 elements share a scale, one warp holds them (8 a lane),
-// so the new scale is a shuffle maximum over registers and every byte is read
-// and written once. The first moment is kept as code x scale with e4m3 codes
+// 8-bit states: 256 elements share a scale, half a warp holds them (16 a
+// lane), so the new scale is a shuffle maximum over registers and every byte
+// is read and written once. The first moment is kept as code x scale with e4m3 codes
 // (largest 448); the second as its root, whose range is half as wide in
 // exponent and which the update needs anyway. A root above zero keeps at
 // least the smallest code: rounded to zero it would leave the moment above it
@@ -29,8 +29,8 @@ namespace eb {
 
 namespace {
 
-constexpr int CHUNK = 2048;
-constexpr int THREADS = 256;
+constexpr int CHUNK = 2048;  // elements of a piece
+constexpr int THREADS = 256, THREADS8 = 128;  // of a block, for 32-bit and 8-bit states
 constexpr float F8_MAX = 448.0f, F8_MIN = 0.001953125f;  // e4m3: largest, smallest (2^-9)
 
 struct Entry {
@@ -122,16 +122,25 @@ __device__ __forceinline__ void piece_f32(const Entry& E, const Hyper& H, float 
   }
 }
 
-__device__ __forceinline__ float f8_value(uint8_t c) {
-  return __half2float(__half(__nv_cvt_fp8_to_halfraw(c, __NV_E4M3)));
+// Two codes at a time, each way.
+__device__ __forceinline__ float2 f8_values(uint16_t c) {
+  return __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(c, __NV_E4M3)));
 }
-__device__ __forceinline__ uint8_t f8_code(float v) {
-  return __nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3);
+__device__ __forceinline__ uint16_t f8_codes(float a, float b) {
+  return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
 }
 
-__device__ __forceinline__ float warp_max(float v) {
+// Larger of two, NaN if either is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// Largest over the 16 lanes of a half warp.
+__device__ __forceinline__ float half_max(float v) {
 #pragma unroll
-  for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  for (int o = 8; o; o >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, o));
   return v;
 }
 
@@ -144,105 +153,163 @@ __device__ __forceinline__ float f8_scale(float top, bool finite, float& inv) {
   return finite ? scale : NAN;
 }
 
+// Eight elements as they are loaded.
+template <typename PT, typename GT>
+struct Raw {
+  Pack<PT, 4> p[2];
+  Pack<GT, 4> g[2];
+  Pack<uint16_t, 4> mc, vc;
+};
+
+// Elements i .. i + 8 of the piece at `at`, zeros past `count`.
+template <typename PT, typename GT>
+__device__ __forceinline__ Raw<PT, GT> load_raw(const Entry& E, size_t at, int i, int count) {
+  Raw<PT, GT> r;
+  const size_t a = at + i;
+  const PT* P = static_cast<const PT*>(E.p) + a;
+  const GT* G = static_cast<const GT*>(E.g) + a;
+  const uint8_t* M = static_cast<const uint8_t*>(E.m) + a;
+  const uint8_t* V = static_cast<const uint8_t*>(E.v) + a;
+  if (i + 8 <= count) {
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      r.p[h] = reinterpret_cast<const Pack<PT, 4>*>(P)[h];
+      r.g[h] = reinterpret_cast<const Pack<GT, 4>*>(G)[h];
+    }
+    r.mc = *reinterpret_cast<const Pack<uint16_t, 4>*>(M);
+    r.vc = *reinterpret_cast<const Pack<uint16_t, 4>*>(V);
+  } else {
+    const int mine = count - i;
+#pragma unroll
+    for (int u = 0; u < 8; u++) {
+      r.p[u / 4].v[u % 4] = u < mine ? P[u] : from_f32<PT>(0.0f);
+      r.g[u / 4].v[u % 4] = u < mine ? G[u] : from_f32<GT>(0.0f);
+    }
+#pragma unroll
+    for (int u = 0; u < 8; u += 2) {
+      r.mc.v[u / 2] = (uint16_t)((u < mine ? M[u] : 0) | (u + 1 < mine ? M[u + 1] : 0) << 8);
+      r.vc.v[u / 2] = (uint16_t)((u < mine ? V[u] : 0) | (u + 1 < mine ? V[u + 1] : 0) << 8);
+    }
+  }
+  return r;
+}
+
+// Half a warp a block of 256, 2 x 8 elements a lane: the block's scales, their
+// inverses and the addresses are worked out once for 16 elements.
 template <typename PT, typename GT>
 __device__ __forceinline__ void piece_f8(const Entry& E, const Hyper& H, float keep, size_t at,
                                          int count) {
-  const int lane = threadIdx.x & 31;
-  static_assert(CHUNK == 8 * THREADS, "one block of 256 a warp");
-  const int i = (threadIdx.x >> 5) * 256 + lane * 8;
-  if (i - lane * 8 >= count) return;  // the whole warp
-  const size_t a = at + i, blk = (at + i) / 256;
-  const int mine = min(max(count - i, 0), 8);
-  PT* P = static_cast<PT*>(E.p) + a;
-  const GT* G = static_cast<const GT*>(E.g) + a;
-  uint8_t* M = static_cast<uint8_t*>(E.m) + a;
-  uint8_t* V = static_cast<uint8_t*>(E.v) + a;
-  const float ms = E.ms[blk], vs = E.vs[blk];
-  float p[8], g[8];
-  Pack<uint8_t, 8> mc, vc;
-  if (mine == 8) {
+  static_assert(CHUNK == 16 * THREADS8, "one pass a piece");
+  const int lane = threadIdx.x & 15, b = (threadIdx.x >> 4) * 256;
+  if ((threadIdx.x >> 5) * 512 >= count) return;  // the whole warp
+  const size_t blk = (at + b) / 256;
+  const bool some = b < count;
+  const float ms = some ? E.ms[blk] : 0.0f, vs = some ? E.vs[blk] : 0.0f;
+  Raw<PT, GT> R[2];
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-      float q[4];
-      load4(P + 4 * h, q);
+  for (int h = 0; h < 2; h++) R[h] = load_raw<PT, GT>(E, at, b + h * 128 + lane * 8, count);
+  // Elements past the end hold zeros, whose moments stay zero.
+  float m[16], r[16], tm = 0.0f, tr = 0.0f;
 #pragma unroll
-      for (int u = 0; u < 4; u++) p[4 * h + u] = q[u];
-      load4(G + 4 * h, q);
+  for (int h = 0; h < 2; h++) {
+    const int i = b + h * 128 + lane * 8;
+    const size_t a = at + i;
+    float p[8];
 #pragma unroll
-      for (int u = 0; u < 4; u++) g[4 * h + u] = q[u];
+    for (int u = 0; u < 8; u += 2) {
+      const float2 mq = f8_values(R[h].mc.v[u / 2]), rq = f8_values(R[h].vc.v[u / 2]);
+#pragma unroll
+      for (int w = 0; w < 2; w++) {
+        const int q = u + w, k = h * 8 + q;
+        const float root = __fmul_rn(w ? rq.y : rq.x, vs);
+        const Step s = step_one(H, keep, to_f32(R[h].p[q / 4].v[q % 4]),
+                                to_f32(R[h].g[q / 4].v[q % 4]), __fmul_rn(w ? mq.y : mq.x, ms),
+                                __fmul_rn(root, root));
+        p[q] = s.p;
+        m[k] = s.m;
+        r[k] = s.root;
+        tm = max_nan(tm, fabsf(s.m));
+        tr = max_nan(tr, s.root);
+      }
     }
-    mc = *reinterpret_cast<const Pack<uint8_t, 8>*>(M);
-    vc = *reinterpret_cast<const Pack<uint8_t, 8>*>(V);
-  } else {
+    PT* P = static_cast<PT*>(E.p) + a;
+    if (i + 8 <= count) {
 #pragma unroll
-    for (int u = 0; u < 8; u++) {
-      p[u] = u < mine ? to_f32(P[u]) : 0.0f;
-      g[u] = u < mine ? to_f32(G[u]) : 0.0f;
-      mc.v[u] = u < mine ? M[u] : 0;
-      vc.v[u] = u < mine ? V[u] : 0;
+      for (int x = 0; x < 2; x++) {
+        const float q[4] = {p[4 * x], p[4 * x + 1], p[4 * x + 2], p[4 * x + 3]};
+        store4(P + 4 * x, q);
+      }
+      if (E.copy) {
+        Pack<__nv_bfloat16, 8> c;
+#pragma unroll
+        for (int u = 0; u < 8; u++) c.v[u] = from_f32<__nv_bfloat16>(p[u]);
+        *reinterpret_cast<Pack<__nv_bfloat16, 8>*>(E.copy + a) = c;
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < 8; u++) {
+        if (i + u < count) {
+          P[u] = from_f32<PT>(p[u]);
+          if (E.copy) E.copy[a + u] = from_f32<__nv_bfloat16>(p[u]);
+        }
+      }
     }
   }
-  float m[8], r[8], tm = 0.0f, tr = 0.0f;
-  bool fine = true;
-#pragma unroll
-  for (int u = 0; u < 8; u++) {
-    const float root = __fmul_rn(f8_value(vc.v[u]), vs);
-    const Step s = step_one(H, keep, p[u], g[u], __fmul_rn(f8_value(mc.v[u]), ms),
-                            __fmul_rn(root, root));
-    p[u] = s.p;
-    m[u] = s.m;
-    r[u] = s.root;
-    if (u < mine) {
-      tm = fmaxf(tm, fabsf(s.m));
-      tr = fmaxf(tr, s.root);
-      fine = fine && isfinite(s.m) && isfinite(s.root);
-    }
-  }
-  fine = __all_sync(0xffffffffu, fine);
+  tm = half_max(tm);
+  tr = half_max(tr);
+  const bool fine = isfinite(tm) && isfinite(tr);
   float im, ir;
-  const float nms = f8_scale(warp_max(tm), fine, im), nvs = f8_scale(warp_max(tr), fine, ir);
-#pragma unroll
-  for (int u = 0; u < 8; u++) {
-    mc.v[u] = f8_code(__fmul_rn(m[u], im));
-    const float q = __fmul_rn(r[u], ir);
-    vc.v[u] = f8_code(r[u] > 0.0f && ir > 0.0f ? fmaxf(q, F8_MIN) : q);
-  }
-  if (lane == 0) {
+  const float nms = f8_scale(tm, fine, im), nvs = f8_scale(tr, fine, ir);
+  const float least = ir > 0.0f ? F8_MIN : 0.0f;
+  if (some && lane == 0) {
     E.ms[blk] = nms;
     E.vs[blk] = nvs;
   }
-  if (mine == 8) {
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-      const float q[4] = {p[4 * h], p[4 * h + 1], p[4 * h + 2], p[4 * h + 3]};
-      store4(P + 4 * h, q);
-      if (E.copy) store4(E.copy + a + 4 * h, q);
+  for (int h = 0; h < 2; h++) {
+    const int i = b + h * 128 + lane * 8;
+    Pack<uint16_t, 4> mc, vc;
+#pragma unroll
+    for (int u = 0; u < 8; u += 2) {
+      const int k = h * 8 + u;
+      mc.v[u / 2] = f8_codes(__fmul_rn(m[k], im), __fmul_rn(m[k + 1], im));
+      float q[2];
+#pragma unroll
+      for (int w = 0; w < 2; w++)
+        q[w] = r[k + w] > 0.0f ? fmaxf(__fmul_rn(r[k + w], ir), least) : 0.0f;
+      vc.v[u / 2] = f8_codes(q[0], q[1]);
     }
-    *reinterpret_cast<Pack<uint8_t, 8>*>(M) = mc;
-    *reinterpret_cast<Pack<uint8_t, 8>*>(V) = vc;
-  } else {
+    uint8_t* M = static_cast<uint8_t*>(E.m) + at + i;
+    uint8_t* V = static_cast<uint8_t*>(E.v) + at + i;
+    if (i + 8 <= count) {
+      *reinterpret_cast<Pack<uint16_t, 4>*>(M) = mc;
+      *reinterpret_cast<Pack<uint16_t, 4>*>(V) = vc;
+    } else {
 #pragma unroll
-    for (int u = 0; u < 8; u++) {
-      if (u < mine) {
-        P[u] = from_f32<PT>(p[u]);
-        M[u] = mc.v[u];
-        V[u] = vc.v[u];
-        if (E.copy) E.copy[a + u] = from_f32<__nv_bfloat16>(p[u]);
+      for (int u = 0; u < 8; u++) {
+        if (i + u < count) {
+          M[u] = (uint8_t)(mc.v[u / 2] >> (u % 2 * 8));
+          V[u] = (uint8_t)(vc.v[u / 2] >> (u % 2 * 8));
+        }
       }
     }
   }
 }
 
-template <typename PT, typename GT>
+template <bool EIGHT, typename PT, typename GT>
 __device__ __forceinline__ void piece(const Entry& E, const Hyper& H, float keep, size_t at,
                                       int count) {
-  if (E.ms)
+  if constexpr (EIGHT)
     piece_f8<PT, GT>(E, H, keep, at, count);
   else
     piece_f32<PT, GT>(E, H, keep, at, count);
 }
 
-__global__ void __launch_bounds__(THREADS)
+// The 8-bit and 32-bit tensors of a plan go to kernels of their own: the
+// 32-bit one then keeps six blocks on an SM (120 M f32 parameters: 488 us; four
+// blocks, as registers for both allow: 524).
+template <bool EIGHT>
+__global__ void __launch_bounds__(EIGHT ? THREADS8 : THREADS, 6)
     k_adamw(const Entry* __restrict__ entries, const uint2* __restrict__ pieces, Hyper H) {
   pdl_wait();
   const uint2 w = pieces[blockIdx.x];
@@ -252,14 +319,14 @@ __global__ void __launch_bounds__(THREADS)
   const float keep = (float)(1.0 - H.lr * E.decay);
   if (E.ptype == EB_F32) {
     if (E.gtype == EB_F32)
-      piece<float, float>(E, H, keep, at, count);
+      piece<EIGHT, float, float>(E, H, keep, at, count);
     else
-      piece<float, __nv_bfloat16>(E, H, keep, at, count);
+      piece<EIGHT, float, __nv_bfloat16>(E, H, keep, at, count);
   } else {
     if (E.gtype == EB_F32)
-      piece<__nv_bfloat16, float>(E, H, keep, at, count);
+      piece<EIGHT, __nv_bfloat16, float>(E, H, keep, at, count);
     else
-      piece<__nv_bfloat16, __nv_bfloat16>(E, H, keep, at, count);
+      piece<EIGHT, __nv_bfloat16, __nv_bfloat16>(E, H, keep, at, count);
   }
 }
 
@@ -267,7 +334,7 @@ __global__ void __launch_bounds__(THREADS)
 
 void adamw_create(eb_engine* e, const eb_adamw_tensor* t, size_t count, eb_adamw* plan) {
   std::vector<Entry> entries;
-  std::vector<uint2> pieces;
+  std::vector<uint2> pieces[2];  // of 32-bit states, of 8-bit states
   for (size_t i = 0; i < count; i++) {
     Entry E{};
     E.p = t[i].p->ptr;
@@ -282,32 +349,41 @@ void adamw_create(eb_engine* e, const eb_adamw_tensor* t, size_t count, eb_adamw
     E.ptype = t[i].p->dtype;
     E.gtype = t[i].g->dtype;
     entries.push_back(E);
+    auto& list = pieces[E.ms != nullptr];
     const size_t np = (E.len + CHUNK - 1) / CHUNK;
-    ensure(pieces.size() + np <= 0x7FFFFFFFull, "too many elements in one plan");
-    for (size_t c = 0; c < np; c++) pieces.push_back(make_uint2((unsigned)i, (unsigned)c));
+    ensure(list.size() + np <= 0x7FFFFFFFull, "too many elements in one plan");
+    for (size_t c = 0; c < np; c++) list.push_back(make_uint2((unsigned)i, (unsigned)c));
   }
-  plan->pieces = pieces.size();
-  if (pieces.empty()) return;
-  const size_t eb = entries.size() * sizeof(Entry), pb = pieces.size() * sizeof(uint2);
-  const size_t off = (eb + 15) / 16 * 16;
-  EB_CUDA(cudaMallocAsync(&plan->table, off + pb, e->stream));
+  size_t off = (entries.size() * sizeof(Entry) + 15) / 16 * 16;
+  for (int k = 0; k < 2; k++) {
+    plan->pieces[k] = pieces[k].size();
+    plan->pieces_at[k] = off;
+    off += pieces[k].size() * sizeof(uint2);
+  }
+  if (!plan->pieces[0] && !plan->pieces[1]) return;
+  EB_CUDA(cudaMallocAsync(&plan->table, off, e->stream));
   e->device_allocs++;
-  plan->pieces_at = off;
-  h2d(e, plan->table, entries.data(), eb, e->stream);
-  h2d(e, static_cast<char*>(plan->table) + off, pieces.data(), pb, e->stream);
+  char* dst = static_cast<char*>(plan->table);
+  h2d(e, dst, entries.data(), entries.size() * sizeof(Entry), e->stream);
+  for (int k = 0; k < 2; k++)
+    if (plan->pieces[k])
+      h2d(e, dst + plan->pieces_at[k], pieces[k].data(), pieces[k].size() * sizeof(uint2),
+          e->stream);
 }
 
 void adamw_step(eb_engine* e, const eb_adamw* plan, double lr, uint64_t step, double b1, double b2,
                 double eps, float gscale) {
-  if (!plan->pieces) return;
-  Hyper H{(float)b1, (float)(1.0 - b1), (float)b2, (float)(1.0 - b2),
-          (float)(lr / (1.0 - std::pow(b1, (double)step))),
-          (float)(1.0 / std::sqrt(1.0 - std::pow(b2, (double)step))), (float)eps, gscale, lr};
+  const Hyper H{(float)b1, (float)(1.0 - b1), (float)b2, (float)(1.0 - b2),
+                (float)(lr / (1.0 - std::pow(b1, (double)step))),
+                (float)(1.0 / std::sqrt(1.0 - std::pow(b2, (double)step))), (float)eps, gscale, lr};
   const char* t = static_cast<const char*>(plan->table);
-  launch_pdl(e, k_adamw, dim3((unsigned)plan->pieces), dim3(THREADS), 0,
-             reinterpret_cast<const Entry*>(t), reinterpret_cast<const uint2*>(t + plan->pieces_at),
-             H);
-  e->stats.kernel_launches++;
+  for (int k = 0; k < 2; k++) {
+    if (!plan->pieces[k]) continue;
+    launch_pdl(e, k ? k_adamw<true> : k_adamw<false>, dim3((unsigned)plan->pieces[k]),
+               dim3(k ? THREADS8 : THREADS), 0, reinterpret_cast<const Entry*>(t),
+               reinterpret_cast<const uint2*>(t + plan->pieces_at[k]), H);
+    e->stats.kernel_launches++;
+  }
 }
 
 }  // namespace eb

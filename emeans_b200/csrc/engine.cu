@@ -48,14 +48,19 @@ struct DeviceGuard {
   }
 };
 
+// Messages are put together only when a check fails.
+[[noreturn]] void refuse(const char* what, const char* why) {
+  throw eb::Error(EB_INVALID_ARGUMENT, std::string(what) + why);
+}
+
 void need(const void* p, const char* what) {
-  eb::ensure(p != nullptr, std::string(what) + " is null");
+  if (!p) refuse(what, " is null");
 }
 
 void need_type(const eb_buf* b, int dtype, const char* what) {
   need(b, what);
-  eb::ensure(b->dtype == dtype,
-             std::string(what) + (dtype == EB_F32 ? " must be an f32 buffer" : " must be a u32 buffer"));
+  if (b->dtype != dtype)
+    refuse(what, dtype == EB_F32 ? " must be an f32 buffer" : " must be a u32 buffer");
 }
 
 // An op wrote `b` on the device: drop the caches derived from its contents.
@@ -73,17 +78,16 @@ bool is_float(int dtype) { return dtype == EB_F32 || dtype == EB_BF16 || dtype =
 
 void need_float(const eb_buf* b, const char* what) {
   need(b, what);
-  eb::ensure(is_float(b->dtype), std::string(what) + " must be an f32, bf16 or f16 buffer");
+  if (!is_float(b->dtype)) refuse(what, " must be an f32, bf16 or f16 buffer");
 }
 
 // The row stride of a matrix argument: `ld`, or the row's length for 0; the
 // buffer must hold rows x d at that stride.
 size_t need_rows(const eb_buf* b, size_t rows, size_t d, size_t ld, const char* what) {
   if (ld == 0) ld = d;
-  eb::ensure(ld >= d, std::string(what) + ": the row stride is shorter than a row");
-  if (rows > 0)
-    eb::ensure(b->len >= d && (rows - 1) <= (b->len - d) / ld,
-               std::string(what) + " is too short for its rows");
+  if (ld < d) refuse(what, ": the row stride is shorter than a row");
+  if (rows > 0 && (b->len < d || rows - 1 > (b->len - d) / ld))
+    refuse(what, " is too short for its rows");
   return ld;
 }
 

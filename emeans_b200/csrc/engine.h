@@ -100,7 +100,7 @@ struct eb_buf {
 // A plan of an AdamW step: the tensors' table and their pieces' on the device.
 struct eb_adamw {
   void* table = nullptr;
-  size_t pieces_at = 0, pieces = 0;
+  size_t pieces_at[2] = {}, pieces[2] = {};  // of 32-bit states, of 8-bit states
   std::vector<eb_buf*> written;  // parameters, states, scales and copies
 };
 
