@@ -61,14 +61,30 @@ __device__ __forceinline__ float split_scale(uint32_t bits) {
   return __uint_as_float((uint32_t)(s + 127) << 23);
 }
 
-struct GemmParams {
+// One product D = A B^T of a launch, cut into units: tiles of CG * 128 rows by
+// 256 columns, times splits of k.
+struct Prob {
   long M, N, K;
-  int mtiles, ntiles, splits, kb_split, kblocks, group;
+  int mtiles, ntiles, kblocks, kb_split, splits, units;
+  int group;        // row tiles that pass over the column tiles together
+  int a_mn;         // A is K x M (MN-major) rather than M x K
+  // OUT: v = acc scale max|dloss| / pscale, to `out`, or through FP32 sums
+  int unscale;      // scal slot of the second operand's split scale, or -1
+  void* out;
+  int otype, ovec;  // ovec: rows of `out` keep 16-byte alignment
+  long ldo;
+  float* accum;     // M x ldacc (+ split * M * ldacc)
+  long ldacc;       // a multiple of 4
+  int read_acc, write_acc;
+};
+
+struct GemmParams {
+  Prob q[2];        // the second only with OUT, after the first's units
   uint32_t fmt;     // operand format of the instruction (0 f16, 1 bf16)
   uint32_t* status;
   const uint32_t* scal;
   float scale;      // of the scores
-  int sx, sw;       // scal slots of the operands' split scales, or -1
+  int split;        // operands are f32 in two terms: scores carry both scales
   // LSE
   float2* part;     // [2 ntiles][M]: (max, sum) of a half tile's columns
   float* zt;        // M: target scores, base 2
@@ -83,12 +99,6 @@ struct GemmParams {
   void* p_lo;
   long ldp;
   float pscale;     // what P is kept times: 1 (bf16) or PSCALE
-  // OUT: v = acc scale max|dloss| / pscale, to `out`, or through FP32 sums
-  void* out;
-  int otype;
-  long ldo;
-  float* accum;     // M x N, row stride N (+ split * M * N)
-  int read_acc, write_acc;
 };
 
 template <int CG, int PARTS>
@@ -134,41 +144,128 @@ __device__ __forceinline__ void fold(float& m, float& s, float2 v) {
 // A warp's 32 x 32 block in shared memory: row r's four-column group g is
 // kept at group g ^ (r & 7), so that rows are written by their own threads
 // and read across lanes without bank conflicts.
-__device__ __forceinline__ float4* block4(float* blk, int r, int g) {
-  return reinterpret_cast<float4*>(blk) + r * 8 + (g ^ (r & 7));
+__device__ __forceinline__ float4& block4(float* blk, int r, int g) {
+  return reinterpret_cast<float4*>(blk)[r * 8 + (g ^ (r & 7))];
 }
-__device__ __forceinline__ float block1(const float* blk, int r, int c) {
-  return blk[r * 32 + (((c >> 2) ^ (r & 7)) << 2) + (c & 3)];
-}
-
-// The tile and k-range of unit u: within a split, groups of `group` row tiles
-// pass over all column tiles, row tile fastest, so that the tiles in flight
-// share operands in L2.
+// The tile and k-range of unit u: within a split, groups of row tiles pass
+// over all column tiles, row tile fastest, so that the tiles in flight share
+// operands in L2.
 struct Unit {
-  int mt, nt, split, kb0, kb1;
+  int prob, mt, nt, split, kb0, kb1;
 };
+template <int EPI>
 __device__ __forceinline__ Unit unit_at(const GemmParams& P, int u) {
   Unit r;
-  const int tiles = P.mtiles * P.ntiles;
+  r.prob = EPI == OUT && u >= P.q[0].units;
+  const Prob& q = P.q[r.prob];
+  if (r.prob) u -= P.q[0].units;
+  const int tiles = q.mtiles * q.ntiles;
   r.split = u / tiles;
-  const int t = u % tiles, gn = P.group * P.ntiles;
+  const int t = u % tiles, gn = q.group * q.ntiles;
   const int g = t / gn, w = t % gn;
-  const int gm = min(P.group, P.mtiles - g * P.group);
-  r.mt = g * P.group + w % gm;
+  const int gm = min(q.group, q.mtiles - g * q.group);
+  r.mt = g * q.group + w % gm;
   r.nt = w / gm;
-  r.kb0 = r.split * P.kb_split;
-  r.kb1 = min(r.kb0 + P.kb_split, P.kblocks);
+  r.kb0 = r.split * q.kb_split;
+  r.kb1 = min(r.kb0 + q.kb_split, q.kblocks);
   return r;
 }
 
-// D = A B^T over tiles of CG * 128 rows by 256 columns. A is M x K (K-major)
-// or K x M (A_MN), B likewise N x K or K x N. With PARTS = 2 each operand is
-// two FP16 terms.
-template <int EPI, int CG, int PARTS, bool A_MN, bool B_MN>
+// A warp's 32 x 32 block of a product, times `factor`, to the FP32 sums (at
+// `sums`, the block's first row) or to the output, in 16-byte groups where
+// the rows allow.
+__device__ __forceinline__ void store_block(const Prob& q, float* sums, float* blk, int lane,
+                                            long row0, int rows, long col, int cols,
+                                            float factor) {
+  if (q.write_acc || q.otype == EB_F32) {
+    // Eight lanes a row, four columns each.
+    const int g = lane & 7, r0 = lane >> 3;
+    const int mine = min(max(cols - g * 4, 0), 4);
+    if (!mine) return;
+    const bool sum_vec = mine == 4 || q.write_acc;  // sums' rows are padded to whole groups
+    float4 old[8];
+    if (q.read_acc) {
+#pragma unroll
+      for (int t = 0; t < 8; t++)
+        if (r0 + t * 4 < rows)
+          old[t] = *reinterpret_cast<const float4*>(sums + (r0 + t * 4) * q.ldacc + col + g * 4);
+    }
+#pragma unroll
+    for (int t = 0; t < 8; t++) {
+      const int r = r0 + t * 4;
+      if (r >= rows) break;
+      float4 v = block4(blk, r, g);
+      v = make_float4(v.x * factor, v.y * factor, v.z * factor, v.w * factor);
+      if (q.read_acc) v = make_float4(v.x + old[t].x, v.y + old[t].y, v.z + old[t].z, v.w + old[t].w);
+      if (q.write_acc) {
+        *reinterpret_cast<float4*>(sums + r * q.ldacc + col + g * 4) = v;
+      } else {
+        float* out = static_cast<float*>(q.out) + (row0 + r) * q.ldo + col + g * 4;
+        if (q.ovec && sum_vec) {
+          *reinterpret_cast<float4*>(out) = v;
+        } else {
+          const float f[4] = {v.x, v.y, v.z, v.w};
+          for (int j = 0; j < mine; j++) out[j] = f[j];
+        }
+      }
+    }
+  } else {
+    // Four lanes a row, eight columns each.
+    const int g = (lane & 3) * 2, r0 = lane >> 2;
+    const int mine = min(max(cols - g * 4, 0), 8);
+    if (!mine) return;
+    float4 old[4][2];
+    if (q.read_acc) {
+#pragma unroll
+      for (int t = 0; t < 4; t++) {
+        if (r0 + t * 8 >= rows) break;
+        const float4* at =
+            reinterpret_cast<const float4*>(sums + (r0 + t * 8) * q.ldacc + col + g * 4);
+        old[t][0] = at[0];
+        old[t][1] = mine > 4 ? at[1] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < 4; t++) {
+      const int r = r0 + t * 8;
+      if (r >= rows) break;
+      const float4 a = block4(blk, r, g);
+      const float4 b = block4(blk, r, g + 1);
+      float f[8] = {a.x * factor, a.y * factor, a.z * factor, a.w * factor,
+                    b.x * factor, b.y * factor, b.z * factor, b.w * factor};
+      if (q.read_acc) {
+        const float o[8] = {old[t][0].x, old[t][0].y, old[t][0].z, old[t][0].w,
+                            old[t][1].x, old[t][1].y, old[t][1].z, old[t][1].w};
+#pragma unroll
+        for (int j = 0; j < 8; j++) f[j] += o[j];
+      }
+      uint16_t* out = static_cast<uint16_t*>(q.out) + (row0 + r) * q.ldo + col + g * 4;
+      Pack<uint16_t, 8> h;
+#pragma unroll
+      for (int j = 0; j < 8; j++)
+        h.v[j] = q.otype == EB_BF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(f[j]))
+                                    : __half_as_ushort(__float2half_rn(f[j]));
+      if (q.ovec && mine == 8) {
+        *reinterpret_cast<Pack<uint16_t, 8>*>(out) = h;
+      } else {
+        for (int j = 0; j < mine; j++) out[j] = h.v[j];
+      }
+    }
+  }
+}
+
+// Every operand arrives in boxes of 64 columns by 64 rows (8 KB, 128-byte
+// swizzle): a K-major operand's boxes follow one another down its rows, an
+// MN-major one's along its columns, so one tensor map serves either reading.
+// LSE and PROB: A = x, B = w, both K-major. OUT: A = P, K-major for dx
+// (B = w) and MN-major for dw (B = x), B MN-major. With PARTS = 2 each operand
+// is two FP16 terms.
+template <int EPI, int CG, int PARTS>
 __global__ void __launch_bounds__(NTHREADS, 1)
     k_gemm(const __grid_constant__ CUtensorMap a0, const __grid_constant__ CUtensorMap a1,
            const __grid_constant__ CUtensorMap b0, const __grid_constant__ CUtensorMap b1,
-           const GemmParams P) {
+           const __grid_constant__ CUtensorMap c0, const __grid_constant__ CUtensorMap c1,
+           const __grid_constant__ GemmParams P) {
   using S = Shape<CG, PARTS>;
   using namespace tc;
   extern __shared__ uint8_t smem_raw[];
@@ -182,7 +279,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
   volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = CG == 2 ? cta_rank() : 0;
-  const int units = P.mtiles * P.ntiles * P.splits;
+  const int units = P.q[0].units + (EPI == OUT ? P.q[1].units : 0);
   const int first = blockIdx.x / CG, step = gridDim.x / CG;
 
   if (threadIdx.x == 0) {
@@ -213,7 +310,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       int it = 0;
       bool stop = false;
       for (int u = first; u < units && !stop; u += step) {
-        const Unit q = unit_at(P, u);
+        const Unit q = unit_at<EPI>(P, u);
         const int am = (q.mt * CG + (int)rank) * BM, bn = q.nt * BN + (int)rank * S::B_ROWS;
         for (int kb = q.kb0; kb < q.kb1; kb++, it++) {
           const int s = it % S::STAGES;
@@ -224,26 +321,21 @@ __global__ void __launch_bounds__(NTHREADS, 1)
           if (rank == 0) mbar_expect_tx(&full[s], CG * S::STAGE);
           const uint32_t bar = CG == 2 ? map_rank(smem_u32(&full[s]), 0) : smem_u32(&full[s]);
           uint8_t* st = smem + s * S::STAGE;
+          const bool a_mn = EPI == OUT && P.q[q.prob].a_mn;
 #pragma unroll
           for (int p = 0; p < PARTS; p++) {
-            const CUtensorMap* am_ = p ? &a1 : &a0;
-            const CUtensorMap* bm_ = p ? &b1 : &b0;
-            if constexpr (A_MN) {
+            const CUtensorMap* ma = p ? &a1 : &a0;
+            const CUtensorMap* mb = q.prob ? (p ? &c1 : &c0) : (p ? &b1 : &b0);
 #pragma unroll
-              for (int c = 0; c < S::A_ROWS / 64; c++)
-                tma_load<CG>(st + c * 8192, am_, bar, am + c * 64, kb * BK);
-            } else {
-              tma_load<CG>(st, am_, bar, kb * BK, am);
+            for (int c = 0; c < S::A_ROWS / 64; c++, st += 8192) {
+              const int m = am + c * 64;
+              tma_load<CG>(st, ma, bar, a_mn ? m : kb * BK, a_mn ? kb * BK : m);
             }
-            st += S::A_BYTES;
-            if constexpr (B_MN) {
 #pragma unroll
-              for (int c = 0; c < S::B_ROWS / 64; c++)
-                tma_load<CG>(st + c * 8192, bm_, bar, bn + c * 64, kb * BK);
-            } else {
-              tma_load<CG>(st, bm_, bar, kb * BK, bn);
+            for (int c = 0; c < S::B_ROWS / 64; c++, st += 8192) {
+              const int n = bn + c * 64;
+              tma_load<CG>(st, mb, bar, EPI == OUT ? n : kb * BK, EPI == OUT ? kb * BK : n);
             }
-            st += S::B_BYTES;
           }
         }
       }
@@ -259,13 +351,14 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       }
     }
     if (warp == 1 && lane == 0 && rank == 0) {
-      const uint32_t idesc = (1u << 4) | (P.fmt << 7) | (P.fmt << 10) | ((A_MN ? 1u : 0u) << 15) |
-                             ((B_MN ? 1u : 0u) << 16) | ((uint32_t)(BN >> 3) << 17) |
-                             ((uint32_t)(CG * BM >> 4) << 24);
       int it = 0, tc = 0;  // tc counts chains
       bool stop = false;
       for (int u = first; u < units && !stop; u += step) {
-        const Unit q = unit_at(P, u);
+        const Unit q = unit_at<EPI>(P, u);
+        const bool a_mn = EPI == OUT && P.q[q.prob].a_mn;
+        const uint32_t idesc = (1u << 4) | (P.fmt << 7) | (P.fmt << 10) | ((a_mn ? 1u : 0u) << 15) |
+                               ((EPI == OUT ? 1u : 0u) << 16) | ((uint32_t)(BN >> 3) << 17) |
+                               ((uint32_t)(CG * BM >> 4) << 24);
         for (int k0 = q.kb0; k0 < q.kb1 && !stop; k0 += S::CHAIN, tc++) {
           const int k1 = min(k0 + S::CHAIN, q.kb1);
           const uint32_t d = tmem + (tc & 1) * BN;
@@ -288,8 +381,8 @@ __global__ void __launch_bounds__(NTHREADS, 1)
 #pragma unroll
               for (int p = 0; p < PARTS; p++) {
                 const uint32_t a = st + p * (S::A_BYTES + S::B_BYTES), b = a + S::A_BYTES;
-                da[p] = A_MN ? desc_mn(a + kk * 2048, 8192) : desc_k(a + kk * 32);
-                db[p] = B_MN ? desc_mn(b + kk * 2048, 8192) : desc_k(b + kk * 32);
+                da[p] = a_mn ? desc_mn(a + kk * 2048, 8192) : desc_k(a + kk * 32);
+                db[p] = EPI == OUT ? desc_mn(b + kk * 2048, 8192) : desc_k(b + kk * 32);
               }
               mma_f16<CG>(d, da[0], db[0], idesc, (kb > k0 || kk > 0) ? 1u : 0u);
               if constexpr (PARTS == 2) {
@@ -316,30 +409,20 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     const int r = (warp & 3) * 32 + lane;
     float* blk = (float*)(smem + S::STAGES * S::STAGE + 256) + (warp - 4) * 1024;
     const uint32_t base = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(hf * HALF);
-    const float sc2 = [&] {
-      float v = P.scale * LOG2E;
-      if (P.sx >= 0) v /= split_scale(P.scal[P.sx]);
-      if (P.sw >= 0) v /= split_scale(P.scal[P.sw]);
-      return v;
-    }();
-    float factor = 1.0f, gmax = 0.0f;
-    if constexpr (EPI != LSE) {
+    float sc2 = P.scale * LOG2E, gmax = 0.0f;
+    if (EPI != OUT && P.split) sc2 = sc2 / split_scale(P.scal[S_X]) / split_scale(P.scal[S_W]);
+    if constexpr (EPI != LSE)
       gmax = P.one_dloss ? fabsf(P.dloss[0]) : __uint_as_float(P.scal[S_G]);
-      if constexpr (EPI == OUT) {
-        factor = P.scale / P.pscale * gmax;
-        if (P.sx >= 0) factor /= split_scale(P.scal[P.sx]);
-        if (P.sw >= 0) factor /= split_scale(P.scal[P.sw]);
-      }
-    }
     const uint32_t release = CG == 2 ? map_rank(smem_u32(tempty), 0) : smem_u32(tempty);
     int tc = 0;
     bool stop = false;
     for (int u = first; u < units && !stop; u += step) {
-      const Unit q = unit_at(P, u);
+      const Unit q = unit_at<EPI>(P, u);
+      const Prob& pr = P.q[q.prob];
       const long i = (long)(q.mt * CG + (int)rank) * BM + r;
-      const bool live = i < P.M;
+      const bool live = i < pr.M;
       const long c0 = (long)q.nt * BN + hf * HALF;
-      const int cols = (int)min((long)HALF, max(P.N - c0, 0l));
+      const int cols = (int)min((long)HALF, max(pr.N - c0, 0l));
       float m2 = -INFINITY, sum = 0.0f, lse2 = 0.0f, gr = 0.0f;
       int tcol = -1;
       if constexpr (EPI != OUT) {
@@ -388,20 +471,27 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         wait_chain();
       }
       if (stop) break;
+      float factor = 1.0f;
+      if constexpr (EPI == OUT) {
+        factor = P.scale / P.pscale * gmax;
+        if (pr.unscale >= 0) factor /= split_scale(P.scal[pr.unscale]);
+      }
+      uint32_t raw[PARTS == 1 ? 32 : 1];
+      if constexpr (PARTS == 1) tmem_ld32(base + (tc & 1) * BN, raw);
 #pragma unroll
       for (int h = 0; h < HALF / 32; h++) {
-        if (EPI != LSE && h * 32 >= cols) break;
         float v[32];
         if constexpr (PARTS == 2) {
 #pragma unroll
           for (int j = 0; j < 32; j++) v[j] = acc[h * 32 + j];
         } else {
-          uint32_t raw[32];
-          tmem_ld32(base + (tc & 1) * BN + h * 32, raw);
           ld_wait(raw);
 #pragma unroll
           for (int j = 0; j < 32; j++) v[j] = __uint_as_float(raw[j]);
+          // The next columns are on their way while these are worked on.
+          if (h + 1 < HALF / 32) tmem_ld32(base + (tc & 1) * BN + (h + 1) * 32, raw);
         }
+        if (EPI != LSE && h * 32 >= cols) continue;
         const int left = cols - h * 32;
         if constexpr (EPI == LSE) {
           float top = -INFINITY;
@@ -430,16 +520,16 @@ __global__ void __launch_bounds__(NTHREADS, 1)
           __syncwarp();
 #pragma unroll
           for (int g = 0; g < 8; g++)
-            *block4(blk, lane, g) = make_float4(v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]);
+            block4(blk, lane, g) = make_float4(v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]);
           __syncwarp();
           const long row0 = i - lane, col = c0 + h * 32;
-          const int rows = (int)min(32l, P.M - row0);
+          const int rows = (int)min(32l, pr.M - row0);
           if constexpr (EPI == PROB) {
             // Four lanes a row, eight columns each.
             const int g = (lane & 3) * 2;
             for (int rr = lane >> 2; rr < rows; rr += 8) {
               if (col + g * 4 >= P.ldp) break;
-              const float4 a = *block4(blk, rr, g), b = *block4(blk, rr, g + 1);
+              const float4 a = block4(blk, rr, g), b = block4(blk, rr, g + 1);
               const float f[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
               Pack<uint16_t, 8> hi, lo;
 #pragma unroll
@@ -457,25 +547,15 @@ __global__ void __launch_bounds__(NTHREADS, 1)
               *reinterpret_cast<Pack<uint16_t, 8>*>((uint16_t*)P.p_hi + at) = hi;
               if (PARTS == 2) *reinterpret_cast<Pack<uint16_t, 8>*>((uint16_t*)P.p_lo + at) = lo;
             }
-          } else if (lane < left) {
-            // One row at a time, one column a lane.
-            float* sum_at = P.accum + ((long)q.split * P.M + row0) * P.N + col + lane;
-            const size_t out_at = (size_t)(row0 * P.ldo + col + lane);
-#pragma unroll 4
-            for (int rr = 0; rr < rows; rr++) {
-              float o = block1(blk, rr, lane) * factor;
-              if (P.read_acc) o += sum_at[rr * P.N];
-              if (P.write_acc)
-                sum_at[rr * P.N] = o;
-              else
-                store_any(P.out, P.otype, out_at + rr * P.ldo, o);
-            }
+          } else {
+            store_block(pr, P.q[q.prob].accum + ((long)q.split * pr.M + row0) * pr.ldacc, blk, lane,
+                        row0, rows, col, min(left, 32), factor);
           }
         }
       }
       if constexpr (PARTS == 1) release_chain();
       if constexpr (EPI == LSE) {
-        if (live) P.part[(long)(q.nt * 2 + hf) * P.M + i] = make_float2(m2, sum);
+        if (live) P.part[(long)(q.nt * 2 + hf) * pr.M + i] = make_float2(m2, sum);
       }
     }
   }
@@ -487,6 +567,21 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     tmem_free<CG>(tmem, 512);
   }
   if (threadIdx.x == 0 && *abort_flag) atomicOr(P.status, ST_WAIT_TIMEOUT);
+}
+
+// One row's lse and loss from its (max, sum).
+__device__ __forceinline__ void finish_row(long i, float m, float s, long k, const float* zt,
+                                           const uint32_t* targets, float* loss, float* lse,
+                                           uint32_t* status) {
+  const float l2 = m + log2f(s);
+  lse[i] = l2 * LN2;
+  const uint32_t t = targets[i];
+  if (t == EB_IGNORE || (long)t >= k) {
+    loss[i] = 0.0f;
+    if (t != EB_IGNORE) atomicOr(status, ST_BAD_LABEL);
+  } else {
+    loss[i] = (l2 - zt[i]) * LN2;
+  }
 }
 
 // lse and loss of 32 rows from their half tiles' (max, sum): 32 threads a row
@@ -501,21 +596,28 @@ __global__ void __launch_bounds__(1024)
   const long i = (long)blockIdx.x * 32 + rx;
   float m = -INFINITY, s = 0.0f;
   if (i < n) {
+#pragma unroll 4
     for (int p = py; p < parts; p += 32) fold(m, s, part[(long)p * n + i]);
   }
   acc[py][rx] = make_float2(m, s);
   __syncthreads();
   if (py || i >= n) return;
   for (int p = 1; p < 32; p++) fold(m, s, acc[p][rx]);
-  const float l2 = m + log2f(s);
-  lse[i] = l2 * LN2;
-  const uint32_t t = targets[i];
-  if (t == EB_IGNORE || (long)t >= k) {
-    loss[i] = 0.0f;
-    if (t != EB_IGNORE) atomicOr(status, ST_BAD_LABEL);
-  } else {
-    loss[i] = (l2 - zt[i]) * LN2;
-  }
+  finish_row(i, m, s, k, zt, targets, loss, lse, status);
+}
+
+// The same for few half tiles: one thread a row.
+__global__ void __launch_bounds__(128)
+    k_ce_join_few(const float2* __restrict__ part, int parts, long n, long k,
+                  const float* __restrict__ zt, const uint32_t* __restrict__ targets, float* loss,
+                  float* lse, uint32_t* status) {
+  pdl_wait();
+  const long i = (long)blockIdx.x * 128 + threadIdx.x;
+  if (i >= n) return;
+  float m = -INFINITY, s = 0.0f;
+#pragma unroll 8
+  for (int p = 0; p < parts; p++) fold(m, s, part[(long)p * n + i]);
+  finish_row(i, m, s, k, zt, targets, loss, lse, status);
 }
 
 // Largest magnitude over the finite elements of rows x d f32 values.
@@ -555,21 +657,44 @@ __global__ void __launch_bounds__(256) k_ce_rows(const void* __restrict__ x, lon
   }
 }
 
-// out = the sum over splits, in order, of the partial products (M x N each),
-// plus the FP32 sums so far.
+// The outputs of a product that ran in splits of k: the sum over the splits,
+// in order, of the partial products (M x ld each), plus the FP32 sums so far.
 __global__ void __launch_bounds__(256)
-    k_ce_reduce(const float* __restrict__ part, int splits, long M, long N, float* accum,
-                int read_acc, int write_acc, void* out, int otype, long ldo) {
+    k_ce_reduce(const float* __restrict__ part, int splits, Prob q) {
   pdl_wait();
-  const long total = M * N;
-  for (long q = (long)blockIdx.x * 256 + threadIdx.x; q < total; q += (long)gridDim.x * 256) {
-    float s = 0.0f;
-    for (int p = 0; p < splits; p++) s += part[(long)p * total + q];
-    if (read_acc) s += accum[q];
-    if (write_acc)
-      accum[q] = s;
-    else
-      store_any(out, otype, (size_t)(q / N * ldo + q % N), s);
+  const long groups = q.ldacc / 4, total = q.M * groups;
+  for (long t = (long)blockIdx.x * 256 + threadIdx.x; t < total; t += (long)gridDim.x * 256) {
+    float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+    for (int p = 0; p < splits; p++) {
+      const float4 v = reinterpret_cast<const float4*>(part)[(long)p * total + t];
+      s = make_float4(s.x + v.x, s.y + v.y, s.z + v.z, s.w + v.w);
+    }
+    if (q.read_acc) {
+      const float4 v = reinterpret_cast<const float4*>(q.accum)[t];
+      s = make_float4(s.x + v.x, s.y + v.y, s.z + v.z, s.w + v.w);
+    }
+    if (q.write_acc) {
+      reinterpret_cast<float4*>(q.accum)[t] = s;
+    } else {
+      const long i = t / groups, c = t % groups * 4;
+      const float f[4] = {s.x, s.y, s.z, s.w};
+      const size_t at = (size_t)(i * q.ldo + c);
+      if (q.ovec && c + 4 <= q.N) {
+        if (q.otype == EB_F32) {
+          *reinterpret_cast<float4*>(static_cast<float*>(q.out) + at) = s;
+        } else {
+          Pack<uint16_t, 4> h;
+#pragma unroll
+          for (int j = 0; j < 4; j++)
+            h.v[j] = q.otype == EB_BF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(f[j]))
+                                        : __half_as_ushort(__float2half_rn(f[j]));
+          *reinterpret_cast<Pack<uint16_t, 4>*>(static_cast<uint16_t*>(q.out) + at) = h;
+        }
+      } else {
+        for (int j = 0; j < 4 && c + j < q.N; j++) store_any(q.out, q.otype, at + j, f[j]);
+      }
+    }
   }
 }
 
@@ -595,13 +720,13 @@ struct Operand {
   long rows, cols, ld;
 };
 
-// Boxes of 64 columns (128 bytes) by box_rows rows, 128-byte swizzle. Every
-// load's first column is a multiple of 64.
-CUtensorMap make_map(const uint16_t* base, const Operand& o, uint32_t box_rows) {
+// Boxes of 64 columns (128 bytes) by 64 rows, 128-byte swizzle. Every load's
+// first column is a multiple of 64.
+CUtensorMap make_map(const uint16_t* base, const Operand& o) {
   CUtensorMap m;
   cuuint64_t dims[2] = {(cuuint64_t)o.cols, (cuuint64_t)o.rows};
   cuuint64_t strides[1] = {(cuuint64_t)o.ld * 2};
-  cuuint32_t box[2] = {64, box_rows};
+  cuuint32_t box[2] = {64, 64};
   cuuint32_t estr[2] = {1, 1};
   CUresult r = encode_fn()(&m, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2,
                            const_cast<uint16_t*>(base), dims, strides, box, estr,
@@ -611,15 +736,21 @@ CUtensorMap make_map(const uint16_t* base, const Operand& o, uint32_t box_rows) 
   return m;
 }
 
-template <int EPI, int CG, int PARTS, bool A_MN, bool B_MN>
-void launch_gemm(eb_engine* e, const Operand& A, const Operand& B, const GemmParams& P) {
+template <int EPI, int CG, int PARTS>
+void launch_gemm(eb_engine* e, const Operand& A, const Operand& B, const Operand& C,
+                 const GemmParams& P) {
   using S = Shape<CG, PARTS>;
-  const auto kern = k_gemm<EPI, CG, PARTS, A_MN, B_MN>;
-  EB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::SMEM));
-  const uint32_t ar = A_MN ? 64 : S::A_ROWS, br = B_MN ? 64 : S::B_ROWS;
-  const CUtensorMap a0 = make_map(A.hi, A, ar), a1 = PARTS == 2 ? make_map(A.lo, A, ar) : a0;
-  const CUtensorMap b0 = make_map(B.hi, B, br), b1 = PARTS == 2 ? make_map(B.lo, B, br) : b0;
-  const int units = P.mtiles * P.ntiles * P.splits;
+  const auto kern = k_gemm<EPI, CG, PARTS>;
+  static const bool set = [&] {
+    EB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::SMEM));
+    return true;
+  }();
+  (void)set;
+  const CUtensorMap a0 = make_map(A.hi, A), a1 = PARTS == 2 ? make_map(A.lo, A) : a0;
+  const CUtensorMap b0 = make_map(B.hi, B), b1 = PARTS == 2 ? make_map(B.lo, B) : b0;
+  const CUtensorMap c0 = EPI == OUT ? make_map(C.hi, C) : b0;
+  const CUtensorMap c1 = EPI == OUT && PARTS == 2 ? make_map(C.lo, C) : c0;
+  const int units = P.q[0].units + P.q[1].units;
   const int clusters = std::min(units, e->num_sms / CG);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(clusters * CG));
@@ -634,26 +765,35 @@ void launch_gemm(eb_engine* e, const Operand& A, const Operand& B, const GemmPar
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = CG == 2 ? 2 : 1;
-  cuda_check(cudaLaunchKernelEx(&cfg, kern, a0, a1, b0, b1, P), "linear cross entropy");
+  cuda_check(cudaLaunchKernelEx(&cfg, kern, a0, a1, b0, b1, c0, c1, P), "linear cross entropy");
   e->stats.kernel_launches++;
 }
 
 constexpr int CGS = 2;
 
-template <int EPI, bool A_MN, bool B_MN>
-void gemm(eb_engine* e, const Operand& A, const Operand& B, GemmParams P) {
-  const int tm = CGS * BM;
-  P.mtiles = (int)((P.M + tm - 1) / tm);
-  P.ntiles = (int)((P.N + BN - 1) / BN);
-  P.kblocks = (int)((P.K + BK - 1) / BK);
-  if (P.kb_split == 0) P.kb_split = P.kblocks;
-  P.splits = (P.kblocks + P.kb_split - 1) / P.kb_split;
-  P.group = std::min(P.mtiles, 16);
+Prob make_prob(long M, long N, long K) {
+  Prob q{};
+  q.M = M;
+  q.N = N;
+  q.K = K;
+  q.mtiles = (int)((M + CGS * BM - 1) / (CGS * BM));
+  q.ntiles = (int)((N + BN - 1) / BN);
+  q.kblocks = (int)((K + BK - 1) / BK);
+  q.kb_split = q.kblocks;
+  q.splits = 1;
+  q.units = q.mtiles * q.ntiles;
+  q.group = std::min(q.mtiles, 16);
+  q.unscale = -1;
+  return q;
+}
+
+template <int EPI>
+void gemm(eb_engine* e, const Operand& A, const Operand& B, const Operand& C, GemmParams P) {
   P.status = e->d_status;
   if (A.lo)
-    launch_gemm<EPI, CGS, 2, A_MN, B_MN>(e, A, B, P);
+    launch_gemm<EPI, CGS, 2>(e, A, B, C, P);
   else
-    launch_gemm<EPI, CGS, 1, A_MN, B_MN>(e, A, B, P);
+    launch_gemm<EPI, CGS, 1>(e, A, B, C, P);
 }
 
 // The 16-bit operand of a matrix: itself where TMA can read it (row stride a
@@ -703,44 +843,84 @@ GemmParams base_params(const LinearCeArgs& a, const uint32_t* scal) {
   P.scal = scal;
   P.scale = a.scale;
   P.fmt = a.dtype == EB_BF16 ? 1u : 0u;
-  P.sx = a.dtype == EB_F32 ? S_X : -1;
-  P.sw = a.dtype == EB_F32 ? S_W : -1;
+  P.split = a.dtype == EB_F32;
   P.targets = a.targets;
   P.k = (long)a.k;
   P.pscale = a.dtype == EB_BF16 ? 1.0f : PSCALE;
   return P;
 }
 
-// A product into an output: over splits of k when the tiles alone would leave
-// most of the GPU idle.
-template <bool A_MN>
-void product(eb_engine* e, const Operand& A, const Operand& B, GemmParams P, float* accum,
-             bool read_acc, bool write_acc, void* out, int otype, long ldo) {
-  const long tiles = ((P.M + CGS * BM - 1) / (CGS * BM)) * ((P.N + BN - 1) / BN);
-  const long kblocks = (P.K + BK - 1) / BK, clusters = e->num_sms / CGS;
-  long splits = std::min(clusters / std::max(tiles, 1l), kblocks / 4);
-  if (splits > 1) {
-    P.kb_split = (int)((kblocks + splits - 1) / splits);
-    splits = (kblocks + P.kb_split - 1) / P.kb_split;
+// Splits of k for the products of one launch. Units go to the clusters in
+// turn, the longer first, so the launch takes a round per `clusters` units, each
+// as long as its first unit. A split product also writes and reads its
+// partial sums again in a launch of its own. Chosen over a few split counts by
+// that estimate, in units of one k-block of one tile (0.28 us, three times
+// that for two-term operands).
+void choose_splits(Prob* q, int count, int clusters, int parts) {
+  const double block_us = 0.28 * (parts == 2 ? 3 : 1);
+  static const int tries[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32, 48, 64};
+  auto len = [](const Prob& p, int s) { return (p.kblocks + s - 1) / s; };
+  double best = 1e300;
+  int pick[2] = {1, 1};
+  for (int s0 : tries) {
+    if (s0 > 1 && len(q[0], s0) < 2) break;
+    for (int s1 : tries) {
+      if (s1 > 1 && (count < 2 || len(q[1], s1) < 2)) break;
+      const int s[2] = {s0, s1};
+      double rounds_us = 0, extra_us = 0;
+      long units[2] = {0, 0}, l[2] = {0, 0};
+      for (int i = 0; i < count; i++) {
+        l[i] = len(q[i], s[i]);
+        units[i] = (long)q[i].mtiles * q[i].ntiles * ((q[i].kblocks + l[i] - 1) / l[i]);
+        if (s[i] > 1) extra_us += 3.0 + (double)q[i].M * q[i].ldacc * 4 * (s[i] + 1) / 4e6;
+      }
+      const int a = l[0] >= l[1] ? 0 : 1;
+      const long ra = (units[a] + clusters - 1) / clusters;
+      const long rb = (units[0] + units[1] + clusters - 1) / clusters - ra;
+      rounds_us = block_us * (double)(ra * (l[a] + 3) + rb * (l[1 - a] + 3));
+      if (rounds_us + extra_us < best) {
+        best = rounds_us + extra_us;
+        pick[0] = s0;
+        pick[1] = s1;
+      }
+    }
   }
-  if (splits > 1) {
-    P.accum = e->scratch_get<float>("ce_splits", (size_t)(splits * P.M * P.N));
-    P.write_acc = 1;
-    gemm<OUT, A_MN, true>(e, A, B, P);
+  for (int i = 0; i < count; i++) {
+    q[i].kb_split = len(q[i], pick[i]);
+    q[i].splits = (q[i].kblocks + q[i].kb_split - 1) / q[i].kb_split;
+    q[i].units = q[i].mtiles * q[i].ntiles * q[i].splits;
+  }
+}
+
+// One or both of a piece's gradient products in one launch: A = P; B of the
+// first product, C of the second.
+void products(eb_engine* e, const Operand& A, Operand B, Operand C, GemmParams P, int count) {
+  choose_splits(P.q, count, e->num_sms / CGS, A.lo ? 2 : 1);
+  if (count == 2 && P.q[1].kb_split > P.q[0].kb_split) {
+    std::swap(P.q[0], P.q[1]);
+    std::swap(B, C);
+  }
+  const Prob whole[2] = {P.q[0], P.q[1]};
+  size_t room = 0, at[2] = {0, 0};
+  for (int i = 0; i < count; i++) {
+    at[i] = room;
+    if (P.q[i].splits > 1) room += (size_t)(P.q[i].splits * P.q[i].M * P.q[i].ldacc);
+  }
+  float* part = room ? e->scratch_get<float>("ce_splits", room) : nullptr;
+  for (int i = 0; i < count; i++) {
+    if (P.q[i].splits == 1) continue;
+    P.q[i].accum = part + at[i];
+    P.q[i].read_acc = 0;
+    P.q[i].write_acc = 1;
+  }
+  gemm<OUT>(e, A, B, count == 2 ? C : B, P);
+  for (int i = 0; i < count; i++) {
+    if (P.q[i].splits == 1) continue;
     const unsigned grid =
-        (unsigned)std::min<long>((P.M * P.N + 255) / 256, (long)e->num_sms * 16);
-    launch_pdl(e, k_ce_reduce, dim3(grid), dim3(256), 0, (const float*)P.accum, (int)splits, P.M,
-               P.N, accum, (int)read_acc, (int)write_acc, out, otype, ldo);
+        (unsigned)std::min<long>((whole[i].M * whole[i].ldacc / 4 + 255) / 256, (long)e->num_sms * 8);
+    launch_pdl(e, k_ce_reduce, dim3(grid), dim3(256), 0, (const float*)(part + at[i]),
+               P.q[i].splits, whole[i]);
     e->stats.kernel_launches++;
-  } else {
-    P.kb_split = 0;
-    P.accum = accum;
-    P.read_acc = read_acc;
-    P.write_acc = write_acc;
-    P.out = out;
-    P.otype = otype;
-    P.ldo = ldo;
-    gemm<OUT, A_MN, true>(e, A, B, P);
   }
 }
 
@@ -756,14 +936,15 @@ void linear_ce(eb_engine* e, const LinearCeArgs& a, float* loss, float* lse) {
   float2* part = e->scratch_get<float2>("ce_part", (size_t)parts * a.n);
   float* zt = e->scratch_get<float>("ce_zt", a.n);
   GemmParams P = base_params(a, scal);
-  P.M = (long)a.n;
-  P.N = (long)a.k;
-  P.K = (long)a.d;
+  P.q[0] = make_prob((long)a.n, (long)a.k, (long)a.d);
   P.part = part;
   P.zt = zt;
-  gemm<LSE, false, false>(e, X, W, P);
-  launch_pdl(e, k_ce_join, dim3((unsigned)((a.n + 31) / 32)), dim3(1024), 0, (const float2*)part,
-             parts, (long)a.n, (long)a.k, (const float*)zt, a.targets, loss, lse, e->d_status);
+  gemm<LSE>(e, X, W, W, P);
+  const bool few = parts <= 32;
+  launch_pdl(e, few ? k_ce_join_few : k_ce_join,
+             dim3((unsigned)(few ? (a.n + 127) / 128 : (a.n + 31) / 32)), dim3(few ? 128 : 1024), 0,
+             (const float2*)part, parts, (long)a.n, (long)a.k, (const float*)zt, a.targets, loss,
+             lse, e->d_status);
   e->stats.kernel_launches++;
 }
 
@@ -785,63 +966,73 @@ void linear_ce_backward(eb_engine* e, const LinearCeArgs& a, const LinearCeGrads
     launch_pdl(e, k_ce_max, dim3(grid), dim3(256), 0, g.dloss, (long)a.n, 1l, 1l, scal + S_G);
     e->stats.kernel_launches++;
   }
-  // Pieces: all rows by as many prototypes as the scratch holds (multiples
-  // of a tile); with so many rows that fewer than 2,048 prototypes would
-  // fit, the rows are cut too.
+  // Pieces of P, as many elements as the scratch holds: the shorter side of
+  // P whole where at least 2,048 of the longer then fit (the sums that run
+  // over pieces are the shorter side's gradient), else pieces of both sides.
   const int parts = a.dtype == EB_F32 ? 2 : 1;
   const size_t room = ((size_t)256 << 20) / 2 / parts;  // elements of P
-  const size_t kpad = (a.k + BN - 1) / BN * BN;
-  size_t rows = a.n;
-  if (room / rows < std::min<size_t>(2048, kpad))
-    rows = std::max<size_t>(room / std::min<size_t>(2048, kpad) / 256 * 256, 256);
-  const size_t cols = std::min(kpad, std::max<size_t>(room / rows / BN * BN, BN));
+  const size_t npad = (a.n + 255) / 256 * 256, kpad = (a.k + 255) / 256 * 256;
+  const size_t side = std::min(std::min(npad, kpad), room / 2048 / 256 * 256);
+  const size_t other = std::max<size_t>(room / side / 256 * 256, 256);
+  const size_t rows = std::min(npad, npad <= kpad ? side : other);
+  const size_t cols = std::min(kpad, npad <= kpad ? other : side);
   uint16_t* p = e->scratch_get<uint16_t>("ce_p", rows * cols * parts);
   const bool many_cols = cols < a.k, many_rows = rows < a.n;
-  float* dxacc = g.dx && many_cols ? e->scratch_get<float>("ce_dx", rows * a.d) : nullptr;
-  float* dwacc = g.dw && many_rows ? e->scratch_get<float>("ce_dw", a.k * a.d) : nullptr;
+  const long ldacc = ((long)a.d + 3) / 4 * 4;
+  float* dxacc = g.dx && many_cols ? e->scratch_get<float>("ce_dx", std::min(rows, a.n) * ldacc) : nullptr;
+  float* dwacc = g.dw && many_rows ? e->scratch_get<float>("ce_dw", a.k * ldacc) : nullptr;
+  auto vec = [](int type, size_t ld) { return ld * dtype_bytes(type) % 16 == 0; };
   for (size_t r0 = 0; r0 < a.n; r0 += rows) {
     const size_t r1 = std::min(a.n, r0 + rows);
     const Operand Xr = rows_of(X, (long)r0, (long)r1);
     for (size_t v0 = 0; v0 < a.k; v0 += cols) {
       const size_t v1 = std::min(a.k, v0 + cols);
       const Operand Wv = rows_of(W, (long)v0, (long)v1);
+      const long pr = (long)(r1 - r0), pc = (long)(v1 - v0);
       GemmParams P = base_params(a, scal);
-      P.M = (long)(r1 - r0);
-      P.N = (long)(v1 - v0);
-      P.K = (long)a.d;
+      P.q[0] = make_prob(pr, pc, (long)a.d);
       P.targets = a.targets + r0;
       P.lse = g.lse + r0;
       P.dloss = g.one_dloss ? g.dloss : g.dloss + r0;
       P.one_dloss = g.one_dloss;
       P.col0 = (long)v0;
-      P.ldp = ((long)(v1 - v0) + 7) / 8 * 8;
+      P.ldp = (pc + 7) / 8 * 8;
       P.p_hi = p;
       P.p_lo = parts == 2 ? p + rows * cols : nullptr;
-      gemm<PROB, false, false>(e, Xr, Wv, P);
-      const Operand Pm{p, parts == 2 ? p + rows * cols : nullptr, P.M, P.N, P.ldp};
-      GemmParams Q = base_params(a, scal);
-      Q.dloss = P.dloss;
-      Q.one_dloss = P.one_dloss;
+      gemm<PROB>(e, Xr, Wv, Wv, P);
+      const Operand Pm{p, parts == 2 ? p + rows * cols : nullptr, pr, pc, P.ldp};
+      int count = 0;
+      Operand B[2];
       if (g.dx) {
-        Q.M = P.M;
-        Q.N = (long)a.d;
-        Q.K = P.N;
-        Q.sx = -1;
-        Q.sw = base_params(a, scal).sw;
-        product<false>(e, Pm, Wv, Q, dxacc, v0 > 0, v1 < a.k,
-                       static_cast<char*>(g.dx) + r0 * g.lddx * dtype_bytes(g.dxtype), g.dxtype,
-                       (long)g.lddx);
+        Prob& q = P.q[count];
+        q = make_prob(pr, (long)a.d, pc);
+        q.unscale = parts == 2 ? S_W : -1;
+        q.out = static_cast<char*>(g.dx) + r0 * g.lddx * dtype_bytes(g.dxtype);
+        q.otype = g.dxtype;
+        q.ldo = (long)g.lddx;
+        q.ovec = vec(g.dxtype, g.lddx);
+        q.accum = dxacc;
+        q.ldacc = ldacc;
+        q.read_acc = v0 > 0;
+        q.write_acc = v1 < a.k;
+        B[count++] = Wv;
       }
       if (g.dw) {
-        Q.M = P.N;
-        Q.N = (long)a.d;
-        Q.K = P.M;
-        Q.sx = base_params(a, scal).sx;
-        Q.sw = -1;
-        product<true>(e, Pm, Xr, Q, dwacc ? dwacc + v0 * a.d : nullptr, r0 > 0, r1 < a.n,
-                      static_cast<char*>(g.dw) + v0 * g.lddw * dtype_bytes(g.dwtype), g.dwtype,
-                      (long)g.lddw);
+        Prob& q = P.q[count];
+        q = make_prob(pc, (long)a.d, pr);
+        q.a_mn = 1;
+        q.unscale = parts == 2 ? S_X : -1;
+        q.out = static_cast<char*>(g.dw) + v0 * g.lddw * dtype_bytes(g.dwtype);
+        q.otype = g.dwtype;
+        q.ldo = (long)g.lddw;
+        q.ovec = vec(g.dwtype, g.lddw);
+        q.accum = dwacc ? dwacc + v0 * ldacc : nullptr;
+        q.ldacc = ldacc;
+        q.read_acc = r0 > 0;
+        q.write_acc = r1 < a.n;
+        B[count++] = Xr;
       }
+      products(e, Pm, B[0], B[1], P, count);
     }
   }
 }
