@@ -127,17 +127,11 @@ __device__ __forceinline__ float ex2(float v) {
   return r;
 }
 
-// Larger of two, NaN if either is (fmaxf would drop it).
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-
 // Folds (m', s') into a running (max, sum of 2^(z - max)); (-inf, 0) is empty.
+// NaN scores are in the sums, not in the maxima.
 __device__ __forceinline__ void fold(float& m, float& s, float2 v) {
-  const float top = max_nan(m, v.x);
-  if (top != -INFINITY) s = s * ex2(m - top) + v.y * ex2(v.x - top);
+  const float top = fmaxf(m, v.x), off = top == -INFINITY ? 0.0f : top;
+  s = s * ex2(m - off) + v.y * ex2(v.x - off);
   m = top;
 }
 
@@ -147,6 +141,31 @@ __device__ __forceinline__ void fold(float& m, float& s, float2 v) {
 __device__ __forceinline__ float4& block4(float* blk, int r, int g) {
   return reinterpret_cast<float4*>(blk)[r * 8 + (g ^ (r & 7))];
 }
+// Eight values times `by` as eight 16-bit elements (bf16, or f16), and with
+// LO what f16 left of them as eight more.
+template <bool F16, bool LO = false>
+__device__ __forceinline__ uint4 pack8(const float (&f)[8], float by, uint4& lo) {
+  uint32_t h[4], l[4];
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    const float2 v = make_float2(f[2 * j] * by, f[2 * j + 1] * by);
+    if constexpr (F16) {
+      const __half2 q = __float22half2_rn(v);
+      h[j] = *reinterpret_cast<const uint32_t*>(&q);
+      if constexpr (LO) {
+        const float2 b = __half22float2(q);
+        const __half2 r = __float22half2_rn(make_float2(v.x - b.x, v.y - b.y));
+        l[j] = *reinterpret_cast<const uint32_t*>(&r);
+      }
+    } else {
+      const __nv_bfloat162 q = __float22bfloat162_rn(v);
+      h[j] = *reinterpret_cast<const uint32_t*>(&q);
+    }
+  }
+  if constexpr (LO) lo = make_uint4(l[0], l[1], l[2], l[3]);
+  return make_uint4(h[0], h[1], h[2], h[3]);
+}
+
 // The tile and k-range of unit u: within a split, groups of row tiles pass
 // over all column tiles, row tile fastest, so that the tiles in flight share
 // operands in L2.
@@ -240,15 +259,12 @@ __device__ __forceinline__ void store_block(const Prob& q, float* sums, float* b
         for (int j = 0; j < 8; j++) f[j] += o[j];
       }
       uint16_t* out = static_cast<uint16_t*>(q.out) + (row0 + r) * q.ldo + col + g * 4;
-      Pack<uint16_t, 8> h;
-#pragma unroll
-      for (int j = 0; j < 8; j++)
-        h.v[j] = q.otype == EB_BF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(f[j]))
-                                    : __half_as_ushort(__float2half_rn(f[j]));
+      uint4 none, h = q.otype == EB_BF16 ? pack8<false>(f, 1.0f, none) : pack8<true>(f, 1.0f, none);
       if (q.ovec && mine == 8) {
-        *reinterpret_cast<Pack<uint16_t, 8>*>(out) = h;
+        *reinterpret_cast<uint4*>(out) = h;
       } else {
-        for (int j = 0; j < mine; j++) out[j] = h.v[j];
+        const uint16_t* e = reinterpret_cast<const uint16_t*>(&h);
+        for (int j = 0; j < mine; j++) out[j] = e[j];
       }
     }
   }
@@ -423,8 +439,8 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       const bool live = i < pr.M;
       const long c0 = (long)q.nt * BN + hf * HALF;
       const int cols = (int)min((long)HALF, max(pr.N - c0, 0l));
-      float m2 = -INFINITY, sum = 0.0f, lse2 = 0.0f, gr = 0.0f;
-      int tcol = -1;
+      float m2 = -INFINITY, sum = 0.0f, zt = 0.0f, lse2 = 0.0f, gr = 0.0f;
+      int tcol = -1;  // the target's column among this warp's, if it is one of them
       if constexpr (EPI != OUT) {
         const uint32_t t = live ? P.targets[i] : EB_IGNORE;
         if (t != EB_IGNORE) {
@@ -494,58 +510,68 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         if (EPI != LSE && h * 32 >= cols) continue;
         const int left = cols - h * 32;
         if constexpr (EPI == LSE) {
-          float top = -INFINITY;
+          if (left < 32) {
 #pragma unroll
-          for (int j = 0; j < 32; j++) {
-            v[j] = j < left ? v[j] * sc2 : -INFINITY;
-            top = max_nan(top, v[j]);
-            if (j + h * 32 == tcol) P.zt[i] = v[j];
+            for (int j = 0; j < 32; j++) v[j] = j < left ? v[j] : -INFINITY;
           }
-          const float m = max_nan(m2, top);
-          if (m != -INFINITY) {  // columns of -inf alone add nothing
-            sum *= ex2(m2 - m);
+          if (tcol >> 5 == h) {  // through shared memory: registers have no index
 #pragma unroll
-            for (int j = 0; j < 32; j++) sum += ex2(v[j] - m);
-            m2 = m;
+            for (int g = 0; g < 8; g++)
+              block4(blk, lane, g) = make_float4(v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]);
+            zt = reinterpret_cast<const float*>(&block4(blk, lane, (tcol & 31) >> 2))[tcol & 3];
           }
+          // The maximum passes over NaN scores; they reach the sum.
+          float top[4] = {m2, v[0], v[1], v[2]};
+#pragma unroll
+          for (int j = 3; j < 32; j++) top[j & 3] = fmaxf(top[j & 3], v[j]);
+          const float m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+          const float off = m == -INFINITY ? 0.0f : -m * sc2;
+          float part[4] = {sum * ex2(fmaf(m2, sc2, off)), 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int j = 0; j < 32; j++) part[j & 3] += ex2(fmaf(v[j], sc2, off));
+          sum = (part[0] + part[1]) + (part[2] + part[3]);
+          m2 = m;
         } else {
           if constexpr (EPI == PROB) {
+            // Columns past the last prototype are never read.
 #pragma unroll
-            for (int j = 0; j < 32; j++) {
-              float p = ex2(fmaf(v[j], sc2, -lse2));
-              if (j + h * 32 == tcol) p -= 1.0f;
-              v[j] = j < left && gr != 0.0f ? p * gr : 0.0f;
-            }
+            for (int j = 0; j < 32; j++) v[j] = ex2(fmaf(v[j], sc2, -lse2)) * gr;
           }
           __syncwarp();
 #pragma unroll
           for (int g = 0; g < 8; g++)
             block4(blk, lane, g) = make_float4(v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]);
+          if constexpr (EPI == PROB) {
+            if (gr == 0.0f) {  // nothing of a row without a gradient, not even its NaN
+#pragma unroll
+              for (int g = 0; g < 8; g++) block4(blk, lane, g) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            } else if (tcol >> 5 == h) {
+              reinterpret_cast<float*>(&block4(blk, lane, (tcol & 31) >> 2))[tcol & 3] -= gr;
+            }
+          }
           __syncwarp();
           const long row0 = i - lane, col = c0 + h * 32;
           const int rows = (int)min(32l, pr.M - row0);
           if constexpr (EPI == PROB) {
             // Four lanes a row, eight columns each.
             const int g = (lane & 3) * 2;
-            for (int rr = lane >> 2; rr < rows; rr += 8) {
-              if (col + g * 4 >= P.ldp) break;
-              const float4 a = block4(blk, rr, g), b = block4(blk, rr, g + 1);
-              const float f[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-              Pack<uint16_t, 8> hi, lo;
+            if (col + g * 4 < P.ldp) {
+              const long at = (row0 + (lane >> 2)) * P.ldp + col + g * 4;
 #pragma unroll
-              for (int w = 0; w < 8; w++) {
-                if (PARTS == 1 && P.fmt) {
-                  hi.v[w] = __bfloat16_as_ushort(__float2bfloat16_rn(f[w]));
-                } else {
-                  const float t = f[w] * PSCALE;
-                  const __half q = __float2half_rn(t);
-                  hi.v[w] = __half_as_ushort(q);
-                  if (PARTS == 2) lo.v[w] = __half_as_ushort(__float2half_rn(t - __half2float(q)));
-                }
+              for (int t = 0; t < 4; t++) {
+                const int rr = (lane >> 2) + t * 8;
+                if (rr >= rows) break;
+                const float4 a = block4(blk, rr, g), b = block4(blk, rr, g + 1);
+                const float f[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+                uint4 hi, lo;
+                if (PARTS == 1 && P.fmt)
+                  hi = pack8<false>(f, 1.0f, lo);
+                else
+                  hi = pack8<true, PARTS == 2>(f, PSCALE, lo);
+                *reinterpret_cast<uint4*>((uint16_t*)P.p_hi + at + t * 8 * P.ldp) = hi;
+                if (PARTS == 2)
+                  *reinterpret_cast<uint4*>((uint16_t*)P.p_lo + at + t * 8 * P.ldp) = lo;
               }
-              const long at = (row0 + rr) * P.ldp + col + g * 4;
-              *reinterpret_cast<Pack<uint16_t, 8>*>((uint16_t*)P.p_hi + at) = hi;
-              if (PARTS == 2) *reinterpret_cast<Pack<uint16_t, 8>*>((uint16_t*)P.p_lo + at) = lo;
             }
           } else {
             store_block(pr, P.q[q.prob].accum + ((long)q.split * pr.M + row0) * pr.ldacc, blk, lane,
@@ -555,7 +581,10 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       }
       if constexpr (PARTS == 1) release_chain();
       if constexpr (EPI == LSE) {
-        if (live) P.part[(long)(q.nt * 2 + hf) * pr.M + i] = make_float2(m2, sum);
+        if (live) {
+          P.part[(long)(q.nt * 2 + hf) * pr.M + i] = make_float2(m2 * sc2, sum);
+          if (tcol >= 0) P.zt[i] = zt * sc2;
+        }
       }
     }
   }
