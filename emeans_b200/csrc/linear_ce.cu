@@ -39,6 +39,8 @@ namespace eb {
 
 namespace {
 
+using tc::pdl_trigger;
+
 constexpr int BM = 128;   // rows of a tile a CTA holds (TMEM lanes)
 constexpr int BN = 256;   // columns of a tile (TMEM columns of one accumulator)
 constexpr int BK = 64;    // k-elements a stage: one 128-byte swizzle row
@@ -293,6 +295,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
   uint64_t* done = tempty + 2;
   uint32_t* tmem_slot = (uint32_t*)(done + 1);
   volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
+  pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = CG == 2 ? cta_rank() : 0;
   const int units = P.q[0].units + (EPI == OUT ? P.q[1].units : 0);
@@ -619,6 +622,7 @@ __global__ void __launch_bounds__(1024)
     k_ce_join(const float2* __restrict__ part, int parts, long n, long k,
               const float* __restrict__ zt, const uint32_t* __restrict__ targets, float* loss,
               float* lse, uint32_t* status) {
+  pdl_trigger();
   pdl_wait();
   __shared__ float2 acc[32][33];
   const int rx = threadIdx.x & 31, py = threadIdx.x >> 5;
@@ -640,6 +644,7 @@ __global__ void __launch_bounds__(128)
     k_ce_join_few(const float2* __restrict__ part, int parts, long n, long k,
                   const float* __restrict__ zt, const uint32_t* __restrict__ targets, float* loss,
                   float* lse, uint32_t* status) {
+  pdl_trigger();
   pdl_wait();
   const long i = (long)blockIdx.x * 128 + threadIdx.x;
   if (i >= n) return;
@@ -649,47 +654,130 @@ __global__ void __launch_bounds__(128)
   finish_row(i, m, s, k, zt, targets, loss, lse, status);
 }
 
-// Largest magnitude over the finite elements of rows x d f32 values.
-__global__ void __launch_bounds__(256) k_ce_max(const float* __restrict__ x, long rows, long d,
-                                                long ld, uint32_t* out) {
-  pdl_wait();
-  uint32_t m = 0;
-  const long total = rows * d;
-  for (long q = (long)blockIdx.x * 256 + threadIdx.x; q < total; q += (long)gridDim.x * 256) {
-    const uint32_t b = __float_as_uint(x[ld == d ? q : q / d * ld + q % d]) & 0x7FFFFFFFu;
-    if (b < 0x7F800000u) m = max(m, b);
-  }
+// Rows of an operand on their way to rows of dp 16-bit elements (zeros past
+// d): f32 as two FP16 terms, 16-bit types as they are. `blocks` of a launch
+// work on it.
+struct Prep {
+  const void* x;
+  long rows, d, ld, dp;
+  uint16_t* hi;
+  uint16_t* lo;
+  unsigned blocks;
+};
+constexpr int PREP_BLOCKS = 512;  // most blocks of a launch for one operand
+
+__device__ __forceinline__ uint32_t finite_bits(float v) {
+  const uint32_t b = __float_as_uint(v) & 0x7FFFFFFFu;
+  return b < 0x7F800000u ? b : 0u;
+}
+__device__ __forceinline__ uint32_t block_max(uint32_t m) {
+  __shared__ uint32_t all[8];
   m = __reduce_max_sync(0xffffffffu, m);
-  if ((threadIdx.x & 31) == 0 && m) atomicMax(out, m);
+  if ((threadIdx.x & 31) == 0) all[threadIdx.x >> 5] = m;
+  __syncthreads();
+  m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; i++) m = max(m, all[i]);
+  return m;
 }
 
-// Rows of x as rows of dp 16-bit elements, zeros past d: f32 as two FP16
-// terms, 16-bit types as they are.
-template <bool SPLIT>
-__global__ void __launch_bounds__(256) k_ce_rows(const void* __restrict__ x, long rows, long d,
-                                                 long ld, long dp, const uint32_t* max_bits,
-                                                 uint16_t* hi, uint16_t* lo) {
+// Eight columns c .. c + 8 of a row, zeros past d.
+__device__ __forceinline__ void load8(const float* row, long c, long d, bool vec, float (&f)[8]) {
+  if (vec && c + 8 <= d) {
+    const float4 a = *reinterpret_cast<const float4*>(row + c);
+    const float4 b = *reinterpret_cast<const float4*>(row + c + 4);
+    f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; j++) f[j] = c + j < d ? row[c + j] : 0.0f;
+  }
+}
+
+// Largest magnitude over the finite elements of both operands' rows: one per
+// block (a warp takes a row at a time), at maxima[block].
+__global__ void __launch_bounds__(256) k_ce_max(Prep X, Prep W, uint32_t* maxima) {
+  pdl_trigger();
   pdl_wait();
-  const float s = SPLIT ? split_scale(*max_bits) : 1.0f;
-  const long total = rows * dp;
-  for (long q = (long)blockIdx.x * 256 + threadIdx.x; q < total; q += (long)gridDim.x * 256) {
-    const long i = q / dp, c = q % dp;
-    if constexpr (SPLIT) {
-      float v = c < d ? static_cast<const float*>(x)[i * ld + c] * s : 0.0f;
-      if (!isfinite(v)) v = NAN;
-      const __half h = __float2half_rn(v);
-      hi[q] = __half_as_ushort(h);
-      lo[q] = __half_as_ushort(__float2half_rn(v - __half2float(h)));
-    } else {
-      hi[q] = c < d ? static_cast<const uint16_t*>(x)[i * ld + c] : (uint16_t)0;
+  const bool second = blockIdx.x >= X.blocks;
+  const Prep& q = second ? W : X;
+  const unsigned b = blockIdx.x - (second ? X.blocks : 0);
+  const bool vec = q.ld % 4 == 0;
+  uint32_t m = 0;
+  for (long i = (long)b * 8 + (threadIdx.x >> 5); i < q.rows; i += (long)q.blocks * 8) {
+    const float* row = static_cast<const float*>(q.x) + i * q.ld;
+#pragma unroll 2
+    for (long c = (threadIdx.x & 31) * 8; c < q.d; c += 256) {
+      float f[8];
+      load8(row, c, q.d, vec, f);
+#pragma unroll
+      for (int j = 0; j < 8; j++) m = max(m, finite_bits(f[j]));
     }
   }
+  m = block_max(m);
+  if (threadIdx.x == 0) maxima[blockIdx.x] = m;
+}
+
+// The operands' 16-bit rows; with SPLIT, scaled by the largest of the blocks'
+// maxima, which the first block of each operand leaves in `scal`.
+template <bool SPLIT>
+__global__ void __launch_bounds__(256)
+    k_ce_rows(Prep X, Prep W, const uint32_t* __restrict__ maxima, uint32_t* scal) {
+  pdl_trigger();
+  pdl_wait();
+  const bool second = blockIdx.x >= X.blocks;
+  const Prep& q = second ? W : X;
+  const unsigned b = blockIdx.x - (second ? X.blocks : 0);
+  float s = 1.0f;
+  if constexpr (SPLIT) {
+    uint32_t m = 0;
+    for (unsigned t = threadIdx.x; t < q.blocks; t += 256)
+      m = max(m, maxima[t + (second ? X.blocks : 0)]);
+    m = block_max(m);
+    s = split_scale(m);
+    if (b == 0 && threadIdx.x == 0) scal[second ? S_W : S_X] = m;
+  }
+  const bool vec = q.ld % 4 == 0;
+  for (long i = (long)b * 8 + (threadIdx.x >> 5); i < q.rows; i += (long)q.blocks * 8) {
+    for (long c = (threadIdx.x & 31) * 8; c < q.dp; c += 256) {
+      uint4 hi, lo;
+      if constexpr (SPLIT) {
+        float f[8];
+        load8(static_cast<const float*>(q.x) + i * q.ld, c, q.d, vec, f);
+#pragma unroll
+        for (int j = 0; j < 8; j++) f[j] = isfinite(f[j]) ? f[j] : NAN;
+        hi = pack8<true, true>(f, s, lo);
+        *reinterpret_cast<uint4*>(q.lo + i * q.dp + c) = lo;
+      } else {
+        const uint16_t* row = static_cast<const uint16_t*>(q.x) + i * q.ld;
+        uint16_t h[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) h[j] = c + j < q.d ? row[c + j] : (uint16_t)0;
+        hi = make_uint4(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16,
+                        h[4] | (uint32_t)h[5] << 16, h[6] | (uint32_t)h[7] << 16);
+      }
+      *reinterpret_cast<uint4*>(q.hi + i * q.dp + c) = hi;
+    }
+  }
+}
+
+// Largest magnitude of the rows' loss gradients (finite ones), into a zeroed
+// word.
+__global__ void __launch_bounds__(256) k_ce_gmax(const float* __restrict__ g, long n,
+                                                 uint32_t* out) {
+  pdl_trigger();
+  pdl_wait();
+  uint32_t m = 0;
+  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long)gridDim.x * 256)
+    m = max(m, finite_bits(g[i]));
+  m = block_max(m);
+  if (threadIdx.x == 0 && m) atomicMax(out, m);
 }
 
 // The outputs of a product that ran in splits of k: the sum over the splits,
 // in order, of the partial products (M x ld each), plus the FP32 sums so far.
 __global__ void __launch_bounds__(256)
     k_ce_reduce(const float* __restrict__ part, int splits, Prob q) {
+  pdl_trigger();
   pdl_wait();
   const long groups = q.ldacc / 4, total = q.M * groups;
   for (long t = (long)blockIdx.x * 256 + threadIdx.x; t < total; t += (long)gridDim.x * 256) {
@@ -811,7 +899,7 @@ Prob make_prob(long M, long N, long K) {
   q.kb_split = q.kblocks;
   q.splits = 1;
   q.units = q.mtiles * q.ntiles;
-  q.group = std::min(q.mtiles, 16);
+  q.group = std::min(q.mtiles, 8);
   q.unscale = -1;
   return q;
 }
@@ -825,38 +913,40 @@ void gemm(eb_engine* e, const Operand& A, const Operand& B, const Operand& C, Ge
     launch_gemm<EPI, CGS, 1>(e, A, B, C, P);
 }
 
-// The 16-bit operand of a matrix: itself where TMA can read it (row stride a
-// multiple of 16 bytes), else a copy in scratch; f32 split into two terms.
-Operand operand(eb_engine* e, const void* x, size_t rows, size_t d, size_t ld, int dtype,
-                uint32_t* max_bits, const char* name) {
-  Operand o{};
-  o.rows = (long)rows;
-  o.cols = (long)d;
-  if (dtype != EB_F32 && ld % 8 == 0) {
-    o.hi = static_cast<const uint16_t*>(x);
-    o.ld = (long)ld;
-    return o;
+// The 16-bit operands of x and w: each itself where TMA can read it (16-bit,
+// row stride a multiple of 16 bytes), else a copy in scratch; f32 split into
+// two terms.
+void operands(eb_engine* e, const LinearCeArgs& a, uint32_t* scal, Operand& X, Operand& W) {
+  const bool split = a.dtype == EB_F32;
+  Prep prep[2] = {};
+  const void* src[2] = {a.x, a.w};
+  const size_t rows[2] = {a.n, a.k}, ld[2] = {a.ldx, a.ldw};
+  Operand* out[2] = {&X, &W};
+  for (int i = 0; i < 2; i++) {
+    Operand& o = *out[i];
+    o = Operand{static_cast<const uint16_t*>(src[i]), nullptr, (long)rows[i], (long)a.d,
+                (long)ld[i]};
+    if (!split && ld[i] % 8 == 0) continue;
+    o.ld = ((long)a.d + 7) / 8 * 8;
+    uint16_t* c = e->scratch_get<uint16_t>(i ? "ce_w" : "ce_x", rows[i] * (size_t)o.ld * (split ? 2 : 1));
+    o.hi = c;
+    if (split) o.lo = c + rows[i] * (size_t)o.ld;
+    prep[i] = Prep{src[i], (long)rows[i], (long)a.d, (long)ld[i], o.ld, c, split ? c + rows[i] * (size_t)o.ld : nullptr,
+                   (unsigned)std::min<size_t>((rows[i] + 7) / 8, PREP_BLOCKS)};
   }
-  const long dp = ((long)d + 7) / 8 * 8;
-  const bool split = dtype == EB_F32;
-  uint16_t* c = e->scratch_get<uint16_t>(name, rows * (size_t)dp * (split ? 2 : 1));
-  o.hi = c;
-  o.lo = split ? c + rows * (size_t)dp : nullptr;
-  o.ld = dp;
-  const unsigned grid =
-      (unsigned)std::min<size_t>((rows * (size_t)dp + 255) / 256, (size_t)e->num_sms * 16);
+  const unsigned grid = prep[0].blocks + prep[1].blocks;
+  if (!grid) return;
   if (split) {
-    launch_pdl(e, k_ce_max, dim3(grid), dim3(256), 0, static_cast<const float*>(x), (long)rows,
-               (long)d, (long)ld, max_bits);
-    launch_pdl(e, k_ce_rows<true>, dim3(grid), dim3(256), 0, x, (long)rows, (long)d, (long)ld, dp,
-               (const uint32_t*)max_bits, c, c + rows * (size_t)dp);
+    uint32_t* maxima = e->scratch_get<uint32_t>("ce_maxima", 2 * PREP_BLOCKS);
+    launch_pdl(e, k_ce_max, dim3(grid), dim3(256), 0, prep[0], prep[1], maxima);
+    launch_pdl(e, k_ce_rows<true>, dim3(grid), dim3(256), 0, prep[0], prep[1],
+               (const uint32_t*)maxima, scal);
     e->stats.kernel_launches += 2;
   } else {
-    launch_pdl(e, k_ce_rows<false>, dim3(grid), dim3(256), 0, x, (long)rows, (long)d, (long)ld, dp,
-               (const uint32_t*)nullptr, c, (uint16_t*)nullptr);
+    launch_pdl(e, k_ce_rows<false>, dim3(grid), dim3(256), 0, prep[0], prep[1],
+               (const uint32_t*)nullptr, (uint32_t*)nullptr);
     e->stats.kernel_launches++;
   }
-  return o;
 }
 
 Operand rows_of(const Operand& o, long r0, long r1) {
@@ -958,9 +1048,8 @@ void products(eb_engine* e, const Operand& A, Operand B, Operand C, GemmParams P
 void linear_ce(eb_engine* e, const LinearCeArgs& a, float* loss, float* lse) {
   if (a.n == 0) return;
   uint32_t* scal = e->scratch_get<uint32_t>("ce_scalars", S_WORDS);
-  if (a.dtype == EB_F32) EB_CUDA(cudaMemsetAsync(scal, 0, S_WORDS * 4, e->stream));
-  const Operand X = operand(e, a.x, a.n, a.d, a.ldx, a.dtype, scal + S_X, "ce_x");
-  const Operand W = operand(e, a.w, a.k, a.d, a.ldw, a.dtype, scal + S_W, "ce_w");
+  Operand X, W;
+  operands(e, a, scal, X, W);
   const int parts = 2 * (int)((a.k + BN - 1) / BN);
   float2* part = e->scratch_get<float2>("ce_part", (size_t)parts * a.n);
   float* zt = e->scratch_get<float>("ce_zt", a.n);
@@ -986,20 +1075,19 @@ void linear_ce_backward(eb_engine* e, const LinearCeArgs& a, const LinearCeGrads
     return;
   }
   uint32_t* scal = e->scratch_get<uint32_t>("ce_scalars", S_WORDS);
-  if (a.dtype == EB_F32 || !g.one_dloss)
-    EB_CUDA(cudaMemsetAsync(scal, 0, S_WORDS * 4, e->stream));
-  const Operand X = operand(e, a.x, a.n, a.d, a.ldx, a.dtype, scal + S_X, "ce_x");
-  const Operand W = operand(e, a.w, a.k, a.d, a.ldw, a.dtype, scal + S_W, "ce_w");
   if (!g.one_dloss) {
+    EB_CUDA(cudaMemsetAsync(scal + S_G, 0, 4, e->stream));
     const unsigned grid = (unsigned)std::min<size_t>((a.n + 255) / 256, (size_t)e->num_sms);
-    launch_pdl(e, k_ce_max, dim3(grid), dim3(256), 0, g.dloss, (long)a.n, 1l, 1l, scal + S_G);
+    launch_pdl(e, k_ce_gmax, dim3(grid), dim3(256), 0, g.dloss, (long)a.n, scal + S_G);
     e->stats.kernel_launches++;
   }
+  Operand X, W;
+  operands(e, a, scal, X, W);
   // Pieces of P, as many elements as the scratch holds: the shorter side of
   // P whole where at least 2,048 of the longer then fit (the sums that run
   // over pieces are the shorter side's gradient), else pieces of both sides.
   const int parts = a.dtype == EB_F32 ? 2 : 1;
-  const size_t room = ((size_t)256 << 20) / 2 / parts;  // elements of P
+  const size_t room = ((size_t)512 << 20) / 2 / parts;  // elements of P
   const size_t npad = (a.n + 255) / 256 * 256, kpad = (a.k + 255) / 256 * 256;
   const size_t side = std::min(std::min(npad, kpad), room / 2048 / 256 * 256);
   const size_t other = std::max<size_t>(room / side / 256 * 256, 256);

@@ -28,6 +28,12 @@ __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// Lets the next kernel on the stream be placed as CTAs of this one leave (its
+// pdl_wait still waits for this one's end): its set-up runs in this one's
+// tail.
+__device__ __forceinline__ void pdl_trigger() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
 // The address of this shared-memory location in CTA `rank` of the cluster.
 __device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank) {
   uint32_t r;

@@ -470,7 +470,7 @@ int eb_linear_ce(eb_engine* e, const eb_buf* x, size_t n, size_t d, size_t ldx, 
  * with P_ij = dloss_i scale (exp(z_ij - lse_i) - [j == targets_i]),
  * dx = P w (n x d) and dw = P^T x (k x d). dloss is f32: n elements, or one
  * for all rows. P is formed a piece of the prototypes (and of the rows, when
- * there are very many) at a time in the engine's scratch (up to 256 MB),
+ * there are very many) at a time in the engine's scratch (up to 512 MB),
  * rounded to x's type (f32: two FP16 terms). dx and dw: x's type or f32;
  * either may be null. Sums are added in a fixed order. */
 int eb_linear_ce_backward(eb_engine* e, const eb_buf* x, size_t n, size_t d, size_t ldx,
