@@ -42,7 +42,7 @@ namespace {
 using tc::pdl_trigger;
 
 constexpr int BM = 128;   // rows of a tile a CTA holds (TMEM lanes)
-constexpr int BN = 256;   // columns of a tile (TMEM columns of one accumulator)
+constexpr int BN = 256;   // most columns of a tile (TMEM columns of one accumulator)
 constexpr int BK = 64;    // k-elements a stage: one 128-byte swizzle row
 constexpr int NTHREADS = 384;  // warp 0 loads, warp 1 issues products, warps 4-11 epilogue
 constexpr int HALF = BN / 2;   // columns an epilogue warp takes
@@ -64,9 +64,10 @@ __device__ __forceinline__ float split_scale(uint32_t bits) {
 }
 
 // One product D = A B^T of a launch, cut into units: tiles of CG * 128 rows by
-// 256 columns, times splits of k.
+// `bn` columns, times splits of k.
 struct Prob {
   long M, N, K;
+  int bn;           // columns of a tile: a multiple of 32, at most BN
   int mtiles, ntiles, kblocks, kb_split, splits, units;
   int group;        // row tiles that pass over the column tiles together
   int a_mn;         // A is K x M (MN-major) rather than M x K
@@ -103,7 +104,7 @@ struct GemmParams {
   float pscale;     // what P is kept times: 1 (bf16) or PSCALE
 };
 
-template <int CG, int PARTS>
+template <int EPI, int CG, int PARTS>
 struct Shape {
   static constexpr int A_ROWS = BM;
   static constexpr int B_ROWS = BN / CG;
@@ -118,7 +119,9 @@ struct Shape {
   // always towards zero): 5.6e-6 of dx at k = 5,003 in one chain of three
   // products a step. Two-term operands, which aim at FP32's own error, end a
   // chain after CHAIN blocks and add it to the epilogue's registers, rounded.
-  static constexpr int CHAIN = PARTS == 2 ? 2 : 1 << 28;
+  // Gradients: 6.7e-7 with chains of two, 1.1e-6 of four (8,192 x 8,192 x
+  // 1024 backward 981 us, 917). Scores bear four (loss 5.5e-7).
+  static constexpr int CHAIN = PARTS == 1 ? 1 << 28 : EPI == OUT ? 2 : 4;
 };
 
 // exp2 of a log2-domain difference (relative error 2^-22; inputs <= 0 but for
@@ -284,7 +287,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
            const __grid_constant__ CUtensorMap b0, const __grid_constant__ CUtensorMap b1,
            const __grid_constant__ CUtensorMap c0, const __grid_constant__ CUtensorMap c1,
            const __grid_constant__ GemmParams P) {
-  using S = Shape<CG, PARTS>;
+  using S = Shape<EPI, CG, PARTS>;
   using namespace tc;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -330,14 +333,16 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       bool stop = false;
       for (int u = first; u < units && !stop; u += step) {
         const Unit q = unit_at<EPI>(P, u);
-        const int am = (q.mt * CG + (int)rank) * BM, bn = q.nt * BN + (int)rank * S::B_ROWS;
+        const int am = (q.mt * CG + (int)rank) * BM, bn = q.nt * P.q[q.prob].bn + (int)rank * (P.q[q.prob].bn / CG);
+        // Boxes of 64 of this CTA's columns (the last may reach past them).
+        const int b_boxes = (P.q[q.prob].bn / CG + 63) / 64;
         for (int kb = q.kb0; kb < q.kb1; kb++, it++) {
           const int s = it % S::STAGES;
           if (!mbar_wait(&empty[s], ((it / S::STAGES) & 1) ^ 1, abort_flag)) {
             stop = true;
             break;
           }
-          if (rank == 0) mbar_expect_tx(&full[s], CG * S::STAGE);
+          if (rank == 0) mbar_expect_tx(&full[s], CG * PARTS * (S::A_BYTES + b_boxes * 8192));
           const uint32_t bar = CG == 2 ? map_rank(smem_u32(&full[s]), 0) : smem_u32(&full[s]);
           uint8_t* st = smem + s * S::STAGE;
           const bool a_mn = EPI == OUT && P.q[q.prob].a_mn;
@@ -353,7 +358,8 @@ __global__ void __launch_bounds__(NTHREADS, 1)
 #pragma unroll
             for (int c = 0; c < S::B_ROWS / 64; c++, st += 8192) {
               const int n = bn + c * 64;
-              tma_load<CG>(st, mb, bar, EPI == OUT ? n : kb * BK, EPI == OUT ? kb * BK : n);
+              if (c < b_boxes)
+                tma_load<CG>(st, mb, bar, EPI == OUT ? n : kb * BK, EPI == OUT ? kb * BK : n);
             }
           }
         }
@@ -376,7 +382,8 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         const Unit q = unit_at<EPI>(P, u);
         const bool a_mn = EPI == OUT && P.q[q.prob].a_mn;
         const uint32_t idesc = (1u << 4) | (P.fmt << 7) | (P.fmt << 10) | ((a_mn ? 1u : 0u) << 15) |
-                               ((EPI == OUT ? 1u : 0u) << 16) | ((uint32_t)(BN >> 3) << 17) |
+                               ((EPI == OUT ? 1u : 0u) << 16) |
+                               ((uint32_t)(P.q[q.prob].bn >> 3) << 17) |
                                ((uint32_t)(CG * BM >> 4) << 24);
         for (int k0 = q.kb0; k0 < q.kb1 && !stop; k0 += S::CHAIN, tc++) {
           const int k1 = min(k0 + S::CHAIN, q.kb1);
@@ -440,8 +447,8 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       const Prob& pr = P.q[q.prob];
       const long i = (long)(q.mt * CG + (int)rank) * BM + r;
       const bool live = i < pr.M;
-      const long c0 = (long)q.nt * BN + hf * HALF;
-      const int cols = (int)min((long)HALF, max(pr.N - c0, 0l));
+      const long c0 = (long)q.nt * pr.bn + hf * HALF;
+      const int cols = (int)min((long)min(HALF, pr.bn - hf * HALF), pr.N - c0);  // may be negative
       float m2 = -INFINITY, sum = 0.0f, zt = 0.0f, lse2 = 0.0f, gr = 0.0f;
       int tcol = -1;  // the target's column among this warp's, if it is one of them
       if constexpr (EPI != OUT) {
@@ -856,7 +863,7 @@ CUtensorMap make_map(const uint16_t* base, const Operand& o) {
 template <int EPI, int CG, int PARTS>
 void launch_gemm(eb_engine* e, const Operand& A, const Operand& B, const Operand& C,
                  const GemmParams& P) {
-  using S = Shape<CG, PARTS>;
+  using S = Shape<EPI, CG, PARTS>;
   const auto kern = k_gemm<EPI, CG, PARTS>;
   static const bool set = [&] {
     EB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::SMEM));
@@ -888,13 +895,21 @@ void launch_gemm(eb_engine* e, const Operand& A, const Operand& B, const Operand
 
 constexpr int CGS = 2;
 
+// Column tiles of a product `n` columns wide: as few as 256 columns allow, all
+// of one width (385 columns: two of 224, a fifth less work than two of 256).
+int tile_width(long n) {
+  const long tiles = (n + BN - 1) / BN;
+  return (int)(((n + tiles - 1) / tiles + 31) / 32 * 32);
+}
+
 Prob make_prob(long M, long N, long K) {
   Prob q{};
+  q.bn = tile_width(N);
   q.M = M;
   q.N = N;
   q.K = K;
   q.mtiles = (int)((M + CGS * BM - 1) / (CGS * BM));
-  q.ntiles = (int)((N + BN - 1) / BN);
+  q.ntiles = (int)((N + q.bn - 1) / q.bn);
   q.kblocks = (int)((K + BK - 1) / BK);
   q.kb_split = q.kblocks;
   q.splits = 1;
@@ -1050,11 +1065,11 @@ void linear_ce(eb_engine* e, const LinearCeArgs& a, float* loss, float* lse) {
   uint32_t* scal = e->scratch_get<uint32_t>("ce_scalars", S_WORDS);
   Operand X, W;
   operands(e, a, scal, X, W);
-  const int parts = 2 * (int)((a.k + BN - 1) / BN);
-  float2* part = e->scratch_get<float2>("ce_part", (size_t)parts * a.n);
-  float* zt = e->scratch_get<float>("ce_zt", a.n);
   GemmParams P = base_params(a, scal);
   P.q[0] = make_prob((long)a.n, (long)a.k, (long)a.d);
+  const int parts = 2 * P.q[0].ntiles;
+  float2* part = e->scratch_get<float2>("ce_part", (size_t)parts * a.n);
+  float* zt = e->scratch_get<float>("ce_zt", a.n);
   P.part = part;
   P.zt = zt;
   gemm<LSE>(e, X, W, W, P);
