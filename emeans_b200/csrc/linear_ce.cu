@@ -195,10 +195,43 @@ __device__ __forceinline__ Unit unit_at(const GemmParams& P, int u) {
   return r;
 }
 
+// A warp's whole 32 x 32 block of a product, times `factor`, to the output or
+// the FP32 sums in 16-byte groups (the common case of store_block).
+template <int BYTES, bool BF16>
+__device__ __forceinline__ void store_whole(float* blk, int lane, uint8_t* out, long ld_bytes,
+                                            float factor) {
+  if constexpr (BYTES == 4) {
+    const int g = lane & 7;
+    out += (lane >> 3) * ld_bytes + g * 16;
+    float4 v[8];
+#pragma unroll
+    for (int t = 0; t < 8; t++) v[t] = block4(blk, (lane >> 3) + t * 4, g);
+#pragma unroll
+    for (int t = 0; t < 8; t++, out += 4 * ld_bytes)
+      *reinterpret_cast<float4*>(out) =
+          make_float4(v[t].x * factor, v[t].y * factor, v[t].z * factor, v[t].w * factor);
+  } else {
+    const int g = (lane & 3) * 2;
+    out += (lane >> 2) * ld_bytes + g * 8;
+    float4 a[4], b[4];
+#pragma unroll
+    for (int t = 0; t < 4; t++) {
+      a[t] = block4(blk, (lane >> 2) + t * 8, g);
+      b[t] = block4(blk, (lane >> 2) + t * 8, g + 1);
+    }
+#pragma unroll
+    for (int t = 0; t < 4; t++, out += 8 * ld_bytes) {
+      const float f[8] = {a[t].x, a[t].y, a[t].z, a[t].w, b[t].x, b[t].y, b[t].z, b[t].w};
+      uint4 none;
+      *reinterpret_cast<uint4*>(out) = pack8<!BF16>(f, factor, none);
+    }
+  }
+}
+
 // A warp's 32 x 32 block of a product, times `factor`, to the FP32 sums (at
 // `sums`, the block's first row) or to the output, in 16-byte groups where
 // the rows allow.
-__device__ __forceinline__ void store_block(const Prob& q, float* sums, float* blk, int lane,
+__device__ __noinline__ void store_block(const Prob& q, float* sums, float* blk, int lane,
                                             long row0, int rows, long col, int cols,
                                             float factor) {
   if (q.write_acc || q.otype == EB_F32) {
@@ -334,15 +367,27 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       for (int u = first; u < units && !stop; u += step) {
         const Unit q = unit_at<EPI>(P, u);
         const int am = (q.mt * CG + (int)rank) * BM, bn = q.nt * P.q[q.prob].bn + (int)rank * (P.q[q.prob].bn / CG);
-        // Boxes of 64 of this CTA's columns (the last may reach past them).
-        const int b_boxes = (P.q[q.prob].bn / CG + 63) / 64;
+        // Boxes of 64 of each CTA's rows and columns; those past the matrix are
+        // left out (what their shared memory holds reaches only rows and
+        // columns that are not stored).
+        const Prob& pr = P.q[q.prob];
+        int a_boxes = 0, b_boxes = 0, all = 0;
+#pragma unroll
+        for (int c = 0; c < CG; c++) {
+          const long m = pr.M - (long)(q.mt * CG + c) * BM;
+          const long n = min((long)(pr.bn / CG), pr.N - (long)q.nt * pr.bn - c * (pr.bn / CG));
+          const int a = (int)min(max(m + 63, 0l) / 64, (long)(S::A_ROWS / 64));
+          const int b = (int)(max(n + 63, 0l) / 64);
+          if (c == (int)rank) a_boxes = a, b_boxes = b;
+          all += a + b;
+        }
         for (int kb = q.kb0; kb < q.kb1; kb++, it++) {
           const int s = it % S::STAGES;
           if (!mbar_wait(&empty[s], ((it / S::STAGES) & 1) ^ 1, abort_flag)) {
             stop = true;
             break;
           }
-          if (rank == 0) mbar_expect_tx(&full[s], CG * PARTS * (S::A_BYTES + b_boxes * 8192));
+          if (rank == 0) mbar_expect_tx(&full[s], PARTS * all * 8192);
           const uint32_t bar = CG == 2 ? map_rank(smem_u32(&full[s]), 0) : smem_u32(&full[s]);
           uint8_t* st = smem + s * S::STAGE;
           const bool a_mn = EPI == OUT && P.q[q.prob].a_mn;
@@ -353,7 +398,8 @@ __global__ void __launch_bounds__(NTHREADS, 1)
 #pragma unroll
             for (int c = 0; c < S::A_ROWS / 64; c++, st += 8192) {
               const int m = am + c * 64;
-              tma_load<CG>(st, ma, bar, a_mn ? m : kb * BK, a_mn ? kb * BK : m);
+              if (c < a_boxes)
+                tma_load<CG>(st, ma, bar, a_mn ? m : kb * BK, a_mn ? kb * BK : m);
             }
 #pragma unroll
             for (int c = 0; c < S::B_ROWS / 64; c++, st += 8192) {
@@ -515,7 +561,10 @@ __global__ void __launch_bounds__(NTHREADS, 1)
 #pragma unroll
           for (int j = 0; j < 32; j++) v[j] = __uint_as_float(raw[j]);
           // The next columns are on their way while these are worked on.
-          if (h + 1 < HALF / 32) tmem_ld32(base + (tc & 1) * BN + (h + 1) * 32, raw);
+          if (h + 1 < HALF / 32)
+            tmem_ld32(base + (tc & 1) * BN + (h + 1) * 32, raw);
+          else
+            release_chain();
         }
         if (EPI != LSE && h * 32 >= cols) continue;
         const int left = cols - h * 32;
@@ -584,12 +633,23 @@ __global__ void __launch_bounds__(NTHREADS, 1)
               }
             }
           } else {
-            store_block(pr, P.q[q.prob].accum + ((long)q.split * pr.M + row0) * pr.ldacc, blk, lane,
-                        row0, rows, col, min(left, 32), factor);
+            float* sums = pr.accum + ((long)q.split * pr.M + row0) * pr.ldacc;
+            if (rows == 32 && left >= 32 && !pr.read_acc && (pr.write_acc || pr.ovec)) {
+              uint8_t* out = static_cast<uint8_t*>(pr.out);
+              if (pr.write_acc)
+                store_whole<4, false>(blk, lane, (uint8_t*)(sums + col), pr.ldacc * 4, factor);
+              else if (pr.otype == EB_F32)
+                store_whole<4, false>(blk, lane, out + (row0 * pr.ldo + col) * 4, pr.ldo * 4, factor);
+              else if (pr.otype == EB_BF16)
+                store_whole<2, true>(blk, lane, out + (row0 * pr.ldo + col) * 2, pr.ldo * 2, factor);
+              else
+                store_whole<2, false>(blk, lane, out + (row0 * pr.ldo + col) * 2, pr.ldo * 2, factor);
+            } else {
+              store_block(pr, sums, blk, lane, row0, rows, col, min(left, 32), factor);
+            }
           }
         }
       }
-      if constexpr (PARTS == 1) release_chain();
       if constexpr (EPI == LSE) {
         if (live) {
           P.part[(long)(q.nt * 2 + hf) * pr.M + i] = make_float2(m2 * sc2, sum);
@@ -893,22 +953,34 @@ void launch_gemm(eb_engine* e, const Operand& A, const Operand& B, const Operand
   e->stats.kernel_launches++;
 }
 
-constexpr int CGS = 2;
+// CTAs that share a tile: pairs hold 256 rows; up to 128 rows one CTA does
+// (a pair's second half would stand idle).
+int ctas(long M) { return M <= BM ? 1 : 2; }
 
-// Column tiles of a product `n` columns wide: as few as 256 columns allow, all
-// of one width (385 columns: two of 224, a fifth less work than two of 256).
-int tile_width(long n) {
-  const long tiles = (n + BN - 1) / BN;
-  return (int)(((n + tiles - 1) / tiles + 31) / 32 * 32);
-}
-
-Prob make_prob(long M, long N, long K) {
+// The product's tiles for `cg` CTAs a tile: columns cut into tiles of one
+// width. By itself as few tiles as 256 columns allow (385 columns: two of 224, a
+// fifth less work than two of 256); with `fill`, the width from 160 up whose
+// rounds of `clusters` tiles take least (65,536 columns of one row tile: 224
+// wide, two full rounds of 148, 36 us against 42).
+Prob make_prob(long M, long N, long K, int cg, int fill_clusters = 0) {
   Prob q{};
-  q.bn = tile_width(N);
   q.M = M;
   q.N = N;
   q.K = K;
-  q.mtiles = (int)((M + CGS * BM - 1) / (CGS * BM));
+  q.mtiles = (int)((M + cg * BM - 1) / (cg * BM));
+  const long few = (N + BN - 1) / BN;
+  q.bn = (int)(((N + few - 1) / few + 31) / 32 * 32);
+  if (fill_clusters && few > 1) {
+    long best = -1;
+    for (int w = BN; w >= 160; w -= 32) {
+      const long tiles = q.mtiles * ((N + w - 1) / w);
+      const long cost = (tiles + fill_clusters - 1) / fill_clusters * (w + 32);
+      if (best < 0 || cost < best) {
+        best = cost;
+        q.bn = w;
+      }
+    }
+  }
   q.ntiles = (int)((N + q.bn - 1) / q.bn);
   q.kblocks = (int)((K + BK - 1) / BK);
   q.kb_split = q.kblocks;
@@ -920,12 +992,20 @@ Prob make_prob(long M, long N, long K) {
 }
 
 template <int EPI>
-void gemm(eb_engine* e, const Operand& A, const Operand& B, const Operand& C, GemmParams P) {
+void gemm(eb_engine* e, const Operand& A, const Operand& B, const Operand& C, int cg,
+          GemmParams P) {
   P.status = e->d_status;
-  if (A.lo)
-    launch_gemm<EPI, CGS, 2>(e, A, B, C, P);
-  else
-    launch_gemm<EPI, CGS, 1>(e, A, B, C, P);
+  if (cg == 1) {
+    if (A.lo)
+      launch_gemm<EPI, 1, 2>(e, A, B, C, P);
+    else
+      launch_gemm<EPI, 1, 1>(e, A, B, C, P);
+  } else {
+    if (A.lo)
+      launch_gemm<EPI, 2, 2>(e, A, B, C, P);
+    else
+      launch_gemm<EPI, 2, 1>(e, A, B, C, P);
+  }
 }
 
 // The 16-bit operands of x and w: each itself where TMA can read it (16-bit,
@@ -1028,8 +1108,9 @@ void choose_splits(Prob* q, int count, int clusters, int parts) {
 
 // One or both of a piece's gradient products in one launch: A = P; B of the
 // first product, C of the second.
-void products(eb_engine* e, const Operand& A, Operand B, Operand C, GemmParams P, int count) {
-  choose_splits(P.q, count, e->num_sms / CGS, A.lo ? 2 : 1);
+void products(eb_engine* e, const Operand& A, Operand B, Operand C, int cg, GemmParams P,
+              int count) {
+  choose_splits(P.q, count, e->num_sms / cg, A.lo ? 2 : 1);
   if (count == 2 && P.q[1].kb_split > P.q[0].kb_split) {
     std::swap(P.q[0], P.q[1]);
     std::swap(B, C);
@@ -1047,7 +1128,7 @@ void products(eb_engine* e, const Operand& A, Operand B, Operand C, GemmParams P
     P.q[i].read_acc = 0;
     P.q[i].write_acc = 1;
   }
-  gemm<OUT>(e, A, B, count == 2 ? C : B, P);
+  gemm<OUT>(e, A, B, count == 2 ? C : B, cg, P);
   for (int i = 0; i < count; i++) {
     if (P.q[i].splits == 1) continue;
     const unsigned grid =
@@ -1066,13 +1147,14 @@ void linear_ce(eb_engine* e, const LinearCeArgs& a, float* loss, float* lse) {
   Operand X, W;
   operands(e, a, scal, X, W);
   GemmParams P = base_params(a, scal);
-  P.q[0] = make_prob((long)a.n, (long)a.k, (long)a.d);
+  const int cg = ctas((long)a.n);
+  P.q[0] = make_prob((long)a.n, (long)a.k, (long)a.d, cg, e->num_sms / cg);
   const int parts = 2 * P.q[0].ntiles;
   float2* part = e->scratch_get<float2>("ce_part", (size_t)parts * a.n);
   float* zt = e->scratch_get<float>("ce_zt", a.n);
   P.part = part;
   P.zt = zt;
-  gemm<LSE>(e, X, W, W, P);
+  gemm<LSE>(e, X, W, W, cg, P);
   const bool few = parts <= 32;
   launch_pdl(e, few ? k_ce_join_few : k_ce_join,
              dim3((unsigned)(few ? (a.n + 127) / 128 : (a.n + 31) / 32)), dim3(few ? 128 : 1024), 0,
@@ -1122,7 +1204,8 @@ void linear_ce_backward(eb_engine* e, const LinearCeArgs& a, const LinearCeGrads
       const Operand Wv = rows_of(W, (long)v0, (long)v1);
       const long pr = (long)(r1 - r0), pc = (long)(v1 - v0);
       GemmParams P = base_params(a, scal);
-      P.q[0] = make_prob(pr, pc, (long)a.d);
+      const int cg = ctas(pr);
+      P.q[0] = make_prob(pr, pc, (long)a.d, cg, e->num_sms / cg);
       P.targets = a.targets + r0;
       P.lse = g.lse + r0;
       P.dloss = g.one_dloss ? g.dloss : g.dloss + r0;
@@ -1131,13 +1214,14 @@ void linear_ce_backward(eb_engine* e, const LinearCeArgs& a, const LinearCeGrads
       P.ldp = (pc + 7) / 8 * 8;
       P.p_hi = p;
       P.p_lo = parts == 2 ? p + rows * cols : nullptr;
-      gemm<PROB>(e, Xr, Wv, Wv, P);
+      gemm<PROB>(e, Xr, Wv, Wv, cg, P);
       const Operand Pm{p, parts == 2 ? p + rows * cols : nullptr, pr, pc, P.ldp};
       int count = 0;
+      const int og = ctas(std::max(g.dx ? pr : 0l, g.dw ? pc : 0l));
       Operand B[2];
       if (g.dx) {
         Prob& q = P.q[count];
-        q = make_prob(pr, (long)a.d, pc);
+        q = make_prob(pr, (long)a.d, pc, og);
         q.unscale = parts == 2 ? S_W : -1;
         q.out = static_cast<char*>(g.dx) + r0 * g.lddx * dtype_bytes(g.dxtype);
         q.otype = g.dxtype;
@@ -1151,7 +1235,7 @@ void linear_ce_backward(eb_engine* e, const LinearCeArgs& a, const LinearCeGrads
       }
       if (g.dw) {
         Prob& q = P.q[count];
-        q = make_prob(pc, (long)a.d, pr);
+        q = make_prob(pc, (long)a.d, pr, og);
         q.a_mn = 1;
         q.unscale = parts == 2 ? S_X : -1;
         q.out = static_cast<char*>(g.dw) + v0 * g.lddw * dtype_bytes(g.dwtype);
@@ -1164,7 +1248,7 @@ void linear_ce_backward(eb_engine* e, const LinearCeArgs& a, const LinearCeGrads
         q.write_acc = r1 < a.n;
         B[count++] = Xr;
       }
-      products(e, Pm, B[0], B[1], P, count);
+      products(e, Pm, B[0], B[1], og, P, count);
     }
   }
 }
