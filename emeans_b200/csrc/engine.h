@@ -421,6 +421,11 @@ struct LinearCeGrads {
   int dwtype;
 };
 void linear_ce_backward(eb_engine* e, const LinearCeArgs& a, const LinearCeGrads& g);
+// linear_ce_small.cu: the same in FP32 on the CUDA cores, for problems whose
+// launches cost more than their products.
+bool linear_ce_is_small(const LinearCeArgs& a);
+void linear_ce_small(eb_engine* e, const LinearCeArgs& a, float* loss, float* lse);
+void linear_ce_small_backward(eb_engine* e, const LinearCeArgs& a, const LinearCeGrads& g);
 
 // ---- adamw.cu: a plan's device tables, and one step over them
 void adamw_create(eb_engine* e, const eb_adamw_tensor* t, size_t count, eb_adamw* plan);

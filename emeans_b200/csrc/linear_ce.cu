@@ -1089,6 +1089,7 @@ void products(eb_engine* e, const Operand& A, Operand B, Operand C, int cg, Gemm
 
 void linear_ce(eb_engine* e, const LinearCeArgs& a, float* loss, float* lse) {
   if (a.n == 0) return;
+  if (linear_ce_is_small(a)) return linear_ce_small(e, a, loss, lse);
   uint32_t* scal = e->scratch_get<uint32_t>("ce_scalars", S_WORDS);
   Operand X, W;
   operands(e, a, scal, X, W);
@@ -1117,6 +1118,7 @@ void linear_ce_backward(eb_engine* e, const LinearCeArgs& a, const LinearCeGrads
                                 a.d * dtype_bytes(g.dwtype), a.k, e->stream));
     return;
   }
+  if (linear_ce_is_small(a)) return linear_ce_small_backward(e, a, g);
   uint32_t* scal = e->scratch_get<uint32_t>("ce_scalars", S_WORDS);
   if (!g.one_dloss) {
     EB_CUDA(cudaMemsetAsync(scal + S_G, 0, 4, e->stream));
