@@ -652,6 +652,31 @@ __global__ void __launch_bounds__(1024)
   finish_row(i, m, s, k, zt, targets, loss, lse, status);
 }
 
+// The same for few rows: a block a row, so that its half tiles are one round of
+// loads (8 rows of 592: 2 us less than 32 rows a block).
+__global__ void __launch_bounds__(256)
+    k_ce_join_row(const float2* __restrict__ part, int parts, long n, long k,
+                  const float* __restrict__ zt, const uint32_t* __restrict__ targets, float* loss,
+                  float* lse, uint32_t* status) {
+  pdl_trigger();
+  pdl_wait();
+  __shared__ float2 acc[8];
+  const long i = blockIdx.x;
+  float m = -INFINITY, s = 0.0f;
+#pragma unroll 4
+  for (int p = threadIdx.x; p < parts; p += 256) fold(m, s, part[(long)p * n + i]);
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const float om = __shfl_xor_sync(0xffffffffu, m, o), os = __shfl_xor_sync(0xffffffffu, s, o);
+    fold(m, s, make_float2(om, os));
+  }
+  if ((threadIdx.x & 31) == 0) acc[threadIdx.x >> 5] = make_float2(m, s);
+  __syncthreads();
+  if (threadIdx.x) return;
+  for (int p = 1; p < 8; p++) fold(m, s, acc[p]);
+  finish_row(i, m, s, k, zt, targets, loss, lse, status);
+}
+
 // The same for few half tiles: one thread a row.
 __global__ void __launch_bounds__(128)
     k_ce_join_few(const float2* __restrict__ part, int parts, long n, long k,
@@ -1102,11 +1127,11 @@ void linear_ce(eb_engine* e, const LinearCeArgs& a, float* loss, float* lse) {
   P.part = part;
   P.zt = zt;
   gemm<LSE>(e, X, W, W, cg, P);
-  const bool few = parts <= 32;
-  launch_pdl(e, few ? k_ce_join_few : k_ce_join,
-             dim3((unsigned)(few ? (a.n + 127) / 128 : (a.n + 31) / 32)), dim3(few ? 128 : 1024), 0,
-             (const float2*)part, parts, (long)a.n, (long)a.k, (const float*)zt, a.targets, loss,
-             lse, e->d_status);
+  const bool few = parts <= 32, row = !few && a.n <= 1024;
+  launch_pdl(e, few ? k_ce_join_few : row ? k_ce_join_row : k_ce_join,
+             dim3((unsigned)(few ? (a.n + 127) / 128 : row ? a.n : (a.n + 31) / 32)),
+             dim3(few ? 128 : row ? 256 : 1024), 0, (const float2*)part, parts, (long)a.n,
+             (long)a.k, (const float*)zt, a.targets, loss, lse, e->d_status);
   e->stats.kernel_launches++;
 }
 

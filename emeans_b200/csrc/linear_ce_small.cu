@@ -4,7 +4,10 @@
 // cores (linear_ce.cu) is its launches: operand preparation, scores, join, P,
 // products, sums. Where the operands would need preparation, one kernel here
 // does the forward pass and one the backward pass (a second adds the blocks'
-// dw). Operands that TMA reads as they lie are no slower there.
+// dw): 1,000 x 32 x 64 f32 forward 5.9 us and backward 11.1 (tensor cores 13.9
+// and 19.0), 60,000 x 64 x 64 23.8 and 63.2 (51.1 and 85.2). With 128
+// prototypes or columns the two are even, and operands that TMA reads as they
+// lie are no slower there (1,000 x 32 x 64 bf16: 7.5 and 12.3).
 //
 // A block of 256 threads holds all prototypes and 16 R rows of x in shared
 // memory; a thread keeps R x 4 scores in registers, and the 16 threads of a
