@@ -46,7 +46,7 @@ constexpr int BN = 256;   // most columns of a tile (TMEM columns of one accumul
 constexpr int BK = 64;    // k-elements a stage: one 128-byte swizzle row
 constexpr int NTHREADS = 384;  // warp 0 loads, warp 1 issues products, warps 4-11 epilogue
 constexpr int HALF = BN / 2;   // columns an epilogue warp takes
-constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr float LOG2E = 1.4426950408889634f;
 constexpr float PSCALE = 16384.0f;  // f16 and f32: P is kept times 2^14
 
 enum Epi { LSE, PROB, OUT };
@@ -90,7 +90,7 @@ struct GemmParams {
   int split;        // operands are f32 in two terms: scores carry both scales
   // LSE
   float2* part;     // [2 ntiles][M]: (max, sum) of a half tile's columns
-  float* zt;        // M: target scores, base 2
+  float* zt;        // M: target scores
   const uint32_t* targets;
   // PROB
   long col0;        // first column of the piece
@@ -104,7 +104,7 @@ struct GemmParams {
   float pscale;     // what P is kept times: 1 (bf16) or PSCALE
 };
 
-template <int EPI, int CG, int PARTS>
+template <int EPI, int CG, int PARTS, bool CHAINED>
 struct Shape {
   static constexpr int A_ROWS = BM;
   static constexpr int B_ROWS = BN / CG;
@@ -117,26 +117,29 @@ struct Shape {
   // k-blocks summed in one TMEM accumulator. The tensor cores' FP32 sums are
   // cut, not rounded, at every step of 16 (about 2^-26 of the sum a product,
   // always towards zero): 5.6e-6 of dx at k = 5,003 in one chain of three
-  // products a step. Two-term operands, which aim at FP32's own error, end a
-  // chain after CHAIN blocks and add it to the epilogue's registers, rounded.
-  // Gradients: 6.7e-7 with chains of two, 1.1e-6 of four (8,192 x 8,192 x
-  // 1024 backward 981 us, 917). Scores bear four (loss 5.5e-7).
-  static constexpr int CHAIN = PARTS == 1 ? 1 << 28 : EPI == OUT ? 2 : 4;
+  // products a step. CHAINED products end a chain after CHAIN blocks and add it
+  // to the epilogue's registers, rounded. Two-term operands, which aim at
+  // FP32's own error, take two: gradients 6e-7 (four: 1.1e-6; 8,192 x 8,192 x
+  // 1024 backward 930 us, 890). Scores of 16-bit rows past 768 columns: eight
+  // (loss 3e-7; unchained 7e-7).
+  static constexpr int CHAIN = !CHAINED ? 1 << 28 : PARTS == 1 ? 8 : 2;
 };
 
-// exp2 of a log2-domain difference (relative error 2^-22; inputs <= 0 but for
-// rounding).
-__device__ __forceinline__ float ex2(float v) {
+// exp of a difference of scores (inputs <= 0 but for rounding; relative error
+// 2^-22 and 2^-24 of the input). Differences are formed in natural units,
+// where the scores' scale needs no rounding (a power of two apart), and only
+// then scaled to base 2.
+__device__ __forceinline__ float ex(float v) {
   float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v * LOG2E));
   return r;
 }
 
-// Folds (m', s') into a running (max, sum of 2^(z - max)); (-inf, 0) is empty.
+// Folds (m', s') into a running (max, sum of exp(z - max)); (-inf, 0) is empty.
 // NaN scores are in the sums, not in the maxima.
 __device__ __forceinline__ void fold(float& m, float& s, float2 v) {
   const float top = fmaxf(m, v.x), off = top == -INFINITY ? 0.0f : top;
-  s = s * ex2(m - off) + v.y * ex2(v.x - off);
+  s = s * ex(m - off) + v.y * ex(v.x - off);
   m = top;
 }
 
@@ -268,14 +271,14 @@ __device__ __forceinline__ void store_block(const Prob& q, float* sums, float* b
 // MN-major one's along its columns, so one tensor map serves either reading.
 // LSE and PROB: A = x, B = w, both K-major. OUT: A = P, K-major for dx
 // (B = w) and MN-major for dw (B = x), B MN-major. With PARTS = 2 each operand
-// is two FP16 terms.
-template <int EPI, int CG, int PARTS>
+// is two FP16 terms; CHAINED, sums are kept in registers between chains.
+template <int EPI, int CG, int PARTS, bool CHAINED>
 __global__ void __launch_bounds__(NTHREADS, 1)
     k_gemm(const __grid_constant__ CUtensorMap a0, const __grid_constant__ CUtensorMap a1,
            const __grid_constant__ CUtensorMap b0, const __grid_constant__ CUtensorMap b1,
            const __grid_constant__ CUtensorMap c0, const __grid_constant__ CUtensorMap c1,
            const __grid_constant__ GemmParams P) {
-  using S = Shape<EPI, CG, PARTS>;
+  using S = Shape<EPI, CG, PARTS, CHAINED>;
   using namespace tc;
   extern __shared__ uint8_t smem_raw[];
   // Aligned by an offset, not by rounding the pointer: the compiler then knows
@@ -318,7 +321,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
   // With the sums in registers, the first warpgroup gives some of its own to
   // the epilogue (128 x 72 + 256 x 216 = 384 x 168).
   if (warp < 4) {
-    if constexpr (PARTS == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if constexpr (CHAINED) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (warp == 0 && lane == 0) {
       int it = 0;
       bool stop = false;
@@ -397,30 +400,47 @@ __global__ void __launch_bounds__(NTHREADS, 1)
             break;
           }
           fence_after();
-          for (int kb = k0; kb < k1; kb++, it++) {
-            const int s = it % S::STAGES;
-            if (!mbar_wait(&full[s], (it / S::STAGES) & 1, abort_flag)) {
-              stop = true;
-              break;
-            }
-            fence_after();
+          // The products of one stage: of the operands' terms a and b.
+          auto multiply = [&](int s, int pa, int pb, uint32_t first) {
             const uint32_t st = smem_u32(smem + s * S::STAGE);
+            const uint32_t a = st + pa * (S::A_BYTES + S::B_BYTES);
+            const uint32_t b = st + pb * (S::A_BYTES + S::B_BYTES) + S::A_BYTES;
 #pragma unroll
-            for (int kk = 0; kk < BK / 16; kk++) {
-              uint64_t da[PARTS], db[PARTS];
+            for (int kk = 0; kk < BK / 16; kk++)
+              mma_f16<CG>(d, a_mn ? desc_mn(a + kk * 2048, 8192) : desc_k(a + kk * 32),
+                          EPI == OUT ? desc_mn(b + kk * 2048, 8192) : desc_k(b + kk * 32), idesc,
+                          kk == 0 ? first : 1u);
+          };
+          // Two-term scores take two stages together, the small products of both
+          // first: sums are then cut at their full size eight times in the two
+          // blocks, not 24. Gradients take a stage at a time (the ring's three
+          // stages are held longer otherwise: 8 % of the time).
+          constexpr int TOGETHER = PARTS == 2 && EPI != OUT ? 2 : 1;
+          for (int kb = k0; kb < k1 && !stop; kb += TOGETHER) {
+            const int n = min(TOGETHER, k1 - kb);
 #pragma unroll
-              for (int p = 0; p < PARTS; p++) {
-                const uint32_t a = st + p * (S::A_BYTES + S::B_BYTES), b = a + S::A_BYTES;
-                da[p] = a_mn ? desc_mn(a + kk * 2048, 8192) : desc_k(a + kk * 32);
-                db[p] = EPI == OUT ? desc_mn(b + kk * 2048, 8192) : desc_k(b + kk * 32);
+            for (int g = 0; g < TOGETHER; g++) {
+              if (g >= n) break;
+              const int s = (it + g) % S::STAGES;
+              if (!mbar_wait(&full[s], ((it + g) / S::STAGES) & 1, abort_flag)) {
+                stop = true;
+                break;
               }
-              mma_f16<CG>(d, da[0], db[0], idesc, (kb > k0 || kk > 0) ? 1u : 0u);
+              fence_after();
               if constexpr (PARTS == 2) {
-                mma_f16<CG>(d, da[0], db[1], idesc, 1u);
-                mma_f16<CG>(d, da[1], db[0], idesc, 1u);
+                multiply(s, 0, 1, (kb > k0 || g > 0) ? 1u : 0u);
+                multiply(s, 1, 0, 1u);
               }
             }
-            mma_commit<CG>(&empty[s]);
+            if (stop) break;
+#pragma unroll
+            for (int g = 0; g < TOGETHER; g++) {
+              if (g >= n) break;
+              const int s = (it + g) % S::STAGES;
+              multiply(s, 0, 0, (PARTS == 2 || kb > k0) ? 1u : 0u);
+              mma_commit<CG>(&empty[s]);
+            }
+            it += n;
           }
           if (!stop) mma_commit<CG>(&tfull[tc & 1]);
         }
@@ -432,15 +452,15 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       }
     }
   } else {
-    if constexpr (PARTS == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    if constexpr (CHAINED) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     // Epilogue: warp w reads TMEM lanes 32 (w % 4) .. + 31, one row a thread,
     // and half (w - 4) / 4 of the tile's columns.
     const int hf = (warp - 4) >> 2;
     const int r = (warp & 3) * 32 + lane;
     float* blk = (float*)(smem + S::STAGES * S::STAGE + 256) + (warp - 4) * 1024;
     const uint32_t base = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(hf * HALF);
-    float sc2 = P.scale * LOG2E, gmax = 0.0f;
-    if (EPI != OUT && P.split) sc2 = sc2 / split_scale(P.scal[S_X]) / split_scale(P.scal[S_W]);
+    float sc = P.scale, gmax = 0.0f;
+    if (EPI != OUT && P.split) sc = sc / split_scale(P.scal[S_X]) / split_scale(P.scal[S_W]);
     if constexpr (EPI != LSE)
       gmax = P.one_dloss ? fabsf(P.dloss[0]) : __uint_as_float(P.scal[S_G]);
     const uint32_t release = CG == 2 ? map_rank(smem_u32(tempty), 0) : smem_u32(tempty);
@@ -453,7 +473,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       const bool live = i < pr.M;
       const long c0 = (long)q.nt * pr.bn + hf * HALF;
       const int cols = (int)min((long)min(HALF, pr.bn - hf * HALF), pr.N - c0);  // may be negative
-      float m2 = -INFINITY, sum = 0.0f, zt = 0.0f, lse2 = 0.0f, gr = 0.0f;
+      float m2 = -INFINITY, sum = 0.0f, zt = 0.0f, lse = 0.0f, gr = 0.0f;
       int tcol = -1;  // the target's column among this warp's, if it is one of them
       if constexpr (EPI != OUT) {
         const uint32_t t = live ? P.targets[i] : EB_IGNORE;
@@ -463,7 +483,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         }
         if constexpr (EPI == PROB) {
           if (live && (long)t < P.k && t != EB_IGNORE) {
-            lse2 = P.lse[i] * LOG2E;
+            lse = P.lse[i];
             const float g = P.dloss[P.one_dloss ? 0 : i];
             gr = gmax > 0.0f ? g / gmax : g;  // g: 0, or NaN
           }
@@ -481,8 +501,8 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         if (lane == 0) mbar_arrive_at(release + (tc & 1) * 8);
         tc++;
       };
-      float acc[PARTS == 2 ? HALF : 1];
-      if constexpr (PARTS == 2) {
+      float acc[CHAINED ? HALF : 1];
+      if constexpr (CHAINED) {
 #pragma unroll
         for (int j = 0; j < HALF; j++) acc[j] = 0.0f;
         for (int k0 = q.kb0; k0 < q.kb1; k0 += S::CHAIN) {
@@ -506,12 +526,12 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         factor = P.scale / P.pscale * gmax;
         if (pr.unscale >= 0) factor /= split_scale(P.scal[pr.unscale]);
       }
-      uint32_t raw[PARTS == 1 ? 32 : 1];
-      if constexpr (PARTS == 1) tmem_ld32(base + (tc & 1) * BN, raw);
+      uint32_t raw[CHAINED ? 1 : 32];
+      if constexpr (!CHAINED) tmem_ld32(base + (tc & 1) * BN, raw);
 #pragma unroll
       for (int h = 0; h < HALF / 32; h++) {
         float v[32];
-        if constexpr (PARTS == 2) {
+        if constexpr (CHAINED) {
 #pragma unroll
           for (int j = 0; j < 32; j++) v[j] = acc[h * 32 + j];
         } else {
@@ -542,17 +562,26 @@ __global__ void __launch_bounds__(NTHREADS, 1)
 #pragma unroll
           for (int j = 3; j < 32; j++) top[j & 3] = fmaxf(top[j & 3], v[j]);
           const float m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-          const float off = m == -INFINITY ? 0.0f : -m * sc2;
-          float part[4] = {sum * ex2(fmaf(m2, sc2, off)), 0.0f, 0.0f, 0.0f};
+          const float off = m == -INFINITY ? 0.0f : -m * sc;
+          float part[4] = {sum * ex(fmaf(m2, sc, off)), 0.0f, 0.0f, 0.0f};
 #pragma unroll
-          for (int j = 0; j < 32; j++) part[j & 3] += ex2(fmaf(v[j], sc2, off));
+          for (int j = 0; j < 32; j++) part[j & 3] += ex(fmaf(v[j], sc, off));
           sum = (part[0] + part[1]) + (part[2] + part[3]);
           m2 = m;
         } else {
+          float less = 0.0f;  // the target's p - 1
           if constexpr (EPI == PROB) {
+            if (tcol >> 5 == h) {
+              // By expm1: near 1, p's own rounding would be all that is left.
+#pragma unroll
+              for (int g = 0; g < 8; g++)
+                block4(blk, lane, g) = make_float4(v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]);
+              const float z = reinterpret_cast<const float*>(&block4(blk, lane, (tcol & 31) >> 2))[tcol & 3];
+              less = expm1f(fmaf(z, sc, -lse));
+            }
             // Columns past the last prototype are never read.
 #pragma unroll
-            for (int j = 0; j < 32; j++) v[j] = ex2(fmaf(v[j], sc2, -lse2)) * gr;
+            for (int j = 0; j < 32; j++) v[j] = ex(fmaf(v[j], sc, -lse)) * gr;
           }
           __syncwarp();
 #pragma unroll
@@ -563,7 +592,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
 #pragma unroll
               for (int g = 0; g < 8; g++) block4(blk, lane, g) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             } else if (tcol >> 5 == h) {
-              reinterpret_cast<float*>(&block4(blk, lane, (tcol & 31) >> 2))[tcol & 3] -= gr;
+              reinterpret_cast<float*>(&block4(blk, lane, (tcol & 31) >> 2))[tcol & 3] = gr * less;
             }
           }
           __syncwarp();
@@ -598,8 +627,8 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       }
       if constexpr (EPI == LSE) {
         if (live) {
-          P.part[(long)(q.nt * 2 + hf) * pr.M + i] = make_float2(m2 * sc2, sum);
-          if (tcol >= 0) P.zt[i] = zt * sc2;
+          P.part[(long)(q.nt * 2 + hf) * pr.M + i] = make_float2(m2 * sc, sum);
+          if (tcol >= 0) P.zt[i] = zt * sc;
         }
       }
     }
@@ -618,14 +647,14 @@ __global__ void __launch_bounds__(NTHREADS, 1)
 __device__ __forceinline__ void finish_row(long i, float m, float s, long k, const float* zt,
                                            const uint32_t* targets, float* loss, float* lse,
                                            uint32_t* status) {
-  const float l2 = m + log2f(s);
-  lse[i] = l2 * LN2;
+  const float l = m + logf(s);
+  lse[i] = l;
   const uint32_t t = targets[i];
   if (t == EB_IGNORE || (long)t >= k) {
     loss[i] = 0.0f;
     if (t != EB_IGNORE) atomicOr(status, ST_BAD_LABEL);
   } else {
-    loss[i] = (l2 - zt[i]) * LN2;
+    loss[i] = l - zt[i];
   }
 }
 
@@ -891,11 +920,11 @@ CUtensorMap make_map(const uint16_t* base, const Operand& o) {
   return m;
 }
 
-template <int EPI, int CG, int PARTS>
+template <int EPI, int CG, int PARTS, bool CHAINED = PARTS == 2>
 void launch_gemm(eb_engine* e, const Operand& A, const Operand& B, const Operand& C,
                  const GemmParams& P) {
-  using S = Shape<EPI, CG, PARTS>;
-  const auto kern = k_gemm<EPI, CG, PARTS>;
+  using S = Shape<EPI, CG, PARTS, CHAINED>;
+  const auto kern = k_gemm<EPI, CG, PARTS, CHAINED>;
   static const bool set = [&] {
     EB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::SMEM));
     return true;
@@ -966,6 +995,15 @@ template <int EPI>
 void gemm(eb_engine* e, const Operand& A, const Operand& B, const Operand& C, int cg,
           GemmParams P) {
   P.status = e->d_status;
+  if constexpr (EPI == LSE) {
+    if (!A.lo && P.q[0].kblocks > 12) {
+      if (cg == 1)
+        launch_gemm<EPI, 1, 1, true>(e, A, B, C, P);
+      else
+        launch_gemm<EPI, 2, 1, true>(e, A, B, C, P);
+      return;
+    }
+  }
   if (cg == 1) {
     if (A.lo)
       launch_gemm<EPI, 1, 2>(e, A, B, C, P);

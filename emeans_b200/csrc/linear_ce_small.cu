@@ -33,7 +33,7 @@ using tc::pdl_trigger;
 constexpr int THREADS = 256;
 constexpr int MOST = 64;           // prototypes, and columns
 constexpr int STRIDE = MOST + 4;   // floats of a shared-memory row
-constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr float LOG2E = 1.4426950408889634f;
 
 struct Small {
   const void* x;
@@ -58,9 +58,10 @@ struct Small {
   float* part;  // blocks x k x d, or null with one block
 };
 
-__device__ __forceinline__ float ex2(float v) {
+// exp of a difference of scores.
+__device__ __forceinline__ float ex(float v) {
   float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v * LOG2E));
   return r;
 }
 
@@ -85,7 +86,7 @@ __device__ __forceinline__ void load_rows(const void* src, long r0, long rows, l
     for (int i = 0; i < EACH; i++) dst[(warp + i * 8) * STRIDE + h * 32 + lane] = v[h][i];
 }
 
-// This thread's scores (base 2): rows R ty .. + R against prototypes tx + 16 c.
+// This thread's scores: rows R ty .. + R against prototypes tx + 16 c.
 template <int R>
 __device__ __forceinline__ void scores(const Small& P, const float* xs, const float* ws, int ty,
                                        int tx, float (&z)[R][4]) {
@@ -108,11 +109,10 @@ __device__ __forceinline__ void scores(const Small& P, const float* xs, const fl
         z[r][c] = fmaf(x[r].w, w.w, fmaf(x[r].z, w.z, fmaf(x[r].y, w.y, fmaf(x[r].x, w.x, z[r][c]))));
     }
   }
-  const float s = P.scale * LOG2E;
 #pragma unroll
   for (int r = 0; r < R; r++)
 #pragma unroll
-    for (int c = 0; c < 4; c++) z[r][c] *= s;
+    for (int c = 0; c < 4; c++) z[r][c] *= P.scale;
 }
 
 template <typename T, int R>
@@ -146,26 +146,26 @@ __global__ void __launch_bounds__(THREADS) k_ce_small(Small P) {
     // The maximum passes over NaN scores; they reach the sum.
     float off = m == -INFINITY ? 0.0f : m;
 #pragma unroll
-    for (int c = 0; c < 4; c++) sum += ex2(z[r][c] - off);
+    for (int c = 0; c < 4; c++) sum += ex(z[r][c] - off);
 #pragma unroll
     for (int o = 1; o < 16; o <<= 1) {
       const float om = __shfl_xor_sync(0xffffffffu, m, o);
       const float os = __shfl_xor_sync(0xffffffffu, sum, o);
       const float top = fmaxf(m, om);
       off = top == -INFINITY ? 0.0f : top;
-      sum = sum * ex2(m - off) + os * ex2(om - off);
+      sum = sum * ex(m - off) + os * ex(om - off);
       m = top;
     }
     __syncwarp();
     const long i = row0 + R * ty + r;
     if (tx == 0 && i < P.n) {
-      const float l2 = m + log2f(sum);
-      P.lse[i] = l2 * LN2;
+      const float l = m + logf(sum);
+      P.lse[i] = l;
       if (t[r] >= (uint32_t)P.k) {
         P.loss[i] = 0.0f;
         if (t[r] != EB_IGNORE) atomicOr(P.status, ST_BAD_LABEL);
       } else {
-        P.loss[i] = (l2 - zt[R * ty + r]) * LN2;
+        P.loss[i] = l - zt[R * ty + r];
       }
     }
   }
@@ -182,14 +182,14 @@ __global__ void __launch_bounds__(THREADS) k_ce_small_grad(Small P) {
   load_rows<T, ROWS>(P.x, row0, P.n, P.ldx, P.d, xs);
   load_rows<T, MOST>(P.w, 0, P.k, P.ldw, P.d, ws);
   uint32_t t[R];
-  float g[R], lse2[R];
+  float g[R], lse[R];
 #pragma unroll
   for (int r = 0; r < R; r++) {
     const long i = row0 + R * ty + r;
     t[r] = i < P.n ? P.targets[i] : EB_IGNORE;
     const bool live = t[r] < (uint32_t)P.k;
     g[r] = live ? P.dloss[P.one_dloss ? 0 : i] * P.scale : 0.0f;
-    lse2[r] = live ? P.lse[i] * LOG2E : 0.0f;
+    lse[r] = live ? P.lse[i] : 0.0f;
   }
   __syncthreads();
   float z[R][4];
@@ -199,8 +199,10 @@ __global__ void __launch_bounds__(THREADS) k_ce_small_grad(Small P) {
 #pragma unroll
     for (int c = 0; c < 4; c++) {
       const int j = tx + 16 * c;
-      float p = ex2(z[r][c] - lse2[r]);
-      if ((uint32_t)j == t[r]) p -= 1.0f;
+      const float e = z[r][c] - lse[r];
+      // The target's p - 1 by expm1: near 1, p's own rounding would be all that
+      // is left.
+      const float p = (uint32_t)j == t[r] ? expm1f(e) : ex(e);
       ps[(R * ty + r) * STRIDE + j] = g[r] != 0.0f && j < P.k ? p * g[r] : 0.0f;
     }
   }
