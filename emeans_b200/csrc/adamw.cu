@@ -14,8 +14,13 @@
 // least the smallest code: rounded to zero it would leave the moment above it
 // divided by eps alone.
 //
-// Bound by HBM: 28 bytes a parameter (f32), or 16 with bf16 gradients, 8-bit
-// states and the bf16 copy.
+// Bound by HBM: 28 bytes a parameter (f32; 120 M parameters in 160 tensors 488
+// us, 6.9 TB/s), or 16 with bf16 gradients, 8-bit states and the bf16 copy (400
+// M 1,214 us, 5.3 TB/s: about 70 instructions a parameter, most of them the
+// IEEE divide and square root and the code conversions, share the bound).
+// Measured and not kept for 8-bit states: longer pieces (4,096 to 32,768
+// elements: 1,490 to 1,660 us, their streams lie further apart), elements in
+// flight through shared memory (1,476), a warp a block of 256 (1,300).
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
 

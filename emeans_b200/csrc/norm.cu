@@ -13,7 +13,11 @@
 // kernel adds the blocks in order (the same bits on every call).
 //
 // Bound by HBM: forward reads x and writes y, backward reads dy and x and
-// writes dx.
+// writes dx. 200,000 x 768 bf16 forward 100 to 105 us (5.9 TB/s), backward
+// 145 (6.4); 131,072 x 1024 bf16 backward 143 (5.6). Rows of odd length keep
+// their 16-byte packs: 200,000 x 767 bf16 141 and 196 us (element by element
+// 191 and 438; packs rounded outwards and trimmed 201 and 335). Rows of up to 16
+// packs share a warp: 200,000 x 64 bf16 13 and 22 us (a warp each: 41 and 55).
 #include <cuda_runtime.h>
 
 #include <cmath>
@@ -53,12 +57,21 @@ struct NormBwd {
 
 constexpr int WARP_BLOCK = 128;  // threads of a block when a group is one warp
 
-// Sum over the group's G threads, in every thread. `slot`: two buffers of
-// G / 32 floats used in turn, so that one barrier per sum is enough.
+// Sum over the group's G threads, in every thread. Groups of a warp's part go
+// by shuffles among their own lanes; wider ones add their warps' sums through
+// `slot`: two buffers used in turn, so that one barrier per sum is enough.
 template <int G>
-__device__ __forceinline__ float group_sum(float v, float (*slot)[G / 32], int& turn) {
+__device__ __forceinline__ uint32_t group_mask() {
+  if constexpr (G >= 32) return 0xffffffffu;
+  return ((1u << (G & 31)) - 1u) << (threadIdx.x & 31 & ~(G - 1));
+}
+template <int G>
+constexpr int group_warps = G > 32 ? G / 32 : 1;
+
+template <int G>
+__device__ __forceinline__ float group_sum(float v, float (*slot)[group_warps<G>], int& turn) {
 #pragma unroll
-  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  for (int o = (G < 32 ? G : 32) / 2; o; o >>= 1) v += __shfl_xor_sync(group_mask<G>(), v, o);
   if constexpr (G > 32) {
     const int warp = threadIdx.x >> 5;
     if ((threadIdx.x & 31) == 0) slot[turn][warp] = v;
@@ -73,11 +86,12 @@ __device__ __forceinline__ float group_sum(float v, float (*slot)[G / 32], int& 
 
 // Two sums at once (one barrier).
 template <int G>
-__device__ __forceinline__ float2 group_sum2(float a, float b, float2 (*slot)[G / 32], int& turn) {
+__device__ __forceinline__ float2 group_sum2(float a, float b, float2 (*slot)[group_warps<G>],
+                                             int& turn) {
 #pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    a += __shfl_xor_sync(0xffffffffu, a, o);
-    b += __shfl_xor_sync(0xffffffffu, b, o);
+  for (int o = (G < 32 ? G : 32) / 2; o; o >>= 1) {
+    a += __shfl_xor_sync(group_mask<G>(), a, o);
+    b += __shfl_xor_sync(group_mask<G>(), b, o);
   }
   if constexpr (G > 32) {
     const int warp = threadIdx.x >> 5;
@@ -94,65 +108,87 @@ __device__ __forceinline__ float2 group_sum2(float a, float b, float2 (*slot)[G 
   return make_float2(a, b);
 }
 
+// How a group's threads hold a row. Its 16-byte aligned middle is cut into
+// packs: pack j of thread t holds the V elements from (j G + t) V of the middle
+// on. EDGES: up to V - 1 elements before the middle and after it are held one
+// by one, element x of thread t being edge t + x G. A group steps through rows
+// whose middles start alike (the number of groups is a multiple of V), so its
+// threads keep the same columns throughout. Without EDGES all rows start and
+// end on 16 bytes, or V is 1 (tensors whose rows are not aligned alike).
+template <typename T, int V_, int NV_, int G_, bool EDGES>
+struct Row {
+  static constexpr int V = V_, NV = NV_, G = G_;
+  static constexpr int NX = EDGES ? (2 * V + G - 1) / G : 0;  // edges a thread
+  static constexpr int THREADS = G > 32 ? G : WARP_BLOCK;
+  using P = Pack<T, V>;
+  int t, head, packs, d;
+  __device__ __forceinline__ Row(long row, long ld, long d_)
+      : t(threadIdx.x % G), head(0), d((int)d_) {
+    if constexpr (EDGES) head = min((int)((V - row * ld % V) % V), d);
+    packs = (d - head) / V;
+  }
+  __device__ __forceinline__ bool live(int j) const { return j * G + t < packs; }  // pack j
+  __device__ __forceinline__ int column(int k) const {  // of element k of the packs
+    return head + ((k / V) * G + t) * V + k % V;
+  }
+  // Column of edge element x, or -1: the first V edges are the head's, then
+  // the tail's.
+  __device__ __forceinline__ int edge(int x) const {
+    const int e = t + x * G;
+    const int c = e < V ? e : head + packs * V + e - V;
+    return (e < V ? e < head : e < 2 * V && c < d) ? c : -1;
+  }
+};
+
 // Rows in flight: each thread copies its own packs of the next rows to shared
 // memory (cp.async, no registers held) and reads them back itself, so no
-// barrier is needed. Pack j of a thread covers elements (j G + t) V ...; what
-// lies past the row's end is left at zero. Elements of less than four bytes
-// (16-bit rows that no 16-byte pack fits) are loaded directly.
+// barrier is needed. Packs of less than four bytes (V = 1 of 16-bit types) are
+// loaded directly. 200,000 x 768 bf16 forward: two stages 105 us, three 107,
+// none 123, the next row in registers 137 (they cost more warps than the row
+// brings).
 constexpr int RING = 2;
 
-template <typename T, int V>
-constexpr bool async_copies = V * sizeof(T) >= 4;
-
-template <typename T, int V, int NV, int G>
+template <typename T, typename R>
 struct Ring {
-  static constexpr int THREADS = G > 32 ? G : WARP_BLOCK;
-  static constexpr bool ASYNC = async_copies<T, V>;
-  using P = Pack<T, V>;
-  static constexpr size_t BYTES = ASYNC ? sizeof(P) * NV * THREADS * RING : 0;
+  static constexpr int V = R::V, NV = R::NV;
+  using P = typename R::P;
+  static constexpr bool ASYNC = sizeof(P) >= 4;
+  static constexpr size_t BYTES = ASYNC ? sizeof(P) * NV * R::THREADS * RING : 0;
   P* slots;  // [RING][NV][THREADS]
   __device__ __forceinline__ Ring(uint8_t* smem) : slots(reinterpret_cast<P*>(smem)) {}
   __device__ __forceinline__ P* at(int stage, int j) {
-    return slots + (stage * NV + j) * THREADS + threadIdx.x;
+    return slots + (stage * NV + j) * R::THREADS + threadIdx.x;
+  }
+  static __device__ __forceinline__ P zero() {
+    P z;
+#pragma unroll
+    for (int u = 0; u < V; u++) z.v[u] = from_f32<T>(0.0f);
+    return z;
   }
   __device__ __forceinline__ void clear() {
     if constexpr (ASYNC) {
 #pragma unroll
-      for (int s = 0; s < RING * NV; s++) {
-        P z;
-#pragma unroll
-        for (int u = 0; u < V; u++) z.v[u] = from_f32<T>(0.0f);
-        slots[s * THREADS + threadIdx.x] = z;
-      }
+      for (int s = 0; s < RING * NV; s++) slots[s * R::THREADS + threadIdx.x] = zero();
     }
   }
-  __device__ __forceinline__ void fetch(int stage, const T* row, int t, int packs) {
+  __device__ __forceinline__ void fetch(int stage, const T* row, const R& r) {
     if constexpr (ASYNC) {
 #pragma unroll
       for (int j = 0; j < NV; j++) {
-        const int c = j * G + t;
-        if (c < packs) {
-          const uint32_t dst = (uint32_t)__cvta_generic_to_shared(at(stage, j));
-          if constexpr (sizeof(P) == 16)
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst),
-                         "l"(reinterpret_cast<const P*>(row) + c)
-                         : "memory");
-          else
-            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst),
-                         "l"(reinterpret_cast<const P*>(row) + c)
-                         : "memory");
-        }
+        if (!r.live(j)) continue;
+        const uint32_t dst = (uint32_t)__cvta_generic_to_shared(at(stage, j));
+        const T* src = row + r.column(j * V);
+        if constexpr (sizeof(P) == 16)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+        else
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
       }
     }
   }
-  // Pack j of the row in `stage` (ASYNC), or of `row` itself.
-  __device__ __forceinline__ P get(int stage, int j, const T* row, int t, int packs) {
+  // Pack j of the row in `stage`, or (not ASYNC) of `row` itself.
+  __device__ __forceinline__ P get(int stage, int j, const T* row, const R& r) {
     if constexpr (ASYNC) return *at(stage, j);
-    P z;
-    const int c = j * G + t;
-#pragma unroll
-    for (int u = 0; u < V; u++) z.v[u] = c < packs ? row[(long)c * V + u] : from_f32<T>(0.0f);
-    return z;
+    return r.live(j) ? *reinterpret_cast<const P*>(row + r.column(j * V)) : zero();
   }
 };
 __device__ __forceinline__ void copies_commit() {
@@ -163,189 +199,220 @@ __device__ __forceinline__ void copies_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(RING - 1) : "memory");
 }
 
-template <typename T, int V, int NV, int G>
+template <typename T, int V, int NV, int G, bool EDGES>
 __global__ void __launch_bounds__(G > 32 ? G : WARP_BLOCK) k_norm_fwd(NormFwd P) {
   pdl_wait();
-  constexpr int EPT = NV * V;
+  using R = Row<T, V, NV, G, EDGES>;
+  constexpr int EPT = NV * V, NX = R::NX;
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ float slot[2][G > 32 ? G / 32 : 1];
+  __shared__ float slot[2][group_warps<G>];
   int turn = 0;
-  const int t = threadIdx.x % G;
-  const int packs = (int)(P.d / V);
   const long groups = (long)gridDim.x * (blockDim.x / G);
   long i = (long)blockIdx.x * (blockDim.x / G) + threadIdx.x / G;
+  const R r(i, P.ldx, P.d);
   const T* x = static_cast<const T*>(P.x);
-  Ring<T, V, NV, G> ring(smem);
+  Ring<T, R> ring(smem);
   ring.clear();
-#pragma unroll
-  for (int s = 0; s < RING; s++) {
-    if (i + s * groups < P.rows) ring.fetch(s, x + (i + s * groups) * P.ldx, t, packs);
+  auto fetch = [&](int stage, long row) {
+    if (row < P.rows) ring.fetch(stage, x + row * P.ldx, r);
     copies_commit();
-  }
-  float w[EPT], b[EPT];
+  };
 #pragma unroll
-  for (int j = 0; j < NV; j++) {
+  for (int s = 0; s < RING; s++) fetch(s, i + s * groups);
+  // Elements 0 .. EPT are the packs', then the edges'.
+  float w[EPT + NX], b[EPT + NX], edge[NX ? NX : 1];
 #pragma unroll
-    for (int u = 0; u < V; u++) {
-      const long c = (long)(j * G + t) * V + u;
-      w[j * V + u] = P.w && c < P.d ? load_any(P.w, P.wtype, c) : 1.0f;
-      b[j * V + u] = P.b && c < P.d ? load_any(P.b, P.wtype, c) : 0.0f;
-    }
+  for (int k = 0; k < EPT + NX; k++) {
+    const int c = k < EPT ? (r.live(k / V) ? r.column(k) : -1) : r.edge(k - EPT);
+    w[k] = P.w && c >= 0 ? load_any(P.w, P.wtype, c) : 1.0f;
+    b[k] = P.b && c >= 0 ? load_any(P.b, P.wtype, c) : 0.0f;
   }
+  auto load_edges = [&](long row) {
+#pragma unroll
+    for (int q = 0; q < NX; q++)
+      edge[q] = row < P.rows && r.edge(q) >= 0 ? to_f32(x[row * P.ldx + r.edge(q)]) : 0.0f;
+  };
+  load_edges(i);
   for (int stage = 0; i < P.rows; i += groups, stage = stage + 1 == RING ? 0 : stage + 1) {
     copies_wait();
-    float v[EPT], s = 0.0f;
+    float v[EPT + NX], s = 0.0f;
 #pragma unroll
     for (int j = 0; j < NV; j++) {
-      const Pack<T, V> raw = ring.get(stage, j, x + i * P.ldx, t, packs);
+      const Pack<T, V> raw = ring.get(stage, j, x + i * P.ldx, r);
 #pragma unroll
       for (int u = 0; u < V; u++) s += v[j * V + u] = to_f32(raw.v[u]);
     }
-    if (i + RING * groups < P.rows) ring.fetch(stage, x + (i + RING * groups) * P.ldx, t, packs);
-    copies_commit();
+#pragma unroll
+    for (int q = 0; q < NX; q++) s += v[EPT + q] = edge[q];
+    fetch(stage, i + RING * groups);
+    load_edges(i + groups);
     const float mean = group_sum<G>(s, slot, turn) * P.inv_d;
     s = 0.0f;
 #pragma unroll
-    for (int k = 0; k < EPT; k++) {
+    for (int k = 0; k < EPT + NX; k++) {
       v[k] -= mean;
-      if ((k / V) * G + t < packs) s = fmaf(v[k], v[k], s);
+      if (k < EPT ? r.live(k / V) : r.edge(k - EPT) >= 0) s = fmaf(v[k], v[k], s);
     }
     const float rstd = 1.0f / sqrtf(group_sum<G>(s, slot, turn) * P.inv_d + P.eps);
     T* out = static_cast<T*>(P.y) + i * P.ldy;
 #pragma unroll
     for (int j = 0; j < NV; j++) {
-      const int c = j * G + t;
-      if (c < packs) {
-        Pack<T, V> o;
+      if (!r.live(j)) continue;
+      Pack<T, V> o;
 #pragma unroll
-        for (int u = 0; u < V; u++)
-          o.v[u] = from_f32<T>(fmaf(v[j * V + u] * rstd, w[j * V + u], b[j * V + u]));
-        reinterpret_cast<Pack<T, V>*>(out)[c] = o;
-      }
+      for (int u = 0; u < V; u++)
+        o.v[u] = from_f32<T>(fmaf(v[j * V + u] * rstd, w[j * V + u], b[j * V + u]));
+      *reinterpret_cast<Pack<T, V>*>(out + r.column(j * V)) = o;
     }
-    if (t == 0) {
+#pragma unroll
+    for (int q = 0; q < NX; q++)
+      if (r.edge(q) >= 0)
+        out[r.edge(q)] = from_f32<T>(fmaf(v[EPT + q] * rstd, w[EPT + q], b[EPT + q]));
+    if (r.t == 0) {
       if (P.mean) P.mean[i] = mean;
       if (P.rstd) P.rstd[i] = rstd;
     }
   }
 }
 
-// Registers hold each thread's own columns of the two sums; w and the rows'
-// elements are read from shared memory where they are needed.
-template <typename T, int V, int NV, int G>
+// Registers hold each thread's own columns of the two sums; w (as this group's
+// threads read it) and the rows' packs come from shared memory.
+template <typename T, int V, int NV, int G, bool EDGES>
 __global__ void __launch_bounds__(G > 32 ? G : WARP_BLOCK) k_norm_bwd(NormBwd P) {
   pdl_wait();
-  constexpr int EPT = NV * V;
-  using R = Ring<T, V, NV, G>;
+  using R = Row<T, V, NV, G, EDGES>;
+  constexpr int EPT = NV * V, NX = R::NX, GROUPS = R::THREADS / G;
+  constexpr int MOST = EPT * G + (EDGES ? 2 * V : 0);  // columns of a row
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ float2 slot[2][G > 32 ? G / 32 : 1];
-  __shared__ __align__(16) float ws[EPT * G];
+  __shared__ float2 slot[2][group_warps<G>];
+  // w of each group, and at the end each column's sums of the block.
+  __shared__ __align__(16) float ws[GROUPS == 1 || GROUPS * EPT * G > 2 * MOST ? GROUPS * EPT * G
+                                                                              : 2 * MOST];
   int turn = 0;
-  const int t = threadIdx.x % G;
-  const int packs = (int)(P.d / V);
-  const long groups = (long)gridDim.x * (blockDim.x / G);
-  long i = (long)blockIdx.x * (blockDim.x / G) + threadIdx.x / G;
+  const int group = threadIdx.x / G;
+  const long groups = (long)gridDim.x * GROUPS;
+  long i = (long)blockIdx.x * GROUPS + group;
+  const R r(i, P.ldx, P.d);
   const T *x = static_cast<const T*>(P.x), *dy = static_cast<const T*>(P.dy);
-  R rx(smem), rg(smem + R::BYTES);
+  Ring<T, R> rx(smem), rg(smem + Ring<T, R>::BYTES);
   rx.clear();
   rg.clear();
   auto fetch = [&](int stage, long row) {
     if (row < P.rows) {
-      rx.fetch(stage, x + row * P.ldx, t, packs);
-      rg.fetch(stage, dy + row * P.lddy, t, packs);
+      rx.fetch(stage, x + row * P.ldx, r);
+      rg.fetch(stage, dy + row * P.lddy, r);
     }
     copies_commit();
   };
 #pragma unroll
   for (int s = 0; s < RING; s++) fetch(s, i + s * groups);
-  for (int c = threadIdx.x; c < EPT * G; c += blockDim.x)
-    ws[c] = P.w && c < P.d ? load_any(P.w, P.wtype, c) : 1.0f;
-  float dw[EPT], db[EPT];
+  float* w = ws + group * EPT * G;
+  // Elements 0 .. EPT are the packs', then the edges'.
+  float dw[EPT + NX], db[EPT + NX], wx[NX ? NX : 1], ex[NX ? NX : 1], eg[NX ? NX : 1];
 #pragma unroll
-  for (int k = 0; k < EPT; k++) dw[k] = db[k] = 0.0f;
-  float mean = 0.0f, rstd = 0.0f;
-  if (i < P.rows) {
-    mean = P.mean[i];
-    rstd = P.rstd[i];
+  for (int k = 0; k < EPT + NX; k++) {
+    const int c = k < EPT ? (r.live(k / V) ? r.column(k) : -1) : r.edge(k - EPT);
+    const float v = P.w && c >= 0 ? load_any(P.w, P.wtype, c) : 1.0f;
+    if (k < EPT)
+      w[((k / V) * G + r.t) * V + k % V] = v;
+    else
+      wx[k - EPT] = v;
+    dw[k] = db[k] = 0.0f;
   }
-  __syncthreads();
-  for (int stage = 0; i < P.rows; i += groups, stage = stage + 1 == RING ? 0 : stage + 1) {
-    const float m = mean, r = rstd;
-    if (i + groups < P.rows) {
-      mean = P.mean[i + groups];
-      rstd = P.rstd[i + groups];
+  float mean = 0.0f, rstd = 0.0f;
+  auto load_edges = [&](long row) {
+#pragma unroll
+    for (int q = 0; q < NX; q++) {
+      const bool is = row < P.rows && r.edge(q) >= 0;
+      ex[q] = is ? to_f32(x[row * P.ldx + r.edge(q)]) : 0.0f;
+      eg[q] = is ? to_f32(dy[row * P.lddy + r.edge(q)]) : 0.0f;
     }
+    if (row < P.rows) {
+      mean = P.mean[row];
+      rstd = P.rstd[row];
+    }
+  };
+  load_edges(i);
+  for (int stage = 0; i < P.rows; i += groups, stage = stage + 1 == RING ? 0 : stage + 1) {
+    const float m = mean, rs = rstd;
+    float xe[NX ? NX : 1], ge[NX ? NX : 1];
+#pragma unroll
+    for (int q = 0; q < NX; q++) {
+      xe[q] = ex[q];
+      ge[q] = eg[q];
+    }
+    load_edges(i + groups);
     copies_wait();
     const T *xi = x + i * P.ldx, *gi = dy + i * P.lddy;
     float s1 = 0.0f, s2 = 0.0f;
+    auto add = [&](int k, float g, float v, float wk) {
+      const float u = (v - m) * rs, h = g * wk;
+      dw[k] = fmaf(g, u, dw[k]);
+      db[k] += g;
+      s1 += h;  // elements outside the row have g = 0
+      s2 = fmaf(h, u, s2);
+    };
 #pragma unroll
     for (int j = 0; j < NV; j++) {
-      const Pack<T, V> xr = rx.get(stage, j, xi, t, packs), gr = rg.get(stage, j, gi, t, packs);
+      const Pack<T, V> xr = rx.get(stage, j, xi, r), gr = rg.get(stage, j, gi, r);
 #pragma unroll
-      for (int q = 0; q < V; q++) {
-        const int k = j * V + q;
-        const float g = to_f32(gr.v[q]), u = (to_f32(xr.v[q]) - m) * r;
-        dw[k] = fmaf(g, u, dw[k]);
-        db[k] += g;
-        const float h = g * ws[(j * G + t) * V + q];
-        s1 += h;  // elements past d have g = 0
-        s2 = fmaf(h, u, s2);
-      }
+      for (int q = 0; q < V; q++)
+        add(j * V + q, to_f32(gr.v[q]), to_f32(xr.v[q]), w[(j * G + r.t) * V + q]);
     }
+#pragma unroll
+    for (int q = 0; q < NX; q++) add(EPT + q, ge[q], xe[q], wx[q]);
     const float2 c = group_sum2<G>(s1, s2, slot, turn);
     const float c1 = c.x * P.inv_d, c2 = c.y * P.inv_d;
     if (P.dx) {
       T* out = static_cast<T*>(P.dx) + i * P.lddx;
+      auto grad = [&](float g, float v, float wk) {
+        return from_f32<T>(rs * (g * wk - c1 - (v - m) * rs * c2));
+      };
 #pragma unroll
       for (int j = 0; j < NV; j++) {
-        const int at = j * G + t;
-        if (at < packs) {
-          const Pack<T, V> xr = rx.get(stage, j, xi, t, packs), gr = rg.get(stage, j, gi, t, packs);
-          Pack<T, V> o;
+        if (!r.live(j)) continue;
+        const Pack<T, V> xr = rx.get(stage, j, xi, r), gr = rg.get(stage, j, gi, r);
+        Pack<T, V> o;
 #pragma unroll
-          for (int q = 0; q < V; q++) {
-            const float h = to_f32(gr.v[q]) * ws[at * V + q], u = (to_f32(xr.v[q]) - m) * r;
-            o.v[q] = from_f32<T>(r * (h - c1 - u * c2));
-          }
-          reinterpret_cast<Pack<T, V>*>(out)[at] = o;
-        }
+        for (int q = 0; q < V; q++)
+          o.v[q] = grad(to_f32(gr.v[q]), to_f32(xr.v[q]), w[(j * G + r.t) * V + q]);
+        *reinterpret_cast<Pack<T, V>*>(out + r.column(j * V)) = o;
       }
+#pragma unroll
+      for (int q = 0; q < NX; q++)
+        if (r.edge(q) >= 0) out[r.edge(q)] = grad(ge[q], xe[q], wx[q]);
     }
     fetch(stage, i + RING * groups);
   }
   if (!P.part_w) return;
-  // The block's groups are added in order, column by column.
-  constexpr int GROUPS = (G > 32 ? G : WARP_BLOCK) / G;
   float* pw = P.part_w + (long)blockIdx.x * P.d;
   float* pb = P.part_b + (long)blockIdx.x * P.d;
   if constexpr (GROUPS == 1) {
 #pragma unroll
-    for (int k = 0; k < EPT; k++) {
-      const long c = (long)((k / V) * G + t) * V + k % V;
-      if (c < P.d) {
-        pw[c] = dw[k];
-        pb[c] = db[k];
-      }
+    for (int k = 0; k < EPT + NX; k++) {
+      const int c = k < EPT ? (r.live(k / V) ? r.column(k) : -1) : r.edge(k - EPT);
+      if (c < 0) continue;
+      pw[c] = dw[k];
+      pb[c] = db[k];
     }
   } else {
-    __shared__ float acc[2][EPT][G];
+    // The block's groups are added in order, column by column.
+    float *aw = ws, *ab = ws + MOST;
     for (int g = 0; g < GROUPS; g++) {
-      if ((int)threadIdx.x / G == g) {
-#pragma unroll
-        for (int k = 0; k < EPT; k++) {
-          acc[0][k][t] = g ? acc[0][k][t] + dw[k] : dw[k];
-          acc[1][k][t] = g ? acc[1][k][t] + db[k] : db[k];
-        }
-      }
       __syncthreads();
-    }
-    for (int q = threadIdx.x; q < EPT * G; q += blockDim.x) {
-      const int k = q / G, tt = q % G;
-      const long c = (long)((k / V) * G + tt) * V + k % V;
-      if (c < P.d) {
-        pw[c] = acc[0][k][tt];
-        pb[c] = acc[1][k][tt];
+      if (group != g) continue;
+#pragma unroll
+      for (int k = 0; k < EPT + NX; k++) {
+        const int c = k < EPT ? (r.live(k / V) ? r.column(k) : -1) : r.edge(k - EPT);
+        if (c < 0) continue;
+        aw[c] = g ? aw[c] + dw[k] : dw[k];
+        ab[c] = g ? ab[c] + db[k] : db[k];
       }
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < P.d; c += R::THREADS) {
+      pw[c] = aw[c];
+      pb[c] = ab[c];
     }
   }
 }
@@ -357,7 +424,7 @@ constexpr int LONG_BLOCK = 512;
 template <typename T>
 __global__ void __launch_bounds__(LONG_BLOCK) k_norm_fwd_long(NormFwd P) {
   pdl_wait();
-  __shared__ float slot[2][LONG_BLOCK / 32];
+  __shared__ float slot[2][group_warps<LONG_BLOCK>];
   int turn = 0;
   for (long i = blockIdx.x; i < P.rows; i += gridDim.x) {
     const T* x = static_cast<const T*>(P.x) + i * P.ldx;
@@ -386,7 +453,7 @@ __global__ void __launch_bounds__(LONG_BLOCK) k_norm_fwd_long(NormFwd P) {
 template <typename T>
 __global__ void __launch_bounds__(LONG_BLOCK) k_norm_bwd_long(NormBwd P) {
   pdl_wait();
-  __shared__ float slot[2][LONG_BLOCK / 32];
+  __shared__ float slot[2][group_warps<LONG_BLOCK>];
   int turn = 0;
   float* pw = P.part_w ? P.part_w + (long)blockIdx.x * P.d : nullptr;
   float* pb = P.part_w ? P.part_b + (long)blockIdx.x * P.d : nullptr;
@@ -455,9 +522,13 @@ int resident_blocks(K kern, int threads, size_t smem = 0) {
   EB_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, threads, smem));
   return per_sm;
 }
-unsigned resident_grid(eb_engine* e, int per_sm, long rows, int groups) {
-  const long need = (rows + groups - 1) / groups;
-  return (unsigned)std::max<long>(1, std::min<long>(need, (long)std::max(per_sm, 1) * e->num_sms));
+// `multiple`: of the number of groups, so that all rows of a group are aligned
+// alike.
+unsigned resident_grid(eb_engine* e, int per_sm, long rows, int groups, int multiple = 1) {
+  const long step = std::max(1, multiple / groups);
+  const long most = std::max<long>((long)std::max(per_sm, 1) * e->num_sms / step * step, step);
+  const long need = ((rows + groups - 1) / groups + step - 1) / step * step;
+  return (unsigned)std::max<long>(step, std::min<long>(need, most));
 }
 
 // One launch each; by_width picks the template arguments.
@@ -465,13 +536,13 @@ template <typename T>
 struct FwdLaunch {
   eb_engine* e;
   const NormFwd& P;
-  template <int V, int NV, int G>
+  template <int V, int NV, int G, bool EDGES>
   void go() {
     constexpr int threads = G > 32 ? G : WARP_BLOCK;
-    const auto kern = k_norm_fwd<T, V, NV, G>;
-    constexpr size_t smem = Ring<T, V, NV, G>::BYTES;
+    const auto kern = k_norm_fwd<T, V, NV, G, EDGES>;
+    constexpr size_t smem = Ring<T, Row<T, V, NV, G, EDGES>>::BYTES;
     static const int per_sm = resident_blocks(kern, threads, smem);
-    const unsigned grid = resident_grid(e, per_sm, P.rows, threads / G);
+    const unsigned grid = resident_grid(e, per_sm, P.rows, threads / G, V);
     launch_pdl(e, kern, dim3(grid), dim3(threads), smem, P);
     e->stats.kernel_launches++;
   }
@@ -490,53 +561,60 @@ struct BwdLaunch {
   NormBwd& P;
   bool sums;
   unsigned grid;
-  template <int V, int NV, int G>
+  template <int V, int NV, int G, bool EDGES>
   void go() {
     constexpr int threads = G > 32 ? G : WARP_BLOCK;
-    const auto kern = k_norm_bwd<T, V, NV, G>;
-    constexpr size_t smem = 2 * Ring<T, V, NV, G>::BYTES;
+    const auto kern = k_norm_bwd<T, V, NV, G, EDGES>;
+    constexpr size_t smem = 2 * Ring<T, Row<T, V, NV, G, EDGES>>::BYTES;
     static const int per_sm = resident_blocks(kern, threads, smem);
-    grid = resident_grid(e, per_sm, P.rows, threads / G);
+    grid = resident_grid(e, per_sm, P.rows, threads / G, V);
     place_partials(e, P, grid, sums);
     launch_pdl(e, kern, dim3(grid), dim3(threads), smem, P);
     e->stats.kernel_launches++;
   }
 };
 
-// Calls f.go<V, NV, G>() for the smallest group and register
-// count that hold a row: one warp up to 1,024 elements, then 128 threads and
-// 512 of WIDE elements each. False when a row does not fit.
-template <typename T, int WIDE, typename F>
-bool by_width(long d, bool packed, F&& f) {
+// Calls f.go<V, NV, G, EDGES>() for the smallest group and register count that hold a
+// row: part of a warp, a warp, 128 threads, 512. `packed`: the tensors' rows
+// are aligned alike. False when a row does not fit (past 8,192 elements).
+template <int V, bool EDGES, typename F>
+bool by_packs(long packs, F& f) {
+  if (packs <= 4) return f.template go<V, 1, 4, EDGES>(), true;
+  if (packs <= 8) return f.template go<V, 1, 8, EDGES>(), true;
+  if (packs <= 16) return f.template go<V, 1, 16, EDGES>(), true;
+  if (packs <= 32) return f.template go<V, 1, 32, EDGES>(), true;
+  if (packs <= 64) return f.template go<V, 2, 32, EDGES>(), true;
+  if (packs <= 96) return f.template go<V, 3, 32, EDGES>(), true;
+  if (packs <= 128) return f.template go<V, 4, 32, EDGES>(), true;
+  if constexpr (V == 4) {
+    if (packs <= 192) return f.template go<V, 6, 32, EDGES>(), true;
+    if (packs <= 256) return f.template go<V, 8, 32, EDGES>(), true;
+  }
+  if (packs <= 128 * (32 / V)) return f.template go<V, 32 / V, 128, EDGES>(), true;
+  if (packs <= 512 * (16 / V)) return f.template go<V, 16 / V, 512, EDGES>(), true;
+  return false;
+}
+template <typename T, typename F>
+bool by_width(long d, long ld, bool packed, F& f) {
   constexpr int V = 16 / sizeof(T);
   if (packed) {
-    const long packs = d / V;
-    if (packs <= 32) return f.template go<V, 1, 32>(), true;
-    if (packs <= 64) return f.template go<V, 2, 32>(), true;
-    if (packs <= 96) return f.template go<V, 3, 32>(), true;
-    if (packs <= 128) return f.template go<V, 4, 32>(), true;
-    if constexpr (V == 4) {
-      if (packs <= 192) return f.template go<V, 6, 32>(), true;
-      if (packs <= 256) return f.template go<V, 8, 32>(), true;
-    }
-    if (packs <= 128 * (32 / V)) return f.template go<V, 32 / V, 128>(), true;
-    if (packs <= 512 * (WIDE / V)) return f.template go<V, WIDE / V, 512>(), true;
-    return false;
+    if (d % V == 0 && ld % V == 0) return by_packs<V, false>(d / V, f);
+    return by_packs<V, true>(d / V, f);
   }
-  if (d <= 32 * 4) return f.template go<1, 4, 32>(), true;
-  if (d <= 32 * 8) return f.template go<1, 8, 32>(), true;
-  if (d <= 32 * 16) return f.template go<1, 16, 32>(), true;
-  if (d <= 32 * 32) return f.template go<1, 32, 32>(), true;
-  if (d <= 128 * 32) return f.template go<1, 32, 128>(), true;
-  if (d <= 512 * WIDE) return f.template go<1, WIDE, 512>(), true;
+  if (d <= 32 * 4) return f.template go<1, 4, 32, false>(), true;
+  if (d <= 32 * 16) return f.template go<1, 16, 32, false>(), true;
+  if (d <= 32 * 32) return f.template go<1, 32, 32, false>(), true;
+  if (d <= 128 * 32) return f.template go<1, 32, 128, false>(), true;
+  if (d <= 512 * 16) return f.template go<1, 16, 512, false>(), true;
   return false;
 }
 
 template <typename T>
 void norm_fwd(eb_engine* e, const NormFwd& P) {
   constexpr int V = 16 / sizeof(T);
-  const bool packed = P.d % V == 0 && P.ldx % V == 0 && P.ldy % V == 0;
-  if (by_width<T, 32>(P.d, packed, FwdLaunch<T>{e, P})) return;
+  const bool packed = P.ldx % V == P.ldy % V;
+  FwdLaunch<T> one{e, P};
+  if (by_width<T>(P.d, P.ldx, packed, one)) return;
   static const int per_sm = resident_blocks(k_norm_fwd_long<T>, LONG_BLOCK);
   const unsigned grid = resident_grid(e, per_sm, P.rows, 1);
   launch_pdl(e, k_norm_fwd_long<T>, dim3(grid), dim3(LONG_BLOCK), 0, P);
@@ -546,10 +624,10 @@ void norm_fwd(eb_engine* e, const NormFwd& P) {
 template <typename T>
 void norm_bwd(eb_engine* e, NormBwd P, void* dw, void* db, int wt, int bt) {
   constexpr int V = 16 / sizeof(T);
-  const bool packed = P.d % V == 0 && P.ldx % V == 0 && P.lddy % V == 0 && P.lddx % V == 0;
+  const bool packed = P.ldx % V == P.lddy % V && P.ldx % V == P.lddx % V;
   const bool sums = dw || db;
   BwdLaunch<T> one{e, P, sums, 0};
-  if (!by_width<T, 16>(P.d, packed, one)) {
+  if (!by_width<T>(P.d, P.ldx, packed, one)) {
     static const int per_sm = resident_blocks(k_norm_bwd_long<T>, LONG_BLOCK);
     one.grid = resident_grid(e, per_sm, P.rows, 1);
     place_partials(e, P, one.grid, sums);

@@ -428,8 +428,7 @@ int eb_internal_scores(eb_engine* e, const float* x, size_t n, size_t d, const u
  * are EB_F32, EB_BF16 and EB_F16; sums, statistics and products are held in
  * 32 bits whatever the type, and outputs are rounded once (to nearest).
  * Matrices are row-major with a row stride of ld elements (>= the row's
- * length; 0: equal to it); elements between rows are neither read nor
- * written. Shapes of zero rows are valid and launch nothing but the zeroing
+ * length; 0: equal to it); elements between rows are not written. Shapes of zero rows are valid and launch nothing but the zeroing
  * of the sums they leave. Outputs must not overlap inputs unless noted. */
 
 /* Layer norm of each of `rows` rows of d elements: y = (x - mean) rstd w + b,
