@@ -5,6 +5,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cstdio>
 #include <memory>
 #include <stdexcept>
@@ -236,6 +237,19 @@ void launch_pdl(eb_engine* e, void (*kern)(KArgs...), dim3 grid, dim3 block, siz
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   cuda_check(cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...), "kernel launch");
+}
+#endif
+
+#ifdef __CUDACC__
+// A kernel's dynamic shared memory limit is an attribute of kernel and device:
+// set on the first launch of `kern` on the engine's device (`done`: one bit a
+// device, the launcher's own).
+template <typename K>
+void allow_smem(eb_engine* e, K kern, size_t bytes, std::atomic<uint64_t>& done) {
+  const uint64_t bit = 1ull << (e->device & 63);
+  if (done.load(std::memory_order_relaxed) & bit) return;
+  EB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+  done.fetch_or(bit, std::memory_order_relaxed);
 }
 #endif
 

@@ -925,11 +925,8 @@ void launch_gemm(eb_engine* e, const Operand& A, const Operand& B, const Operand
                  const GemmParams& P) {
   using S = Shape<EPI, CG, PARTS, CHAINED>;
   const auto kern = k_gemm<EPI, CG, PARTS, CHAINED>;
-  static const bool set = [&] {
-    EB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::SMEM));
-    return true;
-  }();
-  (void)set;
+  static std::atomic<uint64_t> allowed{0};
+  allow_smem(e, kern, S::SMEM, allowed);
   const CUtensorMap a0 = make_map(A.hi, A), a1 = PARTS == 2 ? make_map(A.lo, A) : a0;
   const CUtensorMap b0 = make_map(B.hi, B), b1 = PARTS == 2 ? make_map(B.lo, B) : b0;
   const CUtensorMap c0 = EPI == OUT ? make_map(C.hi, C) : b0;
@@ -1156,21 +1153,27 @@ void linear_ce(eb_engine* e, const LinearCeArgs& a, float* loss, float* lse) {
   uint32_t* scal = e->scratch_get<uint32_t>("ce_scalars", S_WORDS);
   Operand X, W;
   operands(e, a, scal, X, W);
-  GemmParams P = base_params(a, scal);
-  const int cg = ctas((long)a.n);
-  P.q[0] = make_prob((long)a.n, (long)a.k, (long)a.d, cg, e->num_sms / cg);
-  const int parts = 2 * P.q[0].ntiles;
-  float2* part = e->scratch_get<float2>("ce_part", (size_t)parts * a.n);
-  float* zt = e->scratch_get<float>("ce_zt", a.n);
-  P.part = part;
-  P.zt = zt;
-  gemm<LSE>(e, X, W, W, cg, P);
-  const bool few = parts <= 32, row = !few && a.n <= 1024;
-  launch_pdl(e, few ? k_ce_join_few : row ? k_ce_join_row : k_ce_join,
-             dim3((unsigned)(few ? (a.n + 127) / 128 : row ? a.n : (a.n + 31) / 32)),
-             dim3(few ? 128 : row ? 256 : 1024), 0, (const float2*)part, parts, (long)a.n,
-             (long)a.k, (const float*)zt, a.targets, loss, lse, e->d_status);
-  e->stats.kernel_launches++;
+  // Rows a pass: as many as keep the half tiles' (max, sum) to 256 MB.
+  const size_t most = ((size_t)256 << 20) / sizeof(float2) / (2 * (a.k / 160 + 1)) / 256 * 256;
+  const size_t rows = std::max<size_t>(std::min(a.n, most), 256);
+  for (size_t r0 = 0; r0 < a.n; r0 += rows) {
+    const long n = (long)std::min(a.n - r0, rows);
+    GemmParams P = base_params(a, scal);
+    const int cg = ctas(n);
+    P.q[0] = make_prob(n, (long)a.k, (long)a.d, cg, e->num_sms / cg);
+    const int parts = 2 * P.q[0].ntiles;
+    float2* part = e->scratch_get<float2>("ce_part", (size_t)parts * n);
+    P.part = part;
+    P.zt = e->scratch_get<float>("ce_zt", (size_t)n);
+    P.targets = a.targets + r0;
+    gemm<LSE>(e, rows_of(X, (long)r0, (long)r0 + n), W, W, cg, P);
+    const bool few = parts <= 32, row = !few && n <= 1024;
+    launch_pdl(e, few ? k_ce_join_few : row ? k_ce_join_row : k_ce_join,
+               dim3((unsigned)(few ? (n + 127) / 128 : row ? n : (n + 31) / 32)),
+               dim3(few ? 128 : row ? 256 : 1024), 0, (const float2*)part, parts, n, (long)a.k,
+               (const float*)P.zt, P.targets, loss + r0, lse + r0, e->d_status);
+    e->stats.kernel_launches++;
+  }
 }
 
 void linear_ce_backward(eb_engine* e, const LinearCeArgs& a, const LinearCeGrads& g) {

@@ -32,6 +32,7 @@ using tc::pdl_trigger;
 
 constexpr int THREADS = 256;
 constexpr int MOST = 64;           // prototypes, and columns
+constexpr size_t MOST_ROWS = 1 << 19;  // the blocks' partial dw are then at most 256 MB
 constexpr int STRIDE = MOST + 4;   // floats of a shared-memory row
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -329,7 +330,7 @@ void launch(eb_engine* e, const Small& P, int dtype, int r, bool grad) {
 
 bool linear_ce_is_small(const LinearCeArgs& a) {
   const bool prepared = a.dtype == EB_F32 || a.ldx % 8 || a.ldw % 8;
-  return prepared && a.k <= MOST && a.d <= MOST;
+  return prepared && a.k <= MOST && a.d <= MOST && a.n <= MOST_ROWS;
 }
 
 void linear_ce_small(eb_engine* e, const LinearCeArgs& a, float* loss, float* lse) {

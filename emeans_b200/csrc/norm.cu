@@ -517,8 +517,6 @@ __global__ void __launch_bounds__(1024) k_norm_sum(const float* pw, const float*
 template <typename K>
 int resident_blocks(K kern, int threads, size_t smem = 0) {
   int per_sm = 0;
-  if (smem)
-    EB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   EB_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, threads, smem));
   return per_sm;
 }
@@ -541,6 +539,8 @@ struct FwdLaunch {
     constexpr int threads = G > 32 ? G : WARP_BLOCK;
     const auto kern = k_norm_fwd<T, V, NV, G, EDGES>;
     constexpr size_t smem = Ring<T, Row<T, V, NV, G, EDGES>>::BYTES;
+    static std::atomic<uint64_t> allowed{0};
+    if (smem) allow_smem(e, kern, smem, allowed);
     static const int per_sm = resident_blocks(kern, threads, smem);
     const unsigned grid = resident_grid(e, per_sm, P.rows, threads / G, V);
     launch_pdl(e, kern, dim3(grid), dim3(threads), smem, P);
@@ -566,6 +566,8 @@ struct BwdLaunch {
     constexpr int threads = G > 32 ? G : WARP_BLOCK;
     const auto kern = k_norm_bwd<T, V, NV, G, EDGES>;
     constexpr size_t smem = 2 * Ring<T, Row<T, V, NV, G, EDGES>>::BYTES;
+    static std::atomic<uint64_t> allowed{0};
+    if (smem) allow_smem(e, kern, smem, allowed);
     static const int per_sm = resident_blocks(kern, threads, smem);
     grid = resident_grid(e, per_sm, P.rows, threads / G, V);
     place_partials(e, P, grid, sums);

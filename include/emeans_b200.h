@@ -460,7 +460,9 @@ int eb_layer_norm_backward(eb_engine* e, const eb_buf* dy, size_t lddy, const eb
  * target >= k is reported by the next call that waits (EB_INVALID_ARGUMENT)
  * and treated as EB_IGNORE. x and w have one float type; targets u32;
  * loss and lse f32, n each. Products: 16-bit types on the tensor cores as
- * they are; f32 as two scaled FP16 terms each (22 bits), three products. */
+ * they are; f32 as two scaled FP16 terms each (22 bits), three products
+ * (a non-finite element counts as NaN), or in FP32 where k and d are small.
+ * Scratch: f32 operands' copies (as large as x and w), and up to 256 MB. */
 int eb_linear_ce(eb_engine* e, const eb_buf* x, size_t n, size_t d, size_t ldx, const eb_buf* w,
                  size_t k, size_t ldw, const eb_buf* targets, float scale, eb_buf* loss,
                  eb_buf* lse);
@@ -471,7 +473,9 @@ int eb_linear_ce(eb_engine* e, const eb_buf* x, size_t n, size_t d, size_t ldx, 
  * for all rows. P is formed a piece of the prototypes (and of the rows, when
  * there are very many) at a time in the engine's scratch (up to 512 MB),
  * rounded to x's type (f32: two FP16 terms). dx and dw: x's type or f32;
- * either may be null. Sums are added in a fixed order. */
+ * either may be null. Sums are added in a fixed order. A row with EB_IGNORE
+ * has dx = 0 whatever it holds, but dw sums 0 x its elements: a non-finite one
+ * makes its columns of dw NaN, as in the plain formula. */
 int eb_linear_ce_backward(eb_engine* e, const eb_buf* x, size_t n, size_t d, size_t ldx,
                           const eb_buf* w, size_t k, size_t ldw, const eb_buf* targets,
                           float scale, const eb_buf* lse, const eb_buf* dloss, eb_buf* dx,
@@ -497,11 +501,13 @@ typedef struct {
 typedef struct eb_adamw eb_adamw;
 
 /* A plan over `count` tensors: their addresses laid out on the device once.
- * The buffers must outlive it. No buffer may be written by two tensors. */
+ * The buffers must outlive it, and the engine too. No buffer may be written by
+ * two tensors. */
 int eb_adamw_create(eb_engine* e, const eb_adamw_tensor* tensors, size_t count, eb_adamw** out);
 int eb_adamw_destroy(eb_engine* e, eb_adamw* plan);
 
-/* One step over every tensor in one kernel. In f32, each operation rounded
+/* One step over every tensor in one kernel (one for 32-bit and one for 8-bit
+ * states). In f32, each operation rounded
  * by itself: g' = grad_scale g; m = beta1 m + (1 - beta1) g';
  * v = beta2 v + (1 - beta2) (g' g');
  * p = (1 - lr weight_decay) p - lr / (1 - beta1^step) (m / (sqrt(v) c + eps)),
