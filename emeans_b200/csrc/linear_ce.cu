@@ -45,7 +45,6 @@ constexpr int BM = 128;   // rows of a tile a CTA holds (TMEM lanes)
 constexpr int BN = 256;   // most columns of a tile (TMEM columns of one accumulator)
 constexpr int BK = 64;    // k-elements a stage: one 128-byte swizzle row
 constexpr int NTHREADS = 384;  // warp 0 loads, warp 1 issues products, warps 4-11 epilogue
-constexpr int HALF = BN / 2;   // columns an epilogue warp takes
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float PSCALE = 16384.0f;  // f16 and f32: P is kept times 2^14
 
@@ -104,14 +103,16 @@ struct GemmParams {
   float pscale;     // what P is kept times: 1 (bf16) or PSCALE
 };
 
-template <int EPI, int CG, int PARTS, bool CHAINED>
+// CG CTAs a tile, PARTS terms an operand, columns up to WIDTH a tile.
+template <int EPI, int CG, int PARTS, int WIDTH, bool CHAINED>
 struct Shape {
   static constexpr int A_ROWS = BM;
-  static constexpr int B_ROWS = BN / CG;
+  static constexpr int B_ROWS = WIDTH / CG;
+  static constexpr int HALF = WIDTH / 2;  // columns an epilogue warp takes
   static constexpr int A_BYTES = A_ROWS * BK * 2;
   static constexpr int B_BYTES = B_ROWS * BK * 2;
   static constexpr int STAGE = PARTS * (A_BYTES + B_BYTES);
-  static constexpr int STAGES = 196608 / STAGE;
+  static constexpr int STAGES = 196608 / STAGE < 8 ? 196608 / STAGE : 8;
   // Operand ring, barriers, and each epilogue warp's 32 x 32 block.
   static constexpr size_t SMEM = 1024 + (size_t)STAGES * STAGE + 256 + 8 * 4096;
   // k-blocks summed in one TMEM accumulator. The tensor cores' FP32 sums are
@@ -253,15 +254,33 @@ __device__ __forceinline__ void store_block(const Prob& q, float* sums, float* b
     }
   } else if (lane < cols) {
     float* at = sums + col + lane;
-    size_t out = (size_t)(row0 * q.ldo + col + lane);
+    const size_t out = (size_t)(row0 * q.ldo + col + lane);
+    auto value = [&](int r) {
+      return reinterpret_cast<const float*>(&block4(blk, r, lane >> 2))[lane & 3] * factor;
+    };
+    if (q.read_acc) {
 #pragma unroll 4
-    for (int r = 0; r < rows; r++, at += q.ldacc, out += q.ldo) {
-      float v = reinterpret_cast<const float*>(&block4(blk, r, lane >> 2))[lane & 3] * factor;
-      if (q.read_acc) v += *at;
-      if (q.write_acc)
-        *at = v;
-      else
-        store_any(q.out, q.otype, out, v);
+      for (int r = 0; r < rows; r++) {
+        const float v = value(r) + at[r * q.ldacc];
+        if (q.write_acc)
+          at[r * q.ldacc] = v;
+        else
+          store_any(q.out, q.otype, out + r * q.ldo, v);
+      }
+    } else if (q.write_acc) {
+#pragma unroll 8
+      for (int r = 0; r < rows; r++) at[r * q.ldacc] = value(r);
+    } else if (q.otype == EB_F32) {
+#pragma unroll 8
+      for (int r = 0; r < rows; r++) static_cast<float*>(q.out)[out + r * q.ldo] = value(r);
+    } else if (q.otype == EB_BF16) {
+#pragma unroll 8
+      for (int r = 0; r < rows; r++)
+        static_cast<__nv_bfloat16*>(q.out)[out + r * q.ldo] = __float2bfloat16_rn(value(r));
+    } else {
+#pragma unroll 8
+      for (int r = 0; r < rows; r++)
+        static_cast<__half*>(q.out)[out + r * q.ldo] = __float2half_rn(value(r));
     }
   }
 }
@@ -272,13 +291,14 @@ __device__ __forceinline__ void store_block(const Prob& q, float* sums, float* b
 // LSE and PROB: A = x, B = w, both K-major. OUT: A = P, K-major for dx
 // (B = w) and MN-major for dw (B = x), B MN-major. With PARTS = 2 each operand
 // is two FP16 terms; CHAINED, sums are kept in registers between chains.
-template <int EPI, int CG, int PARTS, bool CHAINED>
+template <int EPI, int CG, int PARTS, int WIDTH, bool CHAINED>
 __global__ void __launch_bounds__(NTHREADS, 1)
     k_gemm(const __grid_constant__ CUtensorMap a0, const __grid_constant__ CUtensorMap a1,
            const __grid_constant__ CUtensorMap b0, const __grid_constant__ CUtensorMap b1,
            const __grid_constant__ CUtensorMap c0, const __grid_constant__ CUtensorMap c1,
            const __grid_constant__ GemmParams P) {
-  using S = Shape<EPI, CG, PARTS, CHAINED>;
+  using S = Shape<EPI, CG, PARTS, WIDTH, CHAINED>;
+  constexpr int HALF = S::HALF;
   using namespace tc;
   extern __shared__ uint8_t smem_raw[];
   // Aligned by an offset, not by rounding the pointer: the compiler then knows
@@ -509,6 +529,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
           if (!wait_chain()) break;
 #pragma unroll
           for (int h = 0; h < HALF / 16; h++) {
+            if (h * 16 >= cols) break;
             uint32_t raw[16];
             tmem_ld16(base + (tc & 1) * BN + h * 16, raw);
             ld_wait(raw);
@@ -731,7 +752,7 @@ struct Prep {
   uint16_t* lo;
   unsigned blocks;
 };
-constexpr int PREP_BLOCKS = 512;  // most blocks of a launch for one operand
+constexpr int PREP_BLOCKS = 1024;  // most blocks of a launch for one operand
 
 __device__ __forceinline__ uint32_t finite_bits(float v) {
   const uint32_t b = __float_as_uint(v) & 0x7FFFFFFFu;
@@ -748,38 +769,92 @@ __device__ __forceinline__ uint32_t block_max(uint32_t m) {
   return m;
 }
 
-// Eight columns c .. c + 8 of a row, zeros past d.
-__device__ __forceinline__ void load8(const float* row, long c, long d, bool vec, float (&f)[8]) {
-  if (vec && c + 8 <= d) {
-    const float4 a = *reinterpret_cast<const float4*>(row + c);
-    const float4 b = *reinterpret_cast<const float4*>(row + c + 4);
-    f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+// Eight elements of a matrix from element `at` on, of which the first `live` are
+// wanted (the others come as zeros); `end`: elements the matrix holds. Where
+// `at` is not on 16 bytes, the aligned groups around them are loaded and
+// shifted.
+__device__ __forceinline__ void load8(const float* x, long at, int live, long end, float (&f)[8]) {
+  const int s = (int)(at & 3);
+  if (at - s + 12 <= end) {
+    float v[12];
+#pragma unroll
+    for (int g = 0; g < 3; g++) {
+      if (g == 2 && s == 0) continue;
+      const float4 q = *reinterpret_cast<const float4*>(x + at - s + 4 * g);
+      v[4 * g] = q.x, v[4 * g + 1] = q.y, v[4 * g + 2] = q.z, v[4 * g + 3] = q.w;
+    }
+    if (s == 0) v[8] = v[9] = v[10] = v[11] = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 10; j++) v[j] = s & 2 ? v[j + 2] : v[j];
+#pragma unroll
+    for (int j = 0; j < 8; j++) f[j] = s & 1 ? v[j + 1] : v[j];
+#pragma unroll
+    for (int j = 0; j < 8; j++) f[j] = j < live ? f[j] : 0.0f;
   } else {
 #pragma unroll
-    for (int j = 0; j < 8; j++) f[j] = c + j < d ? row[c + j] : 0.0f;
+    for (int j = 0; j < 8; j++) f[j] = j < live ? x[at + j] : 0.0f;
+  }
+}
+__device__ __forceinline__ uint4 load8(const uint16_t* x, long at, int live, long end) {
+  const int s = (int)(at & 7);
+  uint32_t w[8];
+  if (at - s + 16 <= end) {
+    const uint4* p = reinterpret_cast<const uint4*>(x + at - s);
+    const uint4 a = p[0], b = p[1];
+    w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w, w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
+#pragma unroll
+    for (int j = 0; j < 6; j++) w[j] = s & 4 ? w[j + 2] : w[j];
+#pragma unroll
+    for (int j = 0; j < 5; j++) w[j] = s & 2 ? w[j + 1] : w[j];
+#pragma unroll
+    for (int j = 0; j < 4; j++) w[j] = s & 1 ? __funnelshift_r(w[j], w[j + 1], 16) : w[j];
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const uint32_t lo = 2 * j < live ? x[at + 2 * j] : 0, hi = 2 * j + 1 < live ? x[at + 2 * j + 1] : 0;
+      w[j] = lo | hi << 16;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    if (2 * j >= live)
+      w[j] = 0;
+    else if (2 * j + 1 >= live)
+      w[j] &= 0xFFFFu;
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Calls f(row, column, elements left in the row) for each group of eight
+// columns of the operand's rows, consecutive threads taking consecutive
+// groups whatever the rows' length.
+template <typename F>
+__device__ __forceinline__ void for_groups(const Prep& q, unsigned block, F&& f) {
+  const unsigned groups = (unsigned)(q.dp / 8);
+  const long total = q.rows * groups, step = (long)q.blocks * 256;
+#pragma unroll 2
+  for (long t = (long)block * 256 + threadIdx.x; t < total; t += step) {
+    const long i = total <= 0xFFFFFFFFl ? (long)((unsigned)t / groups) : t / groups;
+    const long c = (t - i * groups) * 8;
+    f(i, c, (int)min(8l, q.d - c));
   }
 }
 
 // Largest magnitude over the finite elements of both operands' rows: one per
-// block (a warp takes a row at a time), at maxima[block].
+// block, at maxima[block].
 __global__ void __launch_bounds__(256) k_ce_max(Prep X, Prep W, uint32_t* maxima) {
   pdl_trigger();
   pdl_wait();
   const bool second = blockIdx.x >= X.blocks;
   const Prep& q = second ? W : X;
-  const unsigned b = blockIdx.x - (second ? X.blocks : 0);
-  const bool vec = q.ld % 4 == 0;
+  const long end = (q.rows - 1) * q.ld + q.d;
   uint32_t m = 0;
-  for (long i = (long)b * 8 + (threadIdx.x >> 5); i < q.rows; i += (long)q.blocks * 8) {
-    const float* row = static_cast<const float*>(q.x) + i * q.ld;
-#pragma unroll 2
-    for (long c = (threadIdx.x & 31) * 8; c < q.d; c += 256) {
-      float f[8];
-      load8(row, c, q.d, vec, f);
+  for_groups(q, blockIdx.x - (second ? X.blocks : 0), [&](long i, long c, int live) {
+    float f[8];
+    load8(static_cast<const float*>(q.x), i * q.ld + c, live, end, f);
 #pragma unroll
-      for (int j = 0; j < 8; j++) m = max(m, finite_bits(f[j]));
-    }
-  }
+    for (int j = 0; j < 8; j++) m = max(m, finite_bits(f[j]));
+  });
   m = block_max(m);
   if (threadIdx.x == 0) maxima[blockIdx.x] = m;
 }
@@ -803,28 +878,21 @@ __global__ void __launch_bounds__(256)
     s = split_scale(m);
     if (b == 0 && threadIdx.x == 0) scal[second ? S_W : S_X] = m;
   }
-  const bool vec = q.ld % 4 == 0;
-  for (long i = (long)b * 8 + (threadIdx.x >> 5); i < q.rows; i += (long)q.blocks * 8) {
-    for (long c = (threadIdx.x & 31) * 8; c < q.dp; c += 256) {
-      uint4 hi, lo;
-      if constexpr (SPLIT) {
-        float f[8];
-        load8(static_cast<const float*>(q.x) + i * q.ld, c, q.d, vec, f);
+  const long end = (q.rows - 1) * q.ld + q.d;
+  for_groups(q, b, [&](long i, long c, int live) {
+    uint4 hi, lo;
+    if constexpr (SPLIT) {
+      float f[8];
+      load8(static_cast<const float*>(q.x), i * q.ld + c, live, end, f);
 #pragma unroll
-        for (int j = 0; j < 8; j++) f[j] = isfinite(f[j]) ? f[j] : NAN;
-        hi = pack8<true, true>(f, s, lo);
-        *reinterpret_cast<uint4*>(q.lo + i * q.dp + c) = lo;
-      } else {
-        const uint16_t* row = static_cast<const uint16_t*>(q.x) + i * q.ld;
-        uint16_t h[8];
-#pragma unroll
-        for (int j = 0; j < 8; j++) h[j] = c + j < q.d ? row[c + j] : (uint16_t)0;
-        hi = make_uint4(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16,
-                        h[4] | (uint32_t)h[5] << 16, h[6] | (uint32_t)h[7] << 16);
-      }
-      *reinterpret_cast<uint4*>(q.hi + i * q.dp + c) = hi;
+      for (int j = 0; j < 8; j++) f[j] = isfinite(f[j]) ? f[j] : NAN;
+      hi = pack8<true, true>(f, s, lo);
+      *reinterpret_cast<uint4*>(q.lo + i * q.dp + c) = lo;
+    } else {
+      hi = load8(static_cast<const uint16_t*>(q.x), i * q.ld + c, live, end);
     }
-  }
+    *reinterpret_cast<uint4*>(q.hi + i * q.dp + c) = hi;
+  });
 }
 
 // Largest magnitude of the rows' loss gradients (finite ones), into a zeroed
@@ -920,11 +988,11 @@ CUtensorMap make_map(const uint16_t* base, const Operand& o) {
   return m;
 }
 
-template <int EPI, int CG, int PARTS, bool CHAINED = PARTS == 2>
+template <int EPI, int CG, int PARTS, int WIDTH, bool CHAINED = PARTS == 2>
 void launch_gemm(eb_engine* e, const Operand& A, const Operand& B, const Operand& C,
                  const GemmParams& P) {
-  using S = Shape<EPI, CG, PARTS, CHAINED>;
-  const auto kern = k_gemm<EPI, CG, PARTS, CHAINED>;
+  using S = Shape<EPI, CG, PARTS, WIDTH, CHAINED>;
+  const auto kern = k_gemm<EPI, CG, PARTS, WIDTH, CHAINED>;
   static std::atomic<uint64_t> allowed{0};
   allow_smem(e, kern, S::SMEM, allowed);
   const CUtensorMap a0 = make_map(A.hi, A), a1 = PARTS == 2 ? make_map(A.lo, A) : a0;
@@ -950,28 +1018,36 @@ void launch_gemm(eb_engine* e, const Operand& A, const Operand& B, const Operand
   e->stats.kernel_launches++;
 }
 
-// CTAs that share a tile: pairs hold 256 rows; up to 128 rows one CTA does
-// (a pair's second half would stand idle).
-int ctas(long M) { return M <= BM ? 1 : 2; }
+// A tile's shape: CTAs that share it (128 rows each) and its most columns.
+enum Tile { PAIR, SINGLE, NARROW };  // 256 x 256, 128 x 256 (f32: 128), 128 x 64
+struct TileCost {
+  int ctas, width;
+  double block_us, tile_us;  // a k-block of 64, and what the last tile adds
+};
+TileCost tile_cost(Tile t, int parts) {
+  if (t == PAIR) return {2, 256, parts == 2 ? 0.84 : 0.28, 3.0};
+  if (t == SINGLE) return {1, parts == 2 ? 128 : 256, parts == 2 ? 0.45 : 0.28, 2.5};
+  return {1, 64, parts == 2 ? 0.3 : 0.15, 1.2};
+}
 
-// The product's tiles for `cg` CTAs a tile: columns cut into tiles of one
-// width. By itself as few tiles as 256 columns allow (385 columns: two of 224, a
-// fifth less work than two of 256); with `fill`, the width from 160 up whose
-// rounds of `clusters` tiles take least (65,536 columns of one row tile: 224
-// wide, two full rounds of 148, 36 us against 42).
-Prob make_prob(long M, long N, long K, int cg, int fill_clusters = 0) {
+// The product in tiles of at most `width` columns, all of one width: as few
+// tiles as that allows (385 columns of 256: two of 224, a fifth less work than
+// two of 256), or with `clusters` the width from 5/8 of the most up whose
+// rounds of that many tiles take least (65,536 columns of one row tile: 224
+// wide, two full rounds of 148).
+Prob make_prob(long M, long N, long K, const TileCost& t, int clusters = 0) {
   Prob q{};
   q.M = M;
   q.N = N;
   q.K = K;
-  q.mtiles = (int)((M + cg * BM - 1) / (cg * BM));
-  const long few = (N + BN - 1) / BN;
+  q.mtiles = (int)((M + t.ctas * BM - 1) / (t.ctas * BM));
+  const long few = (N + t.width - 1) / t.width;
   q.bn = (int)(((N + few - 1) / few + 31) / 32 * 32);
-  if (fill_clusters && few > 1) {
+  if (clusters && few > 1) {
     long best = -1;
-    for (int w = BN; w >= 160; w -= 32) {
+    for (int w = t.width; w >= t.width * 5 / 8; w -= 32) {
       const long tiles = q.mtiles * ((N + w - 1) / w);
-      const long cost = (tiles + fill_clusters - 1) / fill_clusters * (w + 32);
+      const long cost = (tiles + clusters - 1) / clusters * (w + 32);
       if (best < 0 || cost < best) {
         best = cost;
         q.bn = w;
@@ -988,29 +1064,57 @@ Prob make_prob(long M, long N, long K, int cg, int fill_clusters = 0) {
   return q;
 }
 
+// The scores' tiles: by rounds of tiles. A narrow tile spreads a small problem
+// over more SMs and holds more k-blocks in flight (67 x 1,026 x 729 f32: 17 CTAs
+// instead of 5, forward 40 us -> 27); up to 128 rows a pair's second half
+// would stand idle.
+Tile score_tile(eb_engine* e, long M, long N, long K, int parts) {
+  Tile best = PAIR;
+  double least = 1e300;
+  for (Tile t : {PAIR, SINGLE, NARROW}) {
+    if (t == SINGLE && M > BM) continue;
+    const TileCost c = tile_cost(t, parts);
+    const int clusters = e->num_sms / c.ctas;
+    const Prob q = make_prob(M, N, K, c, clusters);
+    const long rounds = (q.units + clusters - 1) / clusters;
+    const double us = (double)rounds * q.kblocks * c.block_us * q.bn / c.width + c.tile_us * rounds;
+    if (us < least) {
+      least = us;
+      best = t;
+    }
+  }
+  return best;
+}
+
 template <int EPI>
-void gemm(eb_engine* e, const Operand& A, const Operand& B, const Operand& C, int cg,
+void gemm(eb_engine* e, const Operand& A, const Operand& B, const Operand& C, Tile t,
           GemmParams P) {
   P.status = e->d_status;
   if constexpr (EPI == LSE) {
     if (!A.lo && P.q[0].kblocks > 12) {
-      if (cg == 1)
-        launch_gemm<EPI, 1, 1, true>(e, A, B, C, P);
+      if (t == NARROW)
+        launch_gemm<EPI, 1, 1, 64, true>(e, A, B, C, P);
+      else if (t == SINGLE)
+        launch_gemm<EPI, 1, 1, 256, true>(e, A, B, C, P);
       else
-        launch_gemm<EPI, 2, 1, true>(e, A, B, C, P);
+        launch_gemm<EPI, 2, 1, 256, true>(e, A, B, C, P);
       return;
     }
   }
-  if (cg == 1) {
-    if (A.lo)
-      launch_gemm<EPI, 1, 2>(e, A, B, C, P);
+  if (A.lo) {
+    if (t == NARROW)
+      launch_gemm<EPI, 1, 2, 64>(e, A, B, C, P);
+    else if (t == SINGLE)
+      launch_gemm<EPI, 1, 2, 128>(e, A, B, C, P);
     else
-      launch_gemm<EPI, 1, 1>(e, A, B, C, P);
+      launch_gemm<EPI, 2, 2, 256>(e, A, B, C, P);
   } else {
-    if (A.lo)
-      launch_gemm<EPI, 2, 2>(e, A, B, C, P);
+    if (t == NARROW)
+      launch_gemm<EPI, 1, 1, 64>(e, A, B, C, P);
+    else if (t == SINGLE)
+      launch_gemm<EPI, 1, 1, 256>(e, A, B, C, P);
     else
-      launch_gemm<EPI, 2, 1>(e, A, B, C, P);
+      launch_gemm<EPI, 2, 1, 256>(e, A, B, C, P);
   }
 }
 
@@ -1033,7 +1137,7 @@ void operands(eb_engine* e, const LinearCeArgs& a, uint32_t* scal, Operand& X, O
     o.hi = c;
     if (split) o.lo = c + rows[i] * (size_t)o.ld;
     prep[i] = Prep{src[i], (long)rows[i], (long)a.d, (long)ld[i], o.ld, c, split ? c + rows[i] * (size_t)o.ld : nullptr,
-                   (unsigned)std::min<size_t>((rows[i] + 7) / 8, PREP_BLOCKS)};
+                   (unsigned)std::min<size_t>((rows[i] * (size_t)(o.ld / 8) + 255) / 256, PREP_BLOCKS)};
   }
   const unsigned grid = prep[0].blocks + prep[1].blocks;
   if (!grid) return;
@@ -1074,10 +1178,8 @@ GemmParams base_params(const LinearCeArgs& a, const uint32_t* scal) {
 // turn, the longer first, so the launch takes a round per `clusters` units, each
 // as long as its first unit. A split product also writes and reads its
 // partial sums again in a launch of its own. Chosen over a few split counts by
-// that estimate, in units of one k-block of one tile (0.28 us, three times
-// that for two-term operands).
-void choose_splits(Prob* q, int count, int clusters, int parts) {
-  const double block_us = 0.28 * (parts == 2 ? 3 : 1);
+// that estimate, which is returned (us).
+double choose_splits(Prob* q, int count, int clusters, const TileCost& t) {
   static const int tries[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32, 48, 64};
   auto len = [](const Prob& p, int s) { return (p.kblocks + s - 1) / s; };
   double best = 1e300;
@@ -1087,7 +1189,7 @@ void choose_splits(Prob* q, int count, int clusters, int parts) {
     for (int s1 : tries) {
       if (s1 > 1 && (count < 2 || len(q[1], s1) < 2)) break;
       const int s[2] = {s0, s1};
-      double rounds_us = 0, extra_us = 0;
+      double extra_us = 0;
       long units[2] = {0, 0}, l[2] = {0, 0};
       for (int i = 0; i < count; i++) {
         l[i] = len(q[i], s[i]);
@@ -1097,9 +1199,13 @@ void choose_splits(Prob* q, int count, int clusters, int parts) {
       const int a = l[0] >= l[1] ? 0 : 1;
       const long ra = (units[a] + clusters - 1) / clusters;
       const long rb = (units[0] + units[1] + clusters - 1) / clusters - ra;
-      rounds_us = block_us * (double)(ra * (l[a] + 3) + rb * (l[1 - a] + 3));
-      if (rounds_us + extra_us < best) {
-        best = rounds_us + extra_us;
+      auto round_us = [&](int i) {  // a narrower tile's blocks take that much less
+        return std::max(l[i] * t.block_us * std::max(q[i].bn, 96) / std::max(t.width, 96),
+                        t.tile_us * q[i].bn / t.width);
+      };
+      const double us = ra * round_us(a) + (rb ? rb * round_us(1 - a) : 0.0) + t.tile_us + extra_us;
+      if (us < best) {
+        best = us;
         pick[0] = s0;
         pick[1] = s1;
       }
@@ -1110,13 +1216,32 @@ void choose_splits(Prob* q, int count, int clusters, int parts) {
     q[i].splits = (q[i].kblocks + q[i].kb_split - 1) / q[i].kb_split;
     q[i].units = q[i].mtiles * q[i].ntiles * q[i].splits;
   }
+  return best;
 }
 
 // One or both of a piece's gradient products in one launch: A = P; B of the
 // first product, C of the second.
-void products(eb_engine* e, const Operand& A, Operand B, Operand C, int cg, GemmParams P,
-              int count) {
-  choose_splits(P.q, count, e->num_sms / cg, A.lo ? 2 : 1);
+void products(eb_engine* e, const Operand& A, Operand B, Operand C, GemmParams P, int count) {
+  Tile tile = PAIR;
+  double least = 1e300;
+  Prob chosen[2] = {};
+  for (Tile t : {PAIR, SINGLE, NARROW}) {
+    if (t == SINGLE && (P.q[0].M > BM || (count == 2 && P.q[1].M > BM))) continue;
+    const TileCost c = tile_cost(t, A.lo ? 2 : 1);
+    Prob q[2] = {P.q[0], P.q[1]};
+    for (int i = 0; i < count; i++) {
+      const Prob m = make_prob(q[i].M, q[i].N, q[i].K, c);
+      q[i].mtiles = m.mtiles, q[i].ntiles = m.ntiles, q[i].bn = m.bn, q[i].group = m.group;
+    }
+    const double us = choose_splits(q, count, e->num_sms / c.ctas, c);
+    if (us < least) {
+      least = us;
+      tile = t;
+      chosen[0] = q[0];
+      chosen[1] = q[1];
+    }
+  }
+  for (int i = 0; i < count; i++) P.q[i] = chosen[i];
   if (count == 2 && P.q[1].kb_split > P.q[0].kb_split) {
     std::swap(P.q[0], P.q[1]);
     std::swap(B, C);
@@ -1134,7 +1259,7 @@ void products(eb_engine* e, const Operand& A, Operand B, Operand C, int cg, Gemm
     P.q[i].read_acc = 0;
     P.q[i].write_acc = 1;
   }
-  gemm<OUT>(e, A, B, count == 2 ? C : B, cg, P);
+  gemm<OUT>(e, A, B, count == 2 ? C : B, tile, P);
   for (int i = 0; i < count; i++) {
     if (P.q[i].splits == 1) continue;
     const unsigned grid =
@@ -1159,14 +1284,16 @@ void linear_ce(eb_engine* e, const LinearCeArgs& a, float* loss, float* lse) {
   for (size_t r0 = 0; r0 < a.n; r0 += rows) {
     const long n = (long)std::min(a.n - r0, rows);
     GemmParams P = base_params(a, scal);
-    const int cg = ctas(n);
-    P.q[0] = make_prob(n, (long)a.k, (long)a.d, cg, e->num_sms / cg);
+    const int terms = a.dtype == EB_F32 ? 2 : 1;
+    const Tile tile = score_tile(e, n, (long)a.k, (long)a.d, terms);
+    const TileCost cost = tile_cost(tile, terms);
+    P.q[0] = make_prob(n, (long)a.k, (long)a.d, cost, e->num_sms / cost.ctas);
     const int parts = 2 * P.q[0].ntiles;
     float2* part = e->scratch_get<float2>("ce_part", (size_t)parts * n);
     P.part = part;
     P.zt = e->scratch_get<float>("ce_zt", (size_t)n);
     P.targets = a.targets + r0;
-    gemm<LSE>(e, rows_of(X, (long)r0, (long)r0 + n), W, W, cg, P);
+    gemm<LSE>(e, rows_of(X, (long)r0, (long)r0 + n), W, W, tile, P);
     const bool few = parts <= 32, row = !few && n <= 1024;
     launch_pdl(e, few ? k_ce_join_few : row ? k_ce_join_row : k_ce_join,
                dim3((unsigned)(few ? (n + 127) / 128 : row ? n : (n + 31) / 32)),
@@ -1218,8 +1345,9 @@ void linear_ce_backward(eb_engine* e, const LinearCeArgs& a, const LinearCeGrads
       const Operand Wv = rows_of(W, (long)v0, (long)v1);
       const long pr = (long)(r1 - r0), pc = (long)(v1 - v0);
       GemmParams P = base_params(a, scal);
-      const int cg = ctas(pr);
-      P.q[0] = make_prob(pr, pc, (long)a.d, cg, e->num_sms / cg);
+      const Tile tile = score_tile(e, pr, pc, (long)a.d, parts);
+      const TileCost cost = tile_cost(tile, parts);
+      P.q[0] = make_prob(pr, pc, (long)a.d, cost, e->num_sms / cost.ctas);
       P.targets = a.targets + r0;
       P.lse = g.lse + r0;
       P.dloss = g.one_dloss ? g.dloss : g.dloss + r0;
@@ -1228,14 +1356,13 @@ void linear_ce_backward(eb_engine* e, const LinearCeArgs& a, const LinearCeGrads
       P.ldp = (pc + 7) / 8 * 8;
       P.p_hi = p;
       P.p_lo = parts == 2 ? p + rows * cols : nullptr;
-      gemm<PROB>(e, Xr, Wv, Wv, cg, P);
+      gemm<PROB>(e, Xr, Wv, Wv, tile, P);
       const Operand Pm{p, parts == 2 ? p + rows * cols : nullptr, pr, pc, P.ldp};
       int count = 0;
-      const int og = ctas(std::max(g.dx ? pr : 0l, g.dw ? pc : 0l));
       Operand B[2];
       if (g.dx) {
         Prob& q = P.q[count];
-        q = make_prob(pr, (long)a.d, pc, og);
+        q = make_prob(pr, (long)a.d, pc, cost);
         q.unscale = parts == 2 ? S_W : -1;
         q.out = static_cast<char*>(g.dx) + r0 * g.lddx * dtype_bytes(g.dxtype);
         q.otype = g.dxtype;
@@ -1249,7 +1376,7 @@ void linear_ce_backward(eb_engine* e, const LinearCeArgs& a, const LinearCeGrads
       }
       if (g.dw) {
         Prob& q = P.q[count];
-        q = make_prob(pc, (long)a.d, pr, og);
+        q = make_prob(pc, (long)a.d, pr, cost);
         q.a_mn = 1;
         q.unscale = parts == 2 ? S_X : -1;
         q.out = static_cast<char*>(g.dw) + v0 * g.lddw * dtype_bytes(g.dwtype);
@@ -1262,7 +1389,7 @@ void linear_ce_backward(eb_engine* e, const LinearCeArgs& a, const LinearCeGrads
         q.write_acc = r1 < a.n;
         B[count++] = Xr;
       }
-      products(e, Pm, B[0], B[1], og, P, count);
+      products(e, Pm, B[0], B[1], P, count);
     }
   }
 }
