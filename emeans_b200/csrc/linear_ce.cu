@@ -486,6 +486,30 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     const uint32_t release = CG == 2 ? map_rank(smem_u32(tempty), 0) : smem_u32(tempty);
     int tc = 0;
     bool stop = false;
+    // A tile's row of this thread. The next tile's is fetched while the current
+    // one is worked on: with few k-blocks a tile, these loads' latency would be
+    // most of its time.
+    struct Row {
+      uint32_t t;
+      float lse, g;
+    };
+    auto row_of = [&](int u) {
+      Row n = {EB_IGNORE, 0.0f, 0.0f};
+      if constexpr (EPI != OUT) {
+        if (u < units) {
+          const long i = (long)(unit_at<EPI>(P, u).mt * CG + (int)rank) * BM + r;
+          if (i < P.q[0].M) {
+            n.t = P.targets[i];
+            if constexpr (EPI == PROB) {
+              n.lse = P.lse[i];
+              n.g = P.dloss[P.one_dloss ? 0 : i];
+            }
+          }
+        }
+      }
+      return n;
+    };
+    Row next = row_of(first);
     for (int u = first; u < units && !stop; u += step) {
       const Unit q = unit_at<EPI>(P, u);
       const Prob& pr = P.q[q.prob];
@@ -496,18 +520,16 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       float m2 = -INFINITY, sum = 0.0f, zt = 0.0f, lse = 0.0f, gr = 0.0f;
       int tcol = -1;  // the target's column among this warp's, if it is one of them
       if constexpr (EPI != OUT) {
-        const uint32_t t = live ? P.targets[i] : EB_IGNORE;
-        if (t != EB_IGNORE) {
-          const long rel = (long)t - (EPI == PROB ? P.col0 : 0l) - c0;
+        const Row row = next;
+        if (row.t != EB_IGNORE) {
+          const long rel = (long)row.t - (EPI == PROB ? P.col0 : 0l) - c0;
           if (rel >= 0 && rel < cols) tcol = (int)rel;
-        }
-        if constexpr (EPI == PROB) {
-          if (live && (long)t < P.k && t != EB_IGNORE) {
-            lse = P.lse[i];
-            const float g = P.dloss[P.one_dloss ? 0 : i];
-            gr = gmax > 0.0f ? g / gmax : g;  // g: 0, or NaN
+          if (EPI == PROB && (long)row.t < P.k) {
+            lse = row.lse;
+            gr = gmax > 0.0f ? row.g / gmax : row.g;  // g: 0, or NaN
           }
         }
+        next = row_of(u + step);
       }
       // Waits for the next chain; then its TMEM columns are this warp's.
       auto wait_chain = [&] {
@@ -908,24 +930,35 @@ __global__ void __launch_bounds__(256) k_ce_gmax(const float* __restrict__ g, lo
   if (threadIdx.x == 0 && m) atomicMax(out, m);
 }
 
-// The outputs of a product that ran in splits of k: the sum over the splits,
-// in order, of the partial products (M x ld each), plus the FP32 sums so far.
+// The outputs of a product that ran in splits of k: the sum of the splits'
+// partial products (M x ld each), plus the FP32 sums so far. A group of four
+// outputs is a thread's; with `slices` as many threads', each taking every
+// slices-th split, joined in order: 105 groups in 74 splits (the gradient of 1 x
+// 420 from 41,524 prototypes) are otherwise one block's, a load at a time.
 __global__ void __launch_bounds__(256)
-    k_ce_reduce(const float* __restrict__ part, int splits, Prob q) {
+    k_ce_reduce(const float* __restrict__ part, int splits, int slices, Prob q) {
+  __shared__ float4 joint[256];
   pdl_trigger();
   pdl_wait();
+  const int each = 256 / slices, lane = threadIdx.x % each, slice = threadIdx.x / each;
   const long groups = q.ldacc / 4, total = q.M * groups;
-  for (long t = (long)blockIdx.x * 256 + threadIdx.x; t < total; t += (long)gridDim.x * 256) {
+  for (long t0 = (long)blockIdx.x * each; t0 < total; t0 += (long)gridDim.x * each) {
+    const long t = t0 + lane;
     float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    auto add = [&](const float4& v) { s = make_float4(s.x + v.x, s.y + v.y, s.z + v.z, s.w + v.w); };
+    if (t < total) {
 #pragma unroll 4
-    for (int p = 0; p < splits; p++) {
-      const float4 v = reinterpret_cast<const float4*>(part)[(long)p * total + t];
-      s = make_float4(s.x + v.x, s.y + v.y, s.z + v.z, s.w + v.w);
+      for (int p = slice; p < splits; p += slices)
+        add(reinterpret_cast<const float4*>(part)[(long)p * total + t]);
     }
-    if (q.read_acc) {
-      const float4 v = reinterpret_cast<const float4*>(q.accum)[t];
-      s = make_float4(s.x + v.x, s.y + v.y, s.z + v.z, s.w + v.w);
+    if (slices > 1) {
+      __syncthreads();
+      joint[threadIdx.x] = s;
+      __syncthreads();
+      for (int j = 1; j < slices && slice == 0; j++) add(joint[j * each + lane]);
     }
+    if (slice || t >= total) continue;
+    if (q.read_acc) add(reinterpret_cast<const float4*>(q.accum)[t]);
     if (q.write_acc) {
       reinterpret_cast<float4*>(q.accum)[t] = s;
     } else {
@@ -1065,14 +1098,13 @@ Prob make_prob(long M, long N, long K, const TileCost& t, int clusters = 0) {
 }
 
 // The scores' tiles: by rounds of tiles. A narrow tile spreads a small problem
-// over more SMs and holds more k-blocks in flight (67 x 1,026 x 729 f32: 17 CTAs
-// instead of 5, forward 40 us -> 27); up to 128 rows a pair's second half
-// would stand idle.
+// over more SMs and holds more k-blocks in flight; where the rows' count of 128
+// is odd a pair's second half would stand idle in the last.
 Tile score_tile(eb_engine* e, long M, long N, long K, int parts) {
   Tile best = PAIR;
   double least = 1e300;
   for (Tile t : {PAIR, SINGLE, NARROW}) {
-    if (t == SINGLE && M > BM) continue;
+    if (t == SINGLE && (M + BM - 1) / BM % 2 == 0) continue;
     const TileCost c = tile_cost(t, parts);
     const int clusters = e->num_sms / c.ctas;
     const Prob q = make_prob(M, N, K, c, clusters);
@@ -1262,10 +1294,11 @@ void products(eb_engine* e, const Operand& A, Operand B, Operand C, GemmParams P
   gemm<OUT>(e, A, B, count == 2 ? C : B, tile, P);
   for (int i = 0; i < count; i++) {
     if (P.q[i].splits == 1) continue;
-    const unsigned grid =
-        (unsigned)std::min<long>((whole[i].M * whole[i].ldacc / 4 + 255) / 256, (long)e->num_sms * 8);
+    const long groups = whole[i].M * whole[i].ldacc / 4;
+    const int slices = P.q[i].splits >= 16 && groups < 64l * e->num_sms ? 16 : 1;
+    const unsigned grid = (unsigned)std::min<long>((groups * slices + 255) / 256, (long)e->num_sms * 8);
     launch_pdl(e, k_ce_reduce, dim3(grid), dim3(256), 0, (const float*)(part + at[i]),
-               P.q[i].splits, whole[i]);
+               P.q[i].splits, slices, whole[i]);
     e->stats.kernel_launches++;
   }
 }
