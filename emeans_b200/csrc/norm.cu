@@ -14,7 +14,8 @@
 //
 // Bound by HBM: forward reads x and writes y, backward reads dy and x and
 // writes dx. 200,000 x 768 bf16 forward 100 to 105 us (5.9 TB/s), backward
-// 145 (6.4); 131,072 x 1024 bf16 backward 143 (5.6). Rows of odd length keep
+// 145 (6.4); 131,072 x 1024 bf16 102 and 143 (5.6). (Forward alone read 105 us on
+// one GPU and 118 on another.) Rows of odd length keep
 // their 16-byte packs: 200,000 x 767 bf16 141 and 196 us (element by element
 // 191 and 438; packs rounded outwards and trimmed 201 and 335). Rows of up to 16
 // packs share a warp: 200,000 x 64 bf16 13 and 22 us (a warp each: 41 and 55).
@@ -576,9 +577,22 @@ struct BwdLaunch {
   }
 };
 
-// Calls f.go<V, NV, G, EDGES>() for the smallest group and register count that hold a
-// row: part of a warp, a warp, 128 threads, 512. `packed`: the tensors' rows
-// are aligned alike. False when a row does not fit (past 8,192 elements).
+// Calls f.go<V, NV, G, EDGES>() for the group that holds a row with the fewest idle
+// packs: part of a warp, one warp, then two to sixteen. More packs a thread
+// mean fewer rows in flight an SM, fewer mean more threads that wait for one
+// another; between them, in us forward and backward:
+//   1,025 to 1,536 elements of 16 bits, two warps of 3 packs against four of 4:
+//     100,000 x 1536 bf16 114 and 174, 204 and 291 (four of 2: 115 and 211);
+//   to 4,096, four warps of 2 or 3 packs against 4 (f32: twice as many):
+//     50,000 x 2496 bf16 87 and 157, 112 and 183; 50,000 x 1537 f32 110 and 160,
+//     133 and 317;
+//   to 6,144, eight warps of 3 (f32: 6) packs: 30,000 x 6144 bf16 122 and 223.
+// With edges, whose threads hold one more element and its place, two warps
+// already from 24 packed elements a thread (f32: 16): 131,072 x 1023 bf16 105 and
+// 180, one warp 129 and 200; 60,000 x 1023 f32 88 and 136, 94 and 155; without
+// edges one warp: 131,072 x 1024 bf16 102 and 143, two 101 and 160. `packed`: the
+// tensors' rows are aligned alike. False when a row does not fit (past 8,192
+// elements).
 template <int V, bool EDGES, typename F>
 bool by_packs(long packs, F& f) {
   if (packs <= 4) return f.template go<V, 1, 4, EDGES>(), true;
@@ -587,12 +601,20 @@ bool by_packs(long packs, F& f) {
   if (packs <= 32) return f.template go<V, 1, 32, EDGES>(), true;
   if (packs <= 64) return f.template go<V, 2, 32, EDGES>(), true;
   if (packs <= 96) return f.template go<V, 3, 32, EDGES>(), true;
-  if (packs <= 128) return f.template go<V, 4, 32, EDGES>(), true;
-  if constexpr (V == 4) {
+  if constexpr (!EDGES || V == 4) {
+    if (packs <= 128) return f.template go<V, 4, 32, EDGES>(), true;
+  }
+  if constexpr (EDGES) {
+    if (packs <= 64 * (16 / V)) return f.template go<V, 16 / V, 64, EDGES>(), true;
+  } else if constexpr (V == 4) {
     if (packs <= 192) return f.template go<V, 6, 32, EDGES>(), true;
     if (packs <= 256) return f.template go<V, 8, 32, EDGES>(), true;
   }
+  if (packs <= 64 * (24 / V)) return f.template go<V, 24 / V, 64, EDGES>(), true;
+  if (packs <= 128 * (16 / V)) return f.template go<V, 16 / V, 128, EDGES>(), true;
+  if (packs <= 128 * (24 / V)) return f.template go<V, 24 / V, 128, EDGES>(), true;
   if (packs <= 128 * (32 / V)) return f.template go<V, 32 / V, 128, EDGES>(), true;
+  if (packs <= 256 * (24 / V)) return f.template go<V, 24 / V, 256, EDGES>(), true;
   if (packs <= 512 * (16 / V)) return f.template go<V, 16 / V, 512, EDGES>(), true;
   return false;
 }

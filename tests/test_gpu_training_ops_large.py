@@ -110,6 +110,16 @@ def test_layer_norm_widths(eng, d, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=NAMES.get)
+@pytest.mark.parametrize("d", [768, 776, 1023, 1025, 1536, 1544, 2049, 3079, 4104, 6144, 6150])
+def test_layer_norm_of_several_warps_a_row(eng, d, dtype):
+    """Both sides of each change of the group that holds a row."""
+    for rows, pad in ((37, 0), (37, 3), (1201, 8)):
+        norm_forward(eng, rows, d, dtype, pad)
+    norm_backward(eng, 37, d, dtype)
+    norm_backward(eng, 1201, d, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=NAMES.get)
 def test_layer_norm_rows_aligned_apart(eng, dtype):
     """Row strides of the tensors that leave their rows aligned differently:
     element by element."""
