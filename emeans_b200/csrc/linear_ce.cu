@@ -62,6 +62,21 @@ __device__ __forceinline__ float split_scale(uint32_t bits) {
   return __uint_as_float((uint32_t)(s + 127) << 23);
 }
 
+// Division of 0 <= n < 2^31 by d >= 1 through a multiplication: q = (n + floor(n m /
+// 2^32)) >> l with l = ceil(log2 d), m = floor(2^32 (2^l - d) / d) + 1 (Granlund and
+// Montgomery, 1994).
+struct Divisor {
+  uint32_t m, l;
+  __host__ static Divisor of(long d) {
+    uint32_t l = 0;
+    while ((1l << l) < d) l++;
+    return {(uint32_t)((((uint64_t)((1l << l) - d)) << 32) / (uint64_t)d + 1), l};
+  }
+  __device__ __forceinline__ int operator()(int n) const {
+    return (int)(((uint32_t)n + __umulhi((uint32_t)n, m)) >> l);
+  }
+};
+
 // One product D = A B^T of a launch, cut into units: tiles of CG * 128 rows by
 // `bn` columns, times splits of k.
 struct Prob {
@@ -69,6 +84,7 @@ struct Prob {
   int bn;           // columns of a tile: a multiple of 32, at most BN
   int mtiles, ntiles, kblocks, kb_split, splits, units;
   int group;        // row tiles that pass over the column tiles together
+  Divisor tiles, whole, rows, last;  // by a split's units, a group's, and its row tiles
   int a_mn;         // A is K x M (MN-major) rather than M x K
   // OUT: v = acc scale max|dloss| / pscale, to `out`, or through FP32 sums
   int unscale;      // scal slot of the second operand's split scale, or -1
@@ -187,13 +203,12 @@ __device__ __forceinline__ Unit unit_at(const GemmParams& P, int u) {
   r.prob = EPI == OUT && u >= P.q[0].units;
   const Prob& q = P.q[r.prob];
   if (r.prob) u -= P.q[0].units;
-  const int tiles = q.mtiles * q.ntiles;
-  r.split = u / tiles;
-  const int t = u % tiles, gn = q.group * q.ntiles;
-  const int g = t / gn, w = t % gn;
+  r.split = q.tiles(u);
+  const int t = u - r.split * q.mtiles * q.ntiles;
+  const int g = q.whole(t), w = t - g * q.group * q.ntiles;
   const int gm = min(q.group, q.mtiles - g * q.group);
-  r.mt = g * q.group + w % gm;
-  r.nt = w / gm;
+  r.nt = gm == q.group ? q.rows(w) : q.last(w);
+  r.mt = g * q.group + w - r.nt * gm;
   r.kb0 = r.split * q.kb_split;
   r.kb1 = min(r.kb0 + q.kb_split, q.kblocks);
   return r;
@@ -493,11 +508,11 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       uint32_t t;
       float lse, g;
     };
-    auto row_of = [&](int u) {
+    auto row_of = [&](int u, const Unit& q) {
       Row n = {EB_IGNORE, 0.0f, 0.0f};
       if constexpr (EPI != OUT) {
         if (u < units) {
-          const long i = (long)(unit_at<EPI>(P, u).mt * CG + (int)rank) * BM + r;
+          const long i = (long)(q.mt * CG + (int)rank) * BM + r;
           if (i < P.q[0].M) {
             n.t = P.targets[i];
             if constexpr (EPI == PROB) {
@@ -509,9 +524,11 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       }
       return n;
     };
-    Row next = row_of(first);
+    Unit after = unit_at<EPI>(P, first);
+    Row next = row_of(first, after);
     for (int u = first; u < units && !stop; u += step) {
-      const Unit q = unit_at<EPI>(P, u);
+      const Unit q = after;
+      after = unit_at<EPI>(P, u + step);  // past the last one: not used
       const Prob& pr = P.q[q.prob];
       const long i = (long)(q.mt * CG + (int)rank) * BM + r;
       const bool live = i < pr.M;
@@ -529,7 +546,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
             gr = gmax > 0.0f ? row.g / gmax : row.g;  // g: 0, or NaN
           }
         }
-        next = row_of(u + step);
+        next = row_of(u + step, after);
       }
       // Waits for the next chain; then its TMEM columns are this warp's.
       auto wait_chain = [&] {
@@ -1122,6 +1139,13 @@ template <int EPI>
 void gemm(eb_engine* e, const Operand& A, const Operand& B, const Operand& C, Tile t,
           GemmParams P) {
   P.status = e->d_status;
+  for (Prob& q : P.q) {
+    if (!q.units) continue;
+    q.tiles = Divisor::of((long)q.mtiles * q.ntiles);
+    q.whole = Divisor::of((long)q.group * q.ntiles);
+    q.rows = Divisor::of(q.group);
+    q.last = Divisor::of(std::max(q.mtiles % q.group, 1));
+  }
   if constexpr (EPI == LSE) {
     if (!A.lo && P.q[0].kblocks > 12) {
       if (t == NARROW)
