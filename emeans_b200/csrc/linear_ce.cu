@@ -357,7 +357,8 @@ __global__ void __launch_bounds__(NTHREADS, 1)
   // the epilogue (128 x 72 + 256 x 216 = 384 x 168).
   if (warp < 4) {
     if constexpr (CHAINED) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-    if (warp == 0 && lane == 0) {
+    if (warp == 0) {
+      const bool one = elect_one();
       int it = 0;
       bool stop = false;
       for (int u = first; u < units && !stop; u += step) {
@@ -379,10 +380,11 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         }
         for (int kb = q.kb0; kb < q.kb1; kb++, it++) {
           const int s = it % S::STAGES;
-          if (!mbar_wait(&empty[s], ((it / S::STAGES) & 1) ^ 1, abort_flag)) {
+          if (!warp_wait(&empty[s], ((it / S::STAGES) & 1) ^ 1, abort_flag)) {
             stop = true;
             break;
           }
+          if (!one) continue;
           if (rank == 0) mbar_expect_tx(&full[s], PARTS * all * 8192);
           const uint32_t bar = CG == 2 ? map_rank(smem_u32(&full[s]), 0) : smem_u32(&full[s]);
           uint8_t* st = smem + s * S::STAGE;
@@ -417,7 +419,8 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         }
       }
     }
-    if (warp == 1 && lane == 0 && rank == 0) {
+    if (warp == 1 && rank == 0) {
+      const bool one = elect_one();
       int it = 0, tc = 0;  // tc counts chains
       bool stop = false;
       for (int u = first; u < units && !stop; u += step) {
@@ -430,7 +433,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         for (int k0 = q.kb0; k0 < q.kb1 && !stop; k0 += S::CHAIN, tc++) {
           const int k1 = min(k0 + S::CHAIN, q.kb1);
           const uint32_t d = tmem + (tc & 1) * BN;
-          if (!mbar_wait(&tempty[tc & 1], ((tc >> 1) & 1) ^ 1, abort_flag)) {
+          if (!warp_wait(&tempty[tc & 1], ((tc >> 1) & 1) ^ 1, abort_flag)) {
             stop = true;
             break;
           }
@@ -457,14 +460,16 @@ __global__ void __launch_bounds__(NTHREADS, 1)
             for (int g = 0; g < TOGETHER; g++) {
               if (g >= n) break;
               const int s = (it + g) % S::STAGES;
-              if (!mbar_wait(&full[s], ((it + g) / S::STAGES) & 1, abort_flag)) {
+              if (!warp_wait(&full[s], ((it + g) / S::STAGES) & 1, abort_flag)) {
                 stop = true;
                 break;
               }
               fence_after();
               if constexpr (PARTS == 2) {
-                multiply(s, 0, 1, (kb > k0 || g > 0) ? 1u : 0u);
-                multiply(s, 1, 0, 1u);
+                if (one) {
+                  multiply(s, 0, 1, (kb > k0 || g > 0) ? 1u : 0u);
+                  multiply(s, 1, 0, 1u);
+                }
               }
             }
             if (stop) break;
@@ -472,16 +477,18 @@ __global__ void __launch_bounds__(NTHREADS, 1)
             for (int g = 0; g < TOGETHER; g++) {
               if (g >= n) break;
               const int s = (it + g) % S::STAGES;
-              multiply(s, 0, 0, (PARTS == 2 || kb > k0) ? 1u : 0u);
-              mma_commit<CG>(&empty[s]);
+              if (one) {
+                multiply(s, 0, 0, (PARTS == 2 || kb > k0) ? 1u : 0u);
+                mma_commit<CG>(&empty[s]);
+              }
             }
             it += n;
           }
-          if (!stop) mma_commit<CG>(&tfull[tc & 1]);
+          if (!stop && one) mma_commit<CG>(&tfull[tc & 1]);
         }
       }
       // Every product this thread issued is complete once `done` flips.
-      mma_commit<CG>(done);
+      if (one) mma_commit<CG>(done);
       const uint64_t t0 = now_ns();
       while (!mbar_try(done, 0) && now_ns() - t0 < WAIT_NS) {
       }

@@ -82,6 +82,23 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
   }
 }
 
+// The same for a whole warp that goes on together: true in all lanes, or false.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort));
+}
+// One lane of a converged warp, the same one each time. What the warp computes
+// around it stays in uniform registers, where tcgen05 and TMA take their
+// operands.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "elect.sync _|q, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(p));
+  return p != 0;
+}
+
 // 2-D tile load into this CTA's shared memory; the bytes are counted on the
 // barrier at `bar` (an address from map_rank: in a pair, the first CTA's).
 template <int CG>
