@@ -97,7 +97,9 @@ struct Prob {
 };
 
 struct GemmParams {
-  Prob q[2];        // the second only with OUT, after the first's units
+  Prob q[2];        // the second only with OUT, after the first's (longer) units
+  int skip;         // rounds of the second's units ahead of those for all clusters
+  int more, ahead;  // clusters with a first unit more; units in those rounds
   uint32_t fmt;     // operand format of the instruction (0 f16, 1 bf16)
   uint32_t* status;
   const uint32_t* scal;
@@ -331,7 +333,22 @@ __global__ void __launch_bounds__(NTHREADS, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = CG == 2 ? cta_rank() : 0;
   const int units = P.q[0].units + (EPI == OUT ? P.q[1].units : 0);
-  const int first = blockIdx.x / CG, step = gridDim.x / CG;
+  // Units go to the clusters in turn. With OUT, `more` clusters get one more of
+  // the first product's than the rest, which meanwhile take `skip` rounds of the
+  // second's among themselves; what is left goes to all, those first.
+  const int cluster = blockIdx.x / CG, step = gridDim.x / CG;
+  auto after_long = [&] {
+    const int c = cluster - P.more;
+    return P.q[0].units + (c < 0 ? P.ahead + c + step : c);
+  };
+  auto next_unit = [&](int u) {
+    if (EPI != OUT) return u + step;
+    if (u < P.q[0].units) return u + step < P.q[0].units ? u + step : after_long();
+    if (u - P.q[0].units >= P.ahead) return u + step;
+    u += step - P.more;
+    return u - P.q[0].units < P.ahead ? u : P.q[0].units + P.ahead + cluster - P.more;
+  };
+  const int first = EPI != OUT || cluster < P.q[0].units ? cluster : after_long();
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < S::STAGES; s++) {
@@ -361,7 +378,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       const bool one = elect_one();
       int it = 0;
       bool stop = false;
-      for (int u = first; u < units && !stop; u += step) {
+      for (int u = first; u < units && !stop; u = next_unit(u)) {
         const Unit q = unit_at<EPI>(P, u);
         const int am = (q.mt * CG + (int)rank) * BM, bn = q.nt * P.q[q.prob].bn + (int)rank * (P.q[q.prob].bn / CG);
         // Boxes of 64 of each CTA's rows and columns; those past the matrix are
@@ -423,7 +440,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       const bool one = elect_one();
       int it = 0, tc = 0;  // tc counts chains
       bool stop = false;
-      for (int u = first; u < units && !stop; u += step) {
+      for (int u = first; u < units && !stop; u = next_unit(u)) {
         const Unit q = unit_at<EPI>(P, u);
         const bool a_mn = EPI == OUT && P.q[q.prob].a_mn;
         const uint32_t idesc = (1u << 4) | (P.fmt << 7) | (P.fmt << 10) | ((a_mn ? 1u : 0u) << 15) |
@@ -531,11 +548,11 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       }
       return n;
     };
-    Unit after = unit_at<EPI>(P, first);
+    Unit after = unit_at<EPI>(P, first);  // the next tile's
     Row next = row_of(first, after);
-    for (int u = first; u < units && !stop; u += step) {
-      const Unit q = after;
-      after = unit_at<EPI>(P, u + step);  // past the last one: not used
+    for (int u = first; u < units && !stop; u = next_unit(u)) {
+      const Unit q = EPI == OUT ? unit_at<EPI>(P, u) : after;
+      if constexpr (EPI != OUT) after = unit_at<EPI>(P, next_unit(u));
       const Prob& pr = P.q[q.prob];
       const long i = (long)(q.mt * CG + (int)rank) * BM + r;
       const bool live = i < pr.M;
@@ -553,7 +570,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
             gr = gmax > 0.0f ? row.g / gmax : row.g;  // g: 0, or NaN
           }
         }
-        next = row_of(u + step, after);
+        next = row_of(next_unit(u), after);
       }
       // Waits for the next chain; then its TMEM columns are this warp's.
       auto wait_chain = [&] {
@@ -1047,7 +1064,7 @@ CUtensorMap make_map(const uint16_t* base, const Operand& o) {
 
 template <int EPI, int CG, int PARTS, int WIDTH, bool CHAINED = PARTS == 2>
 void launch_gemm(eb_engine* e, const Operand& A, const Operand& B, const Operand& C,
-                 const GemmParams& P) {
+                 GemmParams P) {
   using S = Shape<EPI, CG, PARTS, WIDTH, CHAINED>;
   const auto kern = k_gemm<EPI, CG, PARTS, WIDTH, CHAINED>;
   static std::atomic<uint64_t> allowed{0};
@@ -1058,6 +1075,8 @@ void launch_gemm(eb_engine* e, const Operand& A, const Operand& B, const Operand
   const CUtensorMap c1 = EPI == OUT && PARTS == 2 ? make_map(C.lo, C) : c0;
   const int units = P.q[0].units + P.q[1].units;
   const int clusters = std::min(units, e->num_sms / CG);
+  P.more = P.q[0].units % clusters;
+  P.ahead = P.skip * (clusters - P.more);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(clusters * CG));
   cfg.blockDim = dim3(NTHREADS);
@@ -1237,12 +1256,13 @@ GemmParams base_params(const LinearCeArgs& a, const uint32_t* scal) {
   return P;
 }
 
-// Splits of k for the products of one launch. Units go to the clusters in
-// turn, the longer first, so the launch takes a round per `clusters` units, each
-// as long as its first unit. A split product also writes and reads its
-// partial sums again in a launch of its own. Chosen over a few split counts by
-// that estimate, which is returned (us).
-double choose_splits(Prob* q, int count, int clusters, const TileCost& t) {
+// Splits of k for the products of one launch, chosen over a few counts by an
+// estimate (returned, us) of its last cluster's end: units go to the clusters in
+// turn, the longer product's first, and clusters with one of those less go
+// ahead with `skip` rounds of the other's (16,384 x 8,192 x 1024 bf16: 128 units of
+// 256 k-blocks on 74 clusters and 256 of 128, backward 580 us -> 546). A split product also
+// writes and reads its partial sums again in a launch of its own.
+double choose_splits(Prob* q, int count, int clusters, const TileCost& t, int* skip) {
   static const int tries[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32, 48, 64};
   auto len = [](const Prob& p, int s) { return (p.kblocks + s - 1) / s; };
   double best = 1e300;
@@ -1260,17 +1280,29 @@ double choose_splits(Prob* q, int count, int clusters, const TileCost& t) {
         if (s[i] > 1) extra_us += 3.0 + (double)q[i].M * q[i].ldacc * 4 * (s[i] + 1) / 4e6;
       }
       const int a = l[0] >= l[1] ? 0 : 1;
-      const long ra = (units[a] + clusters - 1) / clusters;
-      const long rb = (units[0] + units[1] + clusters - 1) / clusters - ra;
-      auto round_us = [&](int i) {  // a narrower tile's blocks take that much less
+      auto unit_us = [&](int i) {  // a narrower tile's blocks take that much less
         return std::max(l[i] * t.block_us * std::max(q[i].bn, 96) / std::max(t.width, 96),
                         t.tile_us * q[i].bn / t.width);
       };
-      const double us = ra * round_us(a) + (rb ? rb * round_us(1 - a) : 0.0) + t.tile_us + extra_us;
+      const double ua = unit_us(a), ub = units[1 - a] ? unit_us(1 - a) : 0.0;
+      const long ra = (units[a] + clusters - 1) / clusters, rest = units[a] % clusters;
+      const long free = clusters - rest;
+      const int rounds = rest && ub > 0.0 ? (int)(ua / ub) : 0;  // ahead of the others
+      double us = ra * ua;
+      if (units[1 - a] > 0 && units[1 - a] <= rounds * free) {
+        us = std::max(us, (ra - 1) * ua + (units[1 - a] + free - 1) / free * ub);
+      } else if (units[1 - a] > 0) {
+        const long left = units[1 - a] - rounds * free, rb = (left + clusters - 1) / clusters;
+        const bool free_last = rest && left - (rb - 1) * clusters <= free;
+        us = std::max(ra * ua + (rb - free_last) * ub,
+                      (ra - (rest > 0)) * ua + (rounds + rb) * ub);
+      }
+      us += t.tile_us + extra_us;
       if (us < best) {
         best = us;
         pick[0] = s0;
         pick[1] = s1;
+        *skip = rounds;
       }
     }
   }
@@ -1296,9 +1328,11 @@ void products(eb_engine* e, const Operand& A, Operand B, Operand C, GemmParams P
       const Prob m = make_prob(q[i].M, q[i].N, q[i].K, c);
       q[i].mtiles = m.mtiles, q[i].ntiles = m.ntiles, q[i].bn = m.bn, q[i].group = m.group;
     }
-    const double us = choose_splits(q, count, e->num_sms / c.ctas, c);
+    int skip = 0;
+    const double us = choose_splits(q, count, e->num_sms / c.ctas, c, &skip);
     if (us < least) {
       least = us;
+      P.skip = skip;
       tile = t;
       chosen[0] = q[0];
       chosen[1] = q[1];
