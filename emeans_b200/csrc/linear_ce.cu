@@ -119,9 +119,6 @@ struct GemmParams {
   const float* dloss;
   int one_dloss;
   long k;           // columns in all
-  void* p_hi;
-  void* p_lo;
-  long ldp;
   float pscale;     // what P is kept times: 1 (bf16) or PSCALE
 };
 
@@ -135,8 +132,8 @@ struct Shape {
   static constexpr int B_BYTES = B_ROWS * BK * 2;
   static constexpr int STAGE = PARTS * (A_BYTES + B_BYTES);
   static constexpr int STAGES = 196608 / STAGE < 8 ? 196608 / STAGE : 8;
-  // Operand ring, barriers, and each epilogue warp's 32 x 32 block.
-  static constexpr size_t SMEM = 1024 + (size_t)STAGES * STAGE + 256 + 8 * 4096;
+  // Operand ring, each epilogue warp's 32 x 32 block, and barriers.
+  static constexpr size_t SMEM = 1024 + (size_t)STAGES * STAGE + 8 * 4096 + 256;
   // k-blocks summed in one TMEM accumulator. The tensor cores' FP32 sums are
   // cut, not rounded, at every step of 16 (about 2^-26 of the sum a product,
   // always towards zero): 5.6e-6 of dx at k = 5,003 in one chain of three
@@ -316,7 +313,7 @@ template <int EPI, int CG, int PARTS, int WIDTH, bool CHAINED>
 __global__ void __launch_bounds__(NTHREADS, 1)
     k_gemm(const __grid_constant__ CUtensorMap a0, const __grid_constant__ CUtensorMap a1,
            const __grid_constant__ CUtensorMap b0, const __grid_constant__ CUtensorMap b1,
-           const __grid_constant__ CUtensorMap c0, const __grid_constant__ CUtensorMap c1,
+           const __grid_constant__ CUtensorMap c0map, const __grid_constant__ CUtensorMap c1map,
            const __grid_constant__ GemmParams P) {
   using S = Shape<EPI, CG, PARTS, WIDTH, CHAINED>;
   constexpr int HALF = S::HALF;
@@ -326,7 +323,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
   // that it points to shared memory (with generic accesses the step of 16,384
   // x 65,536 x 1024 bf16 took 6.5 ms instead of 6.1).
   uint8_t* smem = smem_raw + (-smem_u32(smem_raw) & 1023u);
-  uint64_t* full = (uint64_t*)(smem + S::STAGES * S::STAGE);
+  uint64_t* full = (uint64_t*)(smem + S::STAGES * S::STAGE + 8 * 4096);
   uint64_t* empty = full + S::STAGES;
   uint64_t* tfull = empty + S::STAGES;
   uint64_t* tempty = tfull + 2;
@@ -413,7 +410,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
 #pragma unroll
           for (int p = 0; p < PARTS; p++) {
             const CUtensorMap* ma = p ? &a1 : &a0;
-            const CUtensorMap* mb = q.prob ? (p ? &c1 : &c0) : (p ? &b1 : &b0);
+            const CUtensorMap* mb = q.prob ? (p ? &c1map : &c0map) : (p ? &b1 : &b0);
 #pragma unroll
             for (int c = 0; c < S::A_ROWS / 64; c++, st += 8192) {
               const int m = am + c * 64;
@@ -524,14 +521,14 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     // and half (w - 4) / 4 of the tile's columns.
     const int hf = (warp - 4) >> 2;
     const int r = (warp & 3) * 32 + lane;
-    float* blk = (float*)(smem + S::STAGES * S::STAGE + 256) + (warp - 4) * 1024;
+    float* blk = (float*)(smem + S::STAGES * S::STAGE) + (warp - 4) * 1024;
     const uint32_t base = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(hf * HALF);
     float sc = P.scale, gmax = 0.0f;
     if (EPI != OUT && P.split) sc = sc / split_scale(P.scal[S_X]) / split_scale(P.scal[S_W]);
     if constexpr (EPI != LSE)
       gmax = P.one_dloss ? fabsf(P.dloss[0]) : __uint_as_float(P.scal[S_G]);
     const uint32_t release = CG == 2 ? map_rank(smem_u32(tempty), 0) : smem_u32(tempty);
-    int tc = 0;
+    int tc = 0, stores = 0;
     bool stop = false;
     // A tile's row of this thread. The next tile's is fetched while the current
     // one is worked on: with few k-blocks a tile, these loads' latency would be
@@ -660,61 +657,72 @@ __global__ void __launch_bounds__(NTHREADS, 1)
           for (int j = 0; j < 32; j++) part[j & 3] += ex(fmaf(v[j], sc, off));
           sum = (part[0] + part[1]) + (part[2] + part[3]);
           m2 = m;
-        } else {
-          float less = 0.0f;  // the target's p - 1
-          if constexpr (EPI == PROB) {
-            if (tcol >> 5 == h) {
-              // By expm1: near 1, p's own rounding would be all that is left.
+        } else if constexpr (EPI == PROB) {
+          const bool target = tcol >> 5 == h;
+          const int e = tcol & 31;
+          float at_target = 0.0f;
+          if (target) {  // by expm1: near 1, p's own rounding would be all that is left
+            float z = 0.0f;
 #pragma unroll
-              for (int g = 0; g < 8; g++)
-                block4(blk, lane, g) = make_float4(v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]);
-              const float z = reinterpret_cast<const float*>(&block4(blk, lane, (tcol & 31) >> 2))[tcol & 3];
-              less = expm1f(fmaf(z, sc, -lse));
-            }
-            // Columns past the last prototype are never read.
-#pragma unroll
-            for (int j = 0; j < 32; j++) v[j] = ex(fmaf(v[j], sc, -lse)) * gr;
+            for (int j = 0; j < 32; j++) z = j == e ? v[j] : z;
+            at_target = gr * expm1f(fmaf(z, sc, -lse));
           }
+#pragma unroll
+          for (int j = 0; j < 32; j++) v[j] = ex(fmaf(v[j], sc, -lse)) * gr;
+          if (gr == 0.0f) {  // nothing of a row without a gradient, not even its NaN
+#pragma unroll
+            for (int j = 0; j < 32; j++) v[j] = 0.0f;
+            at_target = 0.0f;
+          }
+          // A row a thread, 64 bytes a term, 16-byte groups placed by the 64-byte
+          // swizzle; a tile store takes the block to P and cuts it at P's
+          // edges. One-term blocks go through two buffers in turn. (Transposed
+          // in shared memory as FP32 and stored by four lanes a row: backward
+          // 16,384 x 8,192 x 256 bf16 221 us, 211 now, x 1,024 x 768 78 and 74,
+          // 8,192 x 8,192 x 256 f32 272 and 263.)
+          auto pack = [&](const float (&f)[8], uint4& lo) {
+            return PARTS == 1 && P.fmt ? pack8<false>(f, 1.0f, lo)
+                                       : pack8<true, PARTS == 2>(f, PSCALE, lo);
+          };
+          uint8_t* box = (uint8_t*)blk + (PARTS == 1 ? (stores++ & 1) * 2048 : 0);
+          uint8_t* row = box + lane * 64;
+          const int turn = (lane >> 1) & 3;
+          if (lane == 0) stores_read<PARTS == 1 ? 1 : 0>();
+          __syncwarp();
+#pragma unroll
+          for (int g = 0; g < 4; g++) {
+            const float f[8] = {v[8 * g],     v[8 * g + 1], v[8 * g + 2], v[8 * g + 3],
+                                v[8 * g + 4], v[8 * g + 5], v[8 * g + 6], v[8 * g + 7]};
+            uint4 lo;
+            *reinterpret_cast<uint4*>(row + ((g ^ turn) << 4)) = pack(f, lo);
+            if (PARTS == 2) *reinterpret_cast<uint4*>(row + 2048 + ((g ^ turn) << 4)) = lo;
+          }
+          if (target) {
+            const float f[8] = {at_target};
+            uint4 lo;
+            uint8_t* p = row + (((e >> 3) ^ turn) << 4) + (e & 7) * 2;
+            *reinterpret_cast<uint16_t*>(p) = (uint16_t)pack(f, lo).x;
+            if (PARTS == 2) *reinterpret_cast<uint16_t*>(p + 2048) = (uint16_t)lo.x;
+          }
+          store_fence();
+          __syncwarp();
+          if (lane == 0) {
+            const int row0 = (int)i, col = (int)c0 + h * 32;
+            if (row0 < pr.M) {
+              tma_store(&c0map, box, col, row0);
+              if (PARTS == 2) tma_store(&c1map, box + 2048, col, row0);
+            }
+            stores_commit();
+          }
+        } else {
           __syncwarp();
 #pragma unroll
           for (int g = 0; g < 8; g++)
             block4(blk, lane, g) = make_float4(v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]);
-          if constexpr (EPI == PROB) {
-            if (gr == 0.0f) {  // nothing of a row without a gradient, not even its NaN
-#pragma unroll
-              for (int g = 0; g < 8; g++) block4(blk, lane, g) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            } else if (tcol >> 5 == h) {
-              reinterpret_cast<float*>(&block4(blk, lane, (tcol & 31) >> 2))[tcol & 3] = gr * less;
-            }
-          }
           __syncwarp();
           const long row0 = i - lane, col = c0 + h * 32;
-          const int rows = (int)min(32l, pr.M - row0);
-          if constexpr (EPI == PROB) {
-            // Four lanes a row, eight columns each.
-            const int g = (lane & 3) * 2;
-            if (col + g * 4 < P.ldp) {
-              const long at = (row0 + (lane >> 2)) * P.ldp + col + g * 4;
-#pragma unroll
-              for (int t = 0; t < 4; t++) {
-                const int rr = (lane >> 2) + t * 8;
-                if (rr >= rows) break;
-                const float4 a = block4(blk, rr, g), b = block4(blk, rr, g + 1);
-                const float f[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-                uint4 hi, lo;
-                if (PARTS == 1 && P.fmt)
-                  hi = pack8<false>(f, 1.0f, lo);
-                else
-                  hi = pack8<true, PARTS == 2>(f, PSCALE, lo);
-                *reinterpret_cast<uint4*>((uint16_t*)P.p_hi + at + t * 8 * P.ldp) = hi;
-                if (PARTS == 2)
-                  *reinterpret_cast<uint4*>((uint16_t*)P.p_lo + at + t * 8 * P.ldp) = lo;
-              }
-            }
-          } else {
-            store_block(pr, pr.accum + ((long)q.split * pr.M + row0) * pr.ldacc, blk, lane, row0, rows,
-                        col, min(left, 32), factor);
-          }
+          store_block(pr, pr.accum + ((long)q.split * pr.M + row0) * pr.ldacc, blk, lane, row0,
+                      (int)min(32l, pr.M - row0), col, min(left, 32), factor);
         }
       }
       if constexpr (EPI == LSE) {
@@ -724,6 +732,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         }
       }
     }
+    if (EPI == PROB && lane == 0) stores_done();
   }
 
   __syncthreads();
@@ -1054,17 +1063,19 @@ struct Operand {
   long rows, cols, ld;
 };
 
-// Boxes of 64 columns (128 bytes) by 64 rows, 128-byte swizzle. Every load's
-// first column is a multiple of 64.
-CUtensorMap make_map(const uint16_t* base, const Operand& o) {
+// Read in boxes of 64 columns (128 bytes) by 64 rows, 128-byte swizzle; P is
+// written in boxes of 32 by 32, 64-byte swizzle. Every box's first column is a
+// multiple of 64, or 32.
+CUtensorMap make_map(const uint16_t* base, const Operand& o, bool store = false) {
   CUtensorMap m;
   cuuint64_t dims[2] = {(cuuint64_t)o.cols, (cuuint64_t)o.rows};
   cuuint64_t strides[1] = {(cuuint64_t)o.ld * 2};
-  cuuint32_t box[2] = {64, 64};
+  cuuint32_t box[2] = {store ? 32u : 64u, store ? 32u : 64u};
   cuuint32_t estr[2] = {1, 1};
   CUresult r = encode_fn()(&m, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2,
                            const_cast<uint16_t*>(base), dims, strides, box, estr,
-                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           store ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) throw Error(EB_ERROR, "cuTensorMapEncodeTiled failed: " + std::to_string(r));
   return m;
@@ -1079,8 +1090,8 @@ void launch_gemm(eb_engine* e, const Operand& A, const Operand& B, const Operand
   allow_smem(e, kern, S::SMEM, allowed);
   const CUtensorMap a0 = make_map(A.hi, A), a1 = PARTS == 2 ? make_map(A.lo, A) : a0;
   const CUtensorMap b0 = make_map(B.hi, B), b1 = PARTS == 2 ? make_map(B.lo, B) : b0;
-  const CUtensorMap c0 = EPI == OUT ? make_map(C.hi, C) : b0;
-  const CUtensorMap c1 = EPI == OUT && PARTS == 2 ? make_map(C.lo, C) : c0;
+  const CUtensorMap c0 = EPI != LSE ? make_map(C.hi, C, EPI == PROB) : b0;
+  const CUtensorMap c1 = EPI != LSE && PARTS == 2 ? make_map(C.lo, C, EPI == PROB) : c0;
   const int units = P.q[0].units + P.q[1].units;
   const int clusters = std::min(units, e->num_sms / CG);
   P.more = P.q[0].units % clusters;
@@ -1459,11 +1470,8 @@ void linear_ce_backward(eb_engine* e, const LinearCeArgs& a, const LinearCeGrads
       P.dloss = g.one_dloss ? g.dloss : g.dloss + r0;
       P.one_dloss = g.one_dloss;
       P.col0 = (long)v0;
-      P.ldp = (pc + 7) / 8 * 8;
-      P.p_hi = p;
-      P.p_lo = parts == 2 ? p + rows * cols : nullptr;
-      gemm<PROB>(e, Xr, Wv, Wv, tile, P);
-      const Operand Pm{p, parts == 2 ? p + rows * cols : nullptr, pr, pc, P.ldp};
+      const Operand Pm{p, parts == 2 ? p + rows * cols : nullptr, pr, pc, (pc + 7) / 8 * 8};
+      gemm<PROB>(e, Xr, Wv, Pm, tile, P);
       int count = 0;
       Operand B[2];
       if (g.dx) {
