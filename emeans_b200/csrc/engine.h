@@ -440,6 +440,12 @@ void linear_ce_backward(eb_engine* e, const LinearCeArgs& a, const LinearCeGrads
 bool linear_ce_is_small(const LinearCeArgs& a);
 void linear_ce_small(eb_engine* e, const LinearCeArgs& a, float* loss, float* lse);
 void linear_ce_small_backward(eb_engine* e, const LinearCeArgs& a, const LinearCeGrads& g);
+// linear_ce_few.cu: the same for few f32 rows. The forward pass leaves
+// linear_ce_few_parts x n (max, sum of exp) and the target scores.
+bool linear_ce_is_few(const LinearCeArgs& a);
+int linear_ce_few_parts(eb_engine* e, const LinearCeArgs& a);
+void linear_ce_few(eb_engine* e, const LinearCeArgs& a, float2* part, float* zt);
+void linear_ce_few_backward(eb_engine* e, const LinearCeArgs& a, const LinearCeGrads& g);
 
 // ---- adamw.cu: a plan's device tables, and one step over them
 void adamw_create(eb_engine* e, const eb_adamw_tensor* t, size_t count, eb_adamw* plan);

@@ -1387,11 +1387,29 @@ void products(eb_engine* e, const Operand& A, Operand B, Operand C, GemmParams P
   }
 }
 
+// Losses and lse of n rows from their parts.
+void join(eb_engine* e, const float2* part, int parts, long n, long k, const float* zt,
+          const uint32_t* targets, float* loss, float* lse) {
+  const bool few = parts <= 32, row = !few && n <= 1024;
+  launch_pdl(e, few ? k_ce_join_few : row ? k_ce_join_row : k_ce_join,
+             dim3((unsigned)(few ? (n + 127) / 128 : row ? n : (n + 31) / 32)),
+             dim3(few ? 128 : row ? 256 : 1024), 0, part, parts, n, k, zt, targets, loss, lse,
+             e->d_status);
+  e->stats.kernel_launches++;
+}
+
 }  // namespace
 
 void linear_ce(eb_engine* e, const LinearCeArgs& a, float* loss, float* lse) {
   if (a.n == 0) return;
   if (linear_ce_is_small(a)) return linear_ce_small(e, a, loss, lse);
+  if (linear_ce_is_few(a)) {
+    const int parts = linear_ce_few_parts(e, a);
+    float2* part = e->scratch_get<float2>("ce_part", (size_t)parts * a.n);
+    float* zt = e->scratch_get<float>("ce_zt", a.n);
+    linear_ce_few(e, a, part, zt);
+    return join(e, part, parts, (long)a.n, (long)a.k, zt, a.targets, loss, lse);
+  }
   uint32_t* scal = e->scratch_get<uint32_t>("ce_scalars", S_WORDS);
   Operand X, W;
   operands(e, a, scal, X, W);
@@ -1411,12 +1429,7 @@ void linear_ce(eb_engine* e, const LinearCeArgs& a, float* loss, float* lse) {
     P.zt = e->scratch_get<float>("ce_zt", (size_t)n);
     P.targets = a.targets + r0;
     gemm<LSE>(e, rows_of(X, (long)r0, (long)r0 + n), W, W, tile, P);
-    const bool few = parts <= 32, row = !few && n <= 1024;
-    launch_pdl(e, few ? k_ce_join_few : row ? k_ce_join_row : k_ce_join,
-               dim3((unsigned)(few ? (n + 127) / 128 : row ? n : (n + 31) / 32)),
-               dim3(few ? 128 : row ? 256 : 1024), 0, (const float2*)part, parts, n, (long)a.k,
-               (const float*)P.zt, P.targets, loss + r0, lse + r0, e->d_status);
-    e->stats.kernel_launches++;
+    join(e, part, parts, n, (long)a.k, P.zt, P.targets, loss + r0, lse + r0);
   }
 }
 
@@ -1429,6 +1442,7 @@ void linear_ce_backward(eb_engine* e, const LinearCeArgs& a, const LinearCeGrads
     return;
   }
   if (linear_ce_is_small(a)) return linear_ce_small_backward(e, a, g);
+  if (linear_ce_is_few(a)) return linear_ce_few_backward(e, a, g);
   uint32_t* scal = e->scratch_get<uint32_t>("ce_scalars", S_WORDS);
   if (!g.one_dloss) {
     EB_CUDA(cudaMemsetAsync(scal + S_G, 0, 4, e->stream));

@@ -1,0 +1,324 @@
+// The linear cross entropy of few f32 rows, in FP32 on the CUDA cores.
+//
+// On the tensor cores (linear_ce.cu) f32 operands are scaled and split into two
+// FP16 terms first: w is read twice and written once before the products read
+// it again. Up to 16 rows the arithmetic is less than that: 2 n k d operations
+// at n = 16 are 8 a byte of w. Here w is read once forward and twice backward.
+//
+// Scores: x lies in shared memory; a warp takes four prototypes at a time, its
+// lanes the columns in turn, and keeps NR x 4 sums a lane, so that each element
+// of x read from shared memory serves four products. The sums over the lanes
+// are halved from step to step (a lane sends the half that it gives up), 62
+// shuffles for 64 sums. Forward, lanes fold their scores into (max, sum of exp);
+// backward they write P (k x NR floats). The gradients then read P and w: a
+// thread owns a column, keeps x and its part of dx in registers, and writes
+// dw as it goes; the blocks' parts of dx are added in order by a second kernel.
+// Columns copied ahead by cp.async (16 prototypes deep) instead of four in
+// registers: backward 148 us against 156 at 15 x 41,927 x 547, but 154 against 134 at
+// 1 x 40,000 x 1024 and 53 against 41 at 8 x 65,536 x 64: not kept.
+//
+// Bound by reading w (and writing dw): 1 x 40,000 x 1024 forward 43 us, 3.8 TB/s.
+#include <cuda_runtime.h>
+
+#include <cmath>
+
+#include "elem.h"
+#include "engine.h"
+#include "tc.h"
+
+namespace eb {
+
+namespace {
+
+using tc::pdl_trigger;
+
+constexpr int THREADS = 256;
+constexpr long MOST_ROWS = 16, MOST_COLUMNS = 1024;
+constexpr long MOST_PROTOTYPES = 1l << 22;  // P is then at most 256 MB
+constexpr int CHUNK = 32;  // prototypes whose P a block holds (128: the same times)
+constexpr float LOG2E = 1.4426950408889634f;
+
+struct Few {
+  const float* x;
+  const float* w;
+  long n, d, k, ldx, ldw;
+  const uint32_t* targets;
+  float scale;
+  // forward: blocks x n (max, sum of exp), and each row's target score
+  float2* part;
+  float* zt;
+  // backward
+  const float* lse;
+  const float* dloss;
+  int one_dloss;
+  float* p;     // k x NR
+  float* dx;    // blocks x n x d, or null
+  float* dw;    // or null
+  long lddw;
+};
+
+__device__ __forceinline__ float ex(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v * LOG2E));
+  return r;
+}
+// Folds (m', s') into a running (max, sum of exp(z - max)); (-inf, 0) is empty.
+// NaN scores are in the sums, not in the maxima.
+__device__ __forceinline__ void fold(float& m, float& s, float mv, float sv) {
+  const float top = fmaxf(m, mv), off = top == -INFINITY ? 0.0f : top;
+  s = s * ex(m - off) + sv * ex(mv - off);
+  m = top;
+}
+
+template <int NR, bool BACKWARD>
+__global__ void __launch_bounds__(THREADS, 2) k_few_scores(Few F) {
+  pdl_trigger();
+  pdl_wait();
+  extern __shared__ float xs[];  // NR x dp
+  __shared__ float2 joint[THREADS / 32][NR];
+  constexpr int V = NR * 4;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int d = (int)F.d, dp = (d + 31) / 32 * 32;
+  for (int t = threadIdx.x; t < NR * dp; t += THREADS) {
+    const int i = t / dp, c = t % dp;
+    xs[t] = i < F.n && c < d ? F.x[i * F.ldx + c] : 0.0f;
+  }
+  __syncthreads();
+  // After the halving a lane holds the sums of this row, V / 32 (at least one)
+  // of its four prototypes from `q0` on.
+  const int i = lane / (32 / NR);
+  const int q0 = V == 64 ? (lane & 1) * 2 : V == 32 ? lane & 3 : (lane >> 1) & 3;
+  const uint32_t target = i < F.n ? F.targets[i] : EB_IGNORE;
+  float m = -INFINITY, s = 0.0f, lse = 0.0f, g = 0.0f;
+  if (BACKWARD && i < F.n && (long)target < F.k) {
+    lse = F.lse[i];
+    g = F.dloss[F.one_dloss ? 0 : i] * F.scale;
+  }
+  const long step = (long)gridDim.x * (THREADS / 32) * 4;
+  for (long p0 = ((long)blockIdx.x * (THREADS / 32) + warp) * 4; p0 < F.k; p0 += step) {
+    const float* w[4];
+#pragma unroll
+    for (int q = 0; q < 4; q++) w[q] = F.w + min(p0 + q, F.k - 1) * F.ldw;
+    float a[V];
+#pragma unroll
+    for (int j = 0; j < V; j++) a[j] = 0.0f;
+#pragma unroll 4
+    for (int c = lane; c < dp; c += 32) {
+      float v[4];
+#pragma unroll
+      for (int q = 0; q < 4; q++) v[q] = c < d ? w[q][c] : 0.0f;
+#pragma unroll
+      for (int r = 0; r < NR; r++) {
+        const float xv = xs[r * dp + c];
+#pragma unroll
+        for (int q = 0; q < 4; q++) a[r * 4 + q] = fmaf(xv, v[q], a[r * 4 + q]);
+      }
+    }
+#pragma unroll
+    for (int o = 16, have = V; o; o >>= 1) {
+      if (have > 1) {
+        have /= 2;
+        const bool upper = lane & o;
+#pragma unroll
+        for (int j = 0; j < V / 2; j++) {
+          if (j >= have) break;
+          const float keep = upper ? a[j + have] : a[j], give = upper ? a[j] : a[j + have];
+          a[j] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+        }
+      } else {
+        a[0] += __shfl_xor_sync(0xffffffffu, a[0], o);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < (V == 64 ? 2 : 1); j++) {
+      const long p = p0 + q0 + j;
+      if (p >= F.k) continue;
+      const float z = a[j] * F.scale;
+      if constexpr (BACKWARD) {
+        // By expm1 at the target: near 1, p's own rounding would be all that is
+        // left. Nothing of a row without a gradient, not even its NaN.
+        const float v = p == (long)target ? expm1f(z - lse) : ex(z - lse);
+        F.p[p * NR + i] = g == 0.0f ? 0.0f : g * v;
+      } else {
+        fold(m, s, z, 1.0f);
+        if (p == (long)target) F.zt[i] = z;
+      }
+    }
+  }
+  if constexpr (!BACKWARD) {
+    // The lanes of a row, then the block's warps in order.
+#pragma unroll
+    for (int o = V == 16 ? 2 : 1; o < 32 / NR; o <<= 1) {
+      const float mo = __shfl_xor_sync(0xffffffffu, m, o), so = __shfl_xor_sync(0xffffffffu, s, o);
+      fold(m, s, mo, so);
+    }
+    if (lane % (32 / NR) == 0) joint[warp][i] = make_float2(m, s);
+    __syncthreads();
+    if (threadIdx.x < F.n) {
+      m = -INFINITY, s = 0.0f;
+      for (int v = 0; v < THREADS / 32; v++)
+        fold(m, s, joint[v][threadIdx.x].x, joint[v][threadIdx.x].y);
+      F.part[(long)blockIdx.x * F.n + threadIdx.x] = make_float2(m, s);
+    }
+  }
+}
+
+template <int NR>
+__global__ void __launch_bounds__(1024) k_few_grads(Few F, long per) {
+  pdl_trigger();
+  pdl_wait();
+  __shared__ __align__(16) float ps[CHUNK * NR];
+  const long c = threadIdx.x;
+  const bool has = c < F.d;
+  float x[NR], dx[NR];
+#pragma unroll
+  for (int i = 0; i < NR; i++) {
+    x[i] = has && i < F.n ? F.x[i * F.ldx + c] : 0.0f;
+    dx[i] = 0.0f;
+  }
+  const long j0 = blockIdx.x * per, j1 = min(j0 + per, F.k);
+  // The next four prototypes' elements are on their way while four are used;
+  // past the block's last one they are 0.
+  float w[4];
+  auto fetch = [&](long j) {
+#pragma unroll
+    for (int q = 0; q < 4; q++) w[q] = has && j + q < j1 ? F.w[(j + q) * F.ldw + c] : 0.0f;
+  };
+  fetch(j0);
+  for (long base = j0; base < j1; base += CHUNK) {
+    const int count = (int)min((long)CHUNK, j1 - base);
+    __syncthreads();
+    for (int t = threadIdx.x; t < CHUNK * NR; t += blockDim.x)
+      ps[t] = t < count * NR ? F.p[base * NR + t] : 0.0f;
+    __syncthreads();
+    for (int p = 0; p < count; p += 4) {
+      const float now[4] = {w[0], w[1], w[2], w[3]};
+      fetch(base + p + 4);
+#pragma unroll
+      for (int q = 0; q < 4; q++) {
+        float dw = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NR; i += 4) {
+          const float4 pv = *reinterpret_cast<const float4*>(&ps[(p + q) * NR + i]);
+          const float pr[4] = {pv.x, pv.y, pv.z, pv.w};
+#pragma unroll
+          for (int u = 0; u < 4; u++) {
+            dx[i + u] = fmaf(pr[u], now[q], dx[i + u]);
+            dw = fmaf(pr[u], x[i + u], dw);
+          }
+        }
+        if (F.dw && has && p + q < count) F.dw[(base + p + q) * F.lddw + c] = dw;
+      }
+    }
+  }
+  if (!F.dx || !has) return;
+#pragma unroll
+  for (int i = 0; i < NR; i++) {
+    if (i >= F.n) break;
+    F.dx[((long)blockIdx.x * F.n + i) * F.d + c] = dx[i];
+  }
+}
+
+// dx: the blocks' parts in order, 32 elements a block of 8 slices.
+__global__ void __launch_bounds__(THREADS)
+    k_few_sum(const float* __restrict__ part, int blocks, long total, long d, float* dx, long lddx) {
+  pdl_trigger();
+  pdl_wait();
+  __shared__ float joint[8][33];
+  const int c = threadIdx.x & 31, slice = threadIdx.x >> 5;
+  const long t = (long)blockIdx.x * 32 + c;
+  float s = 0.0f;
+  if (t < total) {
+#pragma unroll 8
+    for (int b = slice; b < blocks; b += 8) s += part[b * total + t];
+  }
+  joint[slice][c] = s;
+  __syncthreads();
+  if (slice || t >= total) return;
+  s = 0.0f;
+#pragma unroll
+  for (int v = 0; v < 8; v++) s += joint[v][c];
+  dx[t / d * lddx + t % d] = s;
+}
+
+Few few(const LinearCeArgs& a) {
+  Few F{};
+  F.x = static_cast<const float*>(a.x);
+  F.w = static_cast<const float*>(a.w);
+  F.n = (long)a.n;
+  F.d = (long)a.d;
+  F.k = (long)a.k;
+  F.ldx = (long)a.ldx;
+  F.ldw = (long)a.ldw;
+  F.targets = a.targets;
+  F.scale = a.scale;
+  return F;
+}
+
+template <int NR, bool BACKWARD>
+void scores(eb_engine* e, const Few& F, unsigned grid) {
+  const size_t smem = (size_t)NR * ((F.d + 31) / 32 * 32) * 4;
+  const auto kern = k_few_scores<NR, BACKWARD>;
+  static std::atomic<uint64_t> allowed{0};
+  allow_smem(e, kern, (size_t)NR * MOST_COLUMNS * 4, allowed);
+  launch_pdl(e, kern, dim3(grid), dim3(THREADS), smem, F);
+  e->stats.kernel_launches++;
+}
+template <bool BACKWARD>
+void scores_of(eb_engine* e, const Few& F, unsigned grid) {
+  if (F.n <= 4) return scores<4, BACKWARD>(e, F, grid);
+  if (F.n <= 8) return scores<8, BACKWARD>(e, F, grid);
+  scores<16, BACKWARD>(e, F, grid);
+}
+unsigned scores_grid(eb_engine* e, const LinearCeArgs& a) {
+  return (unsigned)std::min<size_t>((a.k + 31) / 32, (size_t)e->num_sms * 2);
+}
+
+}  // namespace
+
+// Up to 16 rows; forward and backward in us, here and on the tensor cores:
+//   1 x 40,000 x 1024 43 and 134, 152 and 244; 16 x 40,000 x 1024 77 and 214, 151 and 240;
+//   15 x 41,927 x 547 48 and 156, 102 and 190; 5 x 7,689 x 807 13 and 30, 34 and 58;
+//   16 x 60,000 x 8 16 and 47, 41 and 51; 1 x 760 x 506 8 and 12, 18 and 25.
+// With more rows the backward pass would lose: at 16 it is bound by its 4 n k d
+// operations in FP32 as much as by memory.
+bool linear_ce_is_few(const LinearCeArgs& a) {
+  return a.dtype == EB_F32 && (long)a.n <= MOST_ROWS && (long)a.d <= MOST_COLUMNS &&
+         (long)a.k <= MOST_PROTOTYPES;
+}
+
+int linear_ce_few_parts(eb_engine* e, const LinearCeArgs& a) { return (int)scores_grid(e, a); }
+
+void linear_ce_few(eb_engine* e, const LinearCeArgs& a, float2* part, float* zt) {
+  Few F = few(a);
+  F.part = part;
+  F.zt = zt;
+  scores_of<false>(e, F, scores_grid(e, a));
+}
+
+void linear_ce_few_backward(eb_engine* e, const LinearCeArgs& a, const LinearCeGrads& g) {
+  Few F = few(a);
+  const int nr = F.n <= 4 ? 4 : F.n <= 8 ? 8 : 16;
+  F.lse = g.lse;
+  F.dloss = g.dloss;
+  F.one_dloss = g.one_dloss;
+  F.p = e->scratch_get<float>("ce_p", a.k * nr);
+  scores_of<true>(e, F, scores_grid(e, a));
+  const unsigned threads = (unsigned)((a.d + 31) / 32 * 32);  // a column each
+  const long most = (long)e->num_sms * (1024 / std::max(threads, 64u));
+  const long per = std::max<long>((F.k + most - 1) / most, 4);
+  const unsigned grid = (unsigned)((F.k + per - 1) / per);
+  F.dx = g.dx ? e->scratch_get<float>("ce_dx", (size_t)grid * a.n * a.d) : nullptr;
+  F.dw = static_cast<float*>(g.dw);
+  F.lddw = (long)g.lddw;
+  const auto kern = nr == 4 ? k_few_grads<4> : nr == 8 ? k_few_grads<8> : k_few_grads<16>;
+  launch_pdl(e, kern, dim3(grid), dim3(threads), 0, F, per);
+  e->stats.kernel_launches++;
+  if (!g.dx) return;
+  const long total = F.n * F.d;
+  launch_pdl(e, k_few_sum, dim3((unsigned)((total + 31) / 32)), dim3(THREADS), 0,
+             (const float*)F.dx, (int)grid, total, F.d, static_cast<float*>(g.dx), (long)g.lddx);
+  e->stats.kernel_launches++;
+}
+
+}  // namespace eb

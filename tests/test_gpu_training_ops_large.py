@@ -152,6 +152,43 @@ def test_linear_cross_entropy_few_rows(eng, n, dtype):
         c.check(c.run(eng))
 
 
+@pytest.mark.parametrize("n", [1, 3, 4, 5, 8, 9, 16])
+@pytest.mark.parametrize("k,d", [(1, 65), (3, 93), (127, 31), (700, 1), (4097, 333), (31, 1024),
+                                 (9000, 1023), (500, 1025)])
+def test_linear_cross_entropy_few_f32_rows(eng, n, k, d):
+    """Rows up to 16 of 32 bits, to both sides of the widest, with row strides."""
+    for pad in (0, 3):
+        c = Ce(n, k, d, torch.float32, n + k + d, per_row=n % 2 == 0, ignored=0.3)
+        c.check(c.run(eng, pad=pad))
+
+
+def test_linear_cross_entropy_few_f32_rows_one_gradient_and_bits(eng):
+    c = Ce(7, 1003, 129, torch.float32, 5)
+    both, again = c.run(eng), c.run(eng)
+    for a, b in zip(both, again):
+        assert torch.equal(a, b)
+    assert torch.equal(c.run(eng, dw=False)[2], both[2])
+    assert torch.equal(c.run(eng, dx=False)[3], both[3])
+
+
+def test_linear_cross_entropy_few_f32_rows_non_finite(eng):
+    """A row without a gradient stays at zero whatever it holds; another row's
+    infinities reach its own loss only."""
+    c = Ce(6, 300, 70, torch.float32, 9, ignored=0.0)
+    c.t[2] = eb.IGNORE
+    c.x[2, 3], c.x[4, 5] = math.nan, math.inf
+    loss, lse, dx, dw = c.run(eng)
+    assert loss[2] == 0 and (dx[2] == 0).all()
+    assert not torch.isfinite(loss[4])
+    rest = [0, 1, 3, 5]
+    X, W = c.x.double()[rest], c.w.double()
+    Z = c.scale * (X @ W.T)
+    want = torch.logsumexp(Z, 1) - Z.gather(1, c.t[rest][:, None])[:, 0]
+    tol = 2.0 ** -19 * (1 + Z.abs().amax(1)) + (c.d / 4 + 8) * 2.0 ** -22 * c.scale * (
+        X.abs() @ W.abs().T).amax(1)
+    within(loss[rest], want, tol, "loss")
+
+
 def test_linear_cross_entropy_long_rows(eng):
     """Scores of 16-bit rows past 768 columns, summed in chains: FP32's own
     error, well inside Ce.check's bound for one chain."""

@@ -29,3 +29,9 @@ def test_training_kernels_spill_at_most_a_few_words(src, kernels):
         assert any(want in k for k in found), (want, sorted(found))
     worst = {k: v for k, v in found.items() if v[0] > 64 or v[1] > 64}
     assert not worst, worst
+
+
+@pytest.mark.timeout(900)
+def test_few_row_kernels_spill_at_most_a_few_words():
+    test_training_kernels_spill_at_most_a_few_words("linear_ce_few.cu",
+                                                    ["k_few_scores", "k_few_grads"])
