@@ -440,7 +440,7 @@ void linear_ce_backward(eb_engine* e, const LinearCeArgs& a, const LinearCeGrads
 bool linear_ce_is_small(const LinearCeArgs& a);
 void linear_ce_small(eb_engine* e, const LinearCeArgs& a, float* loss, float* lse);
 void linear_ce_small_backward(eb_engine* e, const LinearCeArgs& a, const LinearCeGrads& g);
-// linear_ce_few.cu: the same for few f32 rows. The forward pass leaves
+// linear_ce_few.cu: the same for few rows. The forward pass leaves
 // linear_ce_few_parts x n (max, sum of exp) and the target scores.
 bool linear_ce_is_few(const LinearCeArgs& a);
 int linear_ce_few_parts(eb_engine* e, const LinearCeArgs& a);

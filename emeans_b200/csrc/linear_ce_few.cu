@@ -1,8 +1,8 @@
-// The linear cross entropy of few f32 rows, in FP32 on the CUDA cores.
+// The linear cross entropy of few rows, in FP32 on the CUDA cores.
 //
 // On the tensor cores (linear_ce.cu) f32 operands are scaled and split into two
-// FP16 terms first: w is read twice and written once before the products read
-// it again. Up to 16 rows the arithmetic is less than that: 2 n k d operations
+// FP16 terms first (16-bit ones off TMA's alignment copied): w is read twice and
+// written once before the products read it again. Up to 16 rows the arithmetic is less than that: 2 n k d operations
 // at n = 16 are 8 a byte of w. Here w is read once forward and twice backward.
 //
 // Scores: x lies in shared memory; a warp takes four prototypes at a time, its
@@ -21,6 +21,7 @@
 #include <cuda_runtime.h>
 
 #include <cmath>
+#include <type_traits>
 
 #include "elem.h"
 #include "engine.h"
@@ -33,14 +34,14 @@ namespace {
 using tc::pdl_trigger;
 
 constexpr int THREADS = 256;
-constexpr long MOST_ROWS = 16, MOST_COLUMNS = 1024;
+constexpr long MOST_ROWS = 16, MOST_HALF_ROWS = 4, MOST_COLUMNS = 1024;
 constexpr long MOST_PROTOTYPES = 1l << 22;  // P is then at most 256 MB
 constexpr int CHUNK = 32;  // prototypes whose P a block holds (128: the same times)
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct Few {
-  const float* x;
-  const float* w;
+  const void* x;
+  const void* w;
   long n, d, k, ldx, ldw;
   const uint32_t* targets;
   float scale;
@@ -53,8 +54,9 @@ struct Few {
   int one_dloss;
   float* p;     // k x NR
   float* dx;    // blocks x n x d, or null
-  float* dw;    // or null
+  void* dw;     // or null
   long lddw;
+  int dwtype;
 };
 
 __device__ __forceinline__ float ex(float v) {
@@ -70,7 +72,7 @@ __device__ __forceinline__ void fold(float& m, float& s, float mv, float sv) {
   m = top;
 }
 
-template <int NR, bool BACKWARD>
+template <typename T, int NR, bool BACKWARD>
 __global__ void __launch_bounds__(THREADS, 2) k_few_scores(Few F) {
   pdl_trigger();
   pdl_wait();
@@ -81,7 +83,7 @@ __global__ void __launch_bounds__(THREADS, 2) k_few_scores(Few F) {
   const int d = (int)F.d, dp = (d + 31) / 32 * 32;
   for (int t = threadIdx.x; t < NR * dp; t += THREADS) {
     const int i = t / dp, c = t % dp;
-    xs[t] = i < F.n && c < d ? F.x[i * F.ldx + c] : 0.0f;
+    xs[t] = i < F.n && c < d ? to_f32(static_cast<const T*>(F.x)[i * F.ldx + c]) : 0.0f;
   }
   __syncthreads();
   // After the halving a lane holds the sums of this row, V / 32 (at least one)
@@ -96,9 +98,10 @@ __global__ void __launch_bounds__(THREADS, 2) k_few_scores(Few F) {
   }
   const long step = (long)gridDim.x * (THREADS / 32) * 4;
   for (long p0 = ((long)blockIdx.x * (THREADS / 32) + warp) * 4; p0 < F.k; p0 += step) {
-    const float* w[4];
+    const T* w[4];
 #pragma unroll
-    for (int q = 0; q < 4; q++) w[q] = F.w + min(p0 + q, F.k - 1) * F.ldw;
+    for (int q = 0; q < 4; q++) 
+      w[q] = static_cast<const T*>(F.w) + min(p0 + q, F.k - 1) * F.ldw;
     float a[V];
 #pragma unroll
     for (int j = 0; j < V; j++) a[j] = 0.0f;
@@ -106,7 +109,7 @@ __global__ void __launch_bounds__(THREADS, 2) k_few_scores(Few F) {
     for (int c = lane; c < dp; c += 32) {
       float v[4];
 #pragma unroll
-      for (int q = 0; q < 4; q++) v[q] = c < d ? w[q][c] : 0.0f;
+      for (int q = 0; q < 4; q++) v[q] = c < d ? to_f32(w[q][c]) : 0.0f;
 #pragma unroll
       for (int r = 0; r < NR; r++) {
         const float xv = xs[r * dp + c];
@@ -163,7 +166,7 @@ __global__ void __launch_bounds__(THREADS, 2) k_few_scores(Few F) {
   }
 }
 
-template <int NR>
+template <typename T, int NR>
 __global__ void __launch_bounds__(1024) k_few_grads(Few F, long per) {
   pdl_trigger();
   pdl_wait();
@@ -173,16 +176,17 @@ __global__ void __launch_bounds__(1024) k_few_grads(Few F, long per) {
   float x[NR], dx[NR];
 #pragma unroll
   for (int i = 0; i < NR; i++) {
-    x[i] = has && i < F.n ? F.x[i * F.ldx + c] : 0.0f;
+    x[i] = has && i < F.n ? to_f32(static_cast<const T*>(F.x)[i * F.ldx + c]) : 0.0f;
     dx[i] = 0.0f;
   }
   const long j0 = blockIdx.x * per, j1 = min(j0 + per, F.k);
   // The next four prototypes' elements are on their way while four are used;
   // past the block's last one they are 0.
-  float w[4];
+  T w[4];
   auto fetch = [&](long j) {
 #pragma unroll
-    for (int q = 0; q < 4; q++) w[q] = has && j + q < j1 ? F.w[(j + q) * F.ldw + c] : 0.0f;
+    for (int q = 0; q < 4; q++)
+      w[q] = has && j + q < j1 ? static_cast<const T*>(F.w)[(j + q) * F.ldw + c] : from_f32<T>(0.0f);
   };
   fetch(j0);
   for (long base = j0; base < j1; base += CHUNK) {
@@ -192,7 +196,7 @@ __global__ void __launch_bounds__(1024) k_few_grads(Few F, long per) {
       ps[t] = t < count * NR ? F.p[base * NR + t] : 0.0f;
     __syncthreads();
     for (int p = 0; p < count; p += 4) {
-      const float now[4] = {w[0], w[1], w[2], w[3]};
+      const float now[4] = {to_f32(w[0]), to_f32(w[1]), to_f32(w[2]), to_f32(w[3])};
       fetch(base + p + 4);
 #pragma unroll
       for (int q = 0; q < 4; q++) {
@@ -207,7 +211,13 @@ __global__ void __launch_bounds__(1024) k_few_grads(Few F, long per) {
             dw = fmaf(pr[u], x[i + u], dw);
           }
         }
-        if (F.dw && has && p + q < count) F.dw[(base + p + q) * F.lddw + c] = dw;
+        if (F.dw && has && p + q < count) {
+          const size_t at = (size_t)((base + p + q) * F.lddw + c);
+          if constexpr (sizeof(T) == 4)
+            static_cast<float*>(F.dw)[at] = dw;
+          else
+            store_any(F.dw, F.dwtype, at, dw);
+        }
       }
     }
   }
@@ -221,7 +231,8 @@ __global__ void __launch_bounds__(1024) k_few_grads(Few F, long per) {
 
 // dx: the blocks' parts in order, 32 elements a block of 8 slices.
 __global__ void __launch_bounds__(THREADS)
-    k_few_sum(const float* __restrict__ part, int blocks, long total, long d, float* dx, long lddx) {
+    k_few_sum(const float* __restrict__ part, int blocks, long total, long d, void* dx, long lddx,
+              int type) {
   pdl_trigger();
   pdl_wait();
   __shared__ float joint[8][33];
@@ -238,13 +249,13 @@ __global__ void __launch_bounds__(THREADS)
   s = 0.0f;
 #pragma unroll
   for (int v = 0; v < 8; v++) s += joint[v][c];
-  dx[t / d * lddx + t % d] = s;
+  store_any(dx, type, (size_t)(t / d * lddx + t % d), s);
 }
 
 Few few(const LinearCeArgs& a) {
   Few F{};
-  F.x = static_cast<const float*>(a.x);
-  F.w = static_cast<const float*>(a.w);
+  F.x = a.x;
+  F.w = a.w;
   F.n = (long)a.n;
   F.d = (long)a.d;
   F.k = (long)a.k;
@@ -255,20 +266,28 @@ Few few(const LinearCeArgs& a) {
   return F;
 }
 
-template <int NR, bool BACKWARD>
+template <typename T, int NR, bool BACKWARD>
 void scores(eb_engine* e, const Few& F, unsigned grid) {
   const size_t smem = (size_t)NR * ((F.d + 31) / 32 * 32) * 4;
-  const auto kern = k_few_scores<NR, BACKWARD>;
+  const auto kern = k_few_scores<T, NR, BACKWARD>;
   static std::atomic<uint64_t> allowed{0};
   allow_smem(e, kern, (size_t)NR * MOST_COLUMNS * 4, allowed);
   launch_pdl(e, kern, dim3(grid), dim3(THREADS), smem, F);
   e->stats.kernel_launches++;
 }
-template <bool BACKWARD>
-void scores_of(eb_engine* e, const Few& F, unsigned grid) {
-  if (F.n <= 4) return scores<4, BACKWARD>(e, F, grid);
-  if (F.n <= 8) return scores<8, BACKWARD>(e, F, grid);
-  scores<16, BACKWARD>(e, F, grid);
+template <typename T, int NR>
+void grads(eb_engine* e, const Few& F, unsigned grid, unsigned threads, long per) {
+  launch_pdl(e, k_few_grads<T, NR>, dim3(grid), dim3(threads), 0, F, per);
+  e->stats.kernel_launches++;
+}
+// Calls f(T{}, NR) for x's type and the padded number of rows.
+template <typename F>
+void by_type(int dtype, long n, F&& f) {
+  if (dtype == EB_BF16) return f(__nv_bfloat16{}, std::integral_constant<int, 4>{});
+  if (dtype == EB_F16) return f(__half{}, std::integral_constant<int, 4>{});
+  if (n <= 4) return f(float{}, std::integral_constant<int, 4>{});
+  if (n <= 8) return f(float{}, std::integral_constant<int, 8>{});
+  f(float{}, std::integral_constant<int, 16>{});
 }
 unsigned scores_grid(eb_engine* e, const LinearCeArgs& a) {
   return (unsigned)std::min<size_t>((a.k + 31) / 32, (size_t)e->num_sms * 2);
@@ -276,15 +295,19 @@ unsigned scores_grid(eb_engine* e, const LinearCeArgs& a) {
 
 }  // namespace
 
-// Up to 16 rows; forward and backward in us, here and on the tensor cores:
+// f32 up to 16 rows; forward and backward in us, here and on the tensor cores:
 //   1 x 40,000 x 1024 43 and 134, 152 and 244; 16 x 40,000 x 1024 77 and 214, 151 and 240;
 //   15 x 41,927 x 547 48 and 156, 102 and 190; 5 x 7,689 x 807 13 and 30, 34 and 58;
 //   16 x 60,000 x 8 16 and 47, 41 and 51; 1 x 760 x 506 8 and 12, 18 and 25.
 // With more rows the backward pass would lose: at 16 it is bound by its 4 n k d
-// operations in FP32 as much as by memory.
+// operations in FP32 as much as by memory. 16-bit types whose prototypes TMA
+// cannot read as they lie (a copy of w, not a split) up to 4 rows:
+//   1 x 41,524 x 420 bf16 17 and 59, 31 and 71; 4 x 40,000 x 1023 34 and 122, 62 and 135;
+//   2 x 410 x 924 10 and 14, 12 and 16; with more: 9 x 16,885 x 535 22 and 62, 22 and 48.
 bool linear_ce_is_few(const LinearCeArgs& a) {
-  return a.dtype == EB_F32 && (long)a.n <= MOST_ROWS && (long)a.d <= MOST_COLUMNS &&
-         (long)a.k <= MOST_PROTOTYPES;
+  const bool few = a.dtype == EB_F32 ? (long)a.n <= MOST_ROWS
+                                     : a.ldw % 8 && (long)a.n <= MOST_HALF_ROWS;
+  return few && (long)a.d <= MOST_COLUMNS && (long)a.k <= MOST_PROTOTYPES;
 }
 
 int linear_ce_few_parts(eb_engine* e, const LinearCeArgs& a) { return (int)scores_grid(e, a); }
@@ -293,7 +316,9 @@ void linear_ce_few(eb_engine* e, const LinearCeArgs& a, float2* part, float* zt)
   Few F = few(a);
   F.part = part;
   F.zt = zt;
-  scores_of<false>(e, F, scores_grid(e, a));
+  by_type(a.dtype, F.n, [&](auto t, auto rows) {
+    scores<decltype(t), decltype(rows)::value, false>(e, F, scores_grid(e, a));
+  });
 }
 
 void linear_ce_few_backward(eb_engine* e, const LinearCeArgs& a, const LinearCeGrads& g) {
@@ -303,21 +328,24 @@ void linear_ce_few_backward(eb_engine* e, const LinearCeArgs& a, const LinearCeG
   F.dloss = g.dloss;
   F.one_dloss = g.one_dloss;
   F.p = e->scratch_get<float>("ce_p", a.k * nr);
-  scores_of<true>(e, F, scores_grid(e, a));
+  by_type(a.dtype, F.n, [&](auto t, auto rows) {
+    scores<decltype(t), decltype(rows)::value, true>(e, F, scores_grid(e, a));
+  });
   const unsigned threads = (unsigned)((a.d + 31) / 32 * 32);  // a column each
   const long most = (long)e->num_sms * (1024 / std::max(threads, 64u));
   const long per = std::max<long>((F.k + most - 1) / most, 4);
   const unsigned grid = (unsigned)((F.k + per - 1) / per);
   F.dx = g.dx ? e->scratch_get<float>("ce_dx", (size_t)grid * a.n * a.d) : nullptr;
-  F.dw = static_cast<float*>(g.dw);
+  F.dw = g.dw;
   F.lddw = (long)g.lddw;
-  const auto kern = nr == 4 ? k_few_grads<4> : nr == 8 ? k_few_grads<8> : k_few_grads<16>;
-  launch_pdl(e, kern, dim3(grid), dim3(threads), 0, F, per);
-  e->stats.kernel_launches++;
+  F.dwtype = g.dwtype;
+  by_type(a.dtype, F.n, [&](auto t, auto rows) {
+    grads<decltype(t), decltype(rows)::value>(e, F, grid, threads, per);
+  });
   if (!g.dx) return;
   const long total = F.n * F.d;
   launch_pdl(e, k_few_sum, dim3((unsigned)((total + 31) / 32)), dim3(THREADS), 0,
-             (const float*)F.dx, (int)grid, total, F.d, static_cast<float*>(g.dx), (long)g.lddx);
+             (const float*)F.dx, (int)grid, total, F.d, g.dx, (long)g.lddx, g.dxtype);
   e->stats.kernel_launches++;
 }
 

@@ -462,7 +462,7 @@ int eb_layer_norm_backward(eb_engine* e, const eb_buf* dy, size_t lddy, const eb
  * loss and lse f32, n each. Products: 16-bit types on the tensor cores as
  * they are; f32 as two scaled FP16 terms each (22 bits), three products
  * (a non-finite element counts as NaN), or in FP32 where k and d are small or
- * there are up to 16 rows. Scratch: f32 operands' copies (as large as x and w;
+ * there are few rows (up to 16; of 16-bit types 4, off 16-byte alignment). Scratch: f32 operands' copies (as large as x and w;
  * not for those), and up to 256 MB. */
 int eb_linear_ce(eb_engine* e, const eb_buf* x, size_t n, size_t d, size_t ldx, const eb_buf* w,
                  size_t k, size_t ldw, const eb_buf* targets, float scale, eb_buf* loss,

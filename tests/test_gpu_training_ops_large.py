@@ -162,6 +162,16 @@ def test_linear_cross_entropy_few_f32_rows(eng, n, k, d):
         c.check(c.run(eng, pad=pad))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=NAMES.get)
+@pytest.mark.parametrize("n,k,d", [(1, 3, 93), (4, 700, 1), (5, 4097, 333), (8, 129, 66), (9, 31, 1023),
+                                   (16, 9000, 420), (16, 500, 1025)])
+def test_linear_cross_entropy_few_16_bit_rows_off_alignment(eng, n, k, d, dtype):
+    for pad in (0, 3):
+        c = Ce(n, k, d, dtype, n + k + d, per_row=n % 2 == 0)
+        c.check(c.run(eng, pad=pad))
+    c.check(c.run(eng, dxt=torch.float32, dwt=torch.float32))
+
+
 def test_linear_cross_entropy_few_f32_rows_one_gradient_and_bits(eng):
     c = Ce(7, 1003, 129, torch.float32, 5)
     both, again = c.run(eng), c.run(eng)
