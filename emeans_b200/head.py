@@ -52,31 +52,35 @@ class ClusterHead:
         self.optimizer = eb.AdamW(engine, [tensor(self.weight, self.dweight, 0.0),
                                            tensor(self.bias, self.dbias, 0.0),
                                            tensor(self.w, self.dw, weight_decay)])
+        self.dloss = engine.zeros_f32(1)
         self.steps = 0
         self._rows = 0
+        self._last = None  # (losses, rows, labelled rows) of the last step
 
     def _room(self, n: int):
         """Per-row buffers for batches of up to n rows."""
         if n <= self._rows:
             return
         e, f = self.engine, self.engine.zeros_f32
-        self.mean, self.rstd, self.loss, self.lse = f(n), f(n), f(n), f(n)
+        self.mean, self.rstd, self.lse = f(n), f(n), f(n)
         self.y, self.dy = f(n * self.d), f(n * self.d)
-        self.dloss = f(1)
+        # Losses of the steps and of other calls apart: ``last_loss`` reads the
+        # former whatever was called in between.
+        self.step_loss, self.loss = f(n), f(n)
         self.targets = e.zeros_u32(n)
         self._rows = n
 
-    def _forward(self, x: eb.Buffer, n: int, labels):
+    def _forward(self, x: eb.Buffer, n: int, labels, loss: str):
         labels = np.ascontiguousarray(labels, np.uint32)
         if labels.shape != (n,):
             raise ValueError("one label per row")
         self._room(n)
-        e, d = self.engine, self.d
+        e, d, loss = self.engine, self.d, getattr(self, loss)
         self.targets.write(0, labels)
         e.layer_norm(x, n, d, self.weight, self.bias, self.y, mean=self.mean, rstd=self.rstd)
-        e.linear_cross_entropy(self.y, n, d, self.w, self.k, self.targets, self.loss, self.lse,
+        e.linear_cross_entropy(self.y, n, d, self.w, self.k, self.targets, loss, self.lse,
                                scale=self.scale)
-        return int((labels != eb.IGNORE).sum())
+        return loss, n, int((labels != eb.IGNORE).sum())
 
     def _buffer(self, x):
         if isinstance(x, eb.Buffer):
@@ -84,13 +88,17 @@ class ClusterHead:
         b = self.engine.upload_f32(x)
         return b, len(b) // self.d
 
+    @staticmethod
+    def _mean(loss: eb.Buffer, n: int, kept: int) -> float:
+        return float(loss.read(0, n).sum(dtype=np.float64)) / max(kept, 1)
+
     def step(self, x, labels, lr: float, beta1: float = 0.9, beta2: float = 0.999) -> None:
         """One gradient step on the mean loss of rows x (an f32 Buffer or host
         array, n x d) with ``labels`` (n; ``IGNORE`` for rows without one).
         Queued on the engine's stream; ``last_loss`` waits for it."""
         x, n = self._buffer(x)
-        kept = self._forward(x, n, labels)
-        self._kept = (n, kept)
+        self._last = self._forward(x, n, labels, "step_loss")
+        kept = self._last[2]
         e, d = self.engine, self.d
         self.dloss.write(0, [1.0 / max(kept, 1)])
         e.linear_cross_entropy_backward(self.y, n, d, self.w, self.k, self.targets, self.lse,
@@ -102,14 +110,14 @@ class ClusterHead:
 
     def last_loss(self) -> float:
         """The mean loss of the last ``step``'s labelled rows, before it."""
-        n, kept = self._kept
-        return float(self.loss.read(0, n).sum(dtype=np.float64)) / max(kept, 1)
+        if self._last is None:
+            raise RuntimeError("no step has been taken")
+        return self._mean(*self._last)
 
     def evaluate(self, x, labels) -> float:
         """The mean loss of rows x."""
         x, n = self._buffer(x)
-        kept = self._forward(x, n, labels)
-        return float(self.loss.read(0, n).sum(dtype=np.float64)) / max(kept, 1)
+        return self._mean(*self._forward(x, n, labels, "loss"))
 
     def predict(self, x) -> np.ndarray:
         """The best-scoring prototype of each row: the exact top-1 of the
