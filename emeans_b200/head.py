@@ -54,7 +54,7 @@ class ClusterHead:
                                            tensor(self.w, self.dw, weight_decay)])
         self.dloss = engine.zeros_f32(1)
         self.steps = 0
-        self._rows = 0
+        self._rows = -1
         self._last = None  # (losses, rows, labelled rows) of the last step
 
     def _room(self, n: int):

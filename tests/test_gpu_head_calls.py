@@ -34,3 +34,16 @@ def test_last_loss_is_the_last_steps_whatever_is_called_after_it(engine):
     assert head.last_loss() == before
     head.step(x[:40], labels[:40], lr=1e-2)
     assert head.last_loss() != before
+
+
+def test_batches_of_no_rows(engine):
+    """No loss, no predictions, and a step whose gradients are zero: the first
+    moments stay zero and the weights take the decay alone."""
+    head = ClusterHead(engine, D, K, seed=2, weight_decay=0.5)
+    x, labels = batch(0, 1)
+    w = head.w.read()
+    assert head.evaluate(x, labels) == 0.0 and head.predict(x).shape == (0,)
+    head.step(x, labels, lr=1e-2)
+    assert head.last_loss() == 0.0
+    keep = np.float32(1.0 - 1e-2 * 0.5)
+    assert np.array_equal(head.w.read(), w * keep) and np.array_equal(head.weight.read(), np.ones(D))
