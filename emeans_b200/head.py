@@ -83,10 +83,15 @@ class ClusterHead:
         return loss, n, int((labels != eb.IGNORE).sum())
 
     def _buffer(self, x):
-        if isinstance(x, eb.Buffer):
-            return x, len(x) // self.d
-        b = self.engine.upload_f32(x)
-        return b, len(b) // self.d
+        """x on the engine, and its rows."""
+        if not isinstance(x, eb.Buffer):
+            x = np.asarray(x, np.float32)
+            if x.ndim > 1 and x.shape[-1] != self.d:
+                raise ValueError(f"rows of {x.shape[-1]} elements, the head's have {self.d}")
+            x = self.engine.upload_f32(x)
+        if len(x) % self.d:
+            raise ValueError(f"{len(x)} elements are not rows of {self.d}")
+        return x, len(x) // self.d
 
     @staticmethod
     def _mean(loss: eb.Buffer, n: int, kept: int) -> float:

@@ -47,3 +47,14 @@ def test_batches_of_no_rows(engine):
     assert head.last_loss() == 0.0
     keep = np.float32(1.0 - 1e-2 * 0.5)
     assert np.array_equal(head.w.read(), w * keep) and np.array_equal(head.weight.read(), np.ones(D))
+
+
+def test_rows_of_another_width_are_refused(engine):
+    head = ClusterHead(engine, D, K)
+    for x in (np.zeros((10, 2 * D), np.float32), np.zeros((3 * D, 1), np.float32)):
+        with pytest.raises(ValueError, match="rows of"):
+            head.step(x, np.zeros(x.size // D, np.uint32), lr=1e-3)
+    for x in (np.zeros(5 * D + 1, np.float32), engine.zeros_f32(5 * D + 1)):
+        with pytest.raises(ValueError, match="not rows of"):
+            head.evaluate(x, np.zeros(5, np.uint32))
+    assert np.isfinite(head.evaluate(np.zeros(5 * D, np.float32), np.zeros(5, np.uint32)))
