@@ -346,22 +346,26 @@ __global__ void __launch_bounds__(G > 32 ? G : WARP_BLOCK) k_norm_bwd(NormBwd P)
     copies_wait();
     const T *xi = x + i * P.ldx, *gi = dy + i * P.lddy;
     float s1 = 0.0f, s2 = 0.0f;
-    auto add = [&](int k, float g, float v, float wk) {
-      const float u = (v - m) * rs, h = g * wk;
+    // Elements outside the row have g = 0 and v = 0. Their mean is 0 as well: (0 -
+    // mean) rstd overflows where rows of 1e36 and more have no spread, and 0
+    // times it would be NaN.
+    auto add = [&](int k, float g, float v, float mean, float wk) {
+      const float u = (v - mean) * rs, h = g * wk;
       dw[k] = fmaf(g, u, dw[k]);
       db[k] += g;
-      s1 += h;  // elements outside the row have g = 0
+      s1 += h;
       s2 = fmaf(h, u, s2);
     };
 #pragma unroll
     for (int j = 0; j < NV; j++) {
       const Pack<T, V> xr = rx.get(stage, j, xi, r), gr = rg.get(stage, j, gi, r);
+      const float mean_j = r.live(j) ? m : 0.0f;
 #pragma unroll
       for (int q = 0; q < V; q++)
-        add(j * V + q, to_f32(gr.v[q]), to_f32(xr.v[q]), w[(j * G + r.t) * V + q]);
+        add(j * V + q, to_f32(gr.v[q]), to_f32(xr.v[q]), mean_j, w[(j * G + r.t) * V + q]);
     }
 #pragma unroll
-    for (int q = 0; q < NX; q++) add(EPT + q, ge[q], xe[q], wx[q]);
+    for (int q = 0; q < NX; q++) add(EPT + q, ge[q], xe[q], r.edge(q) >= 0 ? m : 0.0f, wx[q]);
     const float2 c = group_sum2<G>(s1, s2, slot, turn);
     const float c1 = c.x * P.inv_d, c2 = c.y * P.inv_d;
     if (P.dx) {
