@@ -7,6 +7,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstring>
+#include <initializer_list>
 #include <string>
 #include <unordered_set>
 
@@ -96,6 +97,30 @@ bool overlap(const eb_buf* a, const eb_buf* b) {
   if (!a || !b || a->len == 0 || b->len == 0) return false;
   const char *pa = static_cast<const char*>(a->ptr), *pb = static_cast<const char*>(b->ptr);
   return pa < pb + b->len * eb::dtype_bytes(b->dtype) && pb < pa + a->len * eb::dtype_bytes(a->dtype);
+}
+
+// The part of a buffer that a call uses: its first `len` elements, or (rows of d
+// elements `ld` apart) up to the last row's end.
+struct Part {
+  const char* ptr = nullptr;
+  size_t bytes = 0;
+  Part(const eb_buf* b, size_t len)
+      : ptr(b ? static_cast<const char*>(b->ptr) : nullptr),
+        bytes(b ? len * eb::dtype_bytes(b->dtype) : 0) {}
+  Part(const eb_buf* b, size_t rows, size_t d, size_t ld) : Part(b, rows ? (rows - 1) * ld + d : 0) {}
+  bool meets(const Part& o) const {
+    return bytes && o.bytes && ptr < o.ptr + o.bytes && o.ptr < ptr + bytes;
+  }
+};
+
+// The outputs of a call share no memory with one another, nor with its inputs; a
+// pair that may (in place) is not among them.
+void need_apart(std::initializer_list<Part> outputs, std::initializer_list<Part> inputs) {
+  for (auto a = outputs.begin(); a != outputs.end(); ++a) {
+    for (auto b = outputs.begin(); b != a; ++b)
+      eb::ensure(!a->meets(*b), "an output overlaps another");
+    for (const Part& in : inputs) eb::ensure(!a->meets(in), "an output overlaps an input");
+  }
 }
 
 // check_select (core/mod.rs:432-439).
@@ -864,6 +889,9 @@ int eb_layer_norm(eb_engine* e, const eb_buf* x, size_t rows, size_t d, size_t l
       need_type(b, EB_F32, "mean and rstd");
       ensure(b->len >= rows, "mean and rstd must hold one element a row");
     }
+    const Part m(mean, rows), r(rstd, rows);
+    need_apart({Part(y, rows, d, a.ldy), m, r}, {Part(weight, d), Part(bias, d)});
+    need_apart({m, r}, {Part(x, rows, d, a.ldx)});
     DeviceGuard g(e);
     touched(e, y);
     touched(e, mean);
@@ -922,6 +950,10 @@ int eb_layer_norm_backward(eb_engine* e, const eb_buf* dy, size_t lddy, const eb
              "dweight and dbias must be f32 or of x's type");
       ensure(b->len >= d, "dweight and dbias must hold d elements");
     }
+    const Part dwp(dweight, d), dbp(dbias, d);
+    need_apart({Part(dx, rows, d, a.lddx), dwp, dbp},
+               {Part(weight, d), Part(mean, rows), Part(rstd, rows)});
+    need_apart({dwp, dbp}, {Part(dy, rows, d, a.lddy), Part(x, rows, d, a.ldx)});
     DeviceGuard g(e);
     touched(e, dx);
     touched(e, dweight);
