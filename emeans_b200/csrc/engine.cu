@@ -1078,7 +1078,15 @@ int eb_adamw_create(eb_engine* e, const eb_adamw_tensor* t, size_t count, eb_ada
     *out = nullptr;
     if (count) need(t, "tensors");
     ensure(count <= 0x7FFFFFFFull, "too many tensors");
-    std::unordered_set<const void*> seen;
+    struct Range {
+      const char *lo, *hi;
+      bool written;
+    };
+    std::vector<Range> ranges;
+    auto use = [&](const eb_buf* b, size_t n, bool written) {
+      const char* p = static_cast<const char*>(b->ptr);
+      ranges.push_back({p, p + n * eb::dtype_bytes(b->dtype), written});
+    };
     auto plan = std::make_unique<eb_adamw>();
     for (size_t i = 0; i < count; i++) {
       need(t[i].p, "p");
@@ -1111,9 +1119,22 @@ int eb_adamw_create(eb_engine* e, const eb_adamw_tensor* t, size_t count, eb_ada
       if (len == 0) continue;
       for (eb_buf* b : {t[i].p, t[i].m, t[i].v, t[i].m_scale, t[i].v_scale, t[i].copy}) {
         if (!b) continue;
-        ensure(seen.insert(b->ptr).second, "a buffer is written twice");
+        const bool scale = b == t[i].m_scale || b == t[i].v_scale;
+        use(b, scale ? (len + EB_ADAMW_BLOCK - 1) / EB_ADAMW_BLOCK : len, true);
         plan->written.push_back(b);
       }
+      use(t[i].g, len, false);
+    }
+    // Blocks take the tensors in any order: what one writes, no other may touch.
+    // Gradients are only read, and may be shared.
+    std::sort(ranges.begin(), ranges.end(),
+              [](const Range& a, const Range& b) { return a.lo < b.lo; });
+    const char *written = nullptr, *read = nullptr;  // ends of the ranges so far
+    for (const Range& r : ranges) {
+      ensure(r.lo >= written, r.written ? "a buffer is written twice, in part or whole"
+                                        : "g overlaps a buffer that is written");
+      ensure(!r.written || r.lo >= read, "g overlaps a buffer that is written");
+      (r.written ? written : read) = std::max(r.written ? written : read, r.hi);
     }
     DeviceGuard g(e);
     try {

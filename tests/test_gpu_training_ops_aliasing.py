@@ -58,3 +58,35 @@ def test_layer_norm_backward_outputs_apart(engine):
     call(dx=dy)()                   # in place
     call(dweight=at(272, 16), dbias=at(288, 16))()
     engine.sync()
+
+
+def test_adamw_buffers_apart(engine):
+    """Of one tensor and of several: no buffer is written twice, in part either,
+    and no gradient lies over one that is written. Gradients may be shared."""
+    n = 300
+    z = engine.zeros
+
+    def tensor(**kw):
+        return eb.AdamWTensor(**{**dict(p=z(eb.F32, n), g=z(eb.F32, n), m=z(eb.F32, n),
+                                        v=z(eb.F32, n)), **kw})
+
+    at = room(engine, 2000)
+    byte = room(engine, 4000, eb.F8)
+    eight = dict(m=byte(0, n), v=byte(320, n), m_scale=at(0, 2), v_scale=at(4, 2))
+    a = tensor(p=at(0, n))
+    for ts, why in (([tensor(p=at(0, n), m=at(200, n))], "written twice"),
+                    ([a, tensor(v=at(296, n))], "written twice"),
+                    ([a, tensor(p=at(0, n))], "written twice"),
+                    ([tensor(p=at(0, n), g=at(0, n))], "g overlaps"),
+                    ([a, tensor(g=at(100, n))], "g overlaps"),
+                    ([tensor(g=at(100, n)), a], "g overlaps"),
+                    ([tensor(g=at(296, n)), a], "g overlaps"),
+                    ([tensor(**{**eight, "v": byte(288, n)})], "written twice"),
+                    ([tensor(**{**eight, "m_scale": at(4, 2)})], "written twice"),
+                    ([tensor(**eight), tensor(g=at(0, n))], "g overlaps")):
+        refused(lambda: eb.AdamW(engine, ts), why)
+    one = z(eb.F32, n)
+    plan = eb.AdamW(engine, [tensor(p=at(0, n), m=at(300, n), v=at(600, n), g=one), tensor(g=one),
+                             tensor(**{**eight, "m_scale": at(1200, 2), "v_scale": at(1204, 2)})])
+    plan.step(lr=1e-3, step=1)
+    engine.sync()
