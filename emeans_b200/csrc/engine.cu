@@ -99,6 +99,14 @@ bool overlap(const eb_buf* a, const eb_buf* b) {
   return pa < pb + b->len * eb::dtype_bytes(b->dtype) && pb < pa + a->len * eb::dtype_bytes(a->dtype);
 }
 
+// The buffers of a call (null: not given) are on the engine's GPU. Another
+// engine's buffers are taken where it shares the GPU: two engines on one stream,
+// or a caller who orders their streams.
+void need_here(const eb_engine* e, std::initializer_list<const eb_buf*> bufs) {
+  for (const eb_buf* b : bufs)
+    eb::ensure(!b || b->device == e->device, "a buffer is on another GPU than the engine");
+}
+
 // The part of a buffer that a call uses: its first `len` elements, or (rows of d
 // elements `ld` apart) up to the last row's end.
 struct Part {
@@ -139,6 +147,7 @@ namespace eb {
 eb_buf* new_buf(eb_engine* e, int dtype, size_t len) {
   auto* b = new eb_buf;
   b->dtype = dtype;
+  b->device = e->device;
   b->len = len;
   b->owned = true;
   size_t bytes = std::max<size_t>(len * dtype_bytes(dtype), 16);
@@ -406,6 +415,7 @@ int eb_buf_wrap(eb_engine* e, int dtype, void* dev_ptr, size_t len, eb_buf** out
     b->ptr = dev_ptr;
     b->len = len;
     b->dtype = dtype;
+    b->device = e->device;
     b->owned = false;
     *out = b;
   });
@@ -889,6 +899,7 @@ int eb_layer_norm(eb_engine* e, const eb_buf* x, size_t rows, size_t d, size_t l
       need_type(b, EB_F32, "mean and rstd");
       ensure(b->len >= rows, "mean and rstd must hold one element a row");
     }
+    need_here(e, {x, weight, bias, y, mean, rstd});
     const Part m(mean, rows), r(rstd, rows);
     need_apart({Part(y, rows, d, a.ldy), m, r}, {Part(weight, d), Part(bias, d)});
     need_apart({m, r}, {Part(x, rows, d, a.ldx)});
@@ -950,6 +961,7 @@ int eb_layer_norm_backward(eb_engine* e, const eb_buf* dy, size_t lddy, const eb
              "dweight and dbias must be f32 or of x's type");
       ensure(b->len >= d, "dweight and dbias must hold d elements");
     }
+    need_here(e, {dy, x, weight, mean, rstd, dx, dweight, dbias});
     const Part dwp(dweight, d), dbp(dbias, d);
     need_apart({Part(dx, rows, d, a.lddx), dwp, dbp},
                {Part(weight, d), Part(mean, rows), Part(rstd, rows)});
@@ -1022,6 +1034,7 @@ int eb_linear_ce(eb_engine* e, const eb_buf* x, size_t n, size_t d, size_t ldx, 
     need_type(loss, EB_F32, "loss");
     need_type(lse, EB_F32, "lse");
     ensure(loss->len >= n && lse->len >= n, "loss and lse must hold one element a row");
+    need_here(e, {x, w, targets, loss, lse});
     ensure(!overlap(loss, lse), "loss overlaps lse");
     for (const eb_buf* in : {x, w, targets})
       ensure(!overlap(loss, in) && !overlap(lse, in), "an output overlaps an input");
@@ -1042,6 +1055,7 @@ int eb_linear_ce_backward(eb_engine* e, const eb_buf* x, size_t n, size_t d, siz
     ensure(lse->len >= n, "lse must hold one element a row");
     need_type(dloss, EB_F32, "dloss");
     ensure(dloss->len == 1 || dloss->len >= n, "dloss must hold one element, or one a row");
+    need_here(e, {x, w, targets, lse, dloss, dx, dw});
     eb::LinearCeGrads q{};
     for (const eb_buf* b : {dx, dw}) {
       if (!b) continue;
@@ -1093,6 +1107,7 @@ int eb_adamw_create(eb_engine* e, const eb_adamw_tensor* t, size_t count, eb_ada
       need(t[i].g, "g");
       need(t[i].m, "m");
       need(t[i].v, "v");
+      need_here(e, {t[i].p, t[i].g, t[i].m, t[i].v, t[i].m_scale, t[i].v_scale, t[i].copy});
       const size_t len = t[i].p->len;
       for (const eb_buf* b : {(const eb_buf*)t[i].p, t[i].g})
         ensure(b->dtype == EB_F32 || b->dtype == EB_BF16, "p and g must be f32 or bf16 buffers");

@@ -86,6 +86,7 @@ struct eb_buf {
   void* ptr = nullptr;
   size_t len = 0;
   int dtype = EB_F32;
+  int device = -1;  // where the memory is: the engine's that made or wrapped it
   bool owned = false;
   // Bumped by every host write; caches derived from the buffer compare it.
   uint64_t version = 0;

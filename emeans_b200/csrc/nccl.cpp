@@ -343,6 +343,7 @@ extern "C" int eb_group_exchange(eb_engine* e, size_t words, eb_buf** out) {
       b->ptr = e->px->base + eb::kPxFlagWords;
       b->len = words;
       b->dtype = EB_U32;
+      b->device = e->device;
       b->owned = false;
       *out = b;
     } else {
