@@ -55,7 +55,8 @@ constexpr float PSCALE = 16384.0f;  // f16 and f32: P is kept times 2^14
 enum Epi { LSE, PROB, OUT };
 
 // Scalars shared by a call's kernels (device scratch): bits of max|x|,
-// max|w| over the finite elements (f32 operands) and of max|dloss|.
+// max|w| over the finite elements (f32 operands) and of max|dloss| over the
+// rows with a target.
 enum { S_X, S_W, S_G, S_WORDS };
 
 // The power of two that brings a largest magnitude (its bits) below 2^15.
@@ -975,15 +976,16 @@ __global__ void __launch_bounds__(256)
   });
 }
 
-// Largest magnitude of the rows' loss gradients (finite ones), into a zeroed
-// word.
-__global__ void __launch_bounds__(256) k_ce_gmax(const float* __restrict__ g, long n,
-                                                 uint32_t* out) {
+// Largest magnitude of the rows' loss gradients (finite ones, of rows with a
+// target: what the others hold is not used), into a zeroed word.
+__global__ void __launch_bounds__(256)
+    k_ce_gmax(const float* __restrict__ g, const uint32_t* __restrict__ targets, long n, long k,
+              uint32_t* out) {
   pdl_trigger();
   pdl_wait();
   uint32_t m = 0;
   for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long)gridDim.x * 256)
-    m = max(m, finite_bits(g[i]));
+    if ((long)targets[i] < k) m = max(m, finite_bits(g[i]));
   m = block_max(m);
   if (threadIdx.x == 0 && m) atomicMax(out, m);
 }
@@ -1447,7 +1449,8 @@ void linear_ce_backward(eb_engine* e, const LinearCeArgs& a, const LinearCeGrads
   if (!g.one_dloss) {
     EB_CUDA(cudaMemsetAsync(scal + S_G, 0, 4, e->stream));
     const unsigned grid = (unsigned)std::min<size_t>((a.n + 255) / 256, (size_t)e->num_sms);
-    launch_pdl(e, k_ce_gmax, dim3(grid), dim3(256), 0, g.dloss, (long)a.n, scal + S_G);
+    launch_pdl(e, k_ce_gmax, dim3(grid), dim3(256), 0, g.dloss, a.targets, (long)a.n, (long)a.k,
+               scal + S_G);
     e->stats.kernel_launches++;
   }
   Operand X, W;

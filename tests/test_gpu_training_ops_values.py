@@ -42,3 +42,92 @@ def test_layer_norm_backward_of_large_rows_without_spread(eng, d, dtype):
     within(dx, want, tol + HALF_ULP[dtype] * (want.abs() + tol), "dx")
     assert (dw == 0).all()
     within(db, dy.double().sum(0), rows * 2 * U32 * dy.double().abs().sum(0), "dbias")
+
+
+# ---------------------------------------------------------------- linear cross entropy
+
+
+class Values:
+    """One problem, run through the engine and in 64 bits, and the bounds of
+    each output by the row's own size (`check`)."""
+
+    def __init__(self, n, k, d, dtype, seed, ignored=0.1, scale=1.0):
+        g = gen(seed)
+        self.n, self.k, self.d, self.scale, self.dtype = n, k, d, scale, dtype
+        self.x, self.w = randn(g, n, d), 0.3 * randn(g, k, d)
+        t = torch.randint(0, k, (n,), generator=g, device="cuda")
+        drop = torch.rand(n, generator=g, device="cuda") < ignored
+        drop[3] = True
+        self.t = torch.where(drop, torch.full_like(t, eb.IGNORE), t)
+        self.dloss = randn(g, n)
+        self.rand = torch.rand(n, generator=g, device="cuda")
+
+    def run(self, e, outs=None):
+        """loss, lse, dx and dw; dx and dw of `outs`' type, or x's."""
+        n, k, d = self.n, self.k, self.d
+        self.x, self.w = self.x.to(self.dtype), self.w.to(self.dtype)
+        loss, lse = torch.empty(n, device="cuda"), torch.empty(n, device="cuda")
+        dx = torch.empty(n, d, device="cuda", dtype=outs or self.dtype)
+        dw = torch.empty(k, d, device="cuda", dtype=outs or self.dtype)
+        xb, wb, tb, lb = wrap(e, self.x), wrap(e, self.w), wrap(e, self.t.to(torch.uint32)), wrap(e, lse)
+        e.linear_cross_entropy(xb, n, d, wb, k, tb, wrap(e, loss), lb, scale=self.scale)
+        e.linear_cross_entropy_backward(xb, n, d, wb, k, tb, lb, wrap(e, self.dloss), wrap(e, dx),
+                                        wrap(e, dw), scale=self.scale)
+        e.sync()
+        return loss, lse, dx, dw
+
+    def check(self, got):
+        """Against 64 bits. A score is off by its products' roundings (2^-22
+        each for f32's terms) and sums (cut, at most d / 4 + 8 of them), and
+        by 2^-26 of its row's and its prototype's largest element for each of
+        the other's (what the terms of f32 may leave out). P: the scores'
+        errors, the exponential's, its own rounding (`keep`) and 2^-25 of the
+        row's loss gradient. The gradients: P's error through the other
+        operand, the products and sums again, and 2^-26 of each row's largest
+        element for each weight."""
+        loss, lse, dx, dw = got
+        X, W, s = self.x.double(), self.w.double(), self.scale
+        live = self.t != eb.IGNORE
+        t = torch.where(live, self.t, torch.zeros_like(self.t))[:, None]
+        f32 = self.dtype == torch.float32
+        Z = s * (X @ W.T)
+        cross = X.abs() @ W.abs().T
+        top_x, top_w = X.abs().amax(1, keepdim=True), W.abs().amax(1, keepdim=True)
+        ez = s * cross * ((self.d / 4 + 8) * 2.0 ** -23 + (3 * 2.0 ** -22 if f32 else 0))
+        if f32:
+            ez = ez + s * 2.0 ** -26 * (top_x * W.abs().sum(1)[None, :] + top_w.T * X.abs().sum(1, keepdim=True))
+        L = torch.logsumexp(Z, 1)
+        el = ez.amax(1) + 2.0 ** -20 + 6 * 2.0 ** -23 * (L.abs() + Z.abs().amax(1))
+        within(lse, L, el, "lse")
+        zt = Z.gather(1, t)[:, 0]
+        within(loss, torch.where(live, L - zt, 0 * L),
+               torch.where(live, el + ez.gather(1, t)[:, 0] + 4 * 2.0 ** -23 * zt.abs(), 0 * L), "loss")
+        g = torch.where(live, self.dloss.double().expand(self.n), 0 * L)[:, None] * s
+        p = torch.exp(Z - L[:, None])
+        hot = torch.zeros_like(p).scatter_(1, t, 1.0)
+        P = g * (p - hot)
+        keep = {torch.float32: 2.0 ** -21, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -10}[self.dtype]
+        eP = g.abs() * (p * (ez + 2 * el[:, None] + 2.0 ** -20) + 2.0 ** -23 * hot + 2.0 ** -25) + P.abs() * keep
+        for out, A, B, eA, top, what in ((dx, P, W, eP, top_w, "dx"), (dw, P.T, X, eP.T, top_x, "dw")):
+            want = A @ B
+            tol = eA @ B.abs() + ((A.shape[1] / 4 + 40) * 2.0 ** -23 + (2.0 ** -20 if f32 else 0)) * (A.abs() @ B.abs())
+            if f32:
+                tol = tol + 2.0 ** -26 * (A.abs() @ top)
+            within(out, want, tol + HALF_ULP[out.dtype] * (want.abs() + tol) + 2.0 ** -149, what)
+
+
+# Shapes of each kind of tile (pairs, single CTAs, narrow ones), off 16 bytes too.
+SHAPES = [(300, 200, 130), (40, 3000, 72), (700, 1100, 264), (129, 70, 40)]
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=NAMES.get)
+@pytest.mark.parametrize("n,k,d", SHAPES)
+def test_loss_gradient_of_a_row_without_a_target_is_not_used(eng, n, k, d, dtype):
+    """Whatever an ignored row's loss gradient holds, every output is the same."""
+    c = Values(n, k, d, dtype, 1)
+    clean = c.run(eng)
+    c.check(clean)
+    for value in (1e30, -3e38, math.inf, math.nan, 0.0):
+        c.dloss[3] = value
+        for a, b in zip(c.run(eng), clean):
+            assert torch.equal(a, b)
