@@ -526,8 +526,12 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     const uint32_t base = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(hf * HALF);
     float sc = P.scale, gmax = 0.0f;
     if (EPI != OUT && P.split) sc = sc / split_scale(P.scal[S_X]) / split_scale(P.scal[S_W]);
-    if constexpr (EPI != LSE)
+    if constexpr (EPI != LSE) {
       gmax = P.one_dloss ? fabsf(P.dloss[0]) : __uint_as_float(P.scal[S_G]);
+      // Nothing to be relative to: P takes the rows' own (a non-finite one stays with
+      // the rows that have a target).
+      if (!(gmax > 0.0f && gmax < INFINITY)) gmax = 1.0f;
+    }
     const uint32_t release = CG == 2 ? map_rank(smem_u32(tempty), 0) : smem_u32(tempty);
     int tc = 0, stores = 0;
     bool stop = false;
@@ -573,7 +577,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
           if (rel >= 0 && rel < cols) tcol = (int)rel;
           if (EPI == PROB && (long)row.t < P.k) {
             lse = row.lse;
-            gr = gmax > 0.0f ? row.g / gmax : row.g;  // g: 0, or NaN
+            gr = row.g / gmax;
           }
         }
         next = row_of(next_unit(u), after);

@@ -131,3 +131,15 @@ def test_loss_gradient_of_a_row_without_a_target_is_not_used(eng, n, k, d, dtype
         c.dloss[3] = value
         for a, b in zip(c.run(eng), clean):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("dtype", TYPES, ids=NAMES.get)
+@pytest.mark.parametrize("n,k,d", SHAPES + [(50, 30, 20), (9, 300, 65)])
+def test_one_non_finite_loss_gradient_leaves_ignored_rows_at_zero(eng, n, k, d, dtype, value):
+    c = Values(n, k, d, dtype, 2)
+    c.dloss = torch.full((1,), value, device="cuda")
+    _, _, dx, dw = c.run(eng)
+    none = c.t == eb.IGNORE
+    assert none.any() and (dx[none] == 0).all()
+    assert not dx[~none].isfinite().any() and not dw.isfinite().any()
