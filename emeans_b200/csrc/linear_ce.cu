@@ -33,6 +33,7 @@
 #include <cuda_runtime.h>
 #include <cudaTypedefs.h>
 
+#include <cfloat>
 #include <cmath>
 
 #include "elem.h"
@@ -59,12 +60,12 @@ enum Epi { LSE, PROB, OUT };
 // rows with a target.
 enum { S_X, S_W, S_G, S_WORDS };
 
-// The power of two that brings a largest magnitude (its bits) below 2^15.
-__device__ __forceinline__ float split_scale(uint32_t bits) {
-  if (bits == 0) return 1.0f;
+// The power of two that brings a largest magnitude (its bits) below 2^15, as
+// its exponent.
+__device__ __forceinline__ int split_exp(uint32_t bits) {
+  if (bits == 0) return 0;
   const int e = max((int)(bits >> 23), 1) - 127;  // 2^e <= max < 2^(e+1)
-  const int s = min(max(14 - e, -126), 126);
-  return __uint_as_float((uint32_t)(s + 127) << 23);
+  return min(max(14 - e, -126), 126);
 }
 
 // Division of 0 <= n < 2^31 by d >= 1 through a multiplication: q = (n + floor(n m /
@@ -525,7 +526,11 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     float* blk = (float*)(smem + S::STAGES * S::STAGE) + (warp - 4) * 1024;
     const uint32_t base = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(hf * HALF);
     float sc = P.scale, gmax = 0.0f;
-    if (EPI != OUT && P.split) sc = sc / split_scale(P.scal[S_X]) / split_scale(P.scal[S_W]);
+    // Kept finite and above 0: products below or past FP32's range leave scores of 0
+    // or infinities, not 0 x infinity.
+    if (EPI != OUT && P.split)
+      sc = fminf(fmaxf(ldexpf(sc, -(split_exp(P.scal[S_X]) + split_exp(P.scal[S_W]))), FLT_MIN),
+                 FLT_MAX);
     if constexpr (EPI != LSE) {
       gmax = P.one_dloss ? fabsf(P.dloss[0]) : __uint_as_float(P.scal[S_G]);
       // Nothing to be relative to: P takes the rows' own (a non-finite one stays with
@@ -615,10 +620,12 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         wait_chain();
       }
       if (stop) break;
-      float factor = 1.0f;
+      // Two-term sums come to their own size before the scores' scale and the loss
+      // gradients, whose product with a power of two may leave FP32's range.
+      float factor = 1.0f, unit = 1.0f;
       if constexpr (EPI == OUT) {
-        factor = P.scale / P.pscale * gmax;
-        if (pr.unscale >= 0) factor /= split_scale(P.scal[pr.unscale]);
+        factor = PARTS == 2 ? gmax : P.scale / P.pscale * gmax;
+        if (PARTS == 2) unit = ldexpf(1.0f / P.pscale, -split_exp(P.scal[pr.unscale]));
       }
       uint32_t raw[CHAINED ? 1 : 32];
       if constexpr (!CHAINED) tmem_ld32(base + (tc & 1) * BN, raw);
@@ -720,6 +727,10 @@ __global__ void __launch_bounds__(NTHREADS, 1)
             stores_commit();
           }
         } else {
+          if constexpr (PARTS == 2) {
+#pragma unroll
+            for (int j = 0; j < 32; j++) v[j] = v[j] * unit * P.scale;
+          }
           __syncwarp();
 #pragma unroll
           for (int g = 0; g < 8; g++)
@@ -960,7 +971,7 @@ __global__ void __launch_bounds__(256)
     for (unsigned t = threadIdx.x; t < q.blocks; t += 256)
       m = max(m, maxima[t + (second ? X.blocks : 0)]);
     m = block_max(m);
-    s = split_scale(m);
+    s = ldexpf(1.0f, split_exp(m));
     if (b == 0 && threadIdx.x == 0) scal[second ? S_W : S_X] = m;
   }
   const long end = (q.rows - 1) * q.ld + q.d;

@@ -143,3 +143,15 @@ def test_one_non_finite_loss_gradient_leaves_ignored_rows_at_zero(eng, n, k, d, 
     none = c.t == eb.IGNORE
     assert none.any() and (dx[none] == 0).all()
     assert not dx[~none].isfinite().any() and not dw.isfinite().any()
+
+
+@pytest.mark.parametrize("sizes", [(1e-25, 1e-25, 1.0, 1.0), (1e-33, 1e-30, 1.0, 1.0),
+                                   (1e15, 1e-25, 1e10, 1e-5), (1e-25, 1e15, 1e10, 1e5),
+                                   (1e-20, 1e-18, 1e38, 1e-30), (1e17, 1e18, 1e-35, 1.0)], ids=str)
+@pytest.mark.parametrize("n,k,d", SHAPES)
+def test_rows_and_prototypes_of_any_size(eng, n, k, d, sizes):
+    """f32 rows, prototypes, scale and loss gradients whose products stay in
+    range though those of some factors leave it."""
+    c = Values(n, k, d, torch.float32, 3)
+    c.x, c.w, c.scale, c.dloss = c.x * sizes[0], c.w * sizes[1], sizes[2], c.dloss * sizes[3]
+    c.check(c.run(eng))
