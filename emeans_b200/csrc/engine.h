@@ -158,6 +158,8 @@ struct eb_engine {
   // non-finite flag): each conversion of a centroid set tags its atomics with
   // a new generation, so the summary needs no zeroing pass per call.
   uint32_t cinfo_gen = 0;
+  // The cross entropy's "ce_found" words hold a call's magnitudes (linear_ce.cu).
+  bool ce_found_raised = false;
   unsigned long long* counters() { return d_counters; }
   // Events of the two pinned staging buffers of caller copies (hostcopy.cpp).
   cudaEvent_t stage_ev[2] = {nullptr, nullptr};

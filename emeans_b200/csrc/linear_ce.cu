@@ -22,7 +22,15 @@
 // f32 operands: scaled by a power of two so that the largest is below 2^15
 // and split into two FP16 terms (22 bits, absolute floor 2^-39 of the
 // largest); three products hi.hi + hi.lo + lo.hi add into one FP32
-// accumulator. The dropped lo.lo term is 2^-22 of the product.
+// accumulator. The dropped lo.lo term is 2^-22 of the product. That floor is the
+// matrix's, so rows, columns or loss gradients far below the largest would lose
+// their last bits, or all of them. Where the smallest row's or column's largest
+// element, or a row's loss gradient, is below 2^-12 of the largest (of those that
+// are not 0), the operands and P are instead split into three bf16 terms each (24
+// bits, FP32's own range, no scale) and multiplied in six products. The
+// preparation decides it on the device, and the same kernels read it: 3,001 x
+// 5,003 x 385 forward and backward 62 and 150 us one way, 83 and 238 the other;
+// 8,192 x 8,192 x 1024 290 and 905, 506 and 1,867.
 //
 // Bound by the tensor cores, 2 n k d operations forward and 6 n k d backward
 // (three times that for f32); for few rows by reading w once. 16,384 x 65,536 x
@@ -35,6 +43,7 @@
 
 #include <cfloat>
 #include <cmath>
+#include <type_traits>
 
 #include "elem.h"
 #include "engine.h"
@@ -55,10 +64,29 @@ constexpr float PSCALE = 16384.0f;  // f16 and f32: P is kept times 2^14
 
 enum Epi { LSE, PROB, OUT };
 
-// Scalars shared by a call's kernels (device scratch): bits of max|x|,
-// max|w| over the finite elements (f32 operands) and of max|dloss| over the
-// rows with a target.
-enum { S_X, S_W, S_G, S_WORDS };
+// Words shared by a call's kernels (device scratch): bits of max|x| and max|w| over
+// the finite elements (f32 operands) and of max|dloss| over the rows with a target;
+// whether f32 operands are three bf16 terms.
+enum { S_X, S_W, S_G, S_WIDE, S_WORDS };
+
+// Words that an f32 call's first kernels raise, zero between calls: the same
+// magnitudes; the complements of the smallest row's max|x| and max|w| and of the
+// smallest |dloss| that are not 0; the blocks that went by columns; then, for x and
+// for w, each column's largest, and for each range of columns what no column's
+// largest is below. The first product kernel zeroes them.
+enum { R_X, R_W, R_G, R_X_LOW, R_W_LOW, R_G_LOW, R_BY_COLUMN, R_COLUMNS };
+constexpr int RANGE = 1024;  // columns of a range
+__host__ __device__ constexpr long range_count(long d) { return (d + RANGE - 1) / RANGE; }
+__host__ __device__ constexpr long found_count(long d) {
+  return R_COLUMNS + 2 * (d + range_count(d));
+}
+
+// Whether a largest and a smallest magnitude (bits, and the smallest's complement;
+// 0: none) lie more than 2^12 apart: two FP16 terms then leave the smallest fewer
+// than 26 bits.
+__device__ __forceinline__ bool apart(uint32_t top, uint32_t low) {
+  return low && __uint_as_float(top) * 0x1p-12f > __uint_as_float(~low);
+}
 
 // The power of two that brings a largest magnitude (its bits) below 2^15, as
 // its exponent.
@@ -93,7 +121,7 @@ struct Prob {
   Divisor tiles, whole, rows, last;  // by a split's units, a group's, and its row tiles
   int a_mn;         // A is K x M (MN-major) rather than M x K
   // OUT: v = acc scale max|dloss| / pscale, to `out`, or through FP32 sums
-  int unscale;      // scal slot of the second operand's split scale, or -1
+  int unscale;      // scal slot of the second operand's largest (f32 operands)
   void* out;
   int otype, ovec;  // ovec: rows of `out` keep 16-byte alignment
   long ldo;
@@ -109,8 +137,9 @@ struct GemmParams {
   uint32_t fmt;     // operand format of the instruction (0 f16, 1 bf16)
   uint32_t* status;
   const uint32_t* scal;
+  uint32_t* found;  // f32 operands: words to zero for the next call, or null
+  long found_words;
   float scale;      // of the scores
-  int split;        // operands are f32 in two terms: scores carry both scales
   // LSE
   float2* part;     // [2 ntiles][M]: (max, sum) of a half tile's columns
   float* zt;        // M: target scores
@@ -124,27 +153,43 @@ struct GemmParams {
   float pscale;     // what P is kept times: 1 (bf16) or PSCALE
 };
 
-// CG CTAs a tile, PARTS terms an operand, columns up to WIDTH a tile.
-template <int EPI, int CG, int PARTS, int WIDTH, bool CHAINED>
+// CG CTAs a tile, columns up to WIDTH a tile; TERMS: operands of several 16-bit
+// terms.
+template <int EPI, int CG, bool TERMS, int WIDTH, bool CHAINED>
 struct Shape {
   static constexpr int A_ROWS = BM;
   static constexpr int B_ROWS = WIDTH / CG;
   static constexpr int HALF = WIDTH / 2;  // columns an epilogue warp takes
   static constexpr int A_BYTES = A_ROWS * BK * 2;
   static constexpr int B_BYTES = B_ROWS * BK * 2;
-  static constexpr int STAGE = PARTS * (A_BYTES + B_BYTES);
-  static constexpr int STAGES = 196608 / STAGE < 8 ? 196608 / STAGE : 8;
+  static constexpr int RING = 196608, MOST_STAGES = 8;
   // Operand ring, each epilogue warp's 32 x 32 block, and barriers.
-  static constexpr size_t SMEM = 1024 + (size_t)STAGES * STAGE + 8 * 4096 + 256;
+  static constexpr size_t SMEM = 1024 + RING + 8 * 4096 + 256;
   // k-blocks summed in one TMEM accumulator. The tensor cores' FP32 sums are
   // cut, not rounded, at every step of 16 (about 2^-26 of the sum a product,
   // always towards zero): 5.6e-6 of dx at k = 5,003 in one chain of three
   // products a step. CHAINED products end a chain after CHAIN blocks and add it
-  // to the epilogue's registers, rounded. Two-term operands, which aim at
-  // FP32's own error, take two: gradients 6e-7 (four: 1.1e-6; 8,192 x 8,192 x
-  // 1024 backward 930 us, 890). Scores of 16-bit rows past 768 columns: eight
-  // (loss 3e-7; unchained 7e-7).
-  static constexpr int CHAIN = !CHAINED ? 1 << 28 : PARTS == 1 ? 8 : 2;
+  // to the epilogue's registers, rounded. Operands of several terms, which aim
+  // at FP32's own error, take two: gradients 6e-7 (four: 1.1e-6 and 4 % less time),
+  // or with three terms each one (24 products). Scores of 16-bit rows past 768
+  // columns: eight (loss 3e-7; unchained 7e-7).
+  static constexpr int CHAIN = !CHAINED ? 1 << 28 : TERMS ? 2 : 8;
+};
+
+// A launch's tensor maps, one a term: A, B, and C: the second product's B (OUT) or
+// P (PROB).
+template <int T>
+struct Maps {
+  CUtensorMap a[T], b[T], c[T];
+};
+
+// A place of the operand ring, and the parity its barriers have there.
+struct Place {
+  int s;
+  uint32_t parity;
+  __device__ __forceinline__ Place next(int stages) const {
+    return s + 1 == stages ? Place{0, parity ^ 1} : Place{s + 1, parity};
+  }
 };
 
 // exp of a difference of scores (inputs <= 0 but for rounding; relative error
@@ -171,28 +216,26 @@ __device__ __forceinline__ void fold(float& m, float& s, float2 v) {
 __device__ __forceinline__ float4& block4(float* blk, int r, int g) {
   return reinterpret_cast<float4*>(blk)[r * 8 + (g ^ (r & 7))];
 }
-// Eight values times `by` as eight 16-bit elements (bf16, or f16), and with
-// LO what f16 left of them as eight more.
-template <bool F16, bool LO = false>
-__device__ __forceinline__ uint4 pack8(const float (&f)[8], float by, uint4& lo) {
-  uint32_t h[4], l[4];
+// Eight values rounded to 16 bits (bf16, or f16); with REST, what that left of
+// them stays in f (exact), for the next term.
+template <bool F16, bool REST>
+__device__ __forceinline__ uint4 pack8(float (&f)[8]) {
+  uint32_t h[4];
 #pragma unroll
   for (int j = 0; j < 4; j++) {
-    const float2 v = make_float2(f[2 * j] * by, f[2 * j + 1] * by);
+    const float2 v = make_float2(f[2 * j], f[2 * j + 1]);
+    float2 b;
     if constexpr (F16) {
       const __half2 q = __float22half2_rn(v);
       h[j] = *reinterpret_cast<const uint32_t*>(&q);
-      if constexpr (LO) {
-        const float2 b = __half22float2(q);
-        const __half2 r = __float22half2_rn(make_float2(v.x - b.x, v.y - b.y));
-        l[j] = *reinterpret_cast<const uint32_t*>(&r);
-      }
+      b = __half22float2(q);
     } else {
       const __nv_bfloat162 q = __float22bfloat162_rn(v);
       h[j] = *reinterpret_cast<const uint32_t*>(&q);
+      b = __bfloat1622float2(q);
     }
+    if constexpr (REST) f[2 * j] = v.x - b.x, f[2 * j + 1] = v.y - b.y;
   }
-  if constexpr (LO) lo = make_uint4(l[0], l[1], l[2], l[3]);
   return make_uint4(h[0], h[1], h[2], h[3]);
 }
 
@@ -267,10 +310,9 @@ __device__ __forceinline__ void store_block(const Prob& q, float* sums, float* b
         a = make_float4(a.x + o[0].x, a.y + o[0].y, a.z + o[0].z, a.w + o[0].w);
         b = make_float4(b.x + o[1].x, b.y + o[1].y, b.z + o[1].z, b.w + o[1].w);
       }
-      const float f[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-      uint4 none;
+      float f[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
       *reinterpret_cast<uint4*>(out + t * 8 * q.ldo) =
-          q.otype == EB_BF16 ? pack8<false>(f, 1.0f, none) : pack8<true>(f, 1.0f, none);
+          q.otype == EB_BF16 ? pack8<false, false>(f) : pack8<true, false>(f);
     }
   } else if (lane < cols) {
     float* at = sums + col + lane;
@@ -309,15 +351,13 @@ __device__ __forceinline__ void store_block(const Prob& q, float* sums, float* b
 // swizzle): a K-major operand's boxes follow one another down its rows, an
 // MN-major one's along its columns, so one tensor map serves either reading.
 // LSE and PROB: A = x, B = w, both K-major. OUT: A = P, K-major for dx
-// (B = w) and MN-major for dw (B = x), B MN-major. With PARTS = 2 each operand
-// is two FP16 terms; CHAINED, sums are kept in registers between chains.
-template <int EPI, int CG, int PARTS, int WIDTH, bool CHAINED>
+// (B = w) and MN-major for dw (B = x), B MN-major. With TERMS each operand is
+// several 16-bit terms (f32: two f16 or three bf16 ones); CHAINED, sums are kept
+// in registers between chains.
+template <int EPI, int CG, bool TERMS, int WIDTH, bool CHAINED>
 __global__ void __launch_bounds__(NTHREADS, 1)
-    k_gemm(const __grid_constant__ CUtensorMap a0, const __grid_constant__ CUtensorMap a1,
-           const __grid_constant__ CUtensorMap b0, const __grid_constant__ CUtensorMap b1,
-           const __grid_constant__ CUtensorMap c0map, const __grid_constant__ CUtensorMap c1map,
-           const __grid_constant__ GemmParams P) {
-  using S = Shape<EPI, CG, PARTS, WIDTH, CHAINED>;
+    k_gemm(const __grid_constant__ Maps<TERMS ? 3 : 1> maps, const __grid_constant__ GemmParams P) {
+  using S = Shape<EPI, CG, TERMS, WIDTH, CHAINED>;
   constexpr int HALF = S::HALF;
   using namespace tc;
   extern __shared__ uint8_t smem_raw[];
@@ -325,9 +365,9 @@ __global__ void __launch_bounds__(NTHREADS, 1)
   // that it points to shared memory (with generic accesses the step of 16,384
   // x 65,536 x 1024 bf16 took 6.5 ms instead of 6.1).
   uint8_t* smem = smem_raw + (-smem_u32(smem_raw) & 1023u);
-  uint64_t* full = (uint64_t*)(smem + S::STAGES * S::STAGE + 8 * 4096);
-  uint64_t* empty = full + S::STAGES;
-  uint64_t* tfull = empty + S::STAGES;
+  uint64_t* full = (uint64_t*)(smem + S::RING + 8 * 4096);
+  uint64_t* empty = full + S::MOST_STAGES;
+  uint64_t* tfull = empty + S::MOST_STAGES;
   uint64_t* tempty = tfull + 2;
   uint64_t* done = tempty + 2;
   uint32_t* tmem_slot = (uint32_t*)(done + 1);
@@ -354,7 +394,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
   const int first = EPI != OUT || cluster < P.q[0].units ? cluster : after_long();
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < S::STAGES; s++) {
+    for (int s = 0; s < S::MOST_STAGES; s++) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
@@ -372,6 +412,14 @@ __global__ void __launch_bounds__(NTHREADS, 1)
   fence_after();
   const uint32_t tmem = *tmem_slot;
   pdl_wait();
+  // Terms of both operands, and what follows from them. A stage holds A's terms,
+  // then B's.
+  const bool wide = TERMS && P.scal[S_WIDE];
+  const int terms = !TERMS ? 1 : wide ? 3 : 2;
+  const int stage_bytes = terms * (S::A_BYTES + S::B_BYTES);
+  const int stages = min(S::RING / stage_bytes, S::MOST_STAGES);
+  const int chain = wide ? 1 : S::CHAIN;
+  auto stage_at = [&](int s) { return smem + s * stage_bytes; };
 
   // With the sums in registers, the first warpgroup gives some of its own to
   // the epilogue (128 x 72 + 256 x 216 = 384 x 168).
@@ -380,6 +428,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     if (warp == 0) {
       const bool one = elect_one();
       int it = 0;
+      Place at = {0, 1};
       bool stop = false;
       for (int u = first; u < units && !stop; u = next_unit(u)) {
         const Unit q = unit_at<EPI>(P, u);
@@ -398,27 +447,31 @@ __global__ void __launch_bounds__(NTHREADS, 1)
           if (c == (int)rank) a_boxes = a, b_boxes = b;
           all += a + b;
         }
-        for (int kb = q.kb0; kb < q.kb1; kb++, it++) {
-          const int s = it % S::STAGES;
-          if (!warp_wait(&empty[s], ((it / S::STAGES) & 1) ^ 1, abort_flag)) {
+        for (int kb = q.kb0; kb < q.kb1; kb++, it++, at = at.next(stages)) {
+          const int s = at.s;
+          if (!warp_wait(&empty[s], at.parity, abort_flag)) {
             stop = true;
             break;
           }
           if (!one) continue;
-          if (rank == 0) mbar_expect_tx(&full[s], PARTS * all * 8192);
+          if (rank == 0) mbar_expect_tx(&full[s], terms * all * 8192);
           const uint32_t bar = CG == 2 ? map_rank(smem_u32(&full[s]), 0) : smem_u32(&full[s]);
-          uint8_t* st = smem + s * S::STAGE;
+          uint8_t* st = stage_at(s);
           const bool a_mn = EPI == OUT && P.q[q.prob].a_mn;
 #pragma unroll
-          for (int p = 0; p < PARTS; p++) {
-            const CUtensorMap* ma = p ? &a1 : &a0;
-            const CUtensorMap* mb = q.prob ? (p ? &c1map : &c0map) : (p ? &b1 : &b0);
+          for (int p = 0; p < (TERMS ? 3 : 1); p++) {
+            if (p >= terms) break;
 #pragma unroll
             for (int c = 0; c < S::A_ROWS / 64; c++, st += 8192) {
               const int m = am + c * 64;
               if (c < a_boxes)
-                tma_load<CG>(st, ma, bar, a_mn ? m : kb * BK, a_mn ? kb * BK : m);
+                tma_load<CG>(st, &maps.a[p], bar, a_mn ? m : kb * BK, a_mn ? kb * BK : m);
             }
+          }
+#pragma unroll
+          for (int p = 0; p < (TERMS ? 3 : 1); p++) {
+            if (p >= terms) break;
+            const CUtensorMap* mb = q.prob ? &maps.c[p] : &maps.b[p];
 #pragma unroll
             for (int c = 0; c < S::B_ROWS / 64; c++, st += 8192) {
               const int n = bn + c * 64;
@@ -432,9 +485,9 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       // barriers count both CTAs' bytes (on the normal path these waits
       // return at once).
       if (rank == 0) {
-        for (int j = it > S::STAGES ? it - S::STAGES : 0; j < it; j++) {
+        for (int j = it > stages ? it - stages : 0; j < it; j++) {
           const uint64_t t0 = now_ns();
-          while (!mbar_try(&full[j % S::STAGES], (j / S::STAGES) & 1) && now_ns() - t0 < WAIT_NS) {
+          while (!mbar_try(&full[j % stages], (j / stages) & 1) && now_ns() - t0 < WAIT_NS) {
           }
         }
       }
@@ -445,17 +498,19 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     // 202 us, 177 now; 512 columns 108 and 97).
     if (warp == 1 && rank == 0) {
       const bool one = elect_one();
-      int it = 0, tc = 0;  // tc counts chains
+      const uint32_t fmt = wide ? 1u : P.fmt;
+      Place at = {0, 0};
+      int tc = 0;  // counts chains
       bool stop = false;
       for (int u = first; u < units && !stop; u = next_unit(u)) {
         const Unit q = unit_at<EPI>(P, u);
         const bool a_mn = EPI == OUT && P.q[q.prob].a_mn;
-        const uint32_t idesc = (1u << 4) | (P.fmt << 7) | (P.fmt << 10) | ((a_mn ? 1u : 0u) << 15) |
+        const uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((a_mn ? 1u : 0u) << 15) |
                                ((EPI == OUT ? 1u : 0u) << 16) |
                                ((uint32_t)(P.q[q.prob].bn >> 3) << 17) |
                                ((uint32_t)(CG * BM >> 4) << 24);
-        for (int k0 = q.kb0; k0 < q.kb1 && !stop; k0 += S::CHAIN, tc++) {
-          const int k1 = min(k0 + S::CHAIN, q.kb1);
+        for (int k0 = q.kb0; k0 < q.kb1 && !stop; k0 += chain, tc++) {
+          const int k1 = min(k0 + chain, q.kb1);
           const uint32_t d = tmem + (tc & 1) * BN;
           if (!warp_wait(&tempty[tc & 1], ((tc >> 1) & 1) ^ 1, abort_flag)) {
             stop = true;
@@ -464,49 +519,58 @@ __global__ void __launch_bounds__(NTHREADS, 1)
           fence_after();
           // The products of one stage: of the operands' terms a and b.
           auto multiply = [&](int s, int pa, int pb, uint32_t first) {
-            const uint32_t st = smem_u32(smem + s * S::STAGE);
-            const uint32_t a = st + pa * (S::A_BYTES + S::B_BYTES);
-            const uint32_t b = st + pb * (S::A_BYTES + S::B_BYTES) + S::A_BYTES;
+            const uint32_t a = smem_u32(stage_at(s)) + pa * S::A_BYTES;
+            const uint32_t b = smem_u32(stage_at(s)) + terms * S::A_BYTES + pb * S::B_BYTES;
 #pragma unroll
             for (int kk = 0; kk < BK / 16; kk++)
               mma_f16<CG>(d, a_mn ? desc_mn(a + kk * 2048, 8192) : desc_k(a + kk * 32),
                           EPI == OUT ? desc_mn(b + kk * 2048, 8192) : desc_k(b + kk * 32), idesc,
                           kk == 0 ? first : 1u);
           };
+          // All of them but the largest, the smallest first.
+          auto small = [&](int s, uint32_t first) {
+            if (wide) {
+              multiply(s, 0, 2, first);
+              multiply(s, 1, 1, 1u);
+              multiply(s, 2, 0, 1u);
+              first = 1u;
+            }
+            multiply(s, 0, 1, first);
+            multiply(s, 1, 0, 1u);
+          };
           // Two-term scores take two stages together, the small products of both
           // first: sums are then cut at their full size eight times in the two
           // blocks, not 24. Gradients take a stage at a time (the ring's three
-          // stages are held longer otherwise: 8 % of the time).
-          constexpr int TOGETHER = PARTS == 2 && EPI != OUT ? 2 : 1;
-          for (int kb = k0; kb < k1 && !stop; kb += TOGETHER) {
-            const int n = min(TOGETHER, k1 - kb);
+          // stages are held longer otherwise: 8 % of the time), and so do three
+          // terms, whose ring has two.
+          constexpr int MOST = TERMS && EPI != OUT ? 2 : 1;
+          const int together = wide ? 1 : MOST;
+          for (int kb = k0; kb < k1 && !stop; kb += together) {
+            const int n = min(together, k1 - kb);
+            Place p = at;
 #pragma unroll
-            for (int g = 0; g < TOGETHER; g++) {
+            for (int g = 0; g < MOST; g++) {
               if (g >= n) break;
-              const int s = (it + g) % S::STAGES;
-              if (!warp_wait(&full[s], ((it + g) / S::STAGES) & 1, abort_flag)) {
+              if (!warp_wait(&full[p.s], p.parity, abort_flag)) {
                 stop = true;
                 break;
               }
               fence_after();
-              if constexpr (PARTS == 2) {
-                if (one) {
-                  multiply(s, 0, 1, (kb > k0 || g > 0) ? 1u : 0u);
-                  multiply(s, 1, 0, 1u);
-                }
+              if constexpr (TERMS) {
+                if (one) small(p.s, (kb > k0 || g > 0) ? 1u : 0u);
               }
+              p = p.next(stages);
             }
             if (stop) break;
 #pragma unroll
-            for (int g = 0; g < TOGETHER; g++) {
+            for (int g = 0; g < MOST; g++) {
               if (g >= n) break;
-              const int s = (it + g) % S::STAGES;
               if (one) {
-                multiply(s, 0, 0, (PARTS == 2 || kb > k0) ? 1u : 0u);
-                mma_commit<CG>(&empty[s]);
+                multiply(at.s, 0, 0, (TERMS || kb > k0) ? 1u : 0u);
+                mma_commit<CG>(&empty[at.s]);
               }
+              at = at.next(stages);
             }
-            it += n;
           }
           if (!stop && one) mma_commit<CG>(&tfull[tc & 1]);
         }
@@ -519,23 +583,28 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     }
   } else {
     if constexpr (CHAINED) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    if constexpr (TERMS && EPI != OUT) {
+      if (blockIdx.x == 0)
+        for (long t = threadIdx.x - 128; t < P.found_words; t += NTHREADS - 128) P.found[t] = 0;
+    }
     // Epilogue: warp w reads TMEM lanes 32 (w % 4) .. + 31, one row a thread,
     // and half (w - 4) / 4 of the tile's columns.
     const int hf = (warp - 4) >> 2;
     const int r = (warp & 3) * 32 + lane;
-    float* blk = (float*)(smem + S::STAGES * S::STAGE) + (warp - 4) * 1024;
+    float* blk = (float*)(smem + S::RING) + (warp - 4) * 1024;
     const uint32_t base = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(hf * HALF);
     float sc = P.scale, gmax = 0.0f;
     // Kept finite and above 0: products below or past FP32's range leave scores of 0
     // or infinities, not 0 x infinity.
-    if (EPI != OUT && P.split)
+    if (EPI != OUT && TERMS && !wide)
       sc = fminf(fmaxf(ldexpf(sc, -(split_exp(P.scal[S_X]) + split_exp(P.scal[S_W]))), FLT_MIN),
                  FLT_MAX);
     if constexpr (EPI != LSE) {
       gmax = P.one_dloss ? fabsf(P.dloss[0]) : __uint_as_float(P.scal[S_G]);
       // Nothing to be relative to: P takes the rows' own (a non-finite one stays with
       // the rows that have a target).
-      if (!(gmax > 0.0f && gmax < INFINITY)) gmax = 1.0f;
+      // Three bf16 terms of P have FP32's range: they too take the rows' own.
+      if (wide || !(gmax > 0.0f && gmax < INFINITY)) gmax = 1.0f;
     }
     const uint32_t release = CG == 2 ? map_rank(smem_u32(tempty), 0) : smem_u32(tempty);
     int tc = 0, stores = 0;
@@ -603,7 +672,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       if constexpr (CHAINED) {
 #pragma unroll
         for (int j = 0; j < HALF; j++) acc[j] = 0.0f;
-        for (int k0 = q.kb0; k0 < q.kb1; k0 += S::CHAIN) {
+        for (int k0 = q.kb0; k0 < q.kb1; k0 += chain) {
           if (!wait_chain()) break;
 #pragma unroll
           for (int h = 0; h < HALF / 16; h++) {
@@ -620,12 +689,20 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         wait_chain();
       }
       if (stop) break;
-      // Two-term sums come to their own size before the scores' scale and the loss
-      // gradients, whose product with a power of two may leave FP32's range.
+      // Sums of several terms: the operand's power of two, the scores' scale and the
+      // loss gradients at once where that keeps well within FP32's range, else one
+      // after the other.
       float factor = 1.0f, unit = 1.0f;
       if constexpr (EPI == OUT) {
-        factor = PARTS == 2 ? gmax : P.scale / P.pscale * gmax;
-        if (PARTS == 2) unit = ldexpf(1.0f / P.pscale, -split_exp(P.scal[pr.unscale]));
+        if constexpr (TERMS) {
+          if (!wide) unit = ldexpf(1.0f / P.pscale, -split_exp(P.scal[pr.unscale]));
+          const float two = unit * P.scale, all = two * gmax;
+          const bool fine = two > 0x1p-90f && two < 0x1p90f && all > 0x1p-90f && all < 0x1p90f;
+          factor = fine ? all : gmax;
+          if (fine) unit = 1.0f;
+        } else {
+          factor = P.scale / P.pscale * gmax;
+        }
       }
       uint32_t raw[CHAINED ? 1 : 32];
       if constexpr (!CHAINED) tmem_ld32(base + (tc & 1) * BN, raw);
@@ -688,46 +765,78 @@ __global__ void __launch_bounds__(NTHREADS, 1)
           }
           // A row a thread, 64 bytes a term, 16-byte groups placed by the 64-byte
           // swizzle; a tile store takes the block to P and cuts it at P's
-          // edges. One-term blocks go through two buffers in turn. (Transposed
+          // edges. One-term blocks go through two buffers in turn, two terms
+          // through both, and three through them in turn again. (Transposed
           // in shared memory as FP32 and stored by four lanes a row: backward
           // 16,384 x 8,192 x 256 bf16 221 us, 211 now, x 1,024 x 768 78 and 74,
           // 8,192 x 8,192 x 256 f32 272 and 263.)
-          auto pack = [&](const float (&f)[8], uint4& lo) {
-            return PARTS == 1 && P.fmt ? pack8<false>(f, 1.0f, lo)
-                                       : pack8<true, PARTS == 2>(f, PSCALE, lo);
-          };
-          uint8_t* box = (uint8_t*)blk + (PARTS == 1 ? (stores++ & 1) * 2048 : 0);
-          uint8_t* row = box + lane * 64;
           const int turn = (lane >> 1) & 3;
-          if (lane == 0) stores_read<PARTS == 1 ? 1 : 0>();
-          __syncwarp();
+          const bool bf = !TERMS && P.fmt;
+          if (!bf && !wide) {
 #pragma unroll
-          for (int g = 0; g < 4; g++) {
-            const float f[8] = {v[8 * g],     v[8 * g + 1], v[8 * g + 2], v[8 * g + 3],
-                                v[8 * g + 4], v[8 * g + 5], v[8 * g + 6], v[8 * g + 7]};
-            uint4 lo;
-            *reinterpret_cast<uint4*>(row + ((g ^ turn) << 4)) = pack(f, lo);
-            if (PARTS == 2) *reinterpret_cast<uint4*>(row + 2048 + ((g ^ turn) << 4)) = lo;
+            for (int j = 0; j < 32; j++) v[j] *= PSCALE;
+            at_target *= PSCALE;
           }
-          if (target) {
-            const float f[8] = {at_target};
-            uint4 lo;
-            uint8_t* p = row + (((e >> 3) ^ turn) << 4) + (e & 7) * 2;
-            *reinterpret_cast<uint16_t*>(p) = (uint16_t)pack(f, lo).x;
-            if (PARTS == 2) *reinterpret_cast<uint16_t*>(p + 2048) = (uint16_t)lo.x;
-          }
-          store_fence();
-          __syncwarp();
-          if (lane == 0) {
-            const int row0 = (int)i, col = (int)c0 + h * 32;
-            if (row0 < pr.M) {
-              tma_store(&c0map, box, col, row0);
-              if (PARTS == 2) tma_store(&c1map, box + 2048, col, row0);
+          // One round: a term of the block to `box` (and the next to what follows it),
+          // then to P; v and at_target keep the rest.
+          auto round = [&](uint8_t* box, int term, auto as_f16, auto both) {
+            constexpr bool F16 = decltype(as_f16)::value, BOTH = decltype(both)::value;
+            uint8_t* row = box + lane * 64;
+            __syncwarp();
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+              float f[8];
+#pragma unroll
+              for (int j = 0; j < 8; j++) f[j] = v[8 * g + j];
+              uint8_t* at = row + ((g ^ turn) << 4);
+              *reinterpret_cast<uint4*>(at) = pack8<F16, TERMS>(f);
+              if constexpr (BOTH) *reinterpret_cast<uint4*>(at + 2048) = pack8<F16, false>(f);
+              if constexpr (TERMS && !BOTH) {
+#pragma unroll
+                for (int j = 0; j < 8; j++) v[8 * g + j] = f[j];
+              }
             }
-            stores_commit();
+            if (target) {
+              float f[8] = {at_target};
+              uint8_t* at = row + (((e >> 3) ^ turn) << 4) + (e & 7) * 2;
+              *reinterpret_cast<uint16_t*>(at) = (uint16_t)pack8<F16, TERMS>(f).x;
+              if constexpr (BOTH)
+                *reinterpret_cast<uint16_t*>(at + 2048) = (uint16_t)pack8<F16, false>(f).x;
+              at_target = f[0];
+            }
+            store_fence();
+            __syncwarp();
+            if (lane == 0) {
+              const int row0 = (int)i, col = (int)c0 + h * 32;
+              if (row0 < pr.M) {
+                tma_store(&maps.c[term], box, col, row0);
+                if constexpr (BOTH) tma_store(&maps.c[term + 1], box + 2048, col, row0);
+              }
+              stores_commit();
+            }
+          };
+          constexpr std::true_type yes{};
+          constexpr std::false_type no{};
+          uint8_t* boxes = (uint8_t*)blk;
+          if constexpr (!TERMS) {
+            if (lane == 0) stores_read<1>();
+            uint8_t* box = boxes + (stores++ & 1) * 2048;
+            if (bf)
+              round(box, 0, no, no);
+            else
+              round(box, 0, yes, no);
+          } else if (!wide) {
+            if (lane == 0) stores_read<0>();
+            round(boxes, 0, yes, yes);
+          } else {
+#pragma unroll 1
+            for (int p = 0; p < 3; p++, stores++) {
+              if (lane == 0) stores_read<1>();
+              round(boxes + (stores & 1) * 2048, p, no, no);
+            }
           }
         } else {
-          if constexpr (PARTS == 2) {
+          if (TERMS && unit != 1.0f) {
 #pragma unroll
             for (int j = 0; j < 32; j++) v[j] = v[j] * unit * P.scale;
           }
@@ -839,13 +948,13 @@ __global__ void __launch_bounds__(128)
 }
 
 // Rows of an operand on their way to rows of dp 16-bit elements (zeros past
-// d): f32 as two FP16 terms, 16-bit types as they are. `blocks` of a launch
-// work on it.
+// d): f32 as two or three terms (`term` elements apart), 16-bit types as they are.
+// `blocks` of a launch work on it.
 struct Prep {
   const void* x;
   long rows, d, ld, dp;
-  uint16_t* hi;
-  uint16_t* lo;
+  uint16_t* out;
+  long term;
   unsigned blocks;
 };
 constexpr int PREP_BLOCKS = 1024;  // most blocks of a launch for one operand
@@ -936,73 +1045,226 @@ __device__ __forceinline__ void for_groups(const Prep& q, unsigned block, F&& f)
   }
 }
 
-// Largest magnitude over the finite elements of both operands' rows: one per
-// block, at maxima[block].
-__global__ void __launch_bounds__(256) k_ce_max(Prep X, Prep W, uint32_t* maxima) {
-  pdl_trigger();
-  pdl_wait();
-  const bool second = blockIdx.x >= X.blocks;
-  const Prep& q = second ? W : X;
-  const long end = (q.rows - 1) * q.ld + q.d;
-  uint32_t m = 0;
-  for_groups(q, blockIdx.x - (second ? X.blocks : 0), [&](long i, long c, int live) {
-    float f[8];
-    load8(static_cast<const float*>(q.x), i * q.ld + c, live, end, f);
-#pragma unroll
-    for (int j = 0; j < 8; j++) m = max(m, finite_bits(f[j]));
-  });
-  m = block_max(m);
-  if (threadIdx.x == 0) maxima[blockIdx.x] = m;
+// Whether a matrix's columns lie too far apart, for all of a block's 256 threads: no
+// column of a range is below its word (some block saw every column that large), or,
+// where every block had columns of zeros or far smaller ones, from the columns' own
+// words.
+__device__ __forceinline__ bool columns_apart(const uint32_t* found, long d, uint32_t top,
+                                              bool by_column) {
+  bool far = false;
+  for (long r = 0; r < range_count(d); r++) {
+    const uint32_t least = found[d + r];
+    far |= !least || apart(top, ~least);
+  }
+  if (!far || !by_column) return far;
+  uint32_t low = 0;
+#pragma unroll 4
+  for (long c = threadIdx.x; c < d; c += 256) {
+    const uint32_t m = found[c];
+    if (m) low = max(low, ~m);
+  }
+  return __syncthreads_or(apart(top, low));
 }
 
-// The operands' 16-bit rows; with SPLIT, scaled by the largest of the blocks'
-// maxima, which the first block of each operand leaves in `scal`.
-template <bool SPLIT>
-__global__ void __launch_bounds__(256)
-    k_ce_rows(Prep X, Prep W, const uint32_t* __restrict__ maxima, uint32_t* scal) {
+// The magnitudes of both operands' finite elements: the largest, the
+// smallest row's largest (of its part in a range of columns) and each column's. L
+// lanes take a row, eight columns at a time; a block keeps to one range, whose
+// largest elements a lane keeps in registers. A block all of whose columns come
+// within 2^-12 of its largest element leaves their smallest largest, as any other
+// block's can only be added to it; only one that finds columns of zeros or far
+// smaller ones leaves each column's (all blocks: 10 us of atomics at 4,096 x 768). 3,001
+// x 5,003 x 385: 10 us.
+template <int L, int PASSES>
+__global__ void __launch_bounds__(256, 2)
+    k_ce_max(Prep X, Prep W, uint32_t* found) {
+  constexpr int COLS = 8 * L * PASSES;
+  static_assert(COLS <= RANGE, "a block's columns are one range's");
+  __shared__ uint32_t cols[COLS], rows[3];
   pdl_trigger();
   pdl_wait();
   const bool second = blockIdx.x >= X.blocks;
   const Prep& q = second ? W : X;
-  const unsigned b = blockIdx.x - (second ? X.blocks : 0);
+  const int ranges = (int)range_count(q.d);
+  const unsigned block = blockIdx.x - (second ? X.blocks : 0), range = block % ranges;
+  const long c0 = (long)range * RANGE, end = (q.rows - 1) * q.ld + q.d;
+  const long last_c = min(c0 + COLS, q.dp) - 8;  // the last eight columns
+  const int lane = threadIdx.x % L;
+  const float* x = static_cast<const float*>(q.x);
+  for (int t = threadIdx.x; t < COLS; t += 256) cols[t] = 0;
+  if (threadIdx.x < 3) rows[threadIdx.x] = threadIdx.x < 2 ? 0 : ~0u;
+  uint32_t top = 0, low = 0, col[PASSES][8] = {};
+  const long step = (long)(q.blocks / ranges) * (256 / L);
+  for (long r0 = (long)(block / ranges) * (256 / L); r0 < q.rows; r0 += step) {
+    const long i = r0 + threadIdx.x / L;
+    const int s = (int)(i * q.ld & 3);
+    uint32_t m = 0;
+    auto add = [&](int p, const float (&f)[8]) {
+      const long live = q.d - (c0 + (p * L + lane) * 8);
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const uint32_t b = j < live ? finite_bits(f[j]) : 0;
+        col[p][j] = max(col[p][j], b);
+        m = max(m, b);
+      }
+    };
+    if (i < q.rows && i * q.ld + last_c + 12 <= end) {
+      // All loads of the row first: the aligned groups around eight columns (a
+      // lane past the row takes its last ones), shifted as in load8.
+      float4 v[PASSES][3];
+      const float* row = x + (i * q.ld - s);
+#pragma unroll
+      for (int p = 0; p < PASSES; p++) {
+        if (c0 + p * L * 8 > last_c) break;
+        const float* at = row + min(c0 + (p * L + lane) * 8, last_c);
+#pragma unroll
+        for (int g = 0; g < 3; g++) v[p][g] = reinterpret_cast<const float4*>(at)[g];
+      }
+#pragma unroll
+      for (int p = 0; p < PASSES; p++) {
+        if (c0 + p * L * 8 > last_c) break;
+        float f[12];
+#pragma unroll
+        for (int g = 0; g < 3; g++)
+          f[4 * g] = v[p][g].x, f[4 * g + 1] = v[p][g].y, f[4 * g + 2] = v[p][g].z, f[4 * g + 3] = v[p][g].w;
+#pragma unroll
+        for (int j = 0; j < 10; j++) f[j] = s & 2 ? f[j + 2] : f[j];
+        float e[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) e[j] = s & 1 ? f[j + 1] : f[j];
+        add(p, e);
+      }
+    } else if (i < q.rows) {  // the matrix's end
+#pragma unroll 1
+      for (int p = 0; p < PASSES; p++) {
+        const long c = c0 + (p * L + lane) * 8;
+        if (c >= q.d) break;
+        float f[8];
+        load8(x, i * q.ld + c, (int)min(8l, q.d - c), end, f);
+#pragma unroll
+        for (int u = 0; u < PASSES; u++)
+          if (u == p) add(u, f);
+      }
+    }
+#pragma unroll
+    for (int o = L / 2; o; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    top = max(top, m);
+    if (m) low = max(low, ~m);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int p = 0; p < PASSES; p++)
+#pragma unroll
+    for (int j = 0; j < 8; j++)
+      if (col[p][j]) atomicMax(&cols[(p * 8 + j) * L + lane], col[p][j]);
+  top = __reduce_max_sync(0xffffffffu, top);
+  low = __reduce_max_sync(0xffffffffu, low);
+  if (threadIdx.x % 32 == 0) {
+    atomicMax(&rows[0], top);
+    atomicMax(&rows[1], low);
+  }
+  __syncthreads();
+  auto column = [&](int t) { return c0 + (t / (8 * L) * L + t % L) * 8 + t / L % 8; };
+  uint32_t least = ~0u;
+#pragma unroll
+  for (int t = threadIdx.x; t < COLS; t += 256)
+    if (column(t) < q.d) least = min(least, cols[t]);
+  least = __reduce_min_sync(0xffffffffu, least);
+  if (threadIdx.x % 32 == 0) atomicMin(&rows[2], least);
+  __syncthreads();
+  least = rows[2];
+  uint32_t* mine = found + R_COLUMNS + (second ? q.d + ranges : 0);
+  const bool by_column = !least || apart(rows[0], ~least);
+  if (by_column) {
+#pragma unroll
+    for (int t = threadIdx.x; t < COLS; t += 256)
+      if (column(t) < q.d && cols[t]) atomicMax(mine + column(t), cols[t]);
+  }
+  if (threadIdx.x == 0) {
+    atomicMax(found + (second ? R_W : R_X), rows[0]);
+    atomicMax(found + (second ? R_W_LOW : R_X_LOW), rows[1]);
+    if (by_column)
+      atomicAdd(found + R_BY_COLUMN, 1);
+    else
+      atomicMax(mine + q.d + range, least);
+  }
+}
+
+// The operands' 16-bit rows; with SPLIT, in two f16 terms scaled by the largest
+// element, or, where rows, columns or the loss gradients lie too far apart for
+// that, in three bf16 terms; the first block leaves what the products need in
+// `scal`. `blocks`: of k_ce_max.
+template <bool SPLIT>
+__global__ void __launch_bounds__(256)
+    k_ce_rows(Prep X, Prep W, const uint32_t* __restrict__ found, unsigned blocks,
+              uint32_t* scal) {
+  pdl_trigger();
+  pdl_wait();
+  const bool second = blockIdx.x >= X.blocks;
+  const Prep& q = second ? W : X;
+  bool wide = false;
   float s = 1.0f;
   if constexpr (SPLIT) {
-    uint32_t m = 0;
-    for (unsigned t = threadIdx.x; t < q.blocks; t += 256)
-      m = max(m, maxima[t + (second ? X.blocks : 0)]);
-    m = block_max(m);
-    s = ldexpf(1.0f, split_exp(m));
-    if (b == 0 && threadIdx.x == 0) scal[second ? S_W : S_X] = m;
+    uint32_t word[R_COLUMNS];
+#pragma unroll
+    for (int t = 0; t < R_COLUMNS; t++) word[t] = found[t];
+    const uint32_t x = word[R_X], w = word[R_W], g = word[R_G];
+    const bool by_column = word[R_BY_COLUMN] == blocks;
+    const bool far_x = columns_apart(found + R_COLUMNS, q.d, x, by_column);
+    const bool far_w =
+        columns_apart(found + R_COLUMNS + q.d + range_count(q.d), q.d, w, by_column);
+    wide = apart(g, word[R_G_LOW]) || apart(x, word[R_X_LOW]) || apart(w, word[R_W_LOW]) ||
+           far_x || far_w;
+    s = wide ? 1.0f : ldexpf(1.0f, split_exp(second ? w : x));
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+      scal[S_X] = x;
+      scal[S_W] = w;
+      scal[S_G] = g;
+      scal[S_WIDE] = wide;
+    }
   }
   const long end = (q.rows - 1) * q.ld + q.d;
-  for_groups(q, b, [&](long i, long c, int live) {
-    uint4 hi, lo;
+  for_groups(q, blockIdx.x - (second ? X.blocks : 0), [&](long i, long c, int live) {
+    uint16_t* out = q.out + i * q.dp + c;
+    auto put = [&](int term, const uint4& v) { *reinterpret_cast<uint4*>(out + term * q.term) = v; };
     if constexpr (SPLIT) {
       float f[8];
       load8(static_cast<const float*>(q.x), i * q.ld + c, live, end, f);
 #pragma unroll
-      for (int j = 0; j < 8; j++) f[j] = isfinite(f[j]) ? f[j] : NAN;
-      hi = pack8<true, true>(f, s, lo);
-      *reinterpret_cast<uint4*>(q.lo + i * q.dp + c) = lo;
+      for (int j = 0; j < 8; j++) f[j] = isfinite(f[j]) ? f[j] * s : NAN;
+      if (wide) {
+#pragma unroll
+        for (int j = 0; j < 3; j++) put(j, pack8<false, true>(f));
+      } else {
+#pragma unroll
+        for (int j = 0; j < 2; j++) put(j, pack8<true, true>(f));
+      }
     } else {
-      hi = load8(static_cast<const uint16_t*>(q.x), i * q.ld + c, live, end);
+      put(0, load8(static_cast<const uint16_t*>(q.x), i * q.ld + c, live, end));
     }
-    *reinterpret_cast<uint4*>(q.hi + i * q.dp + c) = hi;
   });
 }
 
-// Largest magnitude of the rows' loss gradients (finite ones, of rows with a
-// target: what the others hold is not used), into a zeroed word.
+// Largest and smallest magnitude of the rows' loss gradients (finite ones that
+// are not 0, of rows with a target: what the others hold is not used), into
+// zeroed words; `least` may be null.
 __global__ void __launch_bounds__(256)
     k_ce_gmax(const float* __restrict__ g, const uint32_t* __restrict__ targets, long n, long k,
-              uint32_t* out) {
+              uint32_t* most, uint32_t* least) {
   pdl_trigger();
   pdl_wait();
-  uint32_t m = 0;
-  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long)gridDim.x * 256)
-    if ((long)targets[i] < k) m = max(m, finite_bits(g[i]));
-  m = block_max(m);
-  if (threadIdx.x == 0 && m) atomicMax(out, m);
+  uint32_t top = 0, low = 0;
+  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long)gridDim.x * 256) {
+    const uint32_t m = (long)targets[i] < k ? finite_bits(g[i]) : 0;
+    top = max(top, m);
+    if (m) low = max(low, ~m);
+  }
+  top = block_max(top);
+  __syncthreads();
+  low = block_max(low);
+  if (threadIdx.x == 0 && top) {
+    atomicMax(most, top);
+    if (least) atomicMax(least, low);
+  }
 }
 
 // The outputs of a product that ran in splits of k: the sum of the splits'
@@ -1072,25 +1334,26 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   return fn;
 }
 
-// A 16-bit operand: rows x cols, row stride ld (a multiple of 8), one or two
-// terms.
+// A 16-bit operand: rows x cols, row stride ld (a multiple of 8), and the room
+// of one or three terms, `term` elements apart.
 struct Operand {
-  const uint16_t* hi;
-  const uint16_t* lo;  // null: one term
+  const uint16_t* at;
+  long term;
+  int terms;
   long rows, cols, ld;
 };
 
 // Read in boxes of 64 columns (128 bytes) by 64 rows, 128-byte swizzle; P is
 // written in boxes of 32 by 32, 64-byte swizzle. Every box's first column is a
 // multiple of 64, or 32.
-CUtensorMap make_map(const uint16_t* base, const Operand& o, bool store = false) {
+CUtensorMap make_map(const Operand& o, int term, bool store = false) {
   CUtensorMap m;
   cuuint64_t dims[2] = {(cuuint64_t)o.cols, (cuuint64_t)o.rows};
   cuuint64_t strides[1] = {(cuuint64_t)o.ld * 2};
   cuuint32_t box[2] = {store ? 32u : 64u, store ? 32u : 64u};
   cuuint32_t estr[2] = {1, 1};
   CUresult r = encode_fn()(&m, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2,
-                           const_cast<uint16_t*>(base), dims, strides, box, estr,
+                           const_cast<uint16_t*>(o.at + term * o.term), dims, strides, box, estr,
                            CU_TENSOR_MAP_INTERLEAVE_NONE,
                            store ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -1098,17 +1361,19 @@ CUtensorMap make_map(const uint16_t* base, const Operand& o, bool store = false)
   return m;
 }
 
-template <int EPI, int CG, int PARTS, int WIDTH, bool CHAINED = PARTS == 2>
+template <int EPI, int CG, bool TERMS, int WIDTH, bool CHAINED = TERMS>
 void launch_gemm(eb_engine* e, const Operand& A, const Operand& B, const Operand& C,
                  GemmParams P) {
-  using S = Shape<EPI, CG, PARTS, WIDTH, CHAINED>;
-  const auto kern = k_gemm<EPI, CG, PARTS, WIDTH, CHAINED>;
+  using S = Shape<EPI, CG, TERMS, WIDTH, CHAINED>;
+  const auto kern = k_gemm<EPI, CG, TERMS, WIDTH, CHAINED>;
   static std::atomic<uint64_t> allowed{0};
   allow_smem(e, kern, S::SMEM, allowed);
-  const CUtensorMap a0 = make_map(A.hi, A), a1 = PARTS == 2 ? make_map(A.lo, A) : a0;
-  const CUtensorMap b0 = make_map(B.hi, B), b1 = PARTS == 2 ? make_map(B.lo, B) : b0;
-  const CUtensorMap c0 = EPI != LSE ? make_map(C.hi, C, EPI == PROB) : b0;
-  const CUtensorMap c1 = EPI != LSE && PARTS == 2 ? make_map(C.lo, C, EPI == PROB) : c0;
+  Maps<TERMS ? 3 : 1> maps;
+  for (int t = 0; t < (TERMS ? 3 : 1); t++) {
+    maps.a[t] = make_map(A, t);
+    maps.b[t] = make_map(B, t);
+    maps.c[t] = EPI != LSE ? make_map(C, t, EPI == PROB) : maps.b[t];
+  }
   const int units = P.q[0].units + P.q[1].units;
   const int clusters = std::min(units, e->num_sms / CG);
   P.more = P.q[0].units % clusters;
@@ -1126,7 +1391,7 @@ void launch_gemm(eb_engine* e, const Operand& A, const Operand& B, const Operand
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = CG == 2 ? 2 : 1;
-  cuda_check(cudaLaunchKernelEx(&cfg, kern, a0, a1, b0, b1, c0, c1, P), "linear cross entropy");
+  cuda_check(cudaLaunchKernelEx(&cfg, kern, maps, P), "linear cross entropy");
   e->stats.kernel_launches++;
 }
 
@@ -1172,7 +1437,6 @@ Prob make_prob(long M, long N, long K, const TileCost& t, int clusters = 0) {
   q.splits = 1;
   q.units = q.mtiles * q.ntiles;
   q.group = std::min(q.mtiles, 8);
-  q.unscale = -1;
   return q;
 }
 
@@ -1209,37 +1473,50 @@ void gemm(eb_engine* e, const Operand& A, const Operand& B, const Operand& C, Ti
     q.last = Divisor::of(std::max(q.mtiles % q.group, 1));
   }
   if constexpr (EPI == LSE) {
-    if (!A.lo && P.q[0].kblocks > 12) {
+    if (A.terms == 1 && P.q[0].kblocks > 12) {
       if (t == NARROW)
-        launch_gemm<EPI, 1, 1, 64, true>(e, A, B, C, P);
+        launch_gemm<EPI, 1, false, 64, true>(e, A, B, C, P);
       else if (t == SINGLE)
-        launch_gemm<EPI, 1, 1, 256, true>(e, A, B, C, P);
+        launch_gemm<EPI, 1, false, 256, true>(e, A, B, C, P);
       else
-        launch_gemm<EPI, 2, 1, 256, true>(e, A, B, C, P);
+        launch_gemm<EPI, 2, false, 256, true>(e, A, B, C, P);
       return;
     }
   }
-  if (A.lo) {
+  if (A.terms > 1) {
     if (t == NARROW)
-      launch_gemm<EPI, 1, 2, 64>(e, A, B, C, P);
+      launch_gemm<EPI, 1, true, 64>(e, A, B, C, P);
     else if (t == SINGLE)
-      launch_gemm<EPI, 1, 2, 128>(e, A, B, C, P);
+      launch_gemm<EPI, 1, true, 128>(e, A, B, C, P);
     else
-      launch_gemm<EPI, 2, 2, 256>(e, A, B, C, P);
+      launch_gemm<EPI, 2, true, 256>(e, A, B, C, P);
   } else {
     if (t == NARROW)
-      launch_gemm<EPI, 1, 1, 64>(e, A, B, C, P);
+      launch_gemm<EPI, 1, false, 64>(e, A, B, C, P);
     else if (t == SINGLE)
-      launch_gemm<EPI, 1, 1, 256>(e, A, B, C, P);
+      launch_gemm<EPI, 1, false, 256>(e, A, B, C, P);
     else
-      launch_gemm<EPI, 2, 1, 256>(e, A, B, C, P);
+      launch_gemm<EPI, 2, false, 256>(e, A, B, C, P);
   }
+}
+
+// The words that f32 calls raise, zero between them: a call that failed before its
+// products left them as they were.
+uint32_t* found_words(eb_engine* e, const LinearCeArgs& a) {
+  uint32_t* found = e->scratch_get<uint32_t>("ce_found", found_count(a.d), true);
+  if (e->ce_found_raised) {
+    auto& all = e->scratch["ce_found"];
+    EB_CUDA(cudaMemsetAsync(all.p, 0, all.bytes, e->stream));
+    e->ce_found_raised = false;
+  }
+  return found;
 }
 
 // The 16-bit operands of x and w: each itself where TMA can read it (16-bit,
 // row stride a multiple of 16 bytes), else a copy in scratch; f32 split into
-// two terms.
-void operands(eb_engine* e, const LinearCeArgs& a, uint32_t* scal, Operand& X, Operand& W) {
+// two or three terms.
+void operands(eb_engine* e, const LinearCeArgs& a, uint32_t* found, uint32_t* scal, Operand& X,
+              Operand& W) {
   const bool split = a.dtype == EB_F32;
   Prep prep[2] = {};
   const void* src[2] = {a.x, a.w};
@@ -1247,45 +1524,61 @@ void operands(eb_engine* e, const LinearCeArgs& a, uint32_t* scal, Operand& X, O
   Operand* out[2] = {&X, &W};
   for (int i = 0; i < 2; i++) {
     Operand& o = *out[i];
-    o = Operand{static_cast<const uint16_t*>(src[i]), nullptr, (long)rows[i], (long)a.d,
-                (long)ld[i]};
+    o = Operand{static_cast<const uint16_t*>(src[i]), 0, 1, (long)rows[i], (long)a.d, (long)ld[i]};
     if (!split && ld[i] % 8 == 0) continue;
     o.ld = ((long)a.d + 7) / 8 * 8;
-    uint16_t* c = e->scratch_get<uint16_t>(i ? "ce_w" : "ce_x", rows[i] * (size_t)o.ld * (split ? 2 : 1));
-    o.hi = c;
-    if (split) o.lo = c + rows[i] * (size_t)o.ld;
-    prep[i] = Prep{src[i], (long)rows[i], (long)a.d, (long)ld[i], o.ld, c, split ? c + rows[i] * (size_t)o.ld : nullptr,
+    o.term = (long)rows[i] * o.ld;
+    o.terms = split ? 3 : 1;
+    uint16_t* c = e->scratch_get<uint16_t>(i ? "ce_w" : "ce_x", (size_t)(o.term * o.terms));
+    o.at = c;
+    prep[i] = Prep{src[i], (long)rows[i], (long)a.d, (long)ld[i], o.ld, c, o.term,
                    (unsigned)std::min<size_t>((rows[i] * (size_t)(o.ld / 8) + 255) / 256, PREP_BLOCKS)};
   }
   const unsigned grid = prep[0].blocks + prep[1].blocks;
   if (!grid) return;
   if (split) {
-    uint32_t* maxima = e->scratch_get<uint32_t>("ce_maxima", 2 * PREP_BLOCKS);
-    launch_pdl(e, k_ce_max, dim3(grid), dim3(256), 0, prep[0], prep[1], maxima);
+    // Lanes of a row, and blocks: each takes its share of the rows of one range.
+    e->ce_found_raised = true;
+    const int lanes = a.d <= 64 ? 8 : a.d <= 128 ? 16 : 32;
+    const int passes = (int)std::min<size_t>((a.d + 255) / 256, 4);
+    const auto kern = lanes == 8    ? k_ce_max<8, 1>
+                      : lanes == 16 ? k_ce_max<16, 1>
+                      : passes == 1 ? k_ce_max<32, 1>
+                      : passes == 2 ? k_ce_max<32, 2>
+                      : passes == 3 ? k_ce_max<32, 3>
+                                    : k_ce_max<32, 4>;
+    const long resident = (passes == 1 ? 4 : passes == 2 ? 3 : 2) * (long)e->num_sms;
+    Prep m[2] = {prep[0], prep[1]};
+    for (Prep& q : m) {
+      const long each = 256 / lanes, ranges = range_count(q.d);
+      const long most = (resident * q.rows / (long)(a.n + a.k) + ranges) / ranges;
+      q.blocks = (unsigned)(ranges * std::min((q.rows + each - 1) / each, most));
+    }
+    launch_pdl(e, kern, dim3(m[0].blocks + m[1].blocks), dim3(256), 0, m[0], m[1], found);
     launch_pdl(e, k_ce_rows<true>, dim3(grid), dim3(256), 0, prep[0], prep[1],
-               (const uint32_t*)maxima, scal);
+               (const uint32_t*)found, m[0].blocks + m[1].blocks, scal);
     e->stats.kernel_launches += 2;
   } else {
     launch_pdl(e, k_ce_rows<false>, dim3(grid), dim3(256), 0, prep[0], prep[1],
-               (const uint32_t*)nullptr, (uint32_t*)nullptr);
+               (const uint32_t*)nullptr, 0u, scal);
     e->stats.kernel_launches++;
   }
 }
 
 Operand rows_of(const Operand& o, long r0, long r1) {
   Operand p = o;
-  p.hi += r0 * o.ld;
-  if (p.lo) p.lo += r0 * o.ld;
+  p.at += r0 * o.ld;
   p.rows = r1 - r0;
   return p;
 }
 
-GemmParams base_params(const LinearCeArgs& a, const uint32_t* scal) {
+GemmParams base_params(const LinearCeArgs& a, uint32_t* found, const uint32_t* scal) {
   GemmParams P{};
+  P.found = found;
+  P.found_words = found ? found_count((long)a.d) : 0;
   P.scal = scal;
   P.scale = a.scale;
   P.fmt = a.dtype == EB_BF16 ? 1u : 0u;
-  P.split = a.dtype == EB_F32;
   P.targets = a.targets;
   P.k = (long)a.k;
   P.pscale = a.dtype == EB_BF16 ? 1.0f : PSCALE;
@@ -1358,7 +1651,7 @@ void products(eb_engine* e, const Operand& A, Operand B, Operand C, GemmParams P
   Prob chosen[2] = {};
   for (Tile t : {PAIR, SINGLE, NARROW}) {
     if (t == SINGLE && (P.q[0].M > BM || (count == 2 && P.q[1].M > BM))) continue;
-    const TileCost c = tile_cost(t, A.lo ? 2 : 1);
+    const TileCost c = tile_cost(t, A.terms > 1 ? 2 : 1);
     Prob q[2] = {P.q[0], P.q[1]};
     for (int i = 0; i < count; i++) {
       const Prob m = make_prob(q[i].M, q[i].N, q[i].K, c);
@@ -1428,14 +1721,15 @@ void linear_ce(eb_engine* e, const LinearCeArgs& a, float* loss, float* lse) {
     return join(e, part, parts, (long)a.n, (long)a.k, zt, a.targets, loss, lse);
   }
   uint32_t* scal = e->scratch_get<uint32_t>("ce_scalars", S_WORDS);
+  uint32_t* found = a.dtype == EB_F32 ? found_words(e, a) : nullptr;
   Operand X, W;
-  operands(e, a, scal, X, W);
+  operands(e, a, found, scal, X, W);
   // Rows a pass: as many as keep the half tiles' (max, sum) to 256 MB.
   const size_t most = ((size_t)256 << 20) / sizeof(float2) / (2 * (a.k / 160 + 1)) / 256 * 256;
   const size_t rows = std::max<size_t>(std::min(a.n, most), 256);
   for (size_t r0 = 0; r0 < a.n; r0 += rows) {
     const long n = (long)std::min(a.n - r0, rows);
-    GemmParams P = base_params(a, scal);
+    GemmParams P = base_params(a, found, scal);
     const int terms = a.dtype == EB_F32 ? 2 : 1;
     const Tile tile = score_tile(e, n, (long)a.k, (long)a.d, terms);
     const TileCost cost = tile_cost(tile, terms);
@@ -1446,6 +1740,7 @@ void linear_ce(eb_engine* e, const LinearCeArgs& a, float* loss, float* lse) {
     P.zt = e->scratch_get<float>("ce_zt", (size_t)n);
     P.targets = a.targets + r0;
     gemm<LSE>(e, rows_of(X, (long)r0, (long)r0 + n), W, W, tile, P);
+    e->ce_found_raised = false;
     join(e, part, parts, n, (long)a.k, P.zt, P.targets, loss + r0, lse + r0);
   }
 }
@@ -1461,26 +1756,34 @@ void linear_ce_backward(eb_engine* e, const LinearCeArgs& a, const LinearCeGrads
   if (linear_ce_is_small(a)) return linear_ce_small_backward(e, a, g);
   if (linear_ce_is_few(a)) return linear_ce_few_backward(e, a, g);
   uint32_t* scal = e->scratch_get<uint32_t>("ce_scalars", S_WORDS);
+  uint32_t* found = a.dtype == EB_F32 ? found_words(e, a) : nullptr;
   if (!g.one_dloss) {
-    EB_CUDA(cudaMemsetAsync(scal + S_G, 0, 4, e->stream));
+    uint32_t *most = scal + S_G, *least = nullptr;
+    if (found) {
+      e->ce_found_raised = true;
+      most = found + R_G;
+      least = found + R_G_LOW;
+    } else {
+      EB_CUDA(cudaMemsetAsync(most, 0, 4, e->stream));
+    }
     const unsigned grid = (unsigned)std::min<size_t>((a.n + 255) / 256, (size_t)e->num_sms);
     launch_pdl(e, k_ce_gmax, dim3(grid), dim3(256), 0, g.dloss, a.targets, (long)a.n, (long)a.k,
-               scal + S_G);
+               most, least);
     e->stats.kernel_launches++;
   }
   Operand X, W;
-  operands(e, a, scal, X, W);
+  operands(e, a, found, scal, X, W);
   // Pieces of P, as many elements as the scratch holds: the shorter side of
   // P whole where at least 2,048 of the longer then fit (the sums that run
   // over pieces are the shorter side's gradient), else pieces of both sides.
-  const int parts = a.dtype == EB_F32 ? 2 : 1;
-  const size_t room = ((size_t)512 << 20) / 2 / parts;  // elements of P
+  const int parts = a.dtype == EB_F32 ? 2 : 1, terms = a.dtype == EB_F32 ? 3 : 1;
+  const size_t room = ((size_t)512 << 20) / 2 / terms;  // elements of P
   const size_t npad = (a.n + 255) / 256 * 256, kpad = (a.k + 255) / 256 * 256;
   const size_t side = std::min(std::min(npad, kpad), room / 2048 / 256 * 256);
   const size_t other = std::max<size_t>(room / side / 256 * 256, 256);
   const size_t rows = std::min(npad, npad <= kpad ? side : other);
   const size_t cols = std::min(kpad, npad <= kpad ? other : side);
-  uint16_t* p = e->scratch_get<uint16_t>("ce_p", rows * cols * parts);
+  uint16_t* p = e->scratch_get<uint16_t>("ce_p", rows * cols * terms);
   const bool many_cols = cols < a.k, many_rows = rows < a.n;
   const long ldacc = ((long)a.d + 3) / 4 * 4;
   float* dxacc = g.dx && many_cols ? e->scratch_get<float>("ce_dx", std::min(rows, a.n) * ldacc) : nullptr;
@@ -1493,7 +1796,7 @@ void linear_ce_backward(eb_engine* e, const LinearCeArgs& a, const LinearCeGrads
       const size_t v1 = std::min(a.k, v0 + cols);
       const Operand Wv = rows_of(W, (long)v0, (long)v1);
       const long pr = (long)(r1 - r0), pc = (long)(v1 - v0);
-      GemmParams P = base_params(a, scal);
+      GemmParams P = base_params(a, found, scal);
       const Tile tile = score_tile(e, pr, pc, (long)a.d, parts);
       const TileCost cost = tile_cost(tile, parts);
       P.q[0] = make_prob(pr, pc, (long)a.d, cost, e->num_sms / cost.ctas);
@@ -1502,14 +1805,15 @@ void linear_ce_backward(eb_engine* e, const LinearCeArgs& a, const LinearCeGrads
       P.dloss = g.one_dloss ? g.dloss : g.dloss + r0;
       P.one_dloss = g.one_dloss;
       P.col0 = (long)v0;
-      const Operand Pm{p, parts == 2 ? p + rows * cols : nullptr, pr, pc, (pc + 7) / 8 * 8};
+      const Operand Pm{p, (long)(rows * cols), terms, pr, pc, (pc + 7) / 8 * 8};
       gemm<PROB>(e, Xr, Wv, Pm, tile, P);
+      e->ce_found_raised = false;
       int count = 0;
       Operand B[2];
       if (g.dx) {
         Prob& q = P.q[count];
         q = make_prob(pr, (long)a.d, pc, cost);
-        q.unscale = parts == 2 ? S_W : -1;
+        q.unscale = S_W;
         q.out = static_cast<char*>(g.dx) + r0 * g.lddx * dtype_bytes(g.dxtype);
         q.otype = g.dxtype;
         q.ldo = (long)g.lddx;
@@ -1524,7 +1828,7 @@ void linear_ce_backward(eb_engine* e, const LinearCeArgs& a, const LinearCeGrads
         Prob& q = P.q[count];
         q = make_prob(pc, (long)a.d, pr, cost);
         q.a_mn = 1;
-        q.unscale = parts == 2 ? S_X : -1;
+        q.unscale = S_X;
         q.out = static_cast<char*>(g.dw) + v0 * g.lddw * dtype_bytes(g.dwtype);
         q.otype = g.dwtype;
         q.ldo = (long)g.lddw;

@@ -460,10 +460,14 @@ int eb_layer_norm_backward(eb_engine* e, const eb_buf* dy, size_t lddy, const eb
  * target >= k is reported by the next call that waits (EB_INVALID_ARGUMENT)
  * and treated as EB_IGNORE. x and w have one float type; targets u32;
  * loss and lse f32, n each. Products: 16-bit types on the tensor cores as
- * they are; f32 as two scaled FP16 terms each (22 bits), three products
- * (a non-finite element counts as NaN), or in FP32 where k and d are small or
- * there are few rows (up to 16; of 16-bit types 4, off 16-byte alignment). Scratch: f32 operands' copies (as large as x and w;
- * not for those), and up to 256 MB. */
+ * they are; f32 as two FP16 terms each under one scale a matrix (22 bits, what
+ * lies below 2^-39 of its largest element left out) in three products, or, where
+ * some row's or column's largest element that is not 0 is below 2^-12 of the
+ * matrix's, as three bf16 terms each (24 bits, FP32's range) in six, which takes
+ * up to twice as long; a non-finite element counts as NaN. In FP32 where k and d are
+ * small (64) or there are few rows (up to 16; of 16-bit types 4, off 16-byte
+ * alignment). Scratch: f32 operands' copies (1.5 times x and w; not for
+ * those), and up to 256 MB. */
 int eb_linear_ce(eb_engine* e, const eb_buf* x, size_t n, size_t d, size_t ldx, const eb_buf* w,
                  size_t k, size_t ldw, const eb_buf* targets, float scale, eb_buf* loss,
                  eb_buf* lse);
@@ -473,7 +477,10 @@ int eb_linear_ce(eb_engine* e, const eb_buf* x, size_t n, size_t d, size_t ldx, 
  * dx = P w (n x d) and dw = P^T x (k x d). dloss is f32: n elements, or one
  * for all rows. P is formed a piece of the prototypes (and of the rows, when
  * there are very many) at a time in the engine's scratch (up to 512 MB),
- * rounded to x's type (f32: two FP16 terms). dx and dw: x's type or f32;
+ * rounded to x's type (f32: two FP16 terms, or three bf16 ones as above or
+ * where the rows' dloss lie more than 2^12 apart). Two FP16 terms, and f16, leave out
+ * what of P lies below 2^-38 of the largest |dloss| scale of a row with a target; f16
+ * rows with a dloss far below the largest lose bits by that. dx and dw: x's type or f32;
  * either may be null. Sums are added in a fixed order. A row with EB_IGNORE
  * has dx = 0 whatever it holds, but dw sums 0 x its elements: a non-finite one
  * makes its columns of dw NaN, as in the plain formula. */

@@ -76,8 +76,8 @@ class Values:
         e.sync()
         return loss, lse, dx, dw
 
-    def check(self, got):
-        """Against 64 bits. A score is off by its products' roundings (2^-22
+    def check(self, got, floor=True):
+        """Against 64 bits. (Without `floor`: f32's terms leave nothing out.) A score is off by its products' roundings (2^-22
         each for f32's terms) and sums (cut, at most d / 4 + 8 of them), and
         by 2^-26 of its row's and its prototype's largest element for each of
         the other's (what the terms of f32 may leave out). P: the scores'
@@ -94,7 +94,7 @@ class Values:
         cross = X.abs() @ W.abs().T
         top_x, top_w = X.abs().amax(1, keepdim=True), W.abs().amax(1, keepdim=True)
         ez = s * cross * ((self.d / 4 + 8) * 2.0 ** -23 + (3 * 2.0 ** -22 if f32 else 0))
-        if f32:
+        if f32 and floor:
             ez = ez + s * 2.0 ** -26 * (top_x * W.abs().sum(1)[None, :] + top_w.T * X.abs().sum(1, keepdim=True))
         L = torch.logsumexp(Z, 1)
         el = ez.amax(1) + 2.0 ** -20 + 6 * 2.0 ** -23 * (L.abs() + Z.abs().amax(1))
@@ -107,11 +107,12 @@ class Values:
         hot = torch.zeros_like(p).scatter_(1, t, 1.0)
         P = g * (p - hot)
         keep = {torch.float32: 2.0 ** -21, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -10}[self.dtype]
-        eP = g.abs() * (p * (ez + 2 * el[:, None] + 2.0 ** -20) + 2.0 ** -23 * hot + 2.0 ** -25) + P.abs() * keep
+        least = 2.0 ** -25 if floor else 2.0 ** -100
+        eP = g.abs() * (p * (ez + 2 * el[:, None] + 2.0 ** -20) + 2.0 ** -23 * hot + least) + P.abs() * keep
         for out, A, B, eA, top, what in ((dx, P, W, eP, top_w, "dx"), (dw, P.T, X, eP.T, top_x, "dw")):
             want = A @ B
             tol = eA @ B.abs() + ((A.shape[1] / 4 + 40) * 2.0 ** -23 + (2.0 ** -20 if f32 else 0)) * (A.abs() @ B.abs())
-            if f32:
+            if f32 and floor:
                 tol = tol + 2.0 ** -26 * (A.abs() @ top)
             within(out, want, tol + HALF_ULP[out.dtype] * (want.abs() + tol) + 2.0 ** -149, what)
 
@@ -155,3 +156,106 @@ def test_rows_and_prototypes_of_any_size(eng, n, k, d, sizes):
     c = Values(n, k, d, torch.float32, 3)
     c.x, c.w, c.scale, c.dloss = c.x * sizes[0], c.w * sizes[1], sizes[2], c.dloss * sizes[3]
     c.check(c.run(eng))
+
+
+def masked_row(c):
+    c.x[3] = 1e30  # ignored
+
+
+def small_rows(c):
+    c.x[5::7] *= 1e-9
+    c.x[6] *= 1e-20
+
+
+def small_prototypes(c):
+    c.w[5::7] *= 1e-9
+    c.w[6] *= 1e-20
+
+
+def features_apart(c):
+    c.x[:, 5], c.w[:, 5] = c.x[:, 5] * 1e9, c.w[:, 5] * 1e-9
+    c.x[:, 7], c.w[:, 7] = c.x[:, 7] * 1e-12, c.w[:, 7] * 1e10
+
+
+def loss_gradients_apart(c):
+    c.dloss = c.dloss.sign() * 10.0 ** (-12 * c.rand)
+
+
+def loss_gradients_far_apart(c):
+    c.dloss = c.dloss.sign() * 10.0 ** (-50 * c.rand + 20)
+
+
+def one_row(c):
+    """A single element that is not 0 in a row and in a column."""
+    c.x[9] = 0
+    c.x[9, 2] = 1e-15
+    c.w[:, 4] = 0
+    c.w[11, 4] = 1e-15
+
+
+@pytest.mark.parametrize("edit", [masked_row, small_rows, small_prototypes, features_apart,
+                                  loss_gradients_apart, loss_gradients_far_apart, one_row],
+                         ids=lambda f: f.__name__)
+@pytest.mark.parametrize("n,k,d", SHAPES + [(20, 5000, 520), (257, 513, 1100), (3000, 1000, 392)])
+def test_f32_values_orders_of_magnitude_apart(eng, n, k, d, edit):
+    """What lies far below the largest of its matrix keeps its own 22 bits: rows,
+    prototypes and features, and gradients of rows of little weight."""
+    c = Values(n, k, d, torch.float32, 4)
+    edit(c)
+    got = c.run(eng)
+    c.check(got, floor=False)
+    for a, b in zip(c.run(eng), got):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("n,k,d", SHAPES)
+def test_f32_non_finite_rows_beside_values_apart(eng, n, k, d):
+    """In three terms as in two: a row with a NaN or an infinity stays its own."""
+    c = Values(n, k, d, torch.float32, 5, ignored=0.0)
+    small_rows(c)
+    clean = c.run(eng)
+    c.x[7, 3], c.x[9, 1] = math.nan, math.inf
+    c.t[7] = eb.IGNORE
+    loss, lse, dx, _ = c.run(eng)
+    keep = torch.ones(n, dtype=torch.bool, device="cuda")
+    keep[7] = keep[9] = False
+    assert torch.equal(loss[keep], clean[0][keep]) and torch.equal(lse[keep], clean[1][keep])
+    assert torch.equal(dx[keep], clean[2][keep])
+    assert lse[7].isnan() and lse[9].isnan() and loss[9].isnan() and dx[9].isnan().any()
+    assert loss[7] == 0 and (dx[7] == 0).all()
+
+
+def sparse(c):
+    """Most elements 0, whole columns too: no block of rows sees every column."""
+    c.x = torch.where(c.x > 1.0, c.x, 0 * c.x)
+    c.x[:, 2::9] = 0
+    c.w[:, 1::5] = 0
+    c.w[20:, 3::7] = 0
+
+
+def sparse_and_apart(c):
+    sparse(c)
+    c.x[8, 0], c.w[8, 0] = 1e9, 1e-9
+    c.x[9:, 0] = 0
+
+
+@pytest.mark.parametrize("edit,floor", [(sparse, True), (sparse_and_apart, False)], ids=["sparse", "apart"])
+@pytest.mark.parametrize("n,k,d", SHAPES + [(257, 513, 2100), (3000, 1000, 392), (70, 900, 60)])
+def test_f32_columns_of_zeros(eng, n, k, d, edit, floor):
+    c = Values(n, k, d, torch.float32, 6)
+    edit(c)
+    c.check(c.run(eng), floor)
+
+
+def test_f32_calls_leave_nothing_for_the_next(eng):
+    """What one call finds in its rows is not there in the next one's."""
+    c = Values(300, 200, 130, torch.float32, 7)
+    clean = c.run(eng)
+    big = Values(300, 200, 130, torch.float32, 8)
+    big.x, big.dloss = big.x * 1e20, big.dloss * 1e-20
+    small_prototypes(big)
+    big.run(eng)
+    wider = Values(40, 300, 1500, torch.float32, 9)
+    wider.check(wider.run(eng))
+    for a, b in zip(c.run(eng), clean):
+        assert torch.equal(a, b)
