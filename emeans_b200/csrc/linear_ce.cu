@@ -25,9 +25,11 @@
 // accumulator. The dropped lo.lo term is 2^-22 of the product. That floor is the
 // matrix's, so rows, columns or loss gradients far below the largest would lose
 // their last bits, or all of them. Where the smallest row's or column's largest
-// element, or a row's loss gradient, is below 2^-12 of the largest (of those that
+// element is below 2^-12 of the largest (of those that
 // are not 0), the operands and P are instead split into three bf16 terms each (24
-// bits, FP32's own range, no scale) and multiplied in six products. The
+// bits, FP32's own range, no scale) and multiplied in six products. Where the rows'
+// loss gradients lie that far apart, P and the gradients' products are (the scores
+// again stay the forward pass's, to the last bit). The
 // preparation decides it on the device, and the same kernels read it: 3,001 x
 // 5,003 x 385 forward and backward 62 and 150 us one way, 83 and 238 the other;
 // 8,192 x 8,192 x 1024 290 and 905, 506 and 1,867.
@@ -66,8 +68,9 @@ enum Epi { LSE, PROB, OUT };
 
 // Words shared by a call's kernels (device scratch): bits of max|x| and max|w| over
 // the finite elements (f32 operands) and of max|dloss| over the rows with a target;
-// whether f32 operands are three bf16 terms.
-enum { S_X, S_W, S_G, S_WIDE, S_WORDS };
+// whether f32 operands, and whether P and the gradients' operands are three bf16
+// terms.
+enum { S_X, S_W, S_G, S_WIDE, S_WIDE_P, S_WORDS };
 
 // Words that an f32 call's first kernels raise, zero between calls: the same
 // magnitudes; the complements of the smallest row's max|x| and max|w| and of the
@@ -177,7 +180,8 @@ struct Shape {
 };
 
 // A launch's tensor maps, one a term: A, B, and C: the second product's B (OUT) or
-// P (PROB).
+// P (PROB). Operands that are kept both ways have f16 terms 0 and 1 and bf16 terms 2
+// to 4.
 template <int T>
 struct Maps {
   CUtensorMap a[T], b[T], c[T];
@@ -201,6 +205,12 @@ __device__ __forceinline__ float ex(float v) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v * LOG2E));
   return r;
 }
+
+// The softmax of rows whose largest score is past this size goes by rounded scores:
+// half their last bit is 2^-14 and more, and the exact products of fmaf would leave a
+// row's largest score that much, or (past 2^24) whole units, above or below an lse
+// that is that score rounded.
+constexpr float STEEP = 1024.0f;
 
 // Folds (m', s') into a running (max, sum of exp(z - max)); (-inf, 0) is empty.
 // NaN scores are in the sums, not in the maxima.
@@ -356,7 +366,7 @@ __device__ __forceinline__ void store_block(const Prob& q, float* sums, float* b
 // in registers between chains.
 template <int EPI, int CG, bool TERMS, int WIDTH, bool CHAINED>
 __global__ void __launch_bounds__(NTHREADS, 1)
-    k_gemm(const __grid_constant__ Maps<TERMS ? 3 : 1> maps, const __grid_constant__ GemmParams P) {
+    k_gemm(const __grid_constant__ Maps<TERMS ? 5 : 1> maps, const __grid_constant__ GemmParams P) {
   using S = Shape<EPI, CG, TERMS, WIDTH, CHAINED>;
   constexpr int HALF = S::HALF;
   using namespace tc;
@@ -414,7 +424,9 @@ __global__ void __launch_bounds__(NTHREADS, 1)
   pdl_wait();
   // Terms of both operands, and what follows from them. A stage holds A's terms,
   // then B's.
-  const bool wide = TERMS && P.scal[S_WIDE];
+  const bool wide_p = TERMS && EPI != LSE && P.scal[S_WIDE_P];
+  const bool wide = EPI == OUT ? wide_p : TERMS && P.scal[S_WIDE];
+  const int bf16_at = TERMS && EPI == OUT && wide && !P.scal[S_WIDE] ? 2 : 0;  // of B's terms
   const int terms = !TERMS ? 1 : wide ? 3 : 2;
   const int stage_bytes = terms * (S::A_BYTES + S::B_BYTES);
   const int stages = min(S::RING / stage_bytes, S::MOST_STAGES);
@@ -471,7 +483,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
 #pragma unroll
           for (int p = 0; p < (TERMS ? 3 : 1); p++) {
             if (p >= terms) break;
-            const CUtensorMap* mb = q.prob ? &maps.c[p] : &maps.b[p];
+            const CUtensorMap* mb = q.prob ? &maps.c[p + bf16_at] : &maps.b[p + bf16_at];
 #pragma unroll
             for (int c = 0; c < S::B_ROWS / 64; c++, st += 8192) {
               const int n = bn + c * 64;
@@ -604,7 +616,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       // Nothing to be relative to: P takes the rows' own (a non-finite one stays with
       // the rows that have a target).
       // Three bf16 terms of P have FP32's range: they too take the rows' own.
-      if (wide || !(gmax > 0.0f && gmax < INFINITY)) gmax = 1.0f;
+      if (wide_p || !(gmax > 0.0f && gmax < INFINITY)) gmax = 1.0f;
     }
     const uint32_t release = CG == 2 ? map_rank(smem_u32(tempty), 0) : smem_u32(tempty);
     int tc = 0, stores = 0;
@@ -656,6 +668,9 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         }
         next = row_of(next_unit(u), after);
       }
+      // exp(v psc + poff) is p.
+      const bool steep = EPI == PROB && __any_sync(0xffffffffu, fabsf(lse) > STEEP);
+      const float psc = steep ? 1.0f : sc, poff = steep ? 0.0f : -lse;
       // Waits for the next chain; then its TMEM columns are this warp's.
       auto wait_chain = [&] {
         stop = !mbar_wait(&tfull[tc & 1], (tc >> 1) & 1, abort_flag);
@@ -750,14 +765,21 @@ __global__ void __launch_bounds__(NTHREADS, 1)
           const bool target = tcol >> 5 == h;
           const int e = tcol & 31;
           float at_target = 0.0f;
+          if (steep) {  // no score is above lse (a NaN stays one)
+#pragma unroll
+            for (int j = 0; j < 32; j++) {
+              v[j] = __fmul_rn(v[j], sc) - lse;
+              v[j] = v[j] > 0.0f ? 0.0f : v[j];
+            }
+          }
           if (target) {  // by expm1: near 1, p's own rounding would be all that is left
             float z = 0.0f;
 #pragma unroll
             for (int j = 0; j < 32; j++) z = j == e ? v[j] : z;
-            at_target = gr * expm1f(fmaf(z, sc, -lse));
+            at_target = gr * expm1f(fmaf(z, psc, poff));
           }
 #pragma unroll
-          for (int j = 0; j < 32; j++) v[j] = ex(fmaf(v[j], sc, -lse)) * gr;
+          for (int j = 0; j < 32; j++) v[j] = ex(fmaf(v[j], psc, poff)) * gr;
           if (gr == 0.0f) {  // nothing of a row without a gradient, not even its NaN
 #pragma unroll
             for (int j = 0; j < 32; j++) v[j] = 0.0f;
@@ -772,7 +794,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
           // 8,192 x 8,192 x 256 f32 272 and 263.)
           const int turn = (lane >> 1) & 3;
           const bool bf = !TERMS && P.fmt;
-          if (!bf && !wide) {
+          if (!bf && !wide_p) {
 #pragma unroll
             for (int j = 0; j < 32; j++) v[j] *= PSCALE;
             at_target *= PSCALE;
@@ -825,7 +847,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
               round(box, 0, no, no);
             else
               round(box, 0, yes, no);
-          } else if (!wide) {
+          } else if (!wide_p) {
             if (lane == 0) stores_read<0>();
             round(boxes, 0, yes, yes);
           } else {
@@ -852,7 +874,12 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       }
       if constexpr (EPI == LSE) {
         if (live) {
-          P.part[(long)(q.nt * 2 + hf) * pr.M + i] = make_float2(m2 * sc, sum);
+          // Past STEEP the sum goes by the largest score itself, not its rounded value,
+          // as P will: 1 where the others are nothing beside it.
+          const float top = m2 * sc, off = fmaf(m2, sc, -top);
+          if (fabsf(top) > STEEP && top > -INFINITY)
+            sum = fabsf(off) < 60.0f || isnan(sum) ? sum * ex(-off) : 1.0f;
+          P.part[(long)(q.nt * 2 + hf) * pr.M + i] = make_float2(top, sum);
           if (tcol >= 0) P.zt[i] = zt * sc;
         }
       }
@@ -1190,9 +1217,9 @@ __global__ void __launch_bounds__(256, 2)
 }
 
 // The operands' 16-bit rows; with SPLIT, in two f16 terms scaled by the largest
-// element, or, where rows, columns or the loss gradients lie too far apart for
-// that, in three bf16 terms; the first block leaves what the products need in
-// `scal`. `blocks`: of k_ce_max.
+// element, or, where rows or columns lie too far apart for that, in three bf16
+// terms, or both ways where the loss gradients do; the first block leaves what the
+// products need in `scal`. `blocks`: of k_ce_max.
 template <bool SPLIT>
 __global__ void __launch_bounds__(256)
     k_ce_rows(Prep X, Prep W, const uint32_t* __restrict__ found, unsigned blocks,
@@ -1201,7 +1228,7 @@ __global__ void __launch_bounds__(256)
   pdl_wait();
   const bool second = blockIdx.x >= X.blocks;
   const Prep& q = second ? W : X;
-  bool wide = false;
+  bool wide = false, wide_p = false;
   float s = 1.0f;
   if constexpr (SPLIT) {
     uint32_t word[R_COLUMNS];
@@ -1212,14 +1239,15 @@ __global__ void __launch_bounds__(256)
     const bool far_x = columns_apart(found + R_COLUMNS, q.d, x, by_column);
     const bool far_w =
         columns_apart(found + R_COLUMNS + q.d + range_count(q.d), q.d, w, by_column);
-    wide = apart(g, word[R_G_LOW]) || apart(x, word[R_X_LOW]) || apart(w, word[R_W_LOW]) ||
-           far_x || far_w;
-    s = wide ? 1.0f : ldexpf(1.0f, split_exp(second ? w : x));
+    wide = apart(x, word[R_X_LOW]) || apart(w, word[R_W_LOW]) || far_x || far_w;
+    wide_p = wide || apart(g, word[R_G_LOW]);
+    s = ldexpf(1.0f, split_exp(second ? w : x));
     if (blockIdx.x == 0 && threadIdx.x == 0) {
       scal[S_X] = x;
       scal[S_W] = w;
       scal[S_G] = g;
       scal[S_WIDE] = wide;
+      scal[S_WIDE_P] = wide_p;
     }
   }
   const long end = (q.rows - 1) * q.ld + q.d;
@@ -1230,13 +1258,17 @@ __global__ void __launch_bounds__(256)
       float f[8];
       load8(static_cast<const float*>(q.x), i * q.ld + c, live, end, f);
 #pragma unroll
-      for (int j = 0; j < 8; j++) f[j] = isfinite(f[j]) ? f[j] * s : NAN;
-      if (wide) {
+      for (int j = 0; j < 8; j++) f[j] = isfinite(f[j]) ? f[j] : NAN;
+      if (!wide) {
+        float h[8];
 #pragma unroll
-        for (int j = 0; j < 3; j++) put(j, pack8<false, true>(f));
-      } else {
+        for (int j = 0; j < 8; j++) h[j] = f[j] * s;
 #pragma unroll
-        for (int j = 0; j < 2; j++) put(j, pack8<true, true>(f));
+        for (int j = 0; j < 2; j++) put(j, pack8<true, true>(h));
+      }
+      if (wide_p) {
+#pragma unroll
+        for (int j = 0; j < 3; j++) put(wide ? j : j + 2, pack8<false, true>(f));
       }
     } else {
       put(0, load8(static_cast<const uint16_t*>(q.x), i * q.ld + c, live, end));
@@ -1335,7 +1367,7 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
 }
 
 // A 16-bit operand: rows x cols, row stride ld (a multiple of 8), and the room
-// of one or three terms, `term` elements apart.
+// of one, three or five terms, `term` elements apart.
 struct Operand {
   const uint16_t* at;
   long term;
@@ -1368,11 +1400,11 @@ void launch_gemm(eb_engine* e, const Operand& A, const Operand& B, const Operand
   const auto kern = k_gemm<EPI, CG, TERMS, WIDTH, CHAINED>;
   static std::atomic<uint64_t> allowed{0};
   allow_smem(e, kern, S::SMEM, allowed);
-  Maps<TERMS ? 3 : 1> maps;
-  for (int t = 0; t < (TERMS ? 3 : 1); t++) {
-    maps.a[t] = make_map(A, t);
-    maps.b[t] = make_map(B, t);
-    maps.c[t] = EPI != LSE ? make_map(C, t, EPI == PROB) : maps.b[t];
+  Maps<TERMS ? 5 : 1> maps;
+  for (int t = 0; t < (TERMS ? 5 : 1); t++) {  // what an operand lacks is not read
+    maps.a[t] = t < A.terms ? make_map(A, t) : maps.a[0];
+    maps.b[t] = t < B.terms ? make_map(B, t) : maps.b[0];
+    maps.c[t] = EPI == LSE || t >= C.terms ? maps.b[0] : make_map(C, t, EPI == PROB);
   }
   const int units = P.q[0].units + P.q[1].units;
   const int clusters = std::min(units, e->num_sms / CG);
@@ -1472,7 +1504,9 @@ void gemm(eb_engine* e, const Operand& A, const Operand& B, const Operand& C, Ti
     q.rows = Divisor::of(q.group);
     q.last = Divisor::of(std::max(q.mtiles % q.group, 1));
   }
-  if constexpr (EPI == LSE) {
+  // The same chains in both passes: the scores again are the forward pass's, to the
+  // last bit.
+  if constexpr (EPI != OUT) {
     if (A.terms == 1 && P.q[0].kblocks > 12) {
       if (t == NARROW)
         launch_gemm<EPI, 1, false, 64, true>(e, A, B, C, P);
@@ -1513,10 +1547,10 @@ uint32_t* found_words(eb_engine* e, const LinearCeArgs& a) {
 }
 
 // The 16-bit operands of x and w: each itself where TMA can read it (16-bit,
-// row stride a multiple of 16 bytes), else a copy in scratch; f32 split into
-// two or three terms.
+// row stride a multiple of 16 bytes), else a copy in scratch; f32 split into two or
+// three terms, or (`both`: the loss gradients may ask for it) five.
 void operands(eb_engine* e, const LinearCeArgs& a, uint32_t* found, uint32_t* scal, Operand& X,
-              Operand& W) {
+              Operand& W, bool both = false) {
   const bool split = a.dtype == EB_F32;
   Prep prep[2] = {};
   const void* src[2] = {a.x, a.w};
@@ -1528,7 +1562,7 @@ void operands(eb_engine* e, const LinearCeArgs& a, uint32_t* found, uint32_t* sc
     if (!split && ld[i] % 8 == 0) continue;
     o.ld = ((long)a.d + 7) / 8 * 8;
     o.term = (long)rows[i] * o.ld;
-    o.terms = split ? 3 : 1;
+    o.terms = !split ? 1 : both ? 5 : 3;
     uint16_t* c = e->scratch_get<uint16_t>(i ? "ce_w" : "ce_x", (size_t)(o.term * o.terms));
     o.at = c;
     prep[i] = Prep{src[i], (long)rows[i], (long)a.d, (long)ld[i], o.ld, c, o.term,
@@ -1772,7 +1806,7 @@ void linear_ce_backward(eb_engine* e, const LinearCeArgs& a, const LinearCeGrads
     e->stats.kernel_launches++;
   }
   Operand X, W;
-  operands(e, a, found, scal, X, W);
+  operands(e, a, found, scal, X, W, !g.one_dloss);
   // Pieces of P, as many elements as the scratch holds: the shorter side of
   // P whole where at least 2,048 of the longer then fit (the sums that run
   // over pieces are the shorter side's gradient), else pieces of both sides.

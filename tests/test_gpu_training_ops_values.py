@@ -9,7 +9,8 @@ import pytest
 import torch
 
 import emeans_b200 as eb
-from tests.test_gpu_training_ops import HALF_ULP, NAMES, TYPES, U32, gen, randn, within, wrap
+from tests.test_gpu_training_ops import (HALF_ULP, NAMES, TINY, TYPES, U32, gen, randn, within,
+                                         wrap)
 
 pytestmark = pytest.mark.gpu
 
@@ -114,7 +115,11 @@ class Values:
             tol = eA @ B.abs() + ((A.shape[1] / 4 + 40) * 2.0 ** -23 + (2.0 ** -20 if f32 else 0)) * (A.abs() @ B.abs())
             if f32 and floor:
                 tol = tol + 2.0 ** -26 * (A.abs() @ top)
-            within(out, want, tol + HALF_ULP[out.dtype] * (want.abs() + tol) + 2.0 ** -149, what)
+            tol = tol + HALF_ULP[out.dtype] * (want.abs() + tol) + TINY[out.dtype]
+            most = float(torch.finfo(out.dtype).max)
+            assert out[want.abs() - tol > 1.001 * most].isinf().all(), what  # past the type
+            fits = want.abs() + tol <= most
+            within(out[fits], want[fits], tol[fits], what)
 
 
 # Shapes of each kind of tile (pairs, single CTAs, narrow ones), off 16 bytes too.
@@ -259,3 +264,33 @@ def test_f32_calls_leave_nothing_for_the_next(eng):
     wider.check(wider.run(eng))
     for a, b in zip(c.run(eng), clean):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("size", [1e3, 1e5, 1e9])
+@pytest.mark.parametrize("dtype", TYPES, ids=NAMES.get)
+@pytest.mark.parametrize("n,k,d", SHAPES + [(257, 513, 1100), (300, 4000, 800), (9, 300, 65), (50, 30, 20)])
+def test_rows_of_very_large_scores(eng, n, k, d, dtype, size):
+    """Rows far longer than the rest, whose softmax is one prototype's: their
+    gradient is g scale (w of the best - w of the target), though the last bit
+    of their scores is many units; the other rows' is as ever."""
+    c = Values(n, k, d, dtype, 10, ignored=0.0)
+    c.t[3] = 0
+    big = torch.arange(0, n, 7, device="cuda")
+    c.x[big] *= size if dtype != torch.float16 else min(size, 1e4)
+    loss, lse, dx, dw = c.run(eng)
+    # Rows of 1e3 stay within what two FP16 terms hold, and f16's P has its floor.
+    c.check((loss, lse, dx, dw), floor=size == 1e3 or dtype == torch.float16)
+    X, W = c.x[big].double(), c.w.double()
+    z = X @ W.T
+    two = z.topk(2, 1).values
+    # A best score that no rounding of the scores can bring near another.
+    near = (2.0 ** -20 + d * 2.0 ** -24) * (X.abs() @ W.abs().T).amax(1)
+    clear = two[:, 0] - two[:, 1] > 100.0 + 4 * near
+    assert size < 1e5 or clear.sum() >= len(big) // 2
+    rows = big[clear]
+    g = c.dloss[rows].double()[:, None]
+    want = g * (W[z[clear].argmax(1)] - W[c.t[rows]])
+    tol = g.abs() * 2.0 ** -19 * (W[z[clear].argmax(1)].abs() + W[c.t[rows]].abs())
+    keep = {torch.float32: 0.0, torch.bfloat16: 2.0 ** -7, torch.float16: 2.0 ** -9}[dtype]
+    tol = tol + keep * g.abs() * (W[z[clear].argmax(1)].abs() + W[c.t[rows]].abs())
+    within(dx[rows], want, tol + HALF_ULP[dtype] * want.abs() + 2.0 ** -24, "dx of the clear rows")
