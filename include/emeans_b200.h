@@ -478,7 +478,9 @@ int eb_linear_ce(eb_engine* e, const eb_buf* x, size_t n, size_t d, size_t ldx, 
  * for all rows. P is formed a piece of the prototypes (and of the rows, when
  * there are very many) at a time in the engine's scratch (up to 512 MB),
  * rounded to x's type (f32: two FP16 terms, or three bf16 ones as above or
- * where the rows' dloss lie more than 2^12 apart). Two FP16 terms, and f16, leave out
+ * where the rows' dloss lie more than 2^12 apart). Where dx or dw is f32 and x
+ * 16-bit, P is three bf16 or two f16 terms, for FP32's own error: two to two and a
+ * half times the time of 16-bit gradients. Two FP16 terms, and f16, leave out
  * what of P lies below 2^-38 of the largest |dloss| scale of a row with a target; f16
  * rows with a dloss far below the largest lose bits by that. dx and dw: x's type or f32;
  * either may be null. Sums are added in a fixed order. A row with EB_IGNORE

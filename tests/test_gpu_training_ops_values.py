@@ -294,3 +294,64 @@ def test_rows_of_very_large_scores(eng, n, k, d, dtype, size):
     keep = {torch.float32: 0.0, torch.bfloat16: 2.0 ** -7, torch.float16: 2.0 ** -9}[dtype]
     tol = tol + keep * g.abs() * (W[z[clear].argmax(1)].abs() + W[c.t[rows]].abs())
     within(dx[rows], want, tol + HALF_ULP[dtype] * want.abs() + 2.0 ** -24, "dx of the clear rows")
+
+
+# ---------------------------------------------------------------- long sums, and f32 gradients
+
+
+def uniform_rows(n, k, d, dtype, seed):
+    """Positive rows whose scores are all near 0, and one target: every other
+    prototype's gradient is g scale / k times the sum of the rows."""
+    c = Values(n, k, d, dtype, seed, ignored=0.0, scale=1e-6)
+    c.x, c.t, c.dloss = c.x.abs(), torch.zeros_like(c.t), torch.full((1,), 1.0, device="cuda")
+    return c
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=NAMES.get)
+@pytest.mark.parametrize("n,k,d", [(16384, 96, 80), (70000, 100, 72)])
+def test_f32_gradients_of_long_one_signed_sums(eng, n, k, d, dtype):
+    """Sums of one sign over many rows, in f32: the tensor cores cut their sums
+    (2^-24 a step of 16 rows at worst, 2^-26 in the mean), which one chain over the rows
+    would show (two-term sums 1.8e-5), and P alike in all rows, whose rounding to 16
+    bits would (2e-3). P is off by the last bits of the log-sum (2^-22) and of the
+    exponent (2^-22) and by the exponential (2^-22): 1e-6 at most, alike in all
+    rows; chains of 128 rows by 24 cut steps of three products (2^-26 each: 4e-7),
+    and the rounded additions of their sums by at most 2^-24 a chain of a split
+    (600: 3.6e-5 at worst, but of either sign: 25 times 2^-24). 4e-6, and 2e-6 in the mean."""
+    c = uniform_rows(n, k, d, dtype, 11)
+    _, _, dx, dw = c.run(eng, outs=torch.float32)
+    X, W = c.x.double(), c.w.double()
+    p = torch.softmax(c.scale * (X @ W.T), 1)
+    p[:, 0] -= 1
+    want = c.scale * (p.T @ X)
+    off = ((dw.double() - want) / want)[1:]
+    assert float(off.abs().max()) <= 4e-6 and float(off.mean().abs()) <= 2e-6
+    want = c.scale * (p @ W)
+    assert float((dx.double() - want).abs().max() / want.abs().max()) <= 4e-6
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=NAMES.get)
+@pytest.mark.parametrize("n,k,d", SHAPES + [(257, 513, 1100), (3000, 1000, 392), (20000, 9000, 16)])
+def test_f32_gradients_of_16_bit_rows_keep_p(eng, n, k, d, dtype):
+    """Rows' gradients in f32, against 64 bits of the same 16-bit inputs: FP32's
+    own error (5e-6 of a row's norm at 2,000 products; P in bf16 or f16 alone is 2e-3
+    or 2e-4 off), whichever of the two is wanted in f32."""
+    c = Values(n, k, d, dtype, 12)
+    got = c.run(eng, outs=torch.float32)
+    X, W = c.x.double(), c.w.double()
+    live = c.t != eb.IGNORE
+    t = torch.where(live, c.t, 0 * c.t)[:, None]
+    p = torch.softmax(X @ W.T, 1).scatter_add(1, t, -torch.ones_like(t, dtype=torch.float64))
+    p = p * torch.where(live, c.dloss.double(), 0.0)[:, None]
+    for out, want in ((got[2], p @ W), (got[3], p.T @ X)):
+        norm = want.norm(dim=1)
+        some = norm > 1e-3 * norm.max()
+        off = (out.double() - want).norm(dim=1)[some] / norm[some]
+        assert float(off.max()) <= 3e-5 and float(off.median()) <= 5e-6
+    e, lse = eng, got[1]
+    dw = torch.empty(k, d, device="cuda")
+    dx = torch.empty(n, d, device="cuda", dtype=dtype)
+    e.linear_cross_entropy_backward(wrap(e, c.x), n, d, wrap(e, c.w), k, wrap(e, c.t.to(torch.uint32)),
+                                    wrap(e, lse), wrap(e, c.dloss), wrap(e, dx), wrap(e, dw))
+    e.sync()
+    assert torch.equal(dw, got[3]) and torch.equal(dx, got[2].to(dtype))
