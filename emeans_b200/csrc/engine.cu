@@ -1002,8 +1002,8 @@ eb::LinearCeArgs check_linear_ce(eb_engine* e, const eb_buf* x, size_t n, size_t
   ensure(d > 0 && d <= 0x7FFFFF00ull, "d must be positive and fit 31 bits");
   ensure(k > 0 && k <= 0x7FFFFF00ull, "k must be positive and fit 31 bits");
   ensure(n <= 0x7FFFFF00ull, "n must fit 31 bits");
-  // Units of a launch are counted in 31 bits: tiles of the scores, of dx and of
-  // dw (at least 128 x 160).
+  // A launch works on a pass of rows or a piece of P, whose tiles are far fewer than 31
+  // bits count; a problem whose tiles of 128 x 160 in all are more is refused.
   ensure((n / 128 + 1) * (k / 160 + 1) <= 0x7FFFFFFFull, "n x k is too large");
   ensure(std::isfinite(scale) && scale > 0.0f, "scale must be positive and finite");
   need_type(targets, EB_U32, "targets");

@@ -1772,17 +1772,30 @@ void linear_ce(eb_engine* e, const LinearCeArgs& a, float* loss, float* lse) {
   uint32_t* found = a.dtype == EB_F32 ? found_words(e, a) : nullptr;
   Operand X, W;
   operands(e, a, found, scal, X, W);
-  // Rows a pass: as many as keep the half tiles' (max, sum) to 256 MB.
-  const size_t most = ((size_t)256 << 20) / sizeof(float2) / (2 * (a.k / 160 + 1)) / 256 * 256;
-  const size_t rows = std::max<size_t>(std::min(a.n, most), 256);
+  // Rows a pass: all, or a multiple of 256 that keeps the half tiles' (max, sum) to 256
+  // MB (or 256 where those are more); all passes in tiles of one width.
+  const int terms = a.dtype == EB_F32 ? 2 : 1;
+  constexpr size_t ROOM = ((size_t)256 << 20) / sizeof(float2);
+  size_t rows = a.n;
+  Tile tile;
+  Prob whole;
+  while (true) {
+    tile = score_tile(e, (long)rows, (long)a.k, (long)a.d, terms);
+    const TileCost cost = tile_cost(tile, terms);
+    whole = make_prob((long)rows, (long)a.k, (long)a.d, cost, e->num_sms / cost.ctas);
+    const size_t most = ROOM / (2 * (size_t)whole.ntiles);
+    if (rows <= std::max<size_t>(most, 256)) break;
+    rows = std::max<size_t>(std::min(most, rows - 1) / 256 * 256, 256);
+  }
+  const TileCost cost = tile_cost(tile, terms);
   for (size_t r0 = 0; r0 < a.n; r0 += rows) {
     const long n = (long)std::min(a.n - r0, rows);
     GemmParams P = base_params(a, found, scal);
-    const int terms = a.dtype == EB_F32 ? 2 : 1;
-    const Tile tile = score_tile(e, n, (long)a.k, (long)a.d, terms);
-    const TileCost cost = tile_cost(tile, terms);
     P.q[0] = make_prob(n, (long)a.k, (long)a.d, cost, e->num_sms / cost.ctas);
-    const int parts = 2 * P.q[0].ntiles;
+    P.q[0].bn = whole.bn;
+    P.q[0].ntiles = whole.ntiles;
+    P.q[0].units = P.q[0].mtiles * whole.ntiles;
+    const int parts = 2 * whole.ntiles;
     float2* part = e->scratch_get<float2>("ce_part", (size_t)parts * n);
     P.part = part;
     P.zt = e->scratch_get<float>("ce_zt", (size_t)n);

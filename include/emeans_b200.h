@@ -466,8 +466,10 @@ int eb_layer_norm_backward(eb_engine* e, const eb_buf* dy, size_t lddy, const eb
  * matrix's, as three bf16 terms each (24 bits, FP32's range) in six, which takes
  * up to twice as long; a non-finite element counts as NaN. In FP32 where k and d are
  * small (64) or there are few rows (up to 16; of 16-bit types 4, off 16-byte
- * alignment). Scratch: f32 operands' copies (1.5 times x and w; not for
- * those), and up to 256 MB. */
+ * alignment). Scratch, a quarter more than it needs and kept by the engine: f32
+ * operands' copies (1.5 times x and w; not for those), 16-bit ones' where a row
+ * stride is not a multiple of 16 bytes, and (max, sum) pairs of the rows' half tiles,
+ * up to 256 MB (more where 256 rows alone take more: past 10 M prototypes). */
 int eb_linear_ce(eb_engine* e, const eb_buf* x, size_t n, size_t d, size_t ldx, const eb_buf* w,
                  size_t k, size_t ldw, const eb_buf* targets, float scale, eb_buf* loss,
                  eb_buf* lse);
@@ -476,14 +478,17 @@ int eb_linear_ce(eb_engine* e, const eb_buf* x, size_t n, size_t d, size_t ldx, 
  * with P_ij = dloss_i scale (exp(z_ij - lse_i) - [j == targets_i]),
  * dx = P w (n x d) and dw = P^T x (k x d). dloss is f32: n elements, or one
  * for all rows. P is formed a piece of the prototypes (and of the rows, when
- * there are very many) at a time in the engine's scratch (up to 512 MB),
- * rounded to x's type (f32: two FP16 terms, or three bf16 ones as above or
- * where the rows' dloss lie more than 2^12 apart). Where dx or dw is f32 and x
- * 16-bit, P is three bf16 or two f16 terms, for FP32's own error: two to two and a
- * half times the time of 16-bit gradients. Two FP16 terms, and f16, leave out
- * what of P lies below 2^-38 of the largest |dloss| scale of a row with a target; f16
- * rows with a dloss far below the largest lose bits by that. dx and dw: x's type or f32;
- * either may be null. Sums are added in a fixed order. A row with EB_IGNORE
+ * there are very many) at a time in the engine's scratch (up to 512 MB), beside
+ * the operands' copies (f32 with a dloss a row: 2.5 times x and w), FP32 sums of
+ * dx or dw where more than one piece adds to it, and those of products that are
+ * split (again a quarter more, and kept). P is rounded to x's type (f32: two FP16
+ * terms, or three bf16 ones as above or where the rows' dloss lie more than 2^12
+ * apart). Where dx or dw is f32 and x 16-bit, P is three bf16 or two f16 terms, for
+ * FP32's own error: two to two and a half times the time of 16-bit gradients. Two
+ * FP16 terms, and f16, leave out what of P lies below 2^-38 of the largest |dloss|
+ * scale of a row with a target; f16 rows with a dloss far below the largest lose
+ * bits by that. dx and dw: x's type or f32; either may be null. Sums are added in a
+ * fixed order. A row with EB_IGNORE
  * has dx = 0 whatever it holds, but dw sums 0 x its elements: a non-finite one
  * makes its columns of dw NaN, as in the plain formula. */
 int eb_linear_ce_backward(eb_engine* e, const eb_buf* x, size_t n, size_t d, size_t ldx,

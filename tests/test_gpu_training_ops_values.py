@@ -355,3 +355,20 @@ def test_f32_gradients_of_16_bit_rows_keep_p(eng, n, k, d, dtype):
                                     wrap(e, lse), wrap(e, c.dloss), wrap(e, dx), wrap(e, dw))
     e.sync()
     assert torch.equal(dw, got[3]) and torch.equal(dx, got[2].to(dtype))
+
+
+def test_linear_cross_entropy_passes_hold_the_scratch(eng):
+    """Tiles of 128 columns and fewer leave more half tiles: the rows go in more
+    passes (two launches each), not in more than 256 MB of their sums."""
+    n, k, d = 640, 3490000, 900
+    e = eb.Engine(0, stream=torch.cuda.current_stream().cuda_stream)
+    x, w = torch.zeros(n, d, device="cuda"), torch.zeros(k, d, device="cuda")
+    t = torch.zeros(n, device="cuda", dtype=torch.int32)
+    loss, lse = torch.empty(n, device="cuda"), torch.empty(n, device="cuda")
+    before = e.stats()["kernel_launches"]
+    e.linear_cross_entropy(e.wrap(x), n, d, e.wrap(w), k, e.wrap(t), e.wrap(loss), e.wrap(lse))
+    e.sync()
+    launches = e.stats()["kernel_launches"] - before
+    assert launches >= 2 + 2 * 2
+    assert float((lse - math.log(k)).abs().max()) < 1e-5 and torch.equal(loss, lse)
+    e.close()
