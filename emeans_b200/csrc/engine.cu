@@ -35,6 +35,17 @@ int guard(F&& f) {
   }
 }
 
+// The same for calls that give something back. One that succeeds leaves the last
+// failed call's message: a garbage collector may release objects before the caller
+// has read it.
+template <class F>
+int release(F&& f) {
+  std::string kept = std::move(g_last_error);
+  const int rc = guard(f);
+  if (rc == EB_OK) g_last_error = std::move(kept);
+  return rc;
+}
+
 // Makes the engine's device current for the duration of a call.
 struct DeviceGuard {
   int prev = -1;
@@ -261,7 +272,7 @@ int eb_engine_create_on(int device, void* stream, eb_engine** out) {
 
 int eb_engine_destroy(eb_engine* e) {
   if (!e) return EB_OK;
-  return guard([&] {
+  return release([&] {
     DeviceGuard g(e);
     cudaStreamSynchronize(e->stream);
     eb::group_leave(e);
@@ -423,7 +434,7 @@ int eb_buf_wrap(eb_engine* e, int dtype, void* dev_ptr, size_t len, eb_buf** out
 
 int eb_buf_free(eb_engine* e, eb_buf* b) {
   if (!b) return EB_OK;
-  return guard([&] {
+  return release([&] {
     need(e, "engine");
     DeviceGuard g(e);
     if (e->bound == b) e->bound = nullptr;
@@ -1164,7 +1175,7 @@ int eb_adamw_create(eb_engine* e, const eb_adamw_tensor* t, size_t count, eb_ada
 
 int eb_adamw_destroy(eb_engine* e, eb_adamw* plan) {
   if (!plan) return EB_OK;
-  return guard([&] {
+  return release([&] {
     need(e, "engine");
     DeviceGuard g(e);
     if (plan->table) cudaFreeAsync(plan->table, e->stream);
