@@ -34,15 +34,15 @@
 // loss gradients lie that far apart, P and the gradients' products are (the scores
 // again stay the forward pass's, to the last bit). The
 // preparation decides it on the device, and the same kernels read it: 3,001 x
-// 5,003 x 385 forward and backward 62 and 150 us one way, 83 and 238 the other;
-// 8,192 x 8,192 x 1024 290 and 905, 506 and 1,867.
+// 5,003 x 385 forward and backward 62 and 152 us one way, 83 and 238 the other;
+// 8,192 x 8,192 x 1024 291 and 909, 506 and 1,867.
 //
 // Bound by the tensor cores, 2 n k d operations forward and 6 n k d backward
 // (three times that for f32); for few rows by reading w once. 16,384 x 65,536 x
-// 1024 bf16: forward 1.46 ms (1,500 TFLOP/s), backward 4.2 to 4.8 ms (1,370 to
-// 1,570), under the power cap; 16,384 x 8,192 x 1024: forward 177 us, its kernel's
-// tensor cores active 81 % of the time, the scores again 86 %, the gradients
-// 89 %; 8 x 65,536 x 1024 forward 30 us (4.5 TB/s of w).
+// 1024 bf16, under the power cap: in loops of one call forward 1.46 ms (1,510
+// TFLOP/s) and backward 4.75 ms (1,390), a step of both 7.0 ms; 16,384 x 8,192 x 1024:
+// forward 179 us, its kernel's tensor cores active 82 % of the time, the scores
+// again 79 %, the gradients 92 %; 8 x 65,536 x 1024 forward 30 us (4.5 TB/s of w).
 #include <cuda_runtime.h>
 #include <cudaTypedefs.h>
 
@@ -52,6 +52,7 @@
 
 #include "elem.h"
 #include "engine.h"
+#include "softmax.h"
 #include "tc.h"
 
 namespace eb {
@@ -64,7 +65,6 @@ constexpr int BM = 128;   // rows of a tile a CTA holds (TMEM lanes)
 constexpr int BN = 256;   // most columns of a tile (TMEM columns of one accumulator)
 constexpr int BK = 64;    // k-elements a stage: one 128-byte swizzle row
 constexpr int NTHREADS = 384;  // warp 0 loads, warp 1 issues products, warps 4-11 epilogue
-constexpr float LOG2E = 1.4426950408889634f;
 constexpr float PSCALE = 16384.0f;  // f16 and f32: P is kept times 2^14
 
 enum Epi { LSE, PROB, OUT };
@@ -201,29 +201,11 @@ struct Place {
   }
 };
 
-// exp of a difference of scores (inputs <= 0 but for rounding; relative error
-// 2^-22 and 2^-24 of the input). Differences are formed in natural units,
-// where the scores' scale needs no rounding (a power of two apart), and only
-// then scaled to base 2.
-__device__ __forceinline__ float ex(float v) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v * LOG2E));
-  return r;
-}
-
 // The softmax of rows whose largest score is past this size goes by rounded scores:
 // half their last bit is 2^-14 and more, and the exact products of fmaf would leave a
 // row's largest score that much, or (past 2^24) whole units, above or below an lse
 // that is that score rounded.
 constexpr float STEEP = 1024.0f;
-
-// Folds (m', s') into a running (max, sum of exp(z - max)); (-inf, 0) is empty.
-// NaN scores are in the sums, not in the maxima.
-__device__ __forceinline__ void fold(float& m, float& s, float2 v) {
-  const float top = fmaxf(m, v.x), off = top == -INFINITY ? 0.0f : top;
-  s = s * ex(m - off) + v.y * ex(v.x - off);
-  m = top;
-}
 
 // A warp's 32 x 32 block in shared memory: row r's four-column group g is
 // kept at group g ^ (r & 7), so that rows are written by their own threads
@@ -631,6 +613,24 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       // Three bf16 terms of P have FP32's range: they too take the rows' own.
       if (wide_p || !(gmax > 0.0f && gmax < INFINITY)) gmax = 1.0f;
     }
+    // What sums become in the outputs. Of several terms: the operand's power of two,
+    // the scores' scale and the loss gradients at once where that keeps well within
+    // FP32's range (for both products), else one after the other.
+    float factors[2] = {P.scale / P.pscale * gmax, P.scale / P.pscale * gmax}, scales[2] = {1.0f, 1.0f};
+    bool fine = true;
+    if constexpr (EPI == OUT && TERMS) {
+#pragma unroll
+      for (int r = 0; r < 2; r++) {
+        if (!split || wide)
+          scales[r] = split ? 1.0f : 1.0f / P.pscale;
+        else
+          scales[r] = ldexpf(1.0f / P.pscale, -split_exp(P.scal[P.q[r].unscale]));
+        const float two = scales[r] * P.scale;
+        factors[r] = two * gmax;
+        fine = fine && two > 0x1p-90f && two < 0x1p90f && factors[r] > 0x1p-90f && factors[r] < 0x1p90f;
+      }
+      if (!fine) factors[0] = factors[1] = gmax;
+    }
     const uint32_t release = CG == 2 ? map_rank(smem_u32(tempty), 0) : smem_u32(tempty);
     int tc = 0, stores = 0;
     bool stop = false;
@@ -717,24 +717,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         wait_chain();
       }
       if (stop) break;
-      // Sums of several terms: the operand's power of two, the scores' scale and the
-      // loss gradients at once where that keeps well within FP32's range, else one
-      // after the other.
-      float factor = 1.0f, unit = 1.0f;
-      bool fine = true;
-      if constexpr (EPI == OUT) {
-        if constexpr (TERMS) {
-          if (!split)
-            unit = 1.0f / P.pscale;
-          else if (!wide)
-            unit = ldexpf(1.0f / P.pscale, -split_exp(P.scal[pr.unscale]));
-          const float two = unit * P.scale, all = two * gmax;
-          fine = two > 0x1p-90f && two < 0x1p90f && all > 0x1p-90f && all < 0x1p90f;
-          factor = fine ? all : gmax;
-        } else {
-          factor = P.scale / P.pscale * gmax;
-        }
-      }
+      const float factor = q.prob ? factors[1] : factors[0];
       uint32_t raw[CHAINED ? 1 : 32];
       if constexpr (!CHAINED) tmem_ld32(base + (tc & 1) * BN, raw);
 #pragma unroll
@@ -877,7 +860,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         } else {
           if (TERMS && !fine) {
 #pragma unroll
-            for (int j = 0; j < 32; j++) v[j] = v[j] * unit * P.scale;
+            for (int j = 0; j < 32; j++) v[j] = v[j] * (q.prob ? scales[1] : scales[0]) * P.scale;
           }
           __syncwarp();
 #pragma unroll

@@ -25,6 +25,7 @@
 
 #include "elem.h"
 #include "engine.h"
+#include "softmax.h"
 #include "tc.h"
 
 namespace eb {
@@ -37,7 +38,6 @@ constexpr int THREADS = 256;
 constexpr long MOST_ROWS = 16, MOST_HALF_ROWS = 4, MOST_COLUMNS = 1024;
 constexpr long MOST_PROTOTYPES = 1l << 22;  // P is then at most 256 MB
 constexpr int CHUNK = 32;  // prototypes whose P a block holds (128: the same times)
-constexpr float LOG2E = 1.4426950408889634f;
 
 struct Few {
   const void* x;
@@ -58,19 +58,6 @@ struct Few {
   long lddw;
   int dwtype;
 };
-
-__device__ __forceinline__ float ex(float v) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v * LOG2E));
-  return r;
-}
-// Folds (m', s') into a running (max, sum of exp(z - max)); (-inf, 0) is empty.
-// NaN scores are in the sums, not in the maxima.
-__device__ __forceinline__ void fold(float& m, float& s, float mv, float sv) {
-  const float top = fmaxf(m, mv), off = top == -INFINITY ? 0.0f : top;
-  s = s * ex(m - off) + sv * ex(mv - off);
-  m = top;
-}
 
 template <typename T, int NR, bool BACKWARD>
 __global__ void __launch_bounds__(THREADS, 2) k_few_scores(Few F) {
@@ -143,7 +130,7 @@ __global__ void __launch_bounds__(THREADS, 2) k_few_scores(Few F) {
         const float v = p == (long)target ? expm1f(z - lse) : ex(z - lse);
         F.p[p * NR + i] = g == 0.0f ? 0.0f : g * v;
       } else {
-        fold(m, s, z, 1.0f);
+        fold(m, s, make_float2(z, 1.0f));
         if (p == (long)target) F.zt[i] = z;
       }
     }
@@ -153,14 +140,14 @@ __global__ void __launch_bounds__(THREADS, 2) k_few_scores(Few F) {
 #pragma unroll
     for (int o = V == 16 ? 2 : 1; o < 32 / NR; o <<= 1) {
       const float mo = __shfl_xor_sync(0xffffffffu, m, o), so = __shfl_xor_sync(0xffffffffu, s, o);
-      fold(m, s, mo, so);
+      fold(m, s, make_float2(mo, so));
     }
     if (lane % (32 / NR) == 0) joint[warp][i] = make_float2(m, s);
     __syncthreads();
     if (threadIdx.x < F.n) {
       m = -INFINITY, s = 0.0f;
       for (int v = 0; v < THREADS / 32; v++)
-        fold(m, s, joint[v][threadIdx.x].x, joint[v][threadIdx.x].y);
+        fold(m, s, joint[v][threadIdx.x]);
       F.part[(long)blockIdx.x * F.n + threadIdx.x] = make_float2(m, s);
     }
   }
@@ -295,7 +282,8 @@ unsigned scores_grid(eb_engine* e, const LinearCeArgs& a) {
 
 }  // namespace
 
-// f32 up to 16 rows; forward and backward in us, here and on the tensor cores:
+// f32 up to 16 rows; forward and backward in us, in loops of one call, here and on the
+// tensor cores:
 //   1 x 40,000 x 1024 43 and 134, 152 and 244; 16 x 40,000 x 1024 77 and 214, 151 and 240;
 //   15 x 41,927 x 547 48 and 156, 102 and 190; 5 x 7,689 x 807 13 and 30, 34 and 58;
 //   16 x 60,000 x 8 16 and 47, 41 and 51; 1 x 760 x 506 8 and 12, 18 and 25.

@@ -7,7 +7,8 @@
 // dw): 1,000 x 32 x 64 f32 forward 5.9 us and backward 11.1 (tensor cores 13.9
 // and 19.0), 60,000 x 64 x 64 23.8 and 63.2 (51.1 and 85.2). With 128
 // prototypes or columns the two are even, and operands that TMA reads as they
-// lie are no slower there (1,000 x 32 x 64 bf16: 7.5 and 12.3).
+// lie take 9.1 and 10.8 there (1,000 x 32 x 64 bf16). (In loops of one call;
+// a step of 1,000 x 32 x 64, forward and then backward, takes 12.)
 //
 // A block of 256 threads holds all prototypes and 16 R rows of x in shared
 // memory; a thread keeps R x 4 scores in registers, and the 16 threads of a
@@ -22,6 +23,7 @@
 
 #include "elem.h"
 #include "engine.h"
+#include "softmax.h"
 #include "tc.h"
 
 namespace eb {
@@ -34,7 +36,6 @@ constexpr int THREADS = 256;
 constexpr int MOST = 64;           // prototypes, and columns
 constexpr size_t MOST_ROWS = 1 << 19;  // the blocks' partial dw are then at most 256 MB
 constexpr int STRIDE = MOST + 4;   // floats of a shared-memory row
-constexpr float LOG2E = 1.4426950408889634f;
 
 struct Small {
   const void* x;
@@ -58,13 +59,6 @@ struct Small {
   int dwtype;
   float* part;  // blocks x k x d, or null with one block
 };
-
-// exp of a difference of scores.
-__device__ __forceinline__ float ex(float v) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v * LOG2E));
-  return r;
-}
 
 // COUNT rows of a matrix from row r0 on (zeros past `rows` and past d) into
 // shared memory: a warp takes every eighth row, all of them in flight at once.
@@ -145,17 +139,14 @@ __global__ void __launch_bounds__(THREADS) k_ce_small(Small P) {
       m = fmaxf(m, z[r][c]);
     }
     // The maximum passes over NaN scores; they reach the sum.
-    float off = m == -INFINITY ? 0.0f : m;
+    const float off = m == -INFINITY ? 0.0f : m;
 #pragma unroll
     for (int c = 0; c < 4; c++) sum += ex(z[r][c] - off);
 #pragma unroll
     for (int o = 1; o < 16; o <<= 1) {
       const float om = __shfl_xor_sync(0xffffffffu, m, o);
       const float os = __shfl_xor_sync(0xffffffffu, sum, o);
-      const float top = fmaxf(m, om);
-      off = top == -INFINITY ? 0.0f : top;
-      sum = sum * ex(m - off) + os * ex(om - off);
-      m = top;
+      fold(m, sum, make_float2(om, os));
     }
     __syncwarp();
     const long i = row0 + R * ty + r;
