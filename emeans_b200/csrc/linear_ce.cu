@@ -8,7 +8,7 @@
 // epilogues. Forward: the tile of scores stays in TMEM; its epilogue reduces
 // each row's 128 columns to (max, sum of exp) and k_ce_join adds those up.
 // Backward, a piece of the prototypes at a time: the scores again, turned
-// into P (16 bits, engine scratch), then dx += P w and dw = P^T x read that
+// into P (16-bit terms, engine scratch), then dx += P w and dw = P^T x read that
 // piece. Operands are K-major or MN-major as they lie in memory (w is the
 // K-major operand of the scores and the MN-major one of dx), so nothing is
 // transposed.
@@ -28,14 +28,13 @@
 // accumulator. The dropped lo.lo term is 2^-22 of the product. That floor is the
 // matrix's, so rows, columns or loss gradients far below the largest would lose
 // their last bits, or all of them. Where the smallest row's or column's largest
-// element is below 2^-12 of the largest (of those that
-// are not 0), the operands and P are instead split into three bf16 terms each (24
-// bits, FP32's own range, no scale) and multiplied in six products. Where the rows'
-// loss gradients lie that far apart, P and the gradients' products are (the scores
-// again stay the forward pass's, to the last bit). The
-// preparation decides it on the device, and the same kernels read it: 3,001 x
-// 5,003 x 385 forward and backward 62 and 152 us one way, 83 and 238 the other;
-// 8,192 x 8,192 x 1024 291 and 909, 506 and 1,867.
+// element (of those that are not 0) is below 2^-12 of the largest, the operands and
+// P are instead split into three bf16 terms each (24 bits, FP32's own range, no
+// scale) and multiplied in six products. Where only the rows' loss gradients lie
+// that far apart, P and the gradients' products are: the scores again stay the
+// forward pass's, to the last bit. The preparation decides it on the device, and
+// the same kernels read it. Forward and backward, one way and the other: 3,001 x 5,003
+// x 385 62 and 152 us, 83 and 238; 8,192 x 8,192 x 1024 291 and 909, 506 and 1,867.
 //
 // Bound by the tensor cores, 2 n k d operations forward and 6 n k d backward
 // (three times that for f32); for few rows by reading w once. 16,384 x 65,536 x
@@ -77,10 +76,10 @@ enum { S_X, S_W, S_G, S_WIDE, S_WIDE_P, S_WORDS };
 
 // Words that an f32 call's first kernels raise, zero between calls: the same
 // magnitudes; the complements of the smallest row's max|x| and max|w| and of the
-// smallest |dloss| that are not 0; the blocks that went by columns; then, for x and
-// for w, each column's largest, and for each range of columns what no column's
-// largest is below. The first product kernel zeroes them.
-enum { R_X, R_W, R_G, R_X_LOW, R_W_LOW, R_G_LOW, R_BY_COLUMN, R_COLUMNS };
+// smallest |dloss| that are not 0; then, for x and for w, each column's largest, and
+// for each range of columns what no column's largest is below. The first product
+// kernel zeroes them.
+enum { R_X, R_W, R_G, R_X_LOW, R_W_LOW, R_G_LOW, R_COLUMNS };
 constexpr int RANGE = 1024;  // columns of a range
 __host__ __device__ constexpr long range_count(long d) { return (d + RANGE - 1) / RANGE; }
 __host__ __device__ constexpr long found_count(long d) {
@@ -354,7 +353,8 @@ __device__ __forceinline__ void store_block(const Prob& q, float* sums, float* b
 // registers between chains.
 template <int EPI, int CG, bool TERMS, int WIDTH, bool CHAINED, bool FINE>
 __global__ void __launch_bounds__(NTHREADS, 1)
-    k_gemm(const __grid_constant__ Maps<TERMS || FINE ? 5 : 1> maps, const __grid_constant__ GemmParams P) {
+    k_gemm(const __grid_constant__ Maps<TERMS || FINE ? 5 : 1> maps,
+           const __grid_constant__ GemmParams P) {
   using S = Shape<EPI, CG, TERMS, WIDTH, CHAINED>;
   constexpr int HALF = S::HALF;
   using namespace tc;
@@ -1074,23 +1074,25 @@ __device__ __forceinline__ void for_groups(const Prep& q, unsigned block, F&& f)
 
 // Whether a matrix's columns lie too far apart, for all of a block's 256 threads: no
 // column of a range is below its word (some block saw every column that large), or,
-// where every block had columns of zeros or far smaller ones, from the columns' own
-// words.
-__device__ __forceinline__ bool columns_apart(const uint32_t* found, long d, uint32_t top,
-                                              bool by_column) {
-  bool far = false;
+// where there is none, as every block had columns of zeros or far smaller ones, from the
+// columns' own words.
+__device__ __forceinline__ bool columns_apart(const uint32_t* found, long d, uint32_t top) {
+  bool far = false, by_column = false;
+  uint32_t low = 0;
   for (long r = 0; r < range_count(d); r++) {
     const uint32_t least = found[d + r];
-    far |= !least || apart(top, ~least);
-  }
-  if (!far || !by_column) return far;
-  uint32_t low = 0;
+    if (least) {
+      far |= apart(top, ~least);
+      continue;
+    }
+    by_column = true;
 #pragma unroll 4
-  for (long c = threadIdx.x; c < d; c += 256) {
-    const uint32_t m = found[c];
-    if (m) low = max(low, ~m);
+    for (long c = r * RANGE + threadIdx.x; c < min((r + 1) * RANGE, d); c += 256) {
+      const uint32_t m = found[c];
+      if (m) low = max(low, ~m);
+    }
   }
-  return __syncthreads_or(apart(top, low));
+  return by_column ? __syncthreads_or(far || apart(top, low)) : far;
 }
 
 // The magnitudes of both operands' finite elements: the largest, the
@@ -1209,21 +1211,17 @@ __global__ void __launch_bounds__(256, 2)
   if (threadIdx.x == 0) {
     atomicMax(found + (second ? R_W : R_X), rows[0]);
     atomicMax(found + (second ? R_W_LOW : R_X_LOW), rows[1]);
-    if (by_column)
-      atomicAdd(found + R_BY_COLUMN, 1);
-    else
-      atomicMax(mine + q.d + range, least);
+    if (!by_column) atomicMax(mine + q.d + range, least);
   }
 }
 
 // The operands' 16-bit rows; with SPLIT, in two f16 terms scaled by the largest
 // element, or, where rows or columns lie too far apart for that, in three bf16
 // terms, or both ways where the loss gradients do; the first block leaves what the
-// products need in `scal`. `blocks`: of k_ce_max.
+// products need in `scal`.
 template <bool SPLIT>
 __global__ void __launch_bounds__(256)
-    k_ce_rows(Prep X, Prep W, const uint32_t* __restrict__ found, unsigned blocks,
-              uint32_t* scal) {
+    k_ce_rows(Prep X, Prep W, const uint32_t* __restrict__ found, uint32_t* scal) {
   pdl_trigger();
   pdl_wait();
   const bool second = blockIdx.x >= X.blocks;
@@ -1235,10 +1233,8 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
     for (int t = 0; t < R_COLUMNS; t++) word[t] = found[t];
     const uint32_t x = word[R_X], w = word[R_W], g = word[R_G];
-    const bool by_column = word[R_BY_COLUMN] == blocks;
-    const bool far_x = columns_apart(found + R_COLUMNS, q.d, x, by_column);
-    const bool far_w =
-        columns_apart(found + R_COLUMNS + q.d + range_count(q.d), q.d, w, by_column);
+    const bool far_x = columns_apart(found + R_COLUMNS, q.d, x);
+    const bool far_w = columns_apart(found + R_COLUMNS + q.d + range_count(q.d), q.d, w);
     wide = apart(x, word[R_X_LOW]) || apart(w, word[R_W_LOW]) || far_x || far_w;
     wide_p = wide || apart(g, word[R_G_LOW]);
     s = ldexpf(1.0f, split_exp(second ? w : x));
@@ -1586,11 +1582,11 @@ void operands(eb_engine* e, const LinearCeArgs& a, uint32_t* found, uint32_t* sc
     }
     launch_pdl(e, kern, dim3(m[0].blocks + m[1].blocks), dim3(256), 0, m[0], m[1], found);
     launch_pdl(e, k_ce_rows<true>, dim3(grid), dim3(256), 0, prep[0], prep[1],
-               (const uint32_t*)found, m[0].blocks + m[1].blocks, scal);
+               (const uint32_t*)found, scal);
     e->stats.kernel_launches += 2;
   } else {
     launch_pdl(e, k_ce_rows<false>, dim3(grid), dim3(256), 0, prep[0], prep[1],
-               (const uint32_t*)nullptr, 0u, scal);
+               (const uint32_t*)nullptr, scal);
     e->stats.kernel_launches++;
   }
 }

@@ -244,7 +244,22 @@ def sparse_and_apart(c):
     c.x[9:, 0] = 0
 
 
-@pytest.mark.parametrize("edit,floor", [(sparse, True), (sparse_and_apart, False)], ids=["sparse", "apart"])
+def sparse_rows(c):
+    """The prototypes' columns are all there."""
+    w = c.w.clone()
+    sparse(c)
+    c.w = w
+
+
+def sparse_range(c):
+    """Columns of zeros in one range of columns alone (of 1,024), and a far
+    smaller one there."""
+    c.x[:, :2] = 0
+    c.w[:, 1] *= 1e-6
+
+
+@pytest.mark.parametrize("edit,floor", [(sparse, True), (sparse_and_apart, False), (sparse_rows, True),
+                                        (sparse_range, False)], ids=lambda v: getattr(v, "__name__", ""))
 @pytest.mark.parametrize("n,k,d", SHAPES + [(257, 513, 2100), (3000, 1000, 392), (70, 900, 60)])
 def test_f32_columns_of_zeros(eng, n, k, d, edit, floor):
     c = Values(n, k, d, torch.float32, 6)
