@@ -123,7 +123,7 @@ __global__ void __launch_bounds__(THREADS, 2) k_few_scores(Few F) {
     for (int j = 0; j < (V == 64 ? 2 : 1); j++) {
       const long p = p0 + q0 + j;
       if (p >= F.k) continue;
-      const float z = a[j] * F.scale;
+      const float z = __fmul_rn(a[j], F.scale);  // not fused with what is taken from it
       if constexpr (BACKWARD) {
         // By expm1 at the target: near 1, p's own rounding would be all that is
         // left. Nothing of a row without a gradient, not even its NaN.

@@ -81,7 +81,8 @@ __device__ __forceinline__ void load_rows(const void* src, long r0, long rows, l
     for (int i = 0; i < EACH; i++) dst[(warp + i * 8) * STRIDE + h * 32 + lane] = v[h][i];
 }
 
-// This thread's scores: rows R ty .. + R against prototypes tx + 16 c.
+// This thread's scores, rows R ty .. + R against prototypes tx + 16 c; rounded, so
+// that none is above its row's log-sum.
 template <int R>
 __device__ __forceinline__ void scores(const Small& P, const float* xs, const float* ws, int ty,
                                        int tx, float (&z)[R][4]) {
@@ -107,7 +108,8 @@ __device__ __forceinline__ void scores(const Small& P, const float* xs, const fl
 #pragma unroll
   for (int r = 0; r < R; r++)
 #pragma unroll
-    for (int c = 0; c < 4; c++) z[r][c] *= P.scale;
+    for (int c = 0; c < 4; c++)
+      z[r][c] = __fmul_rn(z[r][c], P.scale);  // not fused with what is taken from it
 }
 
 template <typename T, int R>

@@ -387,3 +387,33 @@ def test_linear_cross_entropy_passes_hold_the_scratch(eng):
     assert launches >= 2 + 2 * 2
     assert float((lse - math.log(k)).abs().max()) < 1e-5 and torch.equal(loss, lse)
     e.close()
+
+
+@pytest.mark.parametrize("size", [1e3, 1e5, 1e9])
+@pytest.mark.parametrize("dtype", TYPES, ids=NAMES.get)
+@pytest.mark.parametrize("n,k,d", SHAPES + [(257, 513, 1100), (9, 300, 65), (4, 5000, 41), (50, 30, 20)])
+def test_rows_of_very_large_scores_under_a_scale(eng, n, k, d, dtype, size):
+    """The same with a scale that scores are rounded by: a score less its row's
+    log-sum is 0 or less, never the rounding of a product."""
+    c = Values(n, k, d, dtype, 13, ignored=0.0, scale=1.3)
+    c.t[:] = torch.arange(n, device="cuda") % k
+    big = torch.arange(0, n, 2, device="cuda")
+    c.x[big] *= size if dtype != torch.float16 else min(size, 1e4)
+    c.dloss = 1e-3 * c.dloss
+    loss, lse, dx, dw = c.run(eng)
+    c.check((loss, lse, dx, dw), floor=size == 1e3 or dtype == torch.float16)
+    X, W = c.x[big].double(), c.w.double()
+    z = c.scale * (X @ W.T)
+    two = z.topk(2, 1).values
+    near = c.scale * (2.0 ** -20 + d * 2.0 ** -24) * (X.abs() @ W.abs().T).amax(1)
+    clear = two[:, 0] - two[:, 1] > 100.0 + 4 * near
+    assert size < 1e5 or clear.sum() >= len(big) // 2
+    rows = big[clear]
+    g = c.scale * c.dloss[rows].double()[:, None]
+    best = W[z[clear].argmax(1)]
+    want = g * (best - W[c.t[rows]])
+    keep = {torch.float32: 0.0, torch.bfloat16: 2.0 ** -7, torch.float16: 2.0 ** -9}[dtype]
+    tol = (2.0 ** -19 + keep) * g.abs() * (best.abs() + W[c.t[rows]].abs())
+    # P of f16 and of two terms leaves out 2^-38 of the largest loss gradient.
+    tol = tol + 2.0 ** -36 * float(c.dloss.abs().max()) * W.abs().sum(0)
+    within(dx[rows], want, tol + HALF_ULP[dtype] * want.abs() + 2 * TINY[dtype], "dx of the clear rows")
